@@ -185,6 +185,77 @@ int ob_attention_decode(ob_ctx *ctx, const float *q, const float *k, const float
 int ob_attention_decode_static(ob_ctx *ctx, const float *q_dev, const void *k_pages_dev, const void *v_pages_dev,
                                const int32_t *page_table_dev, uint32_t n_pos, uint32_t n_head, uint32_t n_head_kv,
                                uint32_t head_dim, float scale, float *out_dev, void *stream);
+/* ------------------------------------------------- pages of a cache that the caller holds
+ * Operators of speculative decoding and of long contexts over caller-owned device memory, beside ob_attention_decode_static.  No
+ * counterpart in the reference, whose caches are contiguous.  A cache is K and V apart, [layer][page][n_head_kv][16][head_dim], f16 or
+ * bfloat16 (queries and outputs are of the same type), and a table of page numbers per sequence: position x of sequence s lies in slot
+ * x % 16 of page tables[s][x / 16].  An entry outside [0, n_pages) holds no positions: nobody sees them, nothing is read or written there.
+ *
+ * All pointers but `desc` are device memory of the context's GPU (refused otherwise).  Calls are asynchronous on `stream` (a cudaStream_t
+ * of that GPU, or NULL for the context's stream), allocate nothing and may be captured.  A handle owns a workspace (64 MiB) that its
+ * calls share: calls on one handle that may overlap on the GPU, replays of captured ones included, have to be ordered by the caller;
+ * handles of the same pages may be used side by side.  Numbers in device memory are not known to the host: where the text below gives
+ * them a range, what lies outside is left out, never followed.  Products accumulate in fp32, softmax statistics are fp32. */
+#define OB_TYPE_F16 1u /* with OB_TYPE_BF16 below: types of pages; neither is a type of weights here */
+typedef struct ob_pages ob_pages;
+typedef struct ob_pages_desc {
+    void *k, *v;            /* aligned to 16 bytes */
+    uint64_t layer_stride;  /* elements from a layer's pages to the next one's, a multiple of 8; unused with one layer */
+    uint32_t type;          /* OB_TYPE_F16 or OB_TYPE_BF16 */
+    uint32_t n_layer, n_pages, n_head_kv;
+    uint32_t head_dim;      /* 64 or 128 */
+    uint32_t n_seq, table_stride; /* tables: [n_seq][table_stride] */
+    int32_t *tables;
+} ob_pages_desc;
+/* The description is copied; the memory it names stays the caller's and has to outlive the handle's calls.  Destroy waits for the device. */
+int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out);
+void ob_pages_destroy(ob_pages *pages);
+
+/* Attention of drafted tokens.  Sequence s has n_ctx[s] positions that all of its drafted tokens see, and drafted tokens first_token[s] ..
+ * first_token[s + 1] - 1 of the packed n_tokens (first_token: [n_seq + 1], ascending; no more than max_drafts <= 64 each, those past it
+ * are left out), whose keys and values are at positions n_ctx[s] + 0, 1, ...  Token i sees drafted token j of its sequence where bit j of
+ * visible[i] is set -- itself, too, only where its own bit is.  out = sum of softmax(scale q.k) v over what is seen, zero where that is
+ * nothing.  q and out: [n_tokens][n_head][head_dim] with q_stride and out_stride elements from token to token (multiples of 8; not the same
+ * memory); at most 16 query heads per key/value head.  max_ctx: about the largest n_ctx; it shares out the work, results do not depend on
+ * its being right.  Tokens of no sequence are left as they were. */
+int ob_pages_attention_tree(ob_pages *pages, uint32_t layer, uint32_t n_seq, const void *q, uint64_t q_stride, uint32_t n_tokens,
+                            const int32_t *first_token, const uint32_t *n_ctx, const uint64_t *visible, uint32_t n_head, uint32_t max_drafts,
+                            uint32_t max_ctx, float scale, void *out, uint64_t out_stride, void *stream);
+
+/* Bounds of the keys of one layer's pages, for ob_pages_select.  For the pages that hold positions first_pos[s] .. n_pos[s] - 1 (no more
+ * than max_new of them a sequence), per page and key/value head, over those of its positions that are below n_pos[s]: the unit
+ * d = max |k| / 127 in scales [n_pages][n_head_kv], and codes [n_pages][n_head_kv][2][head_dim] with ceil(largest / d), then
+ * floor(smallest / d).  A key that is no number does not count, and magnitudes above 1e18 count as 1e18.  After a step that appends a
+ * token, call it with the token's position. */
+int ob_pages_bounds(ob_pages *pages, uint32_t layer, uint32_t n_seq, const uint32_t *first_pos, const uint32_t *n_pos, uint32_t max_new,
+                    int8_t *codes, float *scales, void *stream);
+
+/* The pages each row reads: one query token per row, of sequence row_seq[row] (NULL: row r is of sequence r; a row of no sequence has
+ * no pages), which sees n_pos[row] positions (no more than max_pos).  Per key/value head, with c = rint(q / dq), dq = max |q| / 127 per query head (no
+ * number counts as 0, magnitudes above 1e18 as 1e18): a page's score is the largest over the heads of
+ * (dq * d) * sum_e max(c_e * largest_e, c_e * smallest_e), an upper bound of q.k up to the rounding of c.  The first keep_first and the
+ * last keep_last pages are taken, then those with the largest scores, the first one of equals; a page that is not there scores lowest.
+ * selected: [n_rows][n_head_kv][n_select], ascending, -1 behind the last.  At most 131072 pages a row (OB_ERR_CAPACITY). */
+int ob_pages_select(ob_pages *pages, const int8_t *codes, const float *scales, uint32_t n_rows, const void *q, uint64_t q_stride,
+                    const int32_t *row_seq, const uint32_t *n_pos, uint32_t n_head, uint32_t max_pos, uint32_t n_select, uint32_t keep_first,
+                    uint32_t keep_last, int32_t *selected, void *stream);
+/* Attention of such rows over the positions below n_pos[row] of the pages that `selected` names (numbers within the sequence, any order;
+ * one that is named twice counts twice, one outside the sequence not at all).  q, out, scale as in ob_pages_attention_tree. */
+int ob_pages_attention(ob_pages *pages, uint32_t layer, uint32_t n_rows, const void *q, uint64_t q_stride, const int32_t *row_seq,
+                       const uint32_t *n_pos, uint32_t n_head, const int32_t *selected, uint32_t n_select, float scale, void *out,
+                       uint64_t out_stride, void *stream);
+
+/* Page dst[i] of every layer becomes a copy of page src[i].  A page that one pair writes may be in no other pair. */
+int ob_pages_copy(ob_pages *pages, uint32_t n, const int32_t *src, const int32_t *dst, void *stream);
+/* Sequence child[i] goes on from the first n_pos[i] positions of sequence parent[i]: its table names the parent's full pages, and
+ * page fresh[i], with the contents copied, for a last one that is not full.  Which sequences hold a page is for the caller to count.  A
+ * child may be in no other place of the same call. */
+int ob_pages_fork(ob_pages *pages, uint32_t n, const int32_t *parent, const int32_t *child, const uint32_t *n_pos, const int32_t *fresh, void *stream);
+/* The accepted ones of a tree of drafted tokens move together behind their context: in all layers the key and value at position n_ctx[s] + j
+ * become those that were at n_ctx[s] + kept[s][j], for j < n_kept[s] (at most kept_stride <= 64; kept: [n_seq][kept_stride], numbers below 64 in any
+ * order).  All of a sequence's are read before the first is written; those whose place or source is not there are left out. */
+int ob_pages_keep(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept, void *stream);
+
 /* sampling::apply_repeat_penalty + argmax (E/sampling.rs:336-359); last index wins ties.
  * recent may be NULL; penalty 1.0 disables it. */
 int ob_argmax(ob_ctx *ctx, const float *logits, uint32_t n_vocab, const uint32_t *recent,

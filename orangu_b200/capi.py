@@ -37,7 +37,7 @@ class ModelDesc(C.Structure):
         ("rope_freqs", C.c_void_p), ("tp_presliced", C.c_uint32), ("rope_neox", C.c_uint32)]
 
 
-TYPE_BF16 = 30
+TYPE_F16, TYPE_BF16 = 1, 30
 MIXER_LATENT_ATTENTION, MIXER_RETENTION, MIXER_ATTENTION, MIXER_STATE_SPACE, MIXER_TIME_MIXING = 1, 2, 3, 4, 5
 FF_CLAMPED_GLU, FF_RELU2, FF_EXPERTS, FF_GELU_GLU = 0, 1, 2, 3
 ROUTER_SIGMOID, ROUTER_SOFTMAX, ROUTER_SOFTMAX_ALL = 0, 1, 2
@@ -79,6 +79,11 @@ class MatmulOpC(C.Structure):
 
 class Greedy(C.Structure):
     _fields_ = [("repeat_penalty", C.c_float), ("repeat_last_n", C.c_uint32), ("recent", C.c_void_p), ("n_recent", C.c_void_p)]
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("layer_stride", C.c_uint64)] + [
+        (n, C.c_uint32) for n in ("type", "n_layer", "n_pages", "n_head_kv", "head_dim", "n_seq", "table_stride")] + [("tables", C.c_void_p)]
 
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -124,6 +129,15 @@ SIGNATURES = {
     "ob_quantize_act": (_i32, [_vp, _vp, _u32, _i32, _vp, _vp, _vp]),
     "ob_attention_decode": (_i32, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _f32, _i32, _vp]),
     "ob_attention_decode_static": (_i32, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _f32, _vp, _vp]),
+    "ob_pages_create": (_i32, [_vp, C.POINTER(PagesDesc), _PP]),
+    "ob_pages_destroy": (None, [_vp]),
+    "ob_pages_attention_tree": (_i32, [_vp, _u32, _u32, _vp, _u64, _u32, _vp, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _u64, _vp]),
+    "ob_pages_bounds": (_i32, [_vp, _u32, _u32, _vp, _vp, _u32, _vp, _vp, _vp]),
+    "ob_pages_select": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp]),
+    "ob_pages_attention": (_i32, [_vp, _u32, _u32, _vp, _u64, _vp, _vp, _u32, _vp, _u32, _f32, _vp, _u64, _vp]),
+    "ob_pages_copy": (_i32, [_vp, _u32, _vp, _vp, _vp]),
+    "ob_pages_fork": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp, _vp]),
+    "ob_pages_keep": (_i32, [_vp, _u32, _vp, _vp, _u32, _vp, _vp]),
     "ob_argmax": (_i32, [_vp, _vp, _u32, _vp, _u32, _u32, _f32, _vp]),
     "ob_model_create": (_i32, [_vp, C.POINTER(ModelDesc), _PP]),
     "ob_layered_model_create": (_i32, [_vp, C.POINTER(LayeredDesc), _PP]),

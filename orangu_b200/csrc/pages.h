@@ -1,0 +1,67 @@
+// Operators over the pages of a cache that the caller holds (include/orangu_b200.h, ob_pages_*): what the entry points of
+// pages.cu hand to the kernels of pages_attention.cu, pages_tc5.cu and pages_select.cu.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace ob {
+
+constexpr uint32_t PG_MAX_DRAFTS = 64;   // drafted tokens of a sequence: a bit each
+constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
+constexpr size_t PG_WORKSPACE = 64u << 20;  // partial results of the splits, behind the counters
+constexpr uint32_t PG_COUNTERS = 4096;   // arrival counters, zero between launches
+constexpr size_t PG_PARTIAL = PG_WORKSPACE - PG_COUNTERS * 4;
+
+// One layer's pages and the tables of the sequences.
+struct PageView {
+    const void *k, *v;  // [n_pages][n_kv][KV_PAGE][dim], f16 or bf16
+    bool is_bf16;
+    uint32_t n_pages, n_kv, dim;
+    const int32_t *tables;
+    uint32_t n_seq, stride;
+};
+
+struct PagedAttnArgs {
+    PageView pg;
+    const void *q;   // [token or row][n_kv * group][dim], q_stride elements apart
+    void *out;
+    uint64_t q_stride, out_stride;
+    uint32_t group, n_units;  // n_units: sequences (tree) or rows (list)
+    float scale;
+    // tree
+    const int32_t *first;     // [n_units + 1]
+    const uint32_t *n_ctx;    // [n_units]
+    const uint64_t *visible;  // [n_tokens]
+    uint32_t n_tokens, max_drafts, max_ctx;
+    // list
+    const int32_t *list;      // [n_units][n_kv][n_list]
+    const uint32_t *n_pos;    // [n_units]
+    const int32_t *row_seq;   // [n_units] or null: row r is of sequence r
+    uint32_t n_list;
+    // workspace
+    uint32_t *counters;
+    float *partial;
+    // filled in by the launcher
+    uint32_t row_tiles, chunk, max_chunks;
+};
+cudaError_t launch_pages_attention(PagedAttnArgs a, bool tree, int sm_count, cudaStream_t st);
+
+struct PagedSelectArgs {
+    PageView pg;
+    const int8_t *codes;   // [n_pages][n_kv][2][dim]: largest, smallest
+    const float *scales;   // [n_pages][n_kv]
+    const void *q;
+    uint64_t q_stride;
+    uint32_t group, n_rows;
+    const uint32_t *n_pos;
+    const int32_t *row_seq;
+    uint32_t max_pos, n_select, keep_first, keep_last;
+    int32_t *selected;     // [n_rows][n_kv][n_select]
+};
+cudaError_t launch_pages_select(const PagedSelectArgs &a, int sm_count, cudaStream_t st);
+uint32_t pages_select_most();  // most pages of a row
+
+}  // namespace ob
