@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <vector>
 
 #include "mixers_common.cuh"
 #include "pages.h"
@@ -17,7 +18,8 @@ struct ob_pages {
     ob_ctx *ctx;
     ob_pages_desc d;
     uint64_t layer_bytes;  // from a layer's pages to the next one's
-    uint8_t *workspace;    // PG_COUNTERS words that are zero between launches, then partial results
+    uint8_t *workspace;    // PG_COUNTERS words that are zero between launches, as many PagePiece, then partial results
+    std::vector<PageMaps> maps;  // of every layer; empty: the pool is too large for them
 };
 
 namespace {
@@ -252,13 +254,18 @@ MoveArgs moves(const ob_pages *p) {
     const ob_pages_desc &d = p->d;
     return MoveArgs{static_cast<uint8_t *>(d.k), static_cast<uint8_t *>(d.v), p->layer_bytes, d.n_pages, d.n_head_kv, d.head_dim * 2, d.tables, d.n_seq, d.table_stride};
 }
+void use_workspace(const ob_pages *p, PagedAttnArgs &a) {
+    a.counters = reinterpret_cast<uint32_t *>(p->workspace);
+    a.pieces = reinterpret_cast<PagePiece *>(p->workspace + PG_COUNTERS * 4);
+    a.partial = reinterpret_cast<float *>(p->workspace + PG_COUNTERS * (4 + sizeof(PagePiece)));
+}
 cudaStream_t stream_of(const ob_pages *p, void *stream) { return stream ? static_cast<cudaStream_t>(stream) : p->ctx->stream; }
-int launched(ob_pages *p, const char *who, cudaError_t e) {
+int launched(ob_pages *p, const char *who, cudaError_t e, uint32_t kernels = 1) {
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(p->ctx, OB_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
     }
-    p->ctx->launches += 1;
+    p->ctx->launches += kernels;
     return OB_OK;
 }
 
@@ -282,7 +289,7 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     if (!d.k || !d.v || !d.tables) return fail(ctx, OB_ERR_INVALID, "pages_create: null argument");
     if (!aligned(d.k, 16) || !aligned(d.v, 16) || !aligned(d.tables, 4)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages have to be aligned to 16 bytes, tables to 4");
     if (!on_device(ctx, d.k) || !on_device(ctx, d.v) || !on_device(ctx, d.tables)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages and tables have to be memory of the context's device");
-    ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, nullptr};
+    ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, nullptr, {}};
     if (!p) return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
     void *ws = nullptr;
     cudaError_t e = cudaMalloc(&ws, PG_WORKSPACE);
@@ -297,6 +304,12 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
         return fail(ctx, e == cudaErrorMemoryAllocation ? OB_ERR_OOM : OB_ERR_CUDA, std::string("pages_create: ") + cudaGetErrorString(e));
     }
     p->workspace = static_cast<uint8_t *>(ws);
+    p->maps.resize(d.n_layer);
+    for (uint32_t l = 0; l < d.n_layer; ++l)
+        if (!make_page_maps(view(p, l), &p->maps[l])) {
+            p->maps.clear();
+            break;
+        }
     *out = p;
     return OB_OK;
 }
@@ -330,7 +343,11 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.group = n_head / p->d.n_head_kv, a.n_units = n_seq, a.scale = scale;
     a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx;
-    a.counters = reinterpret_cast<uint32_t *>(p->workspace), a.partial = reinterpret_cast<float *>(p->workspace + PG_COUNTERS * 4);
+    use_workspace(p, a);
+    const uint32_t tc5_rows = 32;
+    const bool many = max_drafts * a.group > tc5_rows && !p->maps.empty() &&
+                      (uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + 7) / 8) * ((max_drafts * a.group + 127) / 128) < (1ull << 31);
+    if (many) return launched(p, who, launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, stream_of(p, stream)), 2);
     return launched(p, who, launch_pages_attention(a, true, p->ctx->sm_count, stream_of(p, stream)));
 }
 
@@ -357,7 +374,7 @@ int ob_pages_attention(ob_pages *p, uint32_t layer, uint32_t n_rows, const void 
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.group = n_head / p->d.n_head_kv, a.n_units = n_rows, a.scale = scale;
     a.list = selected, a.n_list = n_select, a.n_pos = n_pos, a.row_seq = row_seq;
-    a.counters = reinterpret_cast<uint32_t *>(p->workspace), a.partial = reinterpret_cast<float *>(p->workspace + PG_COUNTERS * 4);
+    use_workspace(p, a);
     return launched(p, who, launch_pages_attention(a, false, p->ctx->sm_count, stream_of(p, stream)));
 }
 

@@ -13,7 +13,11 @@ constexpr uint32_t PG_MAX_DRAFTS = 64;   // drafted tokens of a sequence: a bit 
 constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
 constexpr size_t PG_WORKSPACE = 64u << 20;  // partial results of the splits, behind the counters
 constexpr uint32_t PG_COUNTERS = 4096;   // arrival counters, zero between launches
-constexpr size_t PG_PARTIAL = PG_WORKSPACE - PG_COUNTERS * 4;
+struct alignas(32) PagePiece {  // rows whose parts several CTAs have left (pages_tc5.cu), for the kernel that adds them up
+    uint32_t parts, slot;       // 0: none; place of the first part, the others are at every other one from the next even place on
+    uint32_t rows, row, token0, head;  // rows row .. row + rows - 1 of the sequence that begins at token0
+};
+constexpr size_t PG_PARTIAL = PG_WORKSPACE - PG_COUNTERS * (4 + sizeof(PagePiece));
 
 // One layer's pages and the tables of the sequences.
 struct PageView {
@@ -43,11 +47,20 @@ struct PagedAttnArgs {
     uint32_t n_list;
     // workspace
     uint32_t *counters;
+    PagePiece *pieces;
     float *partial;
     // filled in by the launcher
     uint32_t row_tiles, chunk, max_chunks;
 };
 cudaError_t launch_pages_attention(PagedAttnArgs a, bool tree, int sm_count, cudaStream_t st);
+
+// Tensor maps of one layer's keys and values (two CUtensorMap, made once per handle and layer).
+struct alignas(64) PageMaps {
+    uint8_t bytes[256];
+};
+bool make_page_maps(const PageView &pg, PageMaps *out);  // false: the pool has too many rows for them
+cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st);
+int pages_take_status();  // 1 when a bounded wait of that kernel ran out since the last call
 
 struct PagedSelectArgs {
     PageView pg;

@@ -1,0 +1,629 @@
+// Attention of drafted tokens on the fifth-generation tensor cores: the form of ob_pages_attention_tree for more rows (drafted token, query
+// head) a key/value head than the mma.sync kernel of pages_attention.cu keeps up with.  The mathematics is the same.
+//
+// The tiles of 128 positions of all (rows, sequence, key/value head) pieces are laid end to end and shared out evenly: every SM has one CTA with
+// the same number of tiles, whatever the lengths of the contexts, and walks through the pieces that lie in its part.  A piece that
+// is cut leaves (maximum, sum, output) in fp32, and a second kernel, launched along, adds them up over all SMs (the last of a piece's
+// CTAs to arrive doing it alone took as long as all the rest: 181 us for 8 x 64 tokens of 4 heads a key/value head at 8192).
+//
+//   warps 0-7  softmax: four warps per stream, a thread per row.  Scores come from tensor memory, weights go back into the same
+//              columns: f16, or bf16 as value plus remainder.
+//   warp 8     issues the products: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
+//   warp 9     issues the TMA loads of pages, 16 rows x 64 columns each, straight from the cache into the swizzled operand tiles
+//
+// There are two streams of scores, so that one's softmax runs under the other's products.  Up to 128 rows (WIDE false) they are the even and the
+// odd tiles of the same rows, with an output each; above that they are two tiles of 128 rows that share keys and values.  Context
+// positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
+// per thread.  There, values of positions that nobody has, or that are no numbers, are set to zero in shared memory (0 times them
+// would reach rows that do not see them); what rows do see of the latter is added at the end.  All waits are bounded.
+#include <algorithm>
+#include <cstring>
+
+#include "mixers_common.cuh"
+#include "pages.h"
+#include "tc5_common.cuh"
+
+namespace ob {
+
+namespace {
+
+constexpr uint32_t PG_ROWS = 128, PG_KEYS = 128, PG_PAGES = PG_KEYS / KV_PAGE, PG_BLOCK = PG_KEYS * 128;  // block: 128 rows of 64 columns
+constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 9, PG_THREADS = 10 * 32;
+constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
+constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
+constexpr uint32_t PG_LEAST = 2;        // tiles of a CTA: one for each stream
+
+// mbarriers and small arrays, byte offsets
+constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 144, PB_S_FULL = 192, PB_P_FULL = 208, PB_O_FULL = 224, PB_Q_FULL = 240, PB_SLOT = 248, PB_ABORT = 252,
+                   PB_ODD = 256, PB_TOP = 264, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
+template <int HD, bool WIDE>
+struct PgPlan {
+    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, Q = (WIDE ? 2 : 1) * OPERAND;
+    static constexpr uint32_t FIT = (227 * 1024 - PB_BYTES - Q) / (2 * OPERAND), STAGES = FIT < 6 ? FIT : 6;
+    static constexpr uint32_t K = Q, V = K + STAGES * OPERAND, BAR = V + STAGES * OPERAND, BYTES = BAR + PB_BYTES;
+    static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
+    static constexpr uint64_t PART = (uint64_t)MR * (HD + 2);  // floats of a partial result
+    static_assert(STAGES >= 2 && BYTES <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b, float c) {
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void add2(float &d0, float &d1, float a0, float a1) {
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PG_SOFT) : "memory"); }
+
+template <typename T> __device__ __forceinline__ uint32_t pack16(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack16<bf16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float from16(__half v) { return __half2float(v); }
+__device__ __forceinline__ float from16(bf16 v) { return __bfloat162float(v); }
+template <typename T> constexpr uint32_t EXPONENT16 = 0x7c00u;
+template <> constexpr uint32_t EXPONENT16<bf16> = 0x7f80u;
+
+// A sequence as the walk sees it.
+struct PgSeq {
+    uint32_t row0, drafts, ctx, limit, n_pages, n_tiles, n_rt;  // n_rt: tiles of rows
+};
+template <uint32_t MR>
+__device__ __forceinline__ PgSeq pg_seq(const PagedAttnArgs &a, uint32_t s) {
+    PgSeq q{};
+    const int32_t f0 = a.first[s], f1 = a.first[s + 1];
+    if (f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens) return q;
+    const uint32_t room = a.pg.stride * KV_PAGE;
+    q.row0 = (uint32_t)f0;
+    q.drafts = min((uint32_t)(f1 - f0), a.max_drafts);
+    q.ctx = min(a.n_ctx[s], room);
+    q.limit = min(q.ctx + q.drafts, room);
+    q.n_pages = (q.limit + KV_PAGE - 1) / KV_PAGE;
+    q.n_tiles = (q.n_pages + PG_PAGES - 1) / PG_PAGES;
+    q.n_rt = (q.drafts * a.group + MR - 1) / MR;
+    return q;
+}
+// Pieces in the order (tile of rows, sequence, head), so that CTAs half a round apart read the same keys at about the same time.  All of a
+// warp's lanes hold the same walk.
+template <uint32_t MR>
+struct PgWalk {
+    uint32_t at, end, per;       // units (tiles) of this CTA, units a CTA (the launcher sees to it that all of them are below 2^31)
+    uint32_t rt, seq, head, tile;
+    PgSeq q;
+
+    __device__ __forceinline__ void start(const PagedAttnArgs &a) {
+        const uint32_t lane = threadIdx.x & 31;
+        uint32_t total = 0;
+        for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) {
+            const PgSeq x = s0 + lane < a.n_units ? pg_seq<MR>(a, s0 + lane) : PgSeq{};
+            total += (uint32_t)warp_sum_i((int)(x.n_tiles * x.n_rt)) * a.pg.n_kv;
+        }
+        per = max((total + gridDim.x - 1) / gridDim.x, PG_LEAST);
+        at = min(total, blockIdx.x * per), end = min(total, at + per);
+        rt = seq = head = tile = 0;
+        q = PgSeq{};
+        if (at >= end) return;
+        uint32_t before = 0;
+        for (rt = 0; rt < a.row_tiles; ++rt)
+            for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) {
+                const PgSeq x = s0 + lane < a.n_units ? pg_seq<MR>(a, s0 + lane) : PgSeq{};
+                const uint32_t mine = rt < x.n_rt ? x.n_tiles * a.pg.n_kv : 0;
+                uint32_t sum = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= (uint32_t)o) sum += up;
+                }
+                const uint32_t hit = __ballot_sync(0xffffffffu, at < before + sum);
+                if (hit) {
+                    const int src = __ffs(hit) - 1;
+                    seq = s0 + src;
+                    const uint32_t off = at - (before + __shfl_sync(0xffffffffu, sum - mine, src));
+                    q = pg_seq<MR>(a, seq);
+                    head = off / q.n_tiles, tile = off % q.n_tiles;
+                    return;
+                }
+                before += __shfl_sync(0xffffffffu, sum, 31);
+            }
+        at = end;
+    }
+    __device__ __forceinline__ bool more() const { return at < end; }
+    __device__ __forceinline__ uint32_t last() const { return min(q.n_tiles, tile + (end - at)); }  // the present piece is tiles [tile, last())
+    __device__ __forceinline__ void next(const PagedAttnArgs &a) {
+        const uint32_t to = last();
+        at += to - tile;
+        tile = 0;
+        if (at >= end || ++head < a.pg.n_kv) return;
+        head = 0;
+        do {
+            if (++seq == a.n_units) {
+                seq = 0;
+                if (++rt >= a.row_tiles) {  // (not while nobody writes the lengths meanwhile)
+                    at = end;
+                    return;
+                }
+            }
+            q = pg_seq<MR>(a, seq);
+        } while (q.n_rt <= rt);
+    }
+};
+
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(PG_THREADS, 1)
+pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
+    using P = PgPlan<HD, WIDE>;
+    constexpr bool REMAINDER = EXPONENT16<T> == 0x7f80u;
+    constexpr uint32_t ST = P::STAGES, OPERAND = P::OPERAND, NB = P::NB, MR = P::MR;
+    extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
+    const uint32_t sbase = smem_u32(smem);
+    const uint32_t bar = sbase + P::BAR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ABORT);
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < ST; ++s) {
+            mbar_init(bar + PB_K_FULL + 8 * s, 1);
+            mbar_init(bar + PB_K_EMPTY + 8 * s, 1);
+            mbar_init(bar + PB_V_FULL + 8 * s, 1);
+            mbar_init(bar + PB_V_EMPTY + 8 * s, 1);
+        }
+        for (uint32_t s = 0; s < 2; ++s) {
+            mbar_init(bar + PB_S_FULL + 8 * s, 1);
+            mbar_init(bar + PB_P_FULL + 8 * s, 4);
+            mbar_init(bar + PB_O_FULL + 8 * s, 1);
+        }
+        mbar_init(bar + PB_Q_FULL, 8);
+        *abort = 0u;
+        *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD) = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == PG_MMA_WARP) tmem_alloc(bar + PB_SLOT, PG_TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_release();  // (only now: a CTA of the next kernel must not take the tensor memory first, it would keep it until this grid is done)
+    pdl_wait();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_SLOT);
+    PgWalk<MR> w;
+    w.start(a);
+    // Tiles of a piece that a stream takes: all of them, or every other one.  With row tiles the second stream may have no rows.
+    auto has = [&](uint32_t s, uint32_t i, uint32_t rows) { return WIDE ? s == 0 || rows > PG_ROWS : (i & 1u) == s; };
+
+    if (warp == PG_TMA_WARP) {
+        uint32_t n = 0;  // tiles so far
+        bool ok = true;
+        const uint32_t nowhere = a.pg.n_pages * a.pg.n_kv * KV_PAGE;  // the row behind the pool: reads as zero
+        for (; w.more() && ok; w.next(a)) {
+            const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
+            const uint32_t end = w.last();
+            auto row_of = [&](uint32_t tile) {  // lanes 0-7: the first row of a page of the tile
+                const uint32_t p = tile * PG_PAGES + (lane & 7);
+                const int32_t id = tile < end && p < w.q.n_pages ? table[p] : -1;
+                return (uint32_t)id < a.pg.n_pages ? ((uint32_t)id * a.pg.n_kv + w.head) * KV_PAGE : nowhere;
+            };
+            uint32_t y = row_of(w.tile);
+            for (uint32_t i = w.tile; i < end && ok; ++i, ++n) {
+                const uint32_t next = row_of(i + 1), st = n % ST, par = ((n / ST) & 1u) ^ 1u;
+                if (n >= ST && !(ok = mbar_wait_warp(bar + PB_K_EMPTY + 8 * st, par, abort))) break;
+                if (lane == 0) mbar_expect_tx(bar + PB_K_FULL + 8 * st, OPERAND);
+                __syncwarp();
+                if (lane < PG_PAGES)
+                    for (uint32_t b = 0; b < NB; ++b)
+                        tma_load_2d(sbase + P::K + st * OPERAND + b * PG_BLOCK + lane * (KV_PAGE * 128), &tm_k, (int32_t)(b * 64), (int32_t)y, bar + PB_K_FULL + 8 * st);
+                __syncwarp();
+                if (n >= ST && !(ok = mbar_wait_warp(bar + PB_V_EMPTY + 8 * st, par, abort))) break;
+                if (lane == 0) mbar_expect_tx(bar + PB_V_FULL + 8 * st, OPERAND);
+                __syncwarp();
+                if (lane < PG_PAGES)
+                    for (uint32_t b = 0; b < NB; ++b)
+                        tma_load_2d(sbase + P::V + st * OPERAND + b * PG_BLOCK + lane * (KV_PAGE * 128), &tm_v, (int32_t)(b * 64), (int32_t)y, bar + PB_V_FULL + 8 * st);
+                __syncwarp();
+                y = next;
+            }
+        }
+    } else if (warp == PG_MMA_WARP) {
+        constexpr uint32_t F16 = REMAINDER ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
+        const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
+        uint32_t n = 0, turn = 0, used0 = 0, used1 = 0;  // tiles and pieces so far, weights taken from each stream so far
+        bool ok = true;
+        const uint64_t q_desc = umma_desc_sw128(sbase), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
+        auto scores = [&](uint32_t s, uint32_t at) {
+            const uint32_t st = at % ST;
+            if (!mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / ST) & 1u, abort)) return false;
+            tc_fence_after();
+            const uint64_t qd = q_desc + ((WIDE ? s * OPERAND : 0u) >> 4), kd = k_desc + (st * OPERAND >> 4);
+#pragma unroll
+            for (uint32_t b = 0; b < HD / 16; ++b)
+                umma_bf16_warp(tmem + PG_TMEM_S + s * PG_KEYS, qd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
+            umma_commit_warp(bar + PB_S_FULL + 8 * s);
+            return true;
+        };
+        for (; w.more() && ok; w.next(a), ++turn) {
+            const uint32_t tiles = w.last() - w.tile, rows = w.q.drafts * a.group - w.rt * MR;
+            ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);
+            tc_fence_after();
+            if (WIDE) {
+                for (uint32_t s = 0; s < 2 && ok; ++s)
+                    if (has(s, 0, rows)) ok = scores(s, n);
+                if (ok) umma_commit_warp(bar + PB_K_EMPTY + 8 * (n % ST));
+            } else {
+                for (uint32_t s = 0; s < 2 && s < tiles && ok; ++s) {
+                    ok = scores(s, n + s);
+                    if (ok) umma_commit_warp(bar + PB_K_EMPTY + 8 * ((n + s) % ST));
+                }
+            }
+            for (uint32_t i = 0; i < tiles && ok; ++i) {
+                const uint32_t st = (n + i) % ST;
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s) {
+                    if (!ok || !has(s, i, rows)) continue;
+                    uint32_t &used = s ? used1 : used0;
+                    ok = mbar_wait_warp(bar + PB_P_FULL + 8 * s, used & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, ((n + i) / ST) & 1u, abort);
+                    ++used;
+                    if (!ok) continue;
+                    tc_fence_after();
+                    const uint32_t p = tmem + PG_TMEM_S + s * PG_KEYS, d = tmem + PG_TMEM_O + s * 128;
+                    const uint64_t vd = v_desc + (st * OPERAND >> 4);
+                    const uint32_t add = WIDE ? i : i >> 1;  // the stream's first product writes, the others add
+#pragma unroll
+                    for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {
+                        if (REMAINDER) {  // 16 positions: eight columns of values, eight of remainders
+                            umma_bf16_ta_warp(d, p + kk * 16, vd + kk * 128, id_o, add || kk ? 1u : 0u);
+                            umma_bf16_ta_warp(d, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
+                        } else {
+                            umma_bf16_ta_warp(d, p + kk * 8, vd + kk * 128, id_o, add || kk ? 1u : 0u);
+                        }
+                    }
+                    const uint32_t step = WIDE ? 1 : 2;
+                    if (i + step >= tiles) {
+                        umma_commit_warp(bar + PB_O_FULL + 8 * s);
+                    } else {
+                        ok = scores(s, n + i + step);
+                        if (ok && !WIDE) umma_commit_warp(bar + PB_K_EMPTY + 8 * ((n + i + step) % ST));
+                    }
+                }
+                if (!ok) break;
+                umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
+                if (WIDE && i + 1 < tiles) umma_commit_warp(bar + PB_K_EMPTY + 8 * ((n + i + 1) % ST));
+            }
+            n += tiles;
+        }
+    } else if (warp < PG_MMA_WARP) {
+        const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
+        const float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
+        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * PG_KEYS, to = lanes + PG_TMEM_O;
+        volatile float *tops = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r, *sums = tops + 2 * PG_ROWS;  // [stream][row]
+        volatile uint32_t *odd = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD);
+        bool ok = true;
+        uint32_t used = 0, n = 0;   // tiles of scores taken, tiles of the CTA so far
+        bool said = false;          // a piece that others go on with has been written down
+        uint32_t both[2] = {0, 0};  // pieces with tiles of either stream (WIDE false: every warp reads both outputs)
+        for (; w.more(); w.next(a)) {
+            const uint32_t end = w.last(), tiles = end - w.tile, n_rows = w.q.drafts * a.group - w.rt * MR;  // rows from this tile of rows on
+            const uint32_t f_row = (WIDE ? s * PG_ROWS : 0u) + r, warp_row = (WIDE ? s * PG_ROWS : 0u) + quad * 32;
+            const bool live = f_row < n_rows, warm = warp_row < n_rows;  // this row, any row of the warp
+            const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
+            // ---- the queries, 16 bytes a thread and turn
+            constexpr uint32_t WORDS = HD / 8;
+#pragma unroll 8
+            for (uint32_t i = threadIdx.x; i < MR * WORDS; i += PG_SOFT) {
+                const uint32_t row = i / WORDS, c = i % WORDS, f = w.rt * MR + row;
+                const uint64_t token = w.q.row0 + f / a.group;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < n_rows) v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token * a.q_stride + (uint64_t)(w.head * a.group + f % a.group) * HD + 8 * c);
+                *reinterpret_cast<uint4 *>(smem + row / PG_ROWS * OPERAND + c / 8 * PG_BLOCK + row % PG_ROWS * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar + PB_Q_FULL);
+            uint64_t seen = 0;
+            if (live && w.q.ctx < end * PG_KEYS) {
+                seen = a.visible[w.q.row0 + (w.rt * MR + f_row) / a.group];
+                if (w.q.limit - w.q.ctx < 64) seen &= (1ull << (w.q.limit - w.q.ctx)) - 1;
+            }
+            auto pages_of = [&](uint32_t tile) {  // lanes 0-7: whether a page of the tile is there
+                const uint32_t p = tile * PG_PAGES + (lane & 7);
+                return tile < end && p < w.q.n_pages && (uint32_t)table[p] < a.pg.n_pages;
+            };
+            // ---- the tiles
+            const uint32_t step = WIDE ? 1 : 2, first = WIDE ? 0 : s;
+            const bool mine = WIDE ? s == 0 || n_rows > PG_ROWS : s < tiles;  // this stream has tiles here
+            float m = -INFINITY, l = 0.0f;
+            bool there = pages_of(w.tile + first);
+            for (uint32_t i = first; mine && ok && i < tiles; i += step, ++used) {
+                ok = mbar_wait_warp(bar + PB_S_FULL + 8 * s, used & 1u, abort);
+                if (!ok) break;
+                const uint32_t valid = __ballot_sync(0xffffffffu, there) & 0xffu, x0 = (w.tile + i) * PG_KEYS;
+                there = pages_of(w.tile + i + step);
+                const bool masked = valid != 0xffu || x0 + PG_KEYS > w.q.ctx;
+                if (x0 + PG_KEYS > w.q.ctx) {  // values of positions past the context
+                    ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
+                    if (!ok) break;
+                    uint8_t *v = smem + P::V + (n + i) % ST * OPERAND;
+                    const uint32_t from = w.q.ctx > x0 ? w.q.ctx - x0 : 0u;
+                    bool bad = false;
+#pragma unroll 1
+                    for (uint32_t c = from * 8 + (warp % 4) * 32 + lane; c < PG_KEYS * 8; c += 128)
+#pragma unroll 1
+                        for (uint32_t b = 0; b < NB; ++b) {
+                            uint4 *at = reinterpret_cast<uint4 *>(v + b * PG_BLOCK) + c;
+                            uint32_t u[4] = {at->x, at->y, at->z, at->w};
+                            if (x0 + c / 8 >= w.q.limit) {
+                                *at = make_uint4(0, 0, 0, 0);
+                            } else {
+                                bool here = false;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if ((u[e] & EXPONENT16<T>) == EXPONENT16<T>) u[e] &= 0xffff0000u, here = true;
+                                    if ((u[e] >> 16 & EXPONENT16<T>) == EXPONENT16<T>) u[e] &= 0xffffu, here = true;
+                                }
+                                if (here) *at = make_uint4(u[0], u[1], u[2], u[3]), bad = true;
+                            }
+                        }
+                    if (bad) *odd = 1u;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                if (warm) {
+                    tc_fence_after();
+                    uint64_t bits[2] = {~0ull, ~0ull};  // what the row sees of the tile
+                    if (masked)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const uint32_t k0 = x0 + c * 64;
+                            bits[c] = k0 >= w.q.ctx ? 0ull : w.q.ctx - k0 >= 64 ? ~0ull : (1ull << (w.q.ctx - k0)) - 1;  // context
+                            if (k0 + 64 > w.q.ctx) {  // drafted token j at ctx + j
+                                const int shift = (int)(w.q.ctx - k0);  // above -64 where any of them is here
+                                bits[c] |= shift >= 0 ? seen << shift : shift > -64 ? seen >> -shift : 0ull;
+                            }
+#pragma unroll
+                            for (int p = 0; p < 4; ++p)
+                                if (!(valid >> (c * 4 + p) & 1)) bits[c] &= ~(0xffffull << (16 * p));
+                        }
+                    auto hide = [&](uint32_t(&u)[32], int c) {
+                        const uint32_t word = (uint32_t)(bits[c / 2] >> (c % 2 * 32));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(word >> e & 1)) u[e] = 0xff800000u;
+                    };
+                    // the scores are read twice, for the maximum and for the weights: 128 of them at a time would not fit beside the rest
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    uint32_t u[2][32];
+                    tmem_ld32(ts, u[0]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_ld32(ts + 32 * ((c + 1) % 4), u[(c + 1) % 2]);
+                        if (masked) hide(u[c % 2], c);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) top[e % 4] = fmaxf(top[e % 4], __uint_as_float(u[c % 2][e]));
+                        tmem_ld_wait();
+                    }
+                    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                    const bool grown = m > -INFINITY && now > m + PG_SLACK;
+                    if (__any_sync(0xffffffffu, grown)) {  // the product before this tile's scores is done: the output may be rescaled
+                        const float keep = grown ? pow2(m - now) : 1.0f;
+                        if (grown) m = now, l *= keep;
+#pragma unroll 1
+                        for (uint32_t c = 0; c < HD; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + s * 128 + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st16(to + s * 128 + c, o);
+                        }
+                    }
+                    if (m == -INFINITY) m = now;
+                    const float base = m == -INFINITY ? 0.0f : -m;  // a row that has seen nothing yet keeps weights of zero
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {  // 32 positions; the next ones are on their way
+                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), u[(c + 1) % 2]);
+                        uint32_t(&x)[32] = u[c % 2];
+                        if (masked) hide(x, c);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            uint32_t v[16];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                float e0, e1;
+                                fma2(e0, e1, __uint_as_float(x[16 * g + 2 * e]), __uint_as_float(x[16 * g + 2 * e + 1]), scale2, base);
+                                e0 = pow2(e0), e1 = pow2(e1);
+                                add2(sum0, sum1, e0, e1);
+                                v[e] = pack16<T>(e0, e1);
+                                if constexpr (REMAINDER) v[8 + e] = pack16<T>(e0 - __uint_as_float(v[e] << 16), e1 - __uint_as_float(v[e] & 0xffff0000u));
+                            }
+                            if constexpr (REMAINDER) {
+                                tmem_st16(ts + 32 * c + 16 * g, v);
+                            } else {
+                                const uint32_t(&h)[8] = reinterpret_cast<const uint32_t(&)[8]>(v);
+                                tmem_st8(ts + 16 * c + 8 * g, h);
+                            }
+                        }
+                        if (c < 3) tmem_ld_wait();
+                    }
+                    l += sum0 + sum1;
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar + PB_P_FULL + 8 * s);
+            }
+            n += tiles;
+            // ---- the piece is done: the streams' outputs and sums
+            const bool had[2] = {true, WIDE ? n_rows > PG_ROWS : tiles > 1};
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k)
+                if (had[k]) {
+                    if (!WIDE || k == s) ok = ok && mbar_wait_warp(bar + PB_O_FULL + 8 * k, both[k] & 1u, abort);
+                    ++both[k];
+                }
+            tc_fence_after();
+            tops[s * PG_ROWS] = m, sums[s * PG_ROWS] = l;
+            soft_sync();
+            const uint32_t origin = w.at - w.tile;  // of the whole piece in units
+            const uint32_t c0 = origin / w.per, c1 = (origin + w.q.n_tiles - 1) / w.per;  // CTAs that have a part of it
+            const bool whole = c0 == c1;
+            auto slot = [&](uint32_t c) { return a.partial + (2ull * c + (origin > c * w.per ? 1 : 0)) * P::PART; };  // a CTA has a part of two pieces at most
+            float *part_out = slot(blockIdx.x);
+            // this thread's columns of its row: all of them, or (both streams have the same rows) half of them of both outputs
+            constexpr uint32_t COLS = WIDE ? HD : HD / 2;
+            const uint32_t col0 = WIDE ? 0u : s * COLS;
+            float f0 = 1.0f, f1 = 0.0f, sum = l, peak = m;
+            if (!WIDE) {
+                const float m0 = tops[0], m1 = had[1] ? tops[PG_ROWS] : -INFINITY;
+                peak = fmaxf(m0, m1);
+                f0 = m0 == -INFINITY ? 0.0f : pow2(m0 - peak), f1 = m1 == -INFINITY ? 0.0f : pow2(m1 - peak);
+                sum = sums[0] * f0 + (had[1] ? sums[PG_ROWS] * f1 : 0.0f);
+            }
+            const uint32_t f = w.rt * MR + f_row;
+            const uint64_t token = w.q.row0 + f / a.group;
+            T *out = static_cast<T *>(a.out) + token * a.out_stride + (uint64_t)(w.head * a.group + f % a.group) * HD;
+            const float norm = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // nothing seen: 0; a sum that is no number stays none
+            const bool special = *odd != 0u;
+            if (ok && warm && (!WIDE || had[s]))
+#pragma unroll 1
+                for (uint32_t c = 0; c < COLS; c += 16) {
+                    uint32_t o0[16], o1[16];
+                    tmem_ld16(to + (WIDE ? s * 128 : 0u) + col0 + c, o0);
+                    if (!WIDE) tmem_ld16(to + 128 + col0 + c, o1);
+                    tmem_ld_wait();
+                    float x[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        x[e] = f0 != 0.0f ? __uint_as_float(o0[e]) * f0 : 0.0f;  // (a stream without tiles has left nothing there)
+                        if (!WIDE && f1 != 0.0f) x[e] = fmaf(__uint_as_float(o1[e]), f1, x[e]);
+                    }
+                    if (special && live) {  // values that are no numbers, of drafted tokens that this row sees (their weights are above zero)
+#pragma unroll 1
+                        for (uint32_t j = 0; j < w.q.limit - w.q.ctx; ++j) {
+                            const uint32_t pos = w.q.ctx + j;
+                            if (!(seen >> j & 1) || pos < w.tile * PG_KEYS || pos >= end * PG_KEYS) continue;
+                            const int32_t id = table[pos / KV_PAGE];
+                            if ((uint32_t)id >= a.pg.n_pages) continue;
+                            const T *v = static_cast<const T *>(a.pg.v) + (((uint64_t)id * a.pg.n_kv + w.head) * KV_PAGE + pos % KV_PAGE) * HD + col0 + c;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float y = from16(v[e]);
+                                if (!(fabsf(y) <= 3.4028235e38f)) x[e] += y;
+                            }
+                        }
+                    }
+                    if (live && whole) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 8)
+                            *reinterpret_cast<uint4 *>(out + col0 + c + e) = make_uint4(pack16<T>(x[e] * norm, x[e + 1] * norm), pack16<T>(x[e + 2] * norm, x[e + 3] * norm),
+                                                                                       pack16<T>(x[e + 4] * norm, x[e + 5] * norm), pack16<T>(x[e + 6] * norm, x[e + 7] * norm));
+                    } else if (live) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)f_row * HD + col0 + c + e), make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                    }
+                }
+            if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
+            if (!whole && origin >= blockIdx.x * w.per && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
+                a.pieces[blockIdx.x] = PagePiece{c1 - c0 + 1, 2 * c0 + (origin > c0 * w.per ? 1u : 0u), min(n_rows, MR), w.rt * MR, w.q.row0, w.head};
+                said = true;
+            }
+            tc_fence_before();
+            soft_sync();  // outputs, sums and maxima have been read
+            if (threadIdx.x == 0) *odd = 0u;
+        }
+        if (threadIdx.x == 0 && !said) a.pieces[blockIdx.x].parts = 0;
+    }
+    __syncwarp();
+    if (*abort) {  // let copies that are still in flight land before the shared memory goes away
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PG_MMA_WARP) tmem_dealloc(tmem, PG_TMEM_COLS);
+}
+
+// grid (CTAs of the kernel above, rows / ROWS): the parts of the piece that began in a CTA, four columns a thread.
+template <typename T, int HD, uint32_t MR>
+__global__ void __launch_bounds__(256) pages_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr uint32_t VEC = HD / 4, ROWS = 256 / VEC;
+    constexpr uint64_t PART = (uint64_t)MR * (HD + 2);
+    pdl_release();
+    pdl_wait();
+    const PagePiece p = a.pieces[blockIdx.x];
+    const uint32_t row = blockIdx.y * ROWS + threadIdx.x / VEC, c = threadIdx.x % VEC;
+    if (p.parts == 0 || row >= p.rows) return;
+    float top = -INFINITY, total = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (uint32_t k = 0; k < p.parts; ++k) {
+        const float *at = a.partial + (k ? (p.slot & ~1u) + 2 * k : p.slot) * PART;
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(at + (uint64_t)MR * HD + 2 * row));
+        const float4 y = __ldcg(reinterpret_cast<const float4 *>(at + (uint64_t)row * HD + 4 * c));
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+        const float higher = fmaxf(top, ml.x), g0 = top == -INFINITY ? 0.0f : pow2(top - higher), g1 = ml.x == -INFINITY ? 0.0f : pow2(ml.x - higher);
+        top = higher;
+        total = fmaf(ml.y, g1, total * g0);
+        x.x = fmaf(y.x, g1, x.x * g0), x.y = fmaf(y.y, g1, x.y * g0), x.z = fmaf(y.z, g1, x.z * g0), x.w = fmaf(y.w, g1, x.w * g0);
+    }
+    const float g = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;
+    const uint32_t f = p.row + row;
+    *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (uint64_t)(p.token0 + f / a.group) * a.out_stride + (uint64_t)(p.head * a.group + f % a.group) * HD + 4 * c) =
+        make_uint2(pack16<T>(x.x * g, x.y * g), pack16<T>(x.z * g, x.w * g));
+}
+
+template <typename T, int HD, bool WIDE>
+cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStream_t st) {
+    using P = PgPlan<HD, WIDE>;
+    auto kernel = pages_tree_tc5_kernel<T, HD, WIDE>;
+    static PerDeviceOnce once;
+    if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES); })) return e;
+    a.row_tiles = (a.max_drafts * a.group + P::MR - 1) / P::MR;
+    const uint32_t ctas = std::min<uint32_t>({(uint32_t)sm_count, PG_COUNTERS, (uint32_t)(PG_PARTIAL / (2 * P::PART * 4))});
+    static_assert(sizeof(PageMaps) == 2 * sizeof(CUtensorMap), "two maps");
+    CUtensorMap tm[2];
+    memcpy(tm, &maps, sizeof(tm));
+    g_tc5_launched.store(true, std::memory_order_relaxed);
+    if (cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(PG_THREADS), P::BYTES, st, tm[0], tm[1], a)) return e;
+    const uint32_t rows = std::min(P::MR, a.max_drafts * a.group), per = 256 / (HD / 4);
+    return launch_pdl(pages_merge_kernel<T, HD, P::MR>, dim3(ctas, (rows + per - 1) / per), dim3(256), 0, st, a);
+}
+
+}  // namespace
+
+bool make_page_maps(const PageView &pg, PageMaps *out) {
+    const uint64_t rows = (uint64_t)pg.n_pages * pg.n_kv * KV_PAGE;
+    if (rows + PG_KEYS > 0x7fffffffull) return false;  // coordinates have 31 bits
+    const CUtensorMapDataType type = pg.is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap tm[2];
+    if (!make_map_2d(&tm[0], type, 2, pg.k, pg.dim, rows, (uint64_t)pg.dim * 2, 64, KV_PAGE, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !make_map_2d(&tm[1], type, 2, pg.v, pg.dim, rows, (uint64_t)pg.dim * 2, 64, KV_PAGE, CU_TENSOR_MAP_SWIZZLE_128B))
+        return false;
+    memcpy(out, tm, sizeof(tm));
+    return true;
+}
+
+cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st) {
+    const bool wide = a.max_drafts * a.group > PG_ROWS;
+    if (a.pg.is_bf16) {
+        if (a.pg.dim == 64) return wide ? launch<bf16, 64, true>(a, maps, sm_count, st) : launch<bf16, 64, false>(a, maps, sm_count, st);
+        return wide ? launch<bf16, 128, true>(a, maps, sm_count, st) : launch<bf16, 128, false>(a, maps, sm_count, st);
+    }
+    if (a.pg.dim == 64) return wide ? launch<__half, 64, true>(a, maps, sm_count, st) : launch<__half, 64, false>(a, maps, sm_count, st);
+    return wide ? launch<__half, 128, true>(a, maps, sm_count, st) : launch<__half, 128, false>(a, maps, sm_count, st);
+}
+
+int pages_take_status() {
+    if (!g_tc5_launched.load()) return 0;  // (it stays set: replays of captured calls leave no trace on the host)
+    uint32_t v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tc5_status, 4) != cudaSuccess) return 0;
+    if (v) {
+        const uint32_t z = 0;
+        cudaMemcpyToSymbol(g_tc5_status, &z, 4);
+    }
+    return (int)v;
+}
+
+}  // namespace ob
