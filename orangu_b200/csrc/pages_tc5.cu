@@ -54,6 +54,11 @@ __device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, f
 __device__ __forceinline__ void add2(float &d0, float &d1, float a0, float a1) {
     asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PG_SOFT) : "memory"); }
 
 template <typename T> __device__ __forceinline__ uint32_t pack16(float a, float b);
@@ -99,9 +104,11 @@ struct PgWalk {
 
     __device__ __forceinline__ void start(const PagedAttnArgs &a) {
         const uint32_t lane = threadIdx.x & 31;
+        auto load = [&](uint32_t s0) { return s0 + lane < a.n_units ? pg_seq<MR>(a, s0 + lane) : PgSeq{}; };
+        const PgSeq front = load(0);  // (up to 32 sequences are read once)
         uint32_t total = 0;
         for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) {
-            const PgSeq x = s0 + lane < a.n_units ? pg_seq<MR>(a, s0 + lane) : PgSeq{};
+            const PgSeq x = s0 ? load(s0) : front;
             total += (uint32_t)warp_sum_i((int)(x.n_tiles * x.n_rt)) * a.pg.n_kv;
         }
         per = max((total + gridDim.x - 1) / gridDim.x, PG_LEAST);
@@ -112,7 +119,7 @@ struct PgWalk {
         uint32_t before = 0;
         for (rt = 0; rt < a.row_tiles; ++rt)
             for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) {
-                const PgSeq x = s0 + lane < a.n_units ? pg_seq<MR>(a, s0 + lane) : PgSeq{};
+                const PgSeq x = s0 ? load(s0) : front;
                 const uint32_t mine = rt < x.n_rt ? x.n_tiles * a.pg.n_kv : 0;
                 uint32_t sum = mine;
 #pragma unroll
@@ -123,9 +130,10 @@ struct PgWalk {
                 const uint32_t hit = __ballot_sync(0xffffffffu, at < before + sum);
                 if (hit) {
                     const int src = __ffs(hit) - 1;
+                    auto of = [&](uint32_t v) { return __shfl_sync(0xffffffffu, v, src); };
+                    const uint32_t off = at - (before + of(sum - mine));
                     seq = s0 + src;
-                    const uint32_t off = at - (before + __shfl_sync(0xffffffffu, sum - mine, src));
-                    q = pg_seq<MR>(a, seq);
+                    q = PgSeq{of(x.row0), of(x.drafts), of(x.ctx), of(x.limit), of(x.n_pages), of(x.n_tiles), of(x.n_rt)};
                     head = off / q.n_tiles, tile = off % q.n_tiles;
                     return;
                 }
@@ -309,14 +317,22 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             const bool live = f_row < n_rows, warm = warp_row < n_rows;  // this row, any row of the warp
             const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
             // ---- the queries, 16 bytes a thread and turn
-            constexpr uint32_t WORDS = HD / 8;
-#pragma unroll 8
-            for (uint32_t i = threadIdx.x; i < MR * WORDS; i += PG_SOFT) {
-                const uint32_t row = i / WORDS, c = i % WORDS, f = w.rt * MR + row;
-                const uint64_t token = w.q.row0 + f / a.group;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < n_rows) v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token * a.q_stride + (uint64_t)(w.head * a.group + f % a.group) * HD + 8 * c);
-                *reinterpret_cast<uint4 *>(smem + row / PG_ROWS * OPERAND + c / 8 * PG_BLOCK + row % PG_ROWS * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+            constexpr uint32_t WORDS = HD / 8, TURNS = MR * WORDS / PG_SOFT, BATCH = TURNS < 8 ? TURNS : 8;  // (all of a batch's loads before its stores)
+#pragma unroll 1
+            for (uint32_t t = 0; t < TURNS; t += BATCH) {
+                uint4 v[BATCH];
+#pragma unroll
+                for (uint32_t k = 0; k < BATCH; ++k) {
+                    const uint32_t i = (t + k) * PG_SOFT + threadIdx.x, row = i / WORDS, c = i % WORDS, f = w.rt * MR + row;
+                    const uint64_t token = w.q.row0 + f / a.group;
+                    v[k] = make_uint4(0, 0, 0, 0);
+                    if (row < n_rows) v[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token * a.q_stride + (uint64_t)(w.head * a.group + f % a.group) * HD + 8 * c));
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < BATCH; ++k) {
+                    const uint32_t i = (t + k) * PG_SOFT + threadIdx.x, row = i / WORDS, c = i % WORDS;
+                    *reinterpret_cast<uint4 *>(smem + row / PG_ROWS * OPERAND + c / 8 * PG_BLOCK + row % PG_ROWS * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[k];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_before();
@@ -401,7 +417,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         tmem_ld32(ts + 32 * ((c + 1) % 4), u[(c + 1) % 2]);
                         if (masked) hide(u[c % 2], c);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) top[e % 4] = fmaxf(top[e % 4], __uint_as_float(u[c % 2][e]));
+                        for (int e = 0; e < 32; e += 2) top[e / 2 % 4] = max3(top[e / 2 % 4], __uint_as_float(u[c % 2][e]), __uint_as_float(u[c % 2][e + 1]));
                         tmem_ld_wait();
                     }
                     const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
@@ -482,9 +498,6 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 f0 = m0 == -INFINITY ? 0.0f : pow2(m0 - peak), f1 = m1 == -INFINITY ? 0.0f : pow2(m1 - peak);
                 sum = sums[0] * f0 + (had[1] ? sums[PG_ROWS] * f1 : 0.0f);
             }
-            const uint32_t f = w.rt * MR + f_row;
-            const uint64_t token = w.q.row0 + f / a.group;
-            T *out = static_cast<T *>(a.out) + token * a.out_stride + (uint64_t)(w.head * a.group + f % a.group) * HD;
             const float norm = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // nothing seen: 0; a sum that is no number stays none
             const bool special = *odd != 0u;
             if (ok && warm && (!WIDE || had[s]))
@@ -515,14 +528,35 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                             }
                         }
                     }
-                    if (live && whole) {
+                    // a thread per row -> four (two) lanes a row: whole sectors, by way of the queries' place, which no product reads any more
+                    uint8_t *stage = smem + warp * 2048;
+                    __syncwarp();
+                    if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 8)
-                            *reinterpret_cast<uint4 *>(out + col0 + c + e) = make_uint4(pack16<T>(x[e] * norm, x[e + 1] * norm), pack16<T>(x[e + 2] * norm, x[e + 3] * norm),
-                                                                                       pack16<T>(x[e + 4] * norm, x[e + 5] * norm), pack16<T>(x[e + 6] * norm, x[e + 7] * norm));
-                    } else if (live) {
+                        for (int e = 0; e < 2; ++e)
+                            *reinterpret_cast<uint4 *>(stage + lane * 32 + ((e ^ (lane >> 2 & 1)) << 4)) =
+                                make_uint4(pack16<T>(x[8 * e] * norm, x[8 * e + 1] * norm), pack16<T>(x[8 * e + 2] * norm, x[8 * e + 3] * norm),
+                                           pack16<T>(x[8 * e + 4] * norm, x[8 * e + 5] * norm), pack16<T>(x[8 * e + 6] * norm, x[8 * e + 7] * norm));
+                        __syncwarp();
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)f_row * HD + col0 + c + e), make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                        for (uint32_t k = 0; k < 2; ++k) {
+                            const uint32_t row = 16 * k + lane / 2, f = w.rt * MR + warp_row + row;
+                            if (warp_row + row < n_rows)
+                                *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + f / a.group) * a.out_stride + (uint64_t)(w.head * a.group + f % a.group) * HD + col0 + c + 8 * (lane & 1)) =
+                                    *reinterpret_cast<const uint4 *>(stage + row * 32 + (((lane & 1) ^ (row >> 2 & 1)) << 4));
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<float4 *>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            const uint32_t row = 8 * k + lane / 4, e = lane & 3;
+                            if (warp_row + row < n_rows)
+                                __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)(warp_row + row) * HD + col0 + c + 4 * e),
+                                       *reinterpret_cast<const float4 *>(stage + row * 64 + ((e ^ (row >> 1 & 3)) << 4)));
+                        }
                     }
                 }
             if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
