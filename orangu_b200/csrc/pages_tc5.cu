@@ -6,10 +6,10 @@
 // is cut leaves (maximum, sum, output) in fp32, and a second kernel, launched along, adds them up over all SMs (the last of a piece's
 // CTAs to arrive doing it alone took as long as all the rest: 181 us for 8 x 64 tokens of 4 heads a key/value head at 8192).
 //
-//   warps 0-7  softmax: four warps per stream, a thread per row.  Scores come from tensor memory, weights go back into the same
-//              columns: f16, or bf16 as value plus remainder.
-//   warp 8     issues the products: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
-//   warp 9     issues the TMA loads of pages, 16 rows x 64 columns each, straight from the cache into the swizzled operand tiles
+//   warps 0-15 softmax: eight warps per stream, two threads per row with 64 positions each.  Scores come from tensor memory, weights go back
+//              into the same columns: f16, or bf16 as value plus remainder.
+//   warp 16    issues the products: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
+//   warp 17    issues the TMA loads of pages, 16 rows x 64 columns each, straight from the cache into the swizzled operand tiles
 //
 // There are two streams of scores, so that one's softmax runs under the other's products.  Up to 128 rows (WIDE false) they are the even and the
 // odd tiles of the same rows, with an output each; above that they are two tiles of 128 rows that share keys and values.  Context
@@ -28,7 +28,7 @@ namespace ob {
 namespace {
 
 constexpr uint32_t PG_ROWS = 128, PG_KEYS = 128, PG_PAGES = PG_KEYS / KV_PAGE, PG_BLOCK = PG_KEYS * 128;  // block: 128 rows of 64 columns
-constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 9, PG_THREADS = 10 * 32;
+constexpr int PG_SOFT = 512, PG_MMA_WARP = 16, PG_TMA_WARP = 17, PG_THREADS = 18 * 32;
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
 constexpr uint32_t PG_LEAST = 2;        // tiles of a CTA: one for each stream
@@ -38,7 +38,7 @@ constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 
                    PB_ODD = 256, PB_TOP = 264, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
 template <int HD, bool WIDE>
 struct PgPlan {
-    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, Q = (WIDE ? 2 : 1) * OPERAND;
+    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, Q = WIDE || HD == 64 ? 2 * OPERAND : OPERAND;  // (32 KB at least: outputs leave by way of it)
     static constexpr uint32_t FIT = (227 * 1024 - PB_BYTES - Q) / (2 * OPERAND), STAGES = FIT < 6 ? FIT : 6;
     static constexpr uint32_t K = Q, V = K + STAGES * OPERAND, BAR = V + STAGES * OPERAND, BYTES = BAR + PB_BYTES;
     static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
@@ -59,7 +59,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PG_SOFT) : "memory"); }
+__device__ __forceinline__ void pair_sync(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 9, %0;" ::"n"(PG_SOFT) : "memory"); }
 
 template <typename T> __device__ __forceinline__ uint32_t pack16(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
@@ -181,10 +182,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         }
         for (uint32_t s = 0; s < 2; ++s) {
             mbar_init(bar + PB_S_FULL + 8 * s, 1);
-            mbar_init(bar + PB_P_FULL + 8 * s, 4);
+            mbar_init(bar + PB_P_FULL + 8 * s, 8);
             mbar_init(bar + PB_O_FULL + 8 * s, 1);
         }
-        mbar_init(bar + PB_Q_FULL, 8);
+        mbar_init(bar + PB_Q_FULL, 16);
         *abort = 0u;
         *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD) = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -283,8 +284,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         if (REMAINDER) {  // 16 positions: eight columns of values, eight of remainders
                             umma_bf16_ta_warp(d, p + kk * 16, vd + kk * 128, id_o, add || kk ? 1u : 0u);
                             umma_bf16_ta_warp(d, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
-                        } else {
-                            umma_bf16_ta_warp(d, p + kk * 8, vd + kk * 128, id_o, add || kk ? 1u : 0u);
+                        } else {  // 64 positions are the second half of their 64 columns
+                            umma_bf16_ta_warp(d, p + kk / 4 * 64 + 32 + kk % 4 * 8, vd + kk * 128, id_o, add || kk ? 1u : 0u);
                         }
                     }
                     const uint32_t step = WIDE ? 1 : 2;
@@ -302,10 +303,12 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             n += tiles;
         }
     } else if (warp < PG_MMA_WARP) {
-        const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
+        const uint32_t s = warp / 8, part = warp / 4 % 2, quad = warp % 4, r = quad * 32 + lane, pair = 1 + s * 4 + quad;
+        const uint32_t magic = (65536 + a.group - 1) / a.group;  // x / group = x magic / 65536 for x below 4096, group up to 16
         const float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
-        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * PG_KEYS, to = lanes + PG_TMEM_O;
-        volatile float *tops = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r, *sums = tops + 2 * PG_ROWS;  // [stream][row]
+        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * PG_KEYS + part * 64, to = lanes + PG_TMEM_O;
+        volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][half][row]: maxima; at the end [stream][sum, maximum][row]
+        const uint32_t own = (2 * s + part) * PG_ROWS, other = (2 * s + (part ^ 1u)) * PG_ROWS;
         volatile uint32_t *odd = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD);
         bool ok = true;
         uint32_t used = 0, n = 0;   // tiles of scores taken, tiles of the CTA so far
@@ -323,10 +326,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 uint4 v[BATCH];
 #pragma unroll
                 for (uint32_t k = 0; k < BATCH; ++k) {
-                    const uint32_t i = (t + k) * PG_SOFT + threadIdx.x, row = i / WORDS, c = i % WORDS, f = w.rt * MR + row;
-                    const uint64_t token = w.q.row0 + f / a.group;
+                    const uint32_t i = (t + k) * PG_SOFT + threadIdx.x, row = i / WORDS, c = i % WORDS, f = w.rt * MR + row, t0 = f * magic >> 16;
                     v[k] = make_uint4(0, 0, 0, 0);
-                    if (row < n_rows) v[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + token * a.q_stride + (uint64_t)(w.head * a.group + f % a.group) * HD + 8 * c));
+                    if (row < n_rows) v[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (uint64_t)(w.q.row0 + t0) * a.q_stride + (w.head * a.group + f - t0 * a.group) * HD + 8 * c));
                 }
 #pragma unroll
                 for (uint32_t k = 0; k < BATCH; ++k) {
@@ -352,20 +354,22 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             const bool mine = WIDE ? s == 0 || n_rows > PG_ROWS : s < tiles;  // this stream has tiles here
             float m = -INFINITY, l = 0.0f;
             bool there = pages_of(w.tile + first);
-            for (uint32_t i = first; mine && ok && i < tiles; i += step, ++used) {
-                ok = mbar_wait_warp(bar + PB_S_FULL + 8 * s, used & 1u, abort);
-                if (!ok) break;
+            for (uint32_t i = first; mine && i < tiles; i += step, ++used) {
+                ok = ok && mbar_wait_warp(bar + PB_S_FULL + 8 * s, used & 1u, abort);
                 const uint32_t valid = __ballot_sync(0xffffffffu, there) & 0xffu, x0 = (w.tile + i) * PG_KEYS;
                 there = pages_of(w.tile + i + step);
                 const bool masked = valid != 0xffu || x0 + PG_KEYS > w.q.ctx;
+                if (ok && x0 + PG_KEYS > w.q.ctx) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
+                if (!ok) {  // a wait was given up: nothing more is computed, but the other half's barriers are kept company
+                    if (warm) pair_sync(pair);
+                    continue;
+                }
                 if (x0 + PG_KEYS > w.q.ctx) {  // values of positions past the context
-                    ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
-                    if (!ok) break;
                     uint8_t *v = smem + P::V + (n + i) % ST * OPERAND;
                     const uint32_t from = w.q.ctx > x0 ? w.q.ctx - x0 : 0u;
                     bool bad = false;
 #pragma unroll 1
-                    for (uint32_t c = from * 8 + (warp % 4) * 32 + lane; c < PG_KEYS * 8; c += 128)
+                    for (uint32_t c = from * 8 + (warp % 8) * 32 + lane; c < PG_KEYS * 8; c += 256)
 #pragma unroll 1
                         for (uint32_t b = 0; b < NB; ++b) {
                             uint4 *at = reinterpret_cast<uint4 *>(v + b * PG_BLOCK) + c;
@@ -387,46 +391,45 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 }
                 if (warm) {
                     tc_fence_after();
-                    uint64_t bits[2] = {~0ull, ~0ull};  // what the row sees of the tile
-                    if (masked)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const uint32_t k0 = x0 + c * 64;
-                            bits[c] = k0 >= w.q.ctx ? 0ull : w.q.ctx - k0 >= 64 ? ~0ull : (1ull << (w.q.ctx - k0)) - 1;  // context
-                            if (k0 + 64 > w.q.ctx) {  // drafted token j at ctx + j
-                                const int shift = (int)(w.q.ctx - k0);  // above -64 where any of them is here
-                                bits[c] |= shift >= 0 ? seen << shift : shift > -64 ? seen >> -shift : 0ull;
-                            }
-#pragma unroll
-                            for (int p = 0; p < 4; ++p)
-                                if (!(valid >> (c * 4 + p) & 1)) bits[c] &= ~(0xffffull << (16 * p));
+                    uint64_t bits = ~0ull;  // what the row sees of this half of the tile
+                    if (masked) {
+                        const uint32_t k0 = x0 + part * 64;
+                        bits = k0 >= w.q.ctx ? 0ull : w.q.ctx - k0 >= 64 ? ~0ull : (1ull << (w.q.ctx - k0)) - 1;  // context
+                        if (k0 + 64 > w.q.ctx) {  // drafted token j at ctx + j
+                            const int shift = (int)(w.q.ctx - k0);  // above -64 where any of them is here
+                            bits |= shift >= 0 ? seen << shift : shift > -64 ? seen >> -shift : 0ull;
                         }
+#pragma unroll
+                        for (int p = 0; p < 4; ++p)
+                            if (!(valid >> (part * 4 + p) & 1)) bits &= ~(0xffffull << (16 * p));
+                    }
                     auto hide = [&](uint32_t(&u)[32], int c) {
-                        const uint32_t word = (uint32_t)(bits[c / 2] >> (c % 2 * 32));
+                        const uint32_t word = (uint32_t)(bits >> (c * 32));
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (!(word >> e & 1)) u[e] = 0xff800000u;
                     };
-                    // the scores are read twice, for the maximum and for the weights: 128 of them at a time would not fit beside the rest
+                    // The first 32 scores are read twice, for the maximum and for the weights: all 64 would not fit beside the rest.
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    uint32_t u[2][32];
-                    tmem_ld32(ts, u[0]);
-                    tmem_ld_wait();
+                    uint32_t u[32];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld32(ts + 32 * ((c + 1) % 4), u[(c + 1) % 2]);
-                        if (masked) hide(u[c % 2], c);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) top[e / 2 % 4] = max3(top[e / 2 % 4], __uint_as_float(u[c % 2][e]), __uint_as_float(u[c % 2][e + 1]));
+                    for (int c = 0; c < 2; ++c) {
+                        tmem_ld32(ts + 32 * c, u);
                         tmem_ld_wait();
+                        if (masked) hide(u, c);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) top[e / 2 % 4] = max3(top[e / 2 % 4], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
                     }
-                    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                    const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+                    xchg[own] = here;
+                    pair_sync(pair);
+                    const float now = fmaxf(here, xchg[other]);
                     const bool grown = m > -INFINITY && now > m + PG_SLACK;
                     if (__any_sync(0xffffffffu, grown)) {  // the product before this tile's scores is done: the output may be rescaled
                         const float keep = grown ? pow2(m - now) : 1.0f;
                         if (grown) m = now, l *= keep;
 #pragma unroll 1
-                        for (uint32_t c = 0; c < HD; c += 16) {
+                        for (uint32_t c = 16 * part; c < HD; c += 32) {
                             uint32_t o[16];
                             tmem_ld16(to + s * 128 + c, o);
                             tmem_ld_wait();
@@ -439,17 +442,19 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     const float base = m == -INFINITY ? 0.0f : -m;  // a row that has seen nothing yet keeps weights of zero
                     float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {  // 32 positions; the next ones are on their way
-                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), u[(c + 1) % 2]);
-                        uint32_t(&x)[32] = u[c % 2];
-                        if (masked) hide(x, c);
+                    for (int c = 1; c >= 0; --c) {  // 32 positions
+                        if (c == 0) {
+                            tmem_ld32(ts, u);
+                            tmem_ld_wait();
+                            if (masked) hide(u, 0);
+                        }
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             uint32_t v[16];
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 float e0, e1;
-                                fma2(e0, e1, __uint_as_float(x[16 * g + 2 * e]), __uint_as_float(x[16 * g + 2 * e + 1]), scale2, base);
+                                fma2(e0, e1, __uint_as_float(u[16 * g + 2 * e]), __uint_as_float(u[16 * g + 2 * e + 1]), scale2, base);
                                 e0 = pow2(e0), e1 = pow2(e1);
                                 add2(sum0, sum1, e0, e1);
                                 v[e] = pack16<T>(e0, e1);
@@ -459,10 +464,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                                 tmem_st16(ts + 32 * c + 16 * g, v);
                             } else {
                                 const uint32_t(&h)[8] = reinterpret_cast<const uint32_t(&)[8]>(v);
-                                tmem_st8(ts + 16 * c + 8 * g, h);
+                                tmem_st8(ts + 32 + 16 * c + 8 * g, h);
                             }
                         }
-                        if (c < 3) tmem_ld_wait();
                     }
                     l += sum0 + sum1;
                     tmem_st_wait();
@@ -481,22 +485,27 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     ++both[k];
                 }
             tc_fence_after();
-            tops[s * PG_ROWS] = m, sums[s * PG_ROWS] = l;
+            if (part) xchg[own] = l;  // (both halves have read the last maxima: their products are done)
+            pair_sync(pair);
+            if (part == 0) {
+                l += xchg[other];
+                xchg[own] = l, xchg[other] = m;
+            }
             soft_sync();
             const uint32_t origin = w.at - w.tile;  // of the whole piece in units
             const uint32_t c0 = origin / w.per, c1 = (origin + w.q.n_tiles - 1) / w.per;  // CTAs that have a part of it
             const bool whole = c0 == c1;
             auto slot = [&](uint32_t c) { return a.partial + (2ull * c + (origin > c * w.per ? 1 : 0)) * P::PART; };  // a CTA has a part of two pieces at most
             float *part_out = slot(blockIdx.x);
-            // this thread's columns of its row: all of them, or (both streams have the same rows) half of them of both outputs
-            constexpr uint32_t COLS = WIDE ? HD : HD / 2;
-            const uint32_t col0 = WIDE ? 0u : s * COLS;
-            float f0 = 1.0f, f1 = 0.0f, sum = l, peak = m;
+            // this thread's columns of its row: half of them, or (both streams have the same rows) a quarter of them of both outputs
+            constexpr uint32_t COLS = WIDE ? HD / 2 : HD / 4;
+            const uint32_t col0 = (WIDE ? part : warp / 4) * COLS;
+            float f0 = 1.0f, f1 = 0.0f, sum = xchg[2 * s * PG_ROWS], peak = m;
             if (!WIDE) {
-                const float m0 = tops[0], m1 = had[1] ? tops[PG_ROWS] : -INFINITY;
+                const float m0 = xchg[PG_ROWS], m1 = had[1] ? xchg[3 * PG_ROWS] : -INFINITY;
                 peak = fmaxf(m0, m1);
                 f0 = m0 == -INFINITY ? 0.0f : pow2(m0 - peak), f1 = m1 == -INFINITY ? 0.0f : pow2(m1 - peak);
-                sum = sums[0] * f0 + (had[1] ? sums[PG_ROWS] * f1 : 0.0f);
+                sum = xchg[0] * f0 + (had[1] ? xchg[2 * PG_ROWS] * f1 : 0.0f);
             }
             const float norm = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // nothing seen: 0; a sum that is no number stays none
             const bool special = *odd != 0u;
@@ -540,9 +549,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         __syncwarp();
 #pragma unroll
                         for (uint32_t k = 0; k < 2; ++k) {
-                            const uint32_t row = 16 * k + lane / 2, f = w.rt * MR + warp_row + row;
+                            const uint32_t row = 16 * k + lane / 2, f = w.rt * MR + warp_row + row, t0 = f * magic >> 16;
                             if (warp_row + row < n_rows)
-                                *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + f / a.group) * a.out_stride + (uint64_t)(w.head * a.group + f % a.group) * HD + col0 + c + 8 * (lane & 1)) =
+                                *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + t0) * a.out_stride + (w.head * a.group + f - t0 * a.group) * HD + col0 + c + 8 * (lane & 1)) =
                                     *reinterpret_cast<const uint4 *>(stage + row * 32 + (((lane & 1) ^ (row >> 2 & 1)) << 4));
                         }
                     } else {
@@ -559,7 +568,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         }
                     }
                 }
-            if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
+            if (!whole && live && part == 0 && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
             if (!whole && origin >= blockIdx.x * w.per && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
                 a.pieces[blockIdx.x] = PagePiece{c1 - c0 + 1, 2 * c0 + (origin > c0 * w.per ? 1u : 0u), min(n_rows, MR), w.rt * MR, w.q.row0, w.head};
                 said = true;
