@@ -207,7 +207,8 @@ typedef struct ob_pages_desc {
     uint32_t n_seq, table_stride; /* tables: [n_seq][table_stride] */
     int32_t *tables;
 } ob_pages_desc;
-/* The description is copied; the memory it names stays the caller's and has to outlive the handle's calls.  Destroy waits for the device. */
+/* The description is copied; the memory it names stays the caller's and has to outlive the handle's calls.  Destroy waits for the device.  n_pages * n_head_kv * 16 has to be
+ * below 2^31 - 128 (OB_ERR_UNSUPPORTED). */
 int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out);
 void ob_pages_destroy(ob_pages *pages);
 

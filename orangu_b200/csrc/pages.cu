@@ -19,7 +19,7 @@ struct ob_pages {
     ob_pages_desc d;
     uint64_t layer_bytes;  // from a layer's pages to the next one's
     uint8_t *workspace;    // PG_COUNTERS words that are zero between launches, as many PagePiece, then partial results
-    std::vector<PageMaps> maps;  // of every layer; empty: the pool is too large for them
+    std::vector<PageMaps> maps;  // of every layer
 };
 
 namespace {
@@ -291,6 +291,12 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     if (!on_device(ctx, d.k) || !on_device(ctx, d.v) || !on_device(ctx, d.tables)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages and tables have to be memory of the context's device");
     ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, nullptr, {}};
     if (!p) return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
+    p->maps.resize(d.n_layer);
+    for (uint32_t l = 0; l < d.n_layer; ++l)
+        if (!make_page_maps(view(p, l), &p->maps[l])) {
+            delete p;
+            return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: no tensor map of the pages can be made (n_pages * n_head_kv * 16 rows have to be below 2^31)");
+        }
     void *ws = nullptr;
     cudaError_t e = cudaMalloc(&ws, PG_WORKSPACE);
     if (e == cudaSuccess) {
@@ -304,12 +310,6 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
         return fail(ctx, e == cudaErrorMemoryAllocation ? OB_ERR_OOM : OB_ERR_CUDA, std::string("pages_create: ") + cudaGetErrorString(e));
     }
     p->workspace = static_cast<uint8_t *>(ws);
-    p->maps.resize(d.n_layer);
-    for (uint32_t l = 0; l < d.n_layer; ++l)
-        if (!make_page_maps(view(p, l), &p->maps[l])) {
-            p->maps.clear();
-            break;
-        }
     *out = p;
     return OB_OK;
 }
@@ -344,10 +344,12 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     a.group = n_head / p->d.n_head_kv, a.n_units = n_seq, a.scale = scale;
     a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx;
     use_workspace(p, a);
-    const uint32_t tc5_rows = 32;
-    const bool many = max_drafts * a.group > tc5_rows && !p->maps.empty() &&
-                      (uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + 7) / 8) * ((max_drafts * a.group + 127) / 128) < (1ull << 31);
-    if (many) return launched(p, who, launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, stream_of(p, stream)), 2);
+    if (max_drafts * a.group > PG_FEW_ROWS) {
+        // (the walk over all tiles counts them in 31 bits)
+        if ((uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + 7) / 8) * ((max_drafts * a.group + 127) / 128) >= (1ull << 31))
+            return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tree: the tables of all sequences together have room for too many positions");
+        return launched(p, who, launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, stream_of(p, stream)), 2);
+    }
     return launched(p, who, launch_pages_attention(a, true, p->ctx->sm_count, stream_of(p, stream)));
 }
 

@@ -11,6 +11,7 @@ namespace ob {
 
 constexpr uint32_t PG_MAX_DRAFTS = 64;   // drafted tokens of a sequence: a bit each
 constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
+constexpr uint32_t PG_FEW_ROWS = 16;     // drafted tokens times heads of a key/value head: up to here mma.sync tiles, above tcgen05 tiles
 constexpr size_t PG_WORKSPACE = 64u << 20;  // partial results of the splits, behind the counters
 constexpr uint32_t PG_COUNTERS = 4096;   // arrival counters, zero between launches
 struct alignas(32) PagePiece {  // rows whose parts several CTAs have left (pages_tc5.cu), for the kernel that adds them up
@@ -52,7 +53,8 @@ struct PagedAttnArgs {
     // filled in by the launcher
     uint32_t row_tiles, chunk, max_chunks;
 };
-cudaError_t launch_pages_attention(PagedAttnArgs a, bool tree, int sm_count, cudaStream_t st);
+// With `tree`, max_drafts * group is at most PG_FEW_ROWS.
+cudaError_t launch_pages_attention(const PagedAttnArgs &a, bool tree, int sm_count, cudaStream_t st);
 
 // Tensor maps of one layer's keys and values (two CUtensorMap, made once per handle and layer).
 struct alignas(64) PageMaps {

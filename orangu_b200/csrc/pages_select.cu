@@ -45,13 +45,14 @@ __device__ __forceinline__ uint32_t ordered(float s) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_constant__ PagedSelectArgs a, uint32_t n_cta, uint32_t cap) {
+// MANY: more than eight heads a key/value head; the lower half of the product's rows is empty otherwise.
+template <typename T, int HD, bool MANY>
+__global__ void __launch_bounds__(SEL_THREADS, MANY ? 2 : 4) pages_select_kernel(const __grid_constant__ PagedSelectArgs a, uint32_t n_cta, uint32_t cap) {
     constexpr int LOADS = 2 * HD / 64;  // 16-byte loads of a lane per page: a quarter of the page's codes
     extern __shared__ __align__(16) uint32_t keys[];  // [cap]
     __shared__ __align__(16) int8_t s_code[PG_MAX_GROUP][HD];
     __shared__ float s_unit[PG_MAX_GROUP];
-    __shared__ uint32_t s_hist[4][256], s_warp[2][SEL_WARPS], s_pick[2], s_count[2];
+    __shared__ uint32_t s_hist[4][256], s_warp[2][SEL_WARPS], s_pick[3], s_count[2];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = n_cta > 1 ? cg::this_cluster().block_rank() : 0u;
     pdl_release();
     pdl_wait();
@@ -69,7 +70,9 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
     const uint32_t share = (n_pages + n_cta - 1) / n_cta, p0 = min(rank * share, n_pages), n = min(share, n_pages - p0);  // this CTA's pages
 
     // ---- the queries' codes
-    for (uint32_t h = warp; h < PG_MAX_GROUP; h += SEL_WARPS) {
+    constexpr uint32_t HEADS = MANY ? 16 : 8, WORDS = MANY ? 4 : 2;  // words of an A fragment that are not always zero
+#pragma unroll 1
+    for (uint32_t h = warp; h < HEADS; h += SEL_WARPS) {
         float x[HD / 32], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
@@ -87,18 +90,26 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
     for (uint32_t i = threadIdx.x; i < 4 * 256; i += SEL_THREADS) (&s_hist[0][0])[i] = 0u;
     __syncthreads();
     // Load i of a lane is bytes 64 i + 16 (lane % 4) .. + 15 of a page's codes; its words 0, 1 and 2, 3 are the two halves of a step's 32.
-    uint32_t f[LOADS][2][4];
+    uint32_t f[LOADS][2][WORDS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t at = i * 64 + (lane & 3) * 16 + j * 8 + (e >> 1) * 4, h = lane / 4 + (e & 1) * 8;
+            for (int e = 0; e < (int)WORDS; ++e) {
+                const uint32_t at = i * 64 + (lane & 3) * 16 + j * 8 + e / (WORDS / 2) * 4, h = lane / 4 + (MANY ? e & 1 : 0) * 8;
                 const uint32_t c = *reinterpret_cast<const uint32_t *>(&s_code[h][at % HD]);
                 f[i][j][e] = at < HD ? __vmaxs4(c, 0u) : __vmins4(c, 0u);  // largest keys meet the positive codes, smallest the others
             }
-    const float unit0 = s_unit[lane / 4], unit1 = s_unit[lane / 4 + 8];
+    const float unit0 = s_unit[lane / 4], unit1 = MANY ? s_unit[lane / 4 + 8] : -1.0f;
+    auto product = [&](int(&c)[4], const uint32_t(&w)[WORDS], uint32_t b0, uint32_t b1) {
+        if constexpr (MANY) {
+            mma_s8(c, w, b0, b1);
+        } else {
+            const uint32_t x[4] = {w[0], 0u, w[1], 0u};
+            mma_s8(c, x, b0, b1);
+        }
+    };
 
     // ---- scores: a warp takes eight pages at a time, two such groups in flight
     const uint64_t rec = 2 * HD;
@@ -129,16 +140,16 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
             int c[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                mma_s8(c, f[i][0], x[u][i].x, x[u][i].y);
-                mma_s8(c, f[i][1], x[u][i].z, x[u][i].w);
+                product(c, f[i][0], x[u][i].x, x[u][i].y);
+                product(c, f[i][1], x[u][i].z, x[u][i].w);
             }
             float best[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float dp = __shfl_sync(0xffffffffu, d[u], (col + e) * 4);
                 const float s0 = unit0 < 0.0f ? -INFINITY : __fmul_rn(__fmul_rn(unit0, dp), (float)c[e]);
-                const float s1 = unit1 < 0.0f ? -INFINITY : __fmul_rn(__fmul_rn(unit1, dp), (float)c[2 + e]);
-                float y = fmaxf(s0, s1);  // (fmaxf gives -inf only where no head is: heads of a page that is not there are all no numbers)
+                float y = s0;
+                if (MANY && unit1 >= 0.0f) y = fmaxf(y, __fmul_rn(__fmul_rn(unit1, dp), (float)c[2 + e]));  // (fmaxf gives -inf only where no head is: heads of a page that is not there are all no numbers)
                 if (dp != dp) y = dp;
                 y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
                 y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
@@ -159,9 +170,9 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
 
     // ---- the n_select'th largest word
     uint32_t prefix = 0, want = a.n_select;  // of the words that begin with the prefix, the want'th largest is looked for
+    int shift = 24;
 #pragma unroll 1
-    for (int round = 0; round < 4; ++round) {
-        const int shift = 24 - 8 * round;
+    for (int round = 0;; ++round, shift -= 8) {
         uint32_t *hist = s_hist[round];
         for (uint32_t i = threadIdx.x; i < (n + 31) / 32 * 32; i += SEL_THREADS) {
             const uint32_t k = i < n ? keys[i] : 0u;
@@ -188,16 +199,17 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
         if (lane == 31) s_warp[round & 1][warp] = upto;
         __syncthreads();
         for (uint32_t w = 0; w < warp; ++w) upto += s_warp[round & 1][w];
-        if (upto >= want && upto - total < want) s_pick[0] = digit, s_pick[1] = want - (upto - total);
+        if (upto >= want && upto - total < want) s_pick[0] = digit, s_pick[1] = want - (upto - total), s_pick[2] = total;
         __syncthreads();
         prefix = prefix << 8 | s_pick[0];
         want = s_pick[1];
+        if (round == 3 || want == s_pick[2]) break;  // (all words that begin so are taken: no need to look further)
         __syncthreads();
     }
-    // ---- above it: all; equal to it: the first `want` of all CTAs
+    // ---- words that begin with more than the prefix: all; with the prefix: the first `want` of all CTAs
     const uint32_t span = (n + SEL_WARPS - 1) / SEL_WARPS, w0 = min(warp * span, n), w1 = min(w0 + span, n);  // this warp's pages
     uint32_t above = 0, equal = 0;
-    for (uint32_t i = w0 + lane; i < w1; i += 32) above += keys[i] > prefix, equal += keys[i] == prefix;
+    for (uint32_t i = w0 + lane; i < w1; i += 32) above += keys[i] >> shift > prefix, equal += keys[i] >> shift == prefix;
     above = warp_sum_i(above), equal = warp_sum_i(equal);
     if (lane == 0) s_warp[0][warp] = above, s_warp[1][warp] = equal;
     __syncthreads();
@@ -215,7 +227,7 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
     }
     for (uint32_t w = 0; w < warp; ++w) above += s_warp[0][w], equal += s_warp[1][w];
     for (uint32_t i = w0; i < w1; i += 32) {
-        const uint32_t k = i + lane < w1 ? keys[i + lane] : 0u;
+        const uint32_t k = i + lane < w1 ? keys[i + lane] >> shift : 0u;
         const bool live = i + lane < w1;
         const uint32_t gt = __ballot_sync(0xffffffffu, live && k > prefix), eq = __ballot_sync(0xffffffffu, live && k == prefix), below = (1u << lane) - 1;
         const uint32_t ga = above + __popc(gt & below), ea = equal + __popc(eq & below);
@@ -225,17 +237,17 @@ __global__ void __launch_bounds__(SEL_THREADS) pages_select_kernel(const __grid_
     if (n_cta > 1) cg::this_cluster().sync();  // nobody leaves while its counts may still be read
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool MANY>
 cudaError_t launch(const PagedSelectArgs &a, int sm_count, cudaStream_t st) {
-    auto kernel = pages_select_kernel<T, HD>;
+    auto kernel = pages_select_kernel<T, HD, MANY>;
     static PerDeviceOnce once;
     if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_KEYS * 4); })) return e;
     const uint32_t pages = std::max(1u, (std::min(a.max_pos, a.pg.stride * KV_PAGE) + KV_PAGE - 1) / KV_PAGE);
     const uint64_t pairs = (uint64_t)a.n_rows * a.pg.n_kv;
-    // More CTAs a row while the SMs are not all taken twice and a CTA keeps 64 pages (a group of eight for each warp), or while a CTA's
+    // More CTAs a row while the SMs are not all taken four times and a CTA keeps 64 pages (a group of eight for each warp), or while a CTA's
     // words would not fit.
     uint32_t c = 1;
-    while (c < SEL_CLUSTER && ((pairs * c * 2 <= 2ull * sm_count && pages / (2 * c) >= 64) || (pages + c - 1) / c > SEL_KEYS)) c *= 2;
+    while (c < SEL_CLUSTER && ((pairs * c * 2 <= 4ull * sm_count && pages / (2 * c) >= 64) || (pages + c - 1) / c > SEL_KEYS)) c *= 2;
     const uint32_t cap = (pages + c - 1) / c;
     if (pairs * c > 0x7fffffffull || cap > SEL_KEYS) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute at[2];
@@ -258,8 +270,9 @@ cudaError_t launch(const PagedSelectArgs &a, int sm_count, cudaStream_t st) {
 uint32_t pages_select_most() { return SEL_CLUSTER * SEL_KEYS; }
 
 cudaError_t launch_pages_select(const PagedSelectArgs &a, int sm_count, cudaStream_t st) {
-    if (a.pg.is_bf16) return a.pg.dim == 64 ? launch<bf16, 64>(a, sm_count, st) : launch<bf16, 128>(a, sm_count, st);
-    return a.pg.dim == 64 ? launch<__half, 64>(a, sm_count, st) : launch<__half, 128>(a, sm_count, st);
+    auto pick = [&](auto few, auto many) { return a.group > 8 ? many(a, sm_count, st) : few(a, sm_count, st); };
+    if (a.pg.is_bf16) return a.pg.dim == 64 ? pick(launch<bf16, 64, false>, launch<bf16, 64, true>) : pick(launch<bf16, 128, false>, launch<bf16, 128, true>);
+    return a.pg.dim == 64 ? pick(launch<__half, 64, false>, launch<__half, 64, true>) : pick(launch<__half, 128, false>, launch<__half, 128, true>);
 }
 
 }  // namespace ob

@@ -492,11 +492,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 xchg[own] = l, xchg[other] = m;
             }
             soft_sync();
-            const uint32_t origin = w.at - w.tile;  // of the whole piece in units
-            const uint32_t c0 = origin / w.per, c1 = (origin + w.q.n_tiles - 1) / w.per;  // CTAs that have a part of it
-            const bool whole = c0 == c1;
-            auto slot = [&](uint32_t c) { return a.partial + (2ull * c + (origin > c * w.per ? 1 : 0)) * P::PART; };  // a CTA has a part of two pieces at most
-            float *part_out = slot(blockIdx.x);
+            const bool whole = w.tile == 0 && end == w.q.n_tiles;
+            const uint32_t origin = w.at - w.tile, begin = blockIdx.x * w.per;  // of the whole piece and of this CTA, in units
+            float *part_out = a.partial + (2ull * blockIdx.x + (origin > begin ? 1 : 0)) * P::PART;  // a CTA has a part of two pieces at most
             // this thread's columns of its row: half of them, or (both streams have the same rows) a quarter of them of both outputs
             constexpr uint32_t COLS = WIDE ? HD / 2 : HD / 4;
             const uint32_t col0 = (WIDE ? part : warp / 4) * COLS;
@@ -569,8 +567,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     }
                 }
             if (!whole && live && part == 0 && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
-            if (!whole && origin >= blockIdx.x * w.per && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
-                a.pieces[blockIdx.x] = PagePiece{c1 - c0 + 1, 2 * c0 + (origin > c0 * w.per ? 1u : 0u), min(n_rows, MR), w.rt * MR, w.q.row0, w.head};
+            if (!whole && origin >= begin && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
+                a.pieces[blockIdx.x] = PagePiece{(origin + w.q.n_tiles - 1) / w.per - blockIdx.x + 1, 2 * blockIdx.x + (origin > begin ? 1u : 0u), min(n_rows, MR), w.rt * MR, w.q.row0, w.head};
                 said = true;
             }
             tc_fence_before();

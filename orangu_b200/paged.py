@@ -13,19 +13,26 @@ from . import capi
 from .backend import CudaBackend
 
 _PAGE = 16
-_INT = ("torch.int32", "torch.uint32", "int32", "uint32")
+_INT = ("int32", "uint32")
 
 
 def _stream(stream):
     return 1 if stream == 0 else stream  # to the C ABI null is the context's stream; 1 is what the runtime calls the legacy default stream
 
 
+_known = {}  # (dtype, accepted names) -> whether it is one of them
+
+
 def _array(name, a, shape, dtypes):
     """Address of a contiguous array of that shape."""
-    if tuple(a.shape) != shape:
+    if a.shape != shape:
         raise ValueError(f"{name} is {list(a.shape)}, expected {list(shape)}")
-    if str(a.dtype) not in dtypes:
-        raise ValueError(f"{name} is {a.dtype}, expected {dtypes[0]}")
+    dtype = a.dtype
+    ok = _known.get((dtype, dtypes))
+    if ok is None:
+        ok = _known[dtype, dtypes] = str(dtype).replace("torch.", "") in dtypes
+    if not ok:
+        raise ValueError(f"{name} is {dtype}, expected {dtypes[0]}")
     if not a.is_contiguous():
         raise ValueError(f"{name} is not contiguous")
     return a.data_ptr()
@@ -39,9 +46,9 @@ class PagedCache:
         self._h = None
         if len(k.shape) != 5 or k.shape[3] != _PAGE:
             raise ValueError(f"k is {list(k.shape)}, expected [layers, pages, kv heads, {_PAGE}, head_dim]")
-        self._type = str(k.dtype)
-        types = {"torch.float16": capi.TYPE_F16, "torch.bfloat16": capi.TYPE_BF16}
-        if self._type not in types:
+        self._type, name = k.dtype, str(k.dtype).replace("torch.", "")
+        types = {"float16": capi.TYPE_F16, "bfloat16": capi.TYPE_BF16}
+        if name not in types:
             raise ValueError(f"k is {k.dtype}, expected float16 or bfloat16")
         shape = tuple(k.shape)
         if len(tables.shape) != 2:
@@ -49,8 +56,8 @@ class PagedCache:
         self.backend, self._lib, self._arrays = backend, backend._lib, (k, v, tables)
         self.n_layer, self.n_pages, self.n_head_kv, _, self.head_dim = shape
         self.n_seq, self.table_stride = tuple(tables.shape)
-        d = capi.PagesDesc(_array("k", k, shape, (self._type,)), _array("v", v, shape, (self._type,)), self.n_pages * self.n_head_kv * _PAGE * self.head_dim, types[self._type],
-                           self.n_layer, self.n_pages, self.n_head_kv, self.head_dim, self.n_seq, self.table_stride, _array("tables", tables, tuple(tables.shape), ("torch.int32",)))
+        d = capi.PagesDesc(_array("k", k, shape, (name,)), _array("v", v, shape, (name,)), self.n_pages * self.n_head_kv * _PAGE * self.head_dim, types[name],
+                           self.n_layer, self.n_pages, self.n_head_kv, self.head_dim, self.n_seq, self.table_stride, _array("tables", tables, tuple(tables.shape), ("int32",)))
         h = C.c_void_p()
         capi.check(backend._h, self._lib.ob_pages_create(backend._h, C.byref(d), C.byref(h)))
         self._h = h
@@ -73,12 +80,16 @@ class PagedCache:
 
     def _rows(self, name, a):
         """Address, rows, heads and row stride of queries or outputs [rows, heads, head_dim], rows any multiple of eight entries apart."""
-        shape, stride = a.shape, a.stride()
-        if len(shape) != 3 or shape[2] != self.head_dim or str(a.dtype) != self._type:
+        shape = a.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or a.dtype != self._type:
             raise ValueError(f"{name} is {list(shape)} of {a.dtype}, expected [rows, heads, {self.head_dim}] of {self._type}")
-        if stride[2] != 1 or (shape[1] > 1 and stride[1] != self.head_dim):
+        rows, heads, dim = shape
+        if a.is_contiguous():
+            return a.data_ptr(), rows, heads, heads * dim
+        stride = a.stride()
+        if stride[2] != 1 or (heads > 1 and stride[1] != dim):
             raise ValueError(f"{name}: the heads of a row are not contiguous")
-        return a.data_ptr(), shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1] * self.head_dim
+        return a.data_ptr(), rows, heads, stride[0] if rows > 1 else heads * dim
 
     def attention_tree(self, q, first_token, n_ctx, visible, scale: float, out, max_drafts: int, max_context: int, layer: int = 0, stream=None):
         """Attention of drafted tokens ``q`` [tokens, heads, head_dim] into ``out``: token i of sequence s (tokens first_token[s] .. first_token[s + 1] - 1) sees
@@ -91,11 +102,11 @@ class PagedCache:
             raise ValueError(f"out is {list(out.shape)}, expected {list(q.shape)}")
         self._check(self._lib.ob_pages_attention_tree(
             self._h, layer, n_seq, qp, q_stride, n, _array("first_token", first_token, (n_seq + 1,), _INT), _array("n_ctx", n_ctx, (n_seq,), _INT),
-            _array("visible", visible, (n,), ("torch.int64", "torch.uint64")), heads, max_drafts, max_context, scale, op, o_stride, _stream(stream)))
+            _array("visible", visible, (n,), ("int64", "uint64")), heads, max_drafts, max_context, scale, op, o_stride, _stream(stream)))
 
     def _bounds(self, codes, scales):
         pages = (self.n_pages, self.n_head_kv)
-        return _array("codes", codes, pages + (2, self.head_dim), ("torch.int8",)), _array("scales", scales, pages, ("torch.float32",))
+        return _array("codes", codes, pages + (2, self.head_dim), ("int8",)), _array("scales", scales, pages, ("float32",))
 
     def bounds(self, first_pos, n_pos, codes, scales, max_new: int, layer: int = 0, stream=None):
         """8-bit bounds of the keys of the pages that hold positions first_pos[s] .. n_pos[s] - 1 (at most ``max_new`` a sequence): codes [pages, kv heads, 2,
@@ -112,7 +123,7 @@ class PagedCache:
         n_select = selected.shape[-1]
         self._check(self._lib.ob_pages_select(
             self._h, cp, sp, n, qp, q_stride, _array("row_seq", row_seq, (n,), _INT) if row_seq is not None else None, _array("n_pos", n_pos, (n,), _INT), heads, max_pos,
-            n_select, keep_first, keep_last, _array("selected", selected, (n, self.n_head_kv, n_select), ("torch.int32",)), _stream(stream)))
+            n_select, keep_first, keep_last, _array("selected", selected, (n, self.n_head_kv, n_select), ("int32",)), _stream(stream)))
 
     def attention(self, q, selected, n_pos, scale: float, out, row_seq=None, layer: int = 0, stream=None):
         """Attention of every row over the positions below n_pos[row] of the pages in ``selected`` (numbers within the row's sequence)."""
@@ -123,12 +134,12 @@ class PagedCache:
         n_select = selected.shape[-1]
         self._check(self._lib.ob_pages_attention(
             self._h, layer, n, qp, q_stride, _array("row_seq", row_seq, (n,), _INT) if row_seq is not None else None, _array("n_pos", n_pos, (n,), _INT), heads,
-            _array("selected", selected, (n, self.n_head_kv, n_select), ("torch.int32",)), n_select, scale, op, o_stride, _stream(stream)))
+            _array("selected", selected, (n, self.n_head_kv, n_select), ("int32",)), n_select, scale, op, o_stride, _stream(stream)))
 
     def copy(self, src, dst, stream=None):
         """Page dst[i] of every layer becomes a copy of page src[i]; no page is written by one pair and in another."""
         n = src.shape[0]
-        self._check(self._lib.ob_pages_copy(self._h, n, _array("src", src, (n,), ("torch.int32",)), _array("dst", dst, (n,), ("torch.int32",)), _stream(stream)))
+        self._check(self._lib.ob_pages_copy(self._h, n, _array("src", src, (n,), ("int32",)), _array("dst", dst, (n,), ("int32",)), _stream(stream)))
 
     def fork(self, parent, child, n_pos, fresh, stream=None):
         """Sequence child[i] goes on from the first n_pos[i] positions of parent[i]: it shares the full pages; a last one that is not full is copied to page
@@ -140,5 +151,5 @@ class PagedCache:
     def keep(self, n_ctx, kept, n_kept, stream=None):
         """In all layers, position n_ctx[s] + kept[s, j] goes to n_ctx[s] + j for j < n_kept[s]: the accepted path of a tree of drafts moves together."""
         n_seq, width = kept.shape
-        self._check(self._lib.ob_pages_keep(self._h, n_seq, _array("n_ctx", n_ctx, (n_seq,), _INT), _array("kept", kept, (n_seq, width), ("torch.int32",)), width,
+        self._check(self._lib.ob_pages_keep(self._h, n_seq, _array("n_ctx", n_ctx, (n_seq,), _INT), _array("kept", kept, (n_seq, width), ("int32",)), width,
                                             _array("n_kept", n_kept, (n_seq,), _INT), _stream(stream)))
