@@ -51,7 +51,7 @@ struct PagedAttnArgs {
     PagePiece *pieces;
     float *partial;
     // filled in by the launcher
-    uint32_t row_tiles, chunk, max_chunks;
+    uint32_t row_tiles;
 };
 // With `tree`, max_drafts * group is at most PG_FEW_ROWS.
 cudaError_t launch_pages_attention(const PagedAttnArgs &a, bool tree, int sm_count, cudaStream_t st);
