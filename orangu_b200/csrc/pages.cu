@@ -391,8 +391,8 @@ int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint3
     if (n_rows > (1u << 24)) return bad(p, who, "too many rows");
     if (n_select == 0 || n_select > p->d.table_stride) return bad(p, who, "n_select has to be at least 1 and at most table_stride");
     if ((uint64_t)keep_first + keep_last > n_select) return bad(p, who, "keep_first + keep_last is more than n_select");
-    if (std::min<uint64_t>(((uint64_t)max_pos + KV_PAGE - 1) / KV_PAGE, p->d.table_stride) > pages_select_most())
-        return fail(p->ctx, OB_ERR_CAPACITY, "pages_select: a row has more than " + std::to_string(pages_select_most()) + " pages");
+    if (std::min<uint64_t>(((uint64_t)max_pos + KV_PAGE - 1) / KV_PAGE, p->d.table_stride) > PG_SELECT_PAGES)
+        return fail(p->ctx, OB_ERR_CAPACITY, "pages_select: a row has more than " + std::to_string(PG_SELECT_PAGES) + " pages");
     if (int rc = check_rows(p, who, "q_stride", q_stride, n_head)) return rc;
     if (n_rows == 0) return OB_OK;
     if (int rc = check_pointers(p, who, {{codes, "codes", 16}, {scales, "scales", 4}, {q, "q", 16}, {n_pos, "n_pos", 4}, {selected, "selected", 4}})) return rc;
@@ -402,7 +402,10 @@ int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint3
     a.pg = view(p, 0);
     a.codes = codes, a.scales = scales, a.q = q, a.q_stride = q_stride, a.group = n_head / p->d.n_head_kv, a.n_rows = n_rows, a.n_pos = n_pos, a.row_seq = row_seq;
     a.max_pos = max_pos, a.n_select = n_select, a.keep_first = keep_first, a.keep_last = keep_last, a.selected = selected;
-    return launched(p, who, launch_pages_select(a, p->ctx->sm_count, stream_of(p, stream)));
+    a.keys = reinterpret_cast<uint32_t *>(p->workspace + PG_COUNTERS * (4 + sizeof(PagePiece)));
+    uint32_t kernels = 0;
+    const cudaError_t e = launch_pages_select(a, p->ctx->sm_count, stream_of(p, stream), &kernels);
+    return launched(p, who, e, kernels);
 }
 
 int ob_pages_bounds(ob_pages *p, uint32_t layer, uint32_t n_seq, const uint32_t *first_pos, const uint32_t *n_pos, uint32_t max_new, int8_t *codes, float *scales, void *stream) {

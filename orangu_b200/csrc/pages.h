@@ -75,8 +75,10 @@ struct PagedSelectArgs {
     const int32_t *row_seq;
     uint32_t max_pos, n_select, keep_first, keep_last;
     int32_t *selected;     // [n_rows][n_kv][n_select]
+    uint32_t *keys;        // workspace, PG_KEYS_BYTES
 };
-cudaError_t launch_pages_select(const PagedSelectArgs &a, int sm_count, cudaStream_t st);
-uint32_t pages_select_most();  // most pages of a row
+constexpr size_t PG_KEYS_BYTES = PG_PARTIAL;    // (one of the two uses at a time)
+constexpr uint32_t PG_SELECT_PAGES = 131072;    // most pages of a row
+cudaError_t launch_pages_select(const PagedSelectArgs &a, int sm_count, cudaStream_t st, uint32_t *launches);
 
 }  // namespace ob

@@ -5,15 +5,16 @@
 //   score = max over the heads h of  (dq_h d) * sum_e max(c_h,e hi_e, c_h,e lo_e)  =  (dq_h d) * (sum_e max(c, 0) hi_e + sum_e min(c, 0) lo_e)
 //
 // The sum is a whole number below 2^24 and the two products are single roundings, so a score has one value whatever the order of
-// the terms, and so has the choice.  A row's sum over (hi, lo) is one row of an s8 product of length 2 dim: mma.sync m16n8k32 with the
-// heads as the 16 rows and 8 pages as columns, whose codes go from memory straight into the fragments (a lane's 16 bytes serve
-// two steps; the order of the terms inside a step is free).  What bounds it is the reading of the codes, 2 dim + 4 bytes a page.
+// the terms, and so has the choice.  The sums are an s8 product of length 2 dim: mma.sync m16n8k32 with 16 pages as rows, whose codes go
+// from memory straight into the fragments (a lane's 16 bytes serve two steps; the order of the terms inside a step is free), and the
+// heads as columns: a page's best head is two exchanges away.  Nor do the queries need shared memory: four lanes hold a head's codes just
+// where the fragments want them.  What bounds the scores is the reading of the codes, 2 dim + 4 bytes a page; with eight pages as columns and
+// the heads as rows, four times as many instructions did (51 us for 64 rows of 6 to 24 k positions, 8 heads of 128).
 //
-// One cluster per (row, head): its CTAs share the pages, keep the scores as ordered 32-bit words in shared memory, and find the
-// n_select'th by four rounds of 8 bits, adding the CTAs' histograms up through distributed shared memory.  Pages above it are taken, and
-// of those that equal it the first ones; the list is written in ascending order without another pass over memory.
-#include <cooperative_groups.h>
-
+// Scores are kept as 32-bit words in their order.  Many of them are made by a kernel of their own, a warp per 64 pages (16 where there are few), neighbouring warps
+// the heads of the same pages, whose codes lie together; few of them in the CTA that picks.  A CTA per (row, head) then picks: counts in
+// 2048 equal parts of the range, as often as the part with the border still holds more than are wanted (two times as a rule),
+// and the list is written in ascending order.
 #include <algorithm>
 
 #include "mixers_common.cuh"
@@ -23,15 +24,14 @@ namespace ob {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int SEL_WARPS = 8, SEL_THREADS = SEL_WARPS * 32;
-constexpr uint32_t SEL_CLUSTER = 8;        // most CTAs of a cluster
-constexpr uint32_t SEL_KEYS = 16384;       // most pages of a CTA
+constexpr uint32_t SEL_BINS = 2048;
+constexpr uint32_t SEL_HELD = 32768;       // words that the picking CTA holds in shared memory; with more they are read again from the workspace
+constexpr uint32_t SEL_FUSED = 512;        // pages of a row up to which the picking CTA makes the scores, too
+constexpr uint32_t SEL_FORCED = 0xffffffffu;
 constexpr float SEL_MOST = 1e18f;          // what larger queries count as: products of two units and a sum stay finite
 
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float as_float(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float2 as_float2(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
+__device__ __forceinline__ float2 as_float2(uint32_t u, bf16) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -45,232 +45,329 @@ __device__ __forceinline__ uint32_t ordered(float s) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// MANY: more than eight heads a key/value head; the lower half of the product's rows is empty otherwise.
-template <typename T, int HD, bool MANY>
-__global__ void __launch_bounds__(SEL_THREADS, MANY ? 2 : 4) pages_select_kernel(const __grid_constant__ PagedSelectArgs a, uint32_t n_cta, uint32_t cap) {
-    constexpr int LOADS = 2 * HD / 64;  // 16-byte loads of a lane per page: a quarter of the page's codes
-    extern __shared__ __align__(16) uint32_t keys[];  // [cap]
-    __shared__ __align__(16) int8_t s_code[PG_MAX_GROUP][HD];
-    __shared__ float s_unit[PG_MAX_GROUP];
-    __shared__ uint32_t s_hist[4][256], s_warp[2][SEL_WARPS], s_pick[3], s_count[2];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = n_cta > 1 ? cg::this_cluster().block_rank() : 0u;
-    pdl_release();
-    pdl_wait();
-    const uint32_t pair = blockIdx.x / n_cta, head = pair % a.pg.n_kv, row = pair / a.pg.n_kv;
+// A row's sequence and pages.
+struct SelRow {
+    const int32_t *table;
+    uint32_t n_pages;
+};
+__device__ __forceinline__ SelRow sel_row(const PagedSelectArgs &a, uint32_t row) {
     const int32_t s = a.row_seq ? a.row_seq[row] : (int32_t)row;
     const bool known = (uint32_t)s < a.pg.n_seq;
-    const uint32_t n_pos = known ? min(min(a.n_pos[row], a.max_pos), a.pg.stride * KV_PAGE) : 0u, n_pages = (n_pos + KV_PAGE - 1) / KV_PAGE;
-    const int32_t *table = a.pg.tables + (uint64_t)(known ? s : 0) * a.pg.stride;
-    int32_t *out = a.selected + (uint64_t)pair * a.n_select;
-    if (n_pages <= a.n_select) {  // all of them (every CTA of the cluster leaves here)
-        if (rank == 0)
-            for (uint32_t i = threadIdx.x; i < a.n_select; i += SEL_THREADS) out[i] = i < n_pages ? (int32_t)i : -1;
-        return;
-    }
-    const uint32_t share = (n_pages + n_cta - 1) / n_cta, p0 = min(rank * share, n_pages), n = min(share, n_pages - p0);  // this CTA's pages
+    const uint32_t n_pos = known ? min(min(a.n_pos[row], a.max_pos), a.pg.stride * KV_PAGE) : 0u;
+    return SelRow{a.pg.tables + (uint64_t)(known ? s : 0) * a.pg.stride, (n_pos + KV_PAGE - 1) / KV_PAGE};
+}
 
-    // ---- the queries' codes
-    constexpr uint32_t HEADS = MANY ? 16 : 8, WORDS = MANY ? 4 : 2;  // words of an A fragment that are not always zero
-#pragma unroll 1
-    for (uint32_t h = warp; h < HEADS; h += SEL_WARPS) {
-        float x[HD / 32], top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            x[i] = h < a.group ? as_float(static_cast<const T *>(a.q)[(uint64_t)row * a.q_stride + (uint64_t)(head * a.group + h) * HD + i * 32 + lane]) : 0.0f;
-            if (x[i] != x[i]) x[i] = 0.0f;
-            x[i] = fminf(fmaxf(x[i], -SEL_MOST), SEL_MOST);
-            top = fmaxf(top, fabsf(x[i]));
-        }
-        top = warp_max(top);
-        const float d = __fdiv_rn(top, 127.0f), by = d > 0.0f ? d : 1.0f;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) s_code[h][i * 32 + lane] = (int8_t)fminf(fmaxf(rintf(__fdiv_rn(x[i], by)), -127.0f), 127.0f);
-        if (lane == 0) s_unit[h] = h < a.group ? d : -1.0f;
-    }
-    for (uint32_t i = threadIdx.x; i < 4 * 256; i += SEL_THREADS) (&s_hist[0][0])[i] = 0u;
-    __syncthreads();
-    // Load i of a lane is bytes 64 i + 16 (lane % 4) .. + 15 of a page's codes; its words 0, 1 and 2, 3 are the two halves of a step's 32.
-    uint32_t f[LOADS][2][WORDS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < (int)WORDS; ++e) {
-                const uint32_t at = i * 64 + (lane & 3) * 16 + j * 8 + e / (WORDS / 2) * 4, h = lane / 4 + (MANY ? e & 1 : 0) * 8;
-                const uint32_t c = *reinterpret_cast<const uint32_t *>(&s_code[h][at % HD]);
-                f[i][j][e] = at < HD ? __vmaxs4(c, 0u) : __vmins4(c, 0u);  // largest keys meet the positive codes, smallest the others
-            }
-    const float unit0 = s_unit[lane / 4], unit1 = MANY ? s_unit[lane / 4 + 8] : -1.0f;
-    auto product = [&](int(&c)[4], const uint32_t(&w)[WORDS], uint32_t b0, uint32_t b1) {
-        if constexpr (MANY) {
-            mma_s8(c, w, b0, b1);
-        } else {
-            const uint32_t x[4] = {w[0], 0u, w[1], 0u};
-            mma_s8(c, x, b0, b1);
-        }
-    };
+// One warp's queries of a (row, key/value head) as B fragments.  MANY: more than eight heads, in two sets of columns.  Load i of a lane is
+// bytes 64 i + 16 (lane % 4) .. + 15 of a page's codes (largest keys, then smallest); its words 0, 1 and 2, 3 are the two halves of a step's
+// 32.  So lane l has entries 64 i + 16 (l % 4) .. + 15 of heads l / 4 and l / 4 + 8.
+template <typename T, int HD, bool MANY>
+struct SelQuery {
+    static constexpr int LOADS = 2 * HD / 64, SETS = MANY ? 2 : 1, N = LOADS / 2 * 16;  // N: entries of a lane
+    uint32_t pos[SETS][LOADS / 2][4], neg[SETS][LOADS / 2][4];  // codes above and below zero: they meet the largest and the smallest keys
+    float unit[SETS][2];                                        // of this lane's two columns; -1: no such head
 
-    // ---- scores: a warp takes eight pages at a time, two such groups in flight
-    const uint64_t rec = 2 * HD;
-    const uint32_t col = (lane & 3) * 2;  // this lane's two columns of a product
-    auto page_of = [&](uint32_t i) {
-        if (i >= n) return -1;
-        const int32_t id = table[p0 + i];
-        return (uint32_t)id < a.pg.n_pages ? id : -1;
-    };
-    constexpr int AHEAD = 2;
-    int32_t id[AHEAD];
+    __device__ __forceinline__ void load(const PagedSelectArgs &a, uint32_t row, uint32_t head) {
+        constexpr float MAGIC = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers, which are then the low bits
+        const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) id[u] = page_of((warp + u * SEL_WARPS) * 8 + lane / 4);
-    for (uint32_t g = warp; g * 8 < n; g += AHEAD * SEL_WARPS) {
-        uint4 x[AHEAD][LOADS];
-        float d[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const uint64_t at = (uint64_t)(uint32_t)max(id[u], 0) * a.pg.n_kv + head;
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) x[u][i] = id[u] < 0 ? make_uint4(0, 0, 0, 0) : ldg128_stream(a.codes + at * rec + i * 64 + (lane & 3) * 16);
-            d[u] = id[u] < 0 ? __int_as_float(0x7fc00000) : __ldg(a.scales + at);  // a page that is not there: no number
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) id[u] = page_of((g + (AHEAD + u) * SEL_WARPS) * 8 + lane / 4);
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            int c[4] = {0, 0, 0, 0};
+        for (int m = 0; m < SETS; ++m) {
+            const uint32_t h = lane / 4 + 8 * m;
+            const bool live = h < a.group;
+            const T *src = static_cast<const T *>(a.q) + (uint64_t)row * a.q_stride + (uint64_t)(head * a.group + (live ? h : 0)) * HD + (lane & 3) * 16;
+            float x[N], top = 0.0f;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                product(c, f[i][0], x[u][i].x, x[u][i].y);
-                product(c, f[i][1], x[u][i].z, x[u][i].w);
-            }
-            float best[2];
+                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + i / 2 * 64) + i % 2) : make_uint4(0, 0, 0, 0);
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float dp = __shfl_sync(0xffffffffu, d[u], (col + e) * 4);
-                const float s0 = unit0 < 0.0f ? -INFINITY : __fmul_rn(__fmul_rn(unit0, dp), (float)c[e]);
-                float y = s0;
-                if (MANY && unit1 >= 0.0f) y = fmaxf(y, __fmul_rn(__fmul_rn(unit1, dp), (float)c[2 + e]));  // (fmaxf gives -inf only where no head is: heads of a page that is not there are all no numbers)
-                if (dp != dp) y = dp;
-                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
-                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-                best[e] = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = as_float2(u[e], T());
+                    x[8 * i + 2 * e] = f.x, x[8 * i + 2 * e + 1] = f.y;
+                }
             }
-            const uint32_t i = (g + u * SEL_WARPS) * 8 + col;
-            if (lane < 4) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (i + e < n) {
-                        const uint32_t p = p0 + i + e;
-                        keys[i + e] = p < a.keep_first || p + a.keep_last >= n_pages ? 0xffffffffu : ordered(best[e]);
+            for (int e = 0; e < N; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[e])));
+            if (!(top <= SEL_MOST)) {
+                top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -SEL_MOST), SEL_MOST);
+                    top = fmaxf(top, fabsf(x[e]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float d = __fdiv_rn(top, 127.0f), by = d > 0.0f ? d : 1.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) unit[m][e] = __shfl_sync(0xffffffffu, live ? d : -1.0f, (lane & 3) * 8 + e * 4);
+            // rint(x / d) by way of a product with 1 / d, which is off by less than 2^-14 (127 (2^-23 + 2^-24)): only where that may cross a
+            // half, or d is too small for an inverse, is the division done.
+            const float inverse = __fdiv_rn(1.0f, by);
+            float far = 0.0f;  // how far from a whole number
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float t = x[e] * inverse;
+                far = fmaxf(far, fabsf(t - ((t + MAGIC) - MAGIC)));
+            }
+            const bool exact = __any_sync(0xffffffffu, !(far < 0.4999f) || !(by > 1e-37f));
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = x[e] * inverse;
+            if (exact) {
+#pragma unroll 1
+                for (int i = 0; i < LOADS; ++i) {
+                    const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + i / 2 * 64) + i % 2) : make_uint4(0, 0, 0, 0);
+                    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 f = as_float2(u[e / 2], T());
+                        float y = e % 2 ? f.y : f.x;
+                        y = y != y ? 0.0f : fminf(fmaxf(y, -SEL_MOST), SEL_MOST);
+                        y = __fdiv_rn(y, by);
+#pragma unroll
+                        for (int k = 0; k < LOADS; ++k)
+                            if (k == i) x[8 * k + e] = y;
                     }
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < N / 4; ++w) {  // (a quotient is 127 and a little at most, which rounds to 127)
+                uint32_t c[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] = __float_as_uint(x[4 * w + e] + MAGIC);
+                const uint32_t u = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+                pos[m][w / 4][w % 4] = __vmaxs4(u, 0u), neg[m][w / 4][w % 4] = __vmins4(u, 0u);
             }
         }
     }
-    __syncthreads();
+    // Words of pages first + step k + i, i < 16, below `end` of the row, handed to put(page, word) by the lanes that have them.
+    template <typename P>
+    __device__ __forceinline__ void score(const PagedSelectArgs &a, const SelRow &r, uint32_t head, uint32_t first, uint32_t end, uint32_t step, P put) const {
+        const uint32_t lane = threadIdx.x & 31;
+        auto page_of = [&](uint32_t p) {
+            const int32_t id = p < end ? r.table[p] : -1;
+            return (uint32_t)id < a.pg.n_pages ? id : -1;
+        };
+        int32_t id[2] = {page_of(first + lane / 4), page_of(first + lane / 4 + 8)};  // this lane's two rows of a product
+        for (uint32_t p0 = first; p0 < end; p0 += step) {
+            uint4 x[2][LOADS];
+            float d[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint64_t at = (uint64_t)(uint32_t)max(id[u], 0) * a.pg.n_kv + head;
+                const int8_t *src = a.codes + at * (2 * HD) + (lane & 3) * 16;
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) x[u][i] = ldg128_stream(src + i * 64);  // (of page 0 where there is none)
+                d[u] = id[u] < 0 ? __int_as_float(0x7fc00000) : __ldg(a.scales + at);    // a page that is not there: no number
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) id[u] = page_of(p0 + step + lane / 4 + 8 * u);
+            float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int m = 0; m < SETS; ++m) {
+                int c[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const uint32_t(&w)[4] = i < LOADS / 2 ? pos[m][i % (LOADS / 2)] : neg[m][i % (LOADS / 2)];
+                    const uint32_t a0[4] = {x[0][i].x, x[1][i].x, x[0][i].y, x[1][i].y}, a1[4] = {x[0][i].z, x[1][i].z, x[0][i].w, x[1][i].w};
+                    mma_s8(c, a0, w[0], w[1]);
+                    mma_s8(c, a1, w[2], w[3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (unit[m][e & 1] >= 0.0f) best[e >> 1] = fmaxf(best[e >> 1], __fmul_rn(__fmul_rn(unit[m][e & 1], d[e >> 1]), (float)c[e]));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float y = best[u];
+                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+                const uint32_t p = p0 + lane / 4 + 8 * u;
+                if ((lane & 3) == 0 && p < end) put(p, p < a.keep_first || p + a.keep_last >= r.n_pages ? SEL_FORCED : d[u] != d[u] ? 0u : ordered(y));
+            }
+        }
+    }
+};
 
-    // ---- the n_select'th largest word
-    uint32_t prefix = 0, want = a.n_select;  // of the words that begin with the prefix, the want'th largest is looked for
-    int shift = 24;
-#pragma unroll 1
-    for (int round = 0;; ++round, shift -= 8) {
-        uint32_t *hist = s_hist[round];
-        for (uint32_t i = threadIdx.x; i < (n + 31) / 32 * 32; i += SEL_THREADS) {
-            const uint32_t k = i < n ? keys[i] : 0u;
-            const bool in = i < n && (round == 0 || (k >> (shift + 8)) == prefix);
-            const uint32_t digit = in ? (k >> shift) & 255u : 256u;
-            const uint32_t same = __match_any_sync(0xffffffffu, digit);  // scores are close together: one addition for equal digits
-            if (in && lane == (uint32_t)__ffs(same) - 1) atomicAdd(hist + digit, __popc(same));
+// A warp per (row, `unit` pages, key/value head), heads side by side.
+template <typename T, int HD, bool MANY>
+__global__ void __launch_bounds__(256, MANY ? 2 : 4) pages_score_kernel(const __grid_constant__ PagedSelectArgs a, uint32_t row0, uint32_t unit, uint32_t units, uint32_t pitch) {
+    pdl_release();
+    pdl_wait();
+    const uint32_t w = blockIdx.x * 8 + (threadIdx.x >> 5), head = w % a.pg.n_kv, part = w / a.pg.n_kv % units;
+    const uint32_t row = row0 + w / a.pg.n_kv / units;
+    if (row >= a.n_rows) return;
+    const SelRow r = sel_row(a, row);
+    const uint32_t first = part * unit;
+    if (r.n_pages <= a.n_select || first >= r.n_pages) return;  // (all of the row's pages are taken without a score)
+    SelQuery<T, HD, MANY> q;
+    q.load(a, row, head);
+    uint32_t *keys = a.keys + ((uint64_t)(row - row0) * a.pg.n_kv + head) * pitch;
+    q.score(a, r, head, first, min(first + unit, r.n_pages), 16, [&](uint32_t p, uint32_t key) { keys[p] = key; });
+}
+
+// Sum over the warps before this one and over all; every thread gets them.  parts: a word per warp.
+template <uint32_t NW>
+__device__ __forceinline__ uint2 warps_before(uint32_t mine, uint32_t *parts) {  // mine: the warp's, on every lane
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) parts[warp] = mine;
+    __syncthreads();
+    const uint32_t v = lane < NW ? parts[lane] : 0u;
+    return make_uint2((uint32_t)warp_sum_i(lane < warp ? (int)v : 0), (uint32_t)warp_sum_i((int)v));
+}
+
+// The n_select best of n words: those in [lo, hi] are all that are not forced, as far as this thread has seen.  The whole CTA.
+template <uint32_t THREADS>
+__device__ __forceinline__ void pick(const PagedSelectArgs &a, const uint32_t *keys, uint32_t n, uint32_t lo, uint32_t hi, int32_t *out) {
+    constexpr uint32_t NW = THREADS / 32, BINS = SEL_BINS / THREADS;  // bins of a thread
+    __shared__ uint32_t s_hist[SEL_BINS], s_parts[3][32], s_pick[3];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) s_parts[0][warp] = lo, s_parts[1][warp] = hi;
+    __syncthreads();  // (the words are written, too)
+    lo = __reduce_min_sync(0xffffffffu, lane < NW ? s_parts[0][lane] : 0xffffffffu);
+    hi = __reduce_max_sync(0xffffffffu, lane < NW ? s_parts[1][lane] : 0u);
+
+    // ---- the border: of the words in [lo, hi], `want` are taken, of those above all
+    uint32_t want = a.n_select - a.keep_first - a.keep_last;
+    bool all = want == 0;  // all words from lo on
+    if (all) lo = hi = SEL_FORCED;
+    while (!all && lo < hi) {
+        const int shift = max(0, 32 - __clz(hi - lo) - 11);  // (hi - lo) >> shift is below 2048
+        for (uint32_t i = threadIdx.x; i < SEL_BINS; i += THREADS) s_hist[i] = 0u;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+            const uint32_t k = keys[i];
+            if (k >= lo && k <= hi) atomicAdd(s_hist + ((k - lo) >> shift), 1u);
         }
-        if (n_cta > 1) cg::this_cluster().sync();
-        else __syncthreads();
-        uint32_t total = 0;  // thread t: digit 255 - t
-        const uint32_t digit = 255 - threadIdx.x;
-        if (n_cta > 1) {
-            for (uint32_t c = 0; c < n_cta; ++c) total += cg::this_cluster().map_shared_rank(hist, c)[digit];
-        } else {
-            total = hist[digit];
-        }
-        uint32_t upto = total;  // words with this digit or a larger one
+        __syncthreads();
+        const uint32_t bin0 = SEL_BINS - 1 - threadIdx.x * BINS;  // this thread's bins: bin0, bin0 - 1, ...
+        uint32_t count[BINS], mine = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < BINS; ++i) mine += count[i] = s_hist[bin0 - i];
+        uint32_t upto = mine;  // words of this warp's bins up to this thread's
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= (uint32_t)o) upto += up;
         }
-        if (lane == 31) s_warp[round & 1][warp] = upto;
+        uint32_t above = warps_before<NW>(__shfl_sync(0xffffffffu, upto, 31), s_parts[2]).x + upto - mine;
+#pragma unroll
+        for (uint32_t i = 0; i < BINS; ++i) {
+            if (above < want && above + count[i] >= want) s_pick[0] = bin0 - i, s_pick[1] = want - above, s_pick[2] = count[i];
+            above += count[i];
+        }
         __syncthreads();
-        for (uint32_t w = 0; w < warp; ++w) upto += s_warp[round & 1][w];
-        if (upto >= want && upto - total < want) s_pick[0] = digit, s_pick[1] = want - (upto - total), s_pick[2] = total;
-        __syncthreads();
-        prefix = prefix << 8 | s_pick[0];
+        lo += s_pick[0] << shift;
+        hi = min(hi, lo + (1u << shift) - 1);
         want = s_pick[1];
-        if (round == 3 || want == s_pick[2]) break;  // (all words that begin so are taken: no need to look further)
+        all = want == s_pick[2];
         __syncthreads();
     }
-    // ---- words that begin with more than the prefix: all; with the prefix: the first `want` of all CTAs
-    const uint32_t span = (n + SEL_WARPS - 1) / SEL_WARPS, w0 = min(warp * span, n), w1 = min(w0 + span, n);  // this warp's pages
+    // ---- the list: words above hi, all in [lo, hi] or the first `want` of them (which are equal then)
+    const uint32_t span = (n + NW - 1) / NW, w0 = min(warp * span, n), w1 = min(w0 + span, n);  // this warp's pages
     uint32_t above = 0, equal = 0;
-    for (uint32_t i = w0 + lane; i < w1; i += 32) above += keys[i] >> shift > prefix, equal += keys[i] >> shift == prefix;
-    above = warp_sum_i(above), equal = warp_sum_i(equal);
-    if (lane == 0) s_warp[0][warp] = above, s_warp[1][warp] = equal;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        uint32_t x = 0, y = 0;
-        for (int w = 0; w < SEL_WARPS; ++w) x += s_warp[0][w], y += s_warp[1][w];
-        s_count[0] = x, s_count[1] = y;
-    }
-    if (n_cta > 1) cg::this_cluster().sync();
-    else __syncthreads();
-    above = equal = 0;  // before this warp
-    for (uint32_t c = 0; c < rank; ++c) {
-        const uint32_t *r = cg::this_cluster().map_shared_rank(s_count, c);
-        above += r[0], equal += r[1];
-    }
-    for (uint32_t w = 0; w < warp; ++w) above += s_warp[0][w], equal += s_warp[1][w];
+    auto kinds = [&](uint32_t i, bool &gt, bool &eq) {
+        const uint32_t k = i < w1 ? keys[i] : 0u;
+        gt = i < w1 && (all ? k >= lo : k > hi);
+        eq = i < w1 && !all && k == lo;
+    };
     for (uint32_t i = w0; i < w1; i += 32) {
-        const uint32_t k = i + lane < w1 ? keys[i + lane] >> shift : 0u;
-        const bool live = i + lane < w1;
-        const uint32_t gt = __ballot_sync(0xffffffffu, live && k > prefix), eq = __ballot_sync(0xffffffffu, live && k == prefix), below = (1u << lane) - 1;
-        const uint32_t ga = above + __popc(gt & below), ea = equal + __popc(eq & below);
-        if ((gt >> lane & 1) || ((eq >> lane & 1) && ea < want)) out[ga + min(ea, want)] = (int32_t)(p0 + i + lane);
-        above += __popc(gt), equal += __popc(eq);
+        bool gt, eq;
+        kinds(i + lane, gt, eq);
+        above += __popc(__ballot_sync(0xffffffffu, gt)), equal += __popc(__ballot_sync(0xffffffffu, eq));
     }
-    if (n_cta > 1) cg::this_cluster().sync();  // nobody leaves while its counts may still be read
+    above = warps_before<NW>(above, s_parts[0]).x;
+    equal = warps_before<NW>(equal, s_parts[1]).x;
+    for (uint32_t i = w0; i < w1; i += 32) {
+        bool gt, eq;
+        kinds(i + lane, gt, eq);
+        const uint32_t g = __ballot_sync(0xffffffffu, gt), q = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1;
+        const uint32_t ga = above + __popc(g & below), ea = equal + __popc(q & below);
+        if (gt || (eq && ea < want)) out[ga + min(ea, want)] = (int32_t)(i + lane);
+        above += __popc(g), equal += __popc(q);
+    }
+}
+
+// A CTA per (row, key/value head).
+template <typename T, int HD, bool MANY>
+__global__ void __launch_bounds__(256) pages_score_pick_kernel(const __grid_constant__ PagedSelectArgs a) {
+    extern __shared__ __align__(16) uint32_t held[];
+    pdl_release();
+    pdl_wait();
+    const uint32_t head = blockIdx.x % a.pg.n_kv, row = blockIdx.x / a.pg.n_kv, warp = threadIdx.x >> 5;
+    const SelRow r = sel_row(a, row);
+    int32_t *out = a.selected + (uint64_t)blockIdx.x * a.n_select;
+    if (r.n_pages <= a.n_select) {  // all of them
+        for (uint32_t i = threadIdx.x; i < a.n_select; i += 256) out[i] = i < r.n_pages ? (int32_t)i : -1;
+        return;
+    }
+    uint32_t lo = 0xffffffffu, hi = 0;
+    SelQuery<T, HD, MANY> q;
+    q.load(a, row, head);
+    q.score(a, r, head, warp * 16, r.n_pages, 8 * 16, [&](uint32_t p, uint32_t key) {
+        held[p] = key;
+        if (key != SEL_FORCED) lo = min(lo, key), hi = max(hi, key);
+    });
+    pick<256>(a, held, r.n_pages, lo, hi, out);
+}
+template <uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) pages_pick_kernel(const __grid_constant__ PagedSelectArgs a, uint32_t row0, uint32_t pitch) {
+    extern __shared__ __align__(16) uint32_t held[];
+    pdl_release();
+    pdl_wait();
+    const uint32_t head = blockIdx.x % a.pg.n_kv, row = row0 + blockIdx.x / a.pg.n_kv;
+    const uint32_t n = sel_row(a, row).n_pages;
+    int32_t *out = a.selected + ((uint64_t)row * a.pg.n_kv + head) * a.n_select;
+    if (n <= a.n_select) {
+        for (uint32_t i = threadIdx.x; i < a.n_select; i += THREADS) out[i] = i < n ? (int32_t)i : -1;
+        return;
+    }
+    const uint32_t *from = a.keys + (uint64_t)blockIdx.x * pitch;
+    const bool fits = n <= SEL_HELD;
+    uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        const uint32_t key = __ldcg(from + i);
+        if (fits) held[i] = key;
+        if (key != SEL_FORCED) lo = min(lo, key), hi = max(hi, key);
+    }
+    pick<THREADS>(a, fits ? held : from, n, lo, hi, out);
 }
 
 template <typename T, int HD, bool MANY>
-cudaError_t launch(const PagedSelectArgs &a, int sm_count, cudaStream_t st) {
-    auto kernel = pages_select_kernel<T, HD, MANY>;
+cudaError_t launch(PagedSelectArgs a, int sm_count, cudaStream_t st, uint32_t *launches) {
     static PerDeviceOnce once;
-    if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_KEYS * 4); })) return e;
+    if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(pages_pick_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_HELD * 4); })) return e;
     const uint32_t pages = std::max(1u, (std::min(a.max_pos, a.pg.stride * KV_PAGE) + KV_PAGE - 1) / KV_PAGE);
     const uint64_t pairs = (uint64_t)a.n_rows * a.pg.n_kv;
-    // More CTAs a row while the SMs are not all taken four times and a CTA keeps 64 pages (a group of eight for each warp), or while a CTA's
-    // words would not fit.
-    uint32_t c = 1;
-    while (c < SEL_CLUSTER && ((pairs * c * 2 <= 4ull * sm_count && pages / (2 * c) >= 64) || (pages + c - 1) / c > SEL_KEYS)) c *= 2;
-    const uint32_t cap = (pages + c - 1) / c;
-    if (pairs * c > 0x7fffffffull || cap > SEL_KEYS) return cudaErrorInvalidConfiguration;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = c, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((uint32_t)(pairs * c));
-    cfg.blockDim = dim3(SEL_THREADS);
-    cfg.dynamicSmemBytes = (size_t)cap * 4;
-    cfg.stream = st;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, a, c, cap);
+    *launches = 1;
+    // One kernel while a CTA per SM scores its own pages at once.
+    if (pages <= SEL_FUSED && pairs <= (uint64_t)sm_count) return launch_pdl(pages_score_pick_kernel<T, HD, MANY>, dim3((uint32_t)pairs), dim3(256), pages * 4, st, a);
+    const uint32_t unit = pairs * pages >= 64ull * 32 * sm_count ? 64 : 16;  // (32 warps an SM, and all of them busy)
+    const uint32_t pitch = (pages + 7) / 8 * 8, units = (pages + unit - 1) / unit;
+    const uint64_t fit = std::min<uint64_t>(PG_KEYS_BYTES / ((uint64_t)pitch * 4 * a.pg.n_kv), 0x7fffffffu / ((uint64_t)units * a.pg.n_kv));  // rows of a batch
+    if (fit == 0) return cudaErrorInvalidConfiguration;
+    *launches = 0;
+    for (uint64_t row = 0; row < a.n_rows; row += fit) {
+        const uint32_t rows = (uint32_t)std::min<uint64_t>(fit, a.n_rows - row);
+        PagedSelectArgs b = a;
+        b.n_rows = (uint32_t)row + rows;
+        // (no early start for the scores: their CTAs would crowd on the SMs that are done first; 121 us instead of 93 with the attention that follows, 64 rows)
+        pages_score_kernel<T, HD, MANY><<<(uint32_t)(((uint64_t)rows * units * a.pg.n_kv + 7) / 8), 256, 0, st>>>(b, (uint32_t)row, unit, units, pitch);
+        if (cudaError_t e = cudaGetLastError()) return e;
+        const dim3 grid(rows * a.pg.n_kv);
+        const size_t held = (size_t)std::min(pages, SEL_HELD) * 4;
+        if (cudaError_t e = pages <= 4096 ? launch_pdl(pages_pick_kernel<256>, grid, dim3(256), held, st, b, (uint32_t)row, pitch)
+                                          : launch_pdl(pages_pick_kernel<1024>, grid, dim3(1024), held, st, b, (uint32_t)row, pitch)) return e;
+        *launches += 2;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
 
-uint32_t pages_select_most() { return SEL_CLUSTER * SEL_KEYS; }
-
-cudaError_t launch_pages_select(const PagedSelectArgs &a, int sm_count, cudaStream_t st) {
-    auto pick = [&](auto few, auto many) { return a.group > 8 ? many(a, sm_count, st) : few(a, sm_count, st); };
+cudaError_t launch_pages_select(const PagedSelectArgs &a, int sm_count, cudaStream_t st, uint32_t *launches) {
+    auto pick = [&](auto few, auto many) { return a.group > 8 ? many(a, sm_count, st, launches) : few(a, sm_count, st, launches); };
     if (a.pg.is_bf16) return a.pg.dim == 64 ? pick(launch<bf16, 64, false>, launch<bf16, 64, true>) : pick(launch<bf16, 128, false>, launch<bf16, 128, true>);
     return a.pg.dim == 64 ? pick(launch<__half, 64, false>, launch<__half, 64, true>) : pick(launch<__half, 128, false>, launch<__half, 128, true>);
 }
