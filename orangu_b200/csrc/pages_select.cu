@@ -11,7 +11,7 @@
 // where the fragments want them.  What bounds the scores is the reading of the codes, 2 dim + 4 bytes a page; with eight pages as columns and
 // the heads as rows, four times as many instructions did (51 us for 64 rows of 6 to 24 k positions, 8 heads of 128).
 //
-// Scores are kept as 32-bit words in their order.  Many of them are made by a kernel of their own, a warp per 64 pages (16 where there are few), neighbouring warps
+// Scores are kept as 32-bit words in their order.  Many of them are made by a kernel of their own, a warp per 128 pages (fewer where there are few), neighbouring warps
 // the heads of the same pages, whose codes lie together; few of them in the CTA that picks.  A CTA per (row, head) then picks: counts in
 // 2048 equal parts of the range, as often as the part with the border still holds more than are wanted (two times as a rule),
 // and the list is written in ascending order.
@@ -62,80 +62,86 @@ __device__ __forceinline__ SelRow sel_row(const PagedSelectArgs &a, uint32_t row
 // 32.  So lane l has entries 64 i + 16 (l % 4) .. + 15 of heads l / 4 and l / 4 + 8.
 template <typename T, int HD, bool MANY>
 struct SelQuery {
-    static constexpr int LOADS = 2 * HD / 64, SETS = MANY ? 2 : 1, N = LOADS / 2 * 16;  // N: entries of a lane
+    static constexpr int LOADS = 2 * HD / 64, SETS = MANY ? 2 : 1, HEADS = 8 * SETS, PER = HD / 32;  // PER: entries of a lane while codes are made
     uint32_t pos[SETS][LOADS / 2][4], neg[SETS][LOADS / 2][4];  // codes above and below zero: they meet the largest and the smallest keys
     float unit[SETS][2];                                        // of this lane's two columns; -1: no such head
 
-    __device__ __forceinline__ void load(const PagedSelectArgs &a, uint32_t row, uint32_t head) {
-        constexpr float MAGIC = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers, which are then the low bits
-        const uint32_t lane = threadIdx.x & 31;
+    // own: HEADS x HD entries of shared memory that are this warp's: the queries, whose places their codes take.  A head after the other in a
+    // loop that is not unrolled: the instructions are fetched from memory by every SM (32 entries a lane side by side took 8 us), and all
+    // loads at once.
+    __device__ __forceinline__ void load(const PagedSelectArgs &a, uint32_t row, uint32_t head, T *own) {
+        const uint32_t lane = threadIdx.x & 31, words = a.group * HD / 8;  // of 16 bytes
+        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (uint64_t)row * a.q_stride + (uint64_t)head * a.group * HD);
+        uint4 v[HEADS * HD / 256];
 #pragma unroll
-        for (int m = 0; m < SETS; ++m) {
-            const uint32_t h = lane / 4 + 8 * m;
-            const bool live = h < a.group;
-            const T *src = static_cast<const T *>(a.q) + (uint64_t)row * a.q_stride + (uint64_t)(head * a.group + (live ? h : 0)) * HD + (lane & 3) * 16;
-            float x[N], top = 0.0f;
+        for (uint32_t i = 0; i < HEADS * HD / 256; ++i) v[i] = i * 32 + lane < words ? __ldg(src + i * 32 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + i / 2 * 64) + i % 2) : make_uint4(0, 0, 0, 0);
-                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        for (uint32_t i = 0; i < HEADS * HD / 256; ++i) reinterpret_cast<uint4 *>(own)[i * 32 + lane] = v[i];
+        __syncwarp();
+        float mine = -1.0f;  // lane h: head h's unit
+#pragma unroll 1
+        for (uint32_t h = 0; h < a.group; ++h) {  // (the places of the others are zero, as are their codes)
+            constexpr float MAGIC = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers, which are then the low bits
+            const uint32_t *at = reinterpret_cast<const uint32_t *>(own + h * HD) + lane * (PER / 2);
+            float x[PER], top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = as_float2(u[e], T());
-                    x[8 * i + 2 * e] = f.x, x[8 * i + 2 * e + 1] = f.y;
-                }
+            for (int e = 0; e < PER; ++e) {
+                const float2 f = as_float2(at[e / 2], T());
+                x[e] = e % 2 ? f.y : f.x;
+                top = fmaxf(top, fabsf(x[e]));
             }
+            bool odd = !(top <= SEL_MOST);
 #pragma unroll
-            for (int e = 0; e < N; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[e])));
-            if (!(top <= SEL_MOST)) {
+            for (int e = 0; e < PER; ++e) odd |= x[e] != x[e];
+            if (odd) {
                 top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
+                for (int e = 0; e < PER; ++e) {
                     x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -SEL_MOST), SEL_MOST);
                     top = fmaxf(top, fabsf(x[e]));
                 }
             }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // (not negative: ordered as its bits are)
             const float d = __fdiv_rn(top, 127.0f), by = d > 0.0f ? d : 1.0f;
+            if (lane == h) mine = d;
+            // rint(x / d) by way of a product with about 1 / d, which is off by less than 2^-14 (127 times 2^-22 and 2^-24): only where that
+            // may cross a half, or d is too small for an inverse, is the division done.
+            const float inverse = __frcp_rn(by);
+            float far = 0.0f, t[PER];  // far: how far from a whole number
 #pragma unroll
-            for (int e = 0; e < 2; ++e) unit[m][e] = __shfl_sync(0xffffffffu, live ? d : -1.0f, (lane & 3) * 8 + e * 4);
-            // rint(x / d) by way of a product with 1 / d, which is off by less than 2^-14 (127 (2^-23 + 2^-24)): only where that may cross a
-            // half, or d is too small for an inverse, is the division done.
-            const float inverse = __fdiv_rn(1.0f, by);
-            float far = 0.0f;  // how far from a whole number
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float t = x[e] * inverse;
-                far = fmaxf(far, fabsf(t - ((t + MAGIC) - MAGIC)));
+            for (int e = 0; e < PER; ++e) {
+                t[e] = x[e] * inverse;
+                far = fmaxf(far, fabsf(t[e] - ((t[e] + MAGIC) - MAGIC)));
             }
-            const bool exact = __any_sync(0xffffffffu, !(far < 0.4999f) || !(by > 1e-37f));
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = x[e] * inverse;
-            if (exact) {
+            if (!(far < 0.4999f) || !(by > 1e-37f)) {
 #pragma unroll 1
-                for (int i = 0; i < LOADS; ++i) {
-                    const uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + i / 2 * 64) + i % 2) : make_uint4(0, 0, 0, 0);
-                    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+                for (int e = 0; e < PER; ++e) {
+                    float y = x[0];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float2 f = as_float2(u[e / 2], T());
-                        float y = e % 2 ? f.y : f.x;
-                        y = y != y ? 0.0f : fminf(fmaxf(y, -SEL_MOST), SEL_MOST);
-                        y = __fdiv_rn(y, by);
+                    for (int k = 1; k < PER; ++k) y = e == k ? x[k] : y;
+                    y = __fdiv_rn(y, by);
 #pragma unroll
-                        for (int k = 0; k < LOADS; ++k)
-                            if (k == i) x[8 * k + e] = y;
-                    }
+                    for (int k = 0; k < PER; ++k) t[k] = e == k ? y : t[k];
                 }
             }
+            uint32_t c = 0;  // (a quotient is 127 and a little at most, which rounds to 127)
 #pragma unroll
-            for (int w = 0; w < N / 4; ++w) {  // (a quotient is 127 and a little at most, which rounds to 127)
-                uint32_t c[4];
+            for (int e = 0; e < PER; ++e) c |= (__float_as_uint(t[e] + MAGIC) & 255u) << (8 * e);
+            int8_t *code = reinterpret_cast<int8_t *>(own + h * HD);  // (all lanes have read: the maximum is theirs)
+            if constexpr (PER == 4) reinterpret_cast<uint32_t *>(code)[lane] = c;
+            else reinterpret_cast<uint16_t *>(code)[lane] = (uint16_t)c;
+        }
+        __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[e] = __float_as_uint(x[4 * w + e] + MAGIC);
-                const uint32_t u = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-                pos[m][w / 4][w % 4] = __vmaxs4(u, 0u), neg[m][w / 4][w % 4] = __vmins4(u, 0u);
+        for (int m = 0; m < SETS; ++m) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) unit[m][e] = __shfl_sync(0xffffffffu, mine, (lane & 3) * 2 + e + 8 * m);
+#pragma unroll
+            for (int i = 0; i < LOADS / 2; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const int8_t *>(own + (lane / 4 + 8 * m) * HD) + i * 64 + (lane & 3) * 16);
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) pos[m][i][w] = __vmaxs4(u[w], 0u), neg[m][i][w] = __vmins4(u[w], 0u);
             }
         }
     }
@@ -148,6 +154,7 @@ struct SelQuery {
             return (uint32_t)id < a.pg.n_pages ? id : -1;
         };
         int32_t id[2] = {page_of(first + lane / 4), page_of(first + lane / 4 + 8)};  // this lane's two rows of a product
+#pragma unroll 1
         for (uint32_t p0 = first; p0 < end; p0 += step) {
             uint4 x[2][LOADS];
             float d[2];
@@ -191,6 +198,7 @@ struct SelQuery {
 // A warp per (row, `unit` pages, key/value head), heads side by side.
 template <typename T, int HD, bool MANY>
 __global__ void __launch_bounds__(256, MANY ? 2 : 4) pages_score_kernel(const __grid_constant__ PagedSelectArgs a, uint32_t row0, uint32_t unit, uint32_t units, uint32_t pitch) {
+    __shared__ __align__(16) T s_query[8][MANY ? 16 : 8][HD];
     pdl_release();
     pdl_wait();
     const uint32_t w = blockIdx.x * 8 + (threadIdx.x >> 5), head = w % a.pg.n_kv, part = w / a.pg.n_kv % units;
@@ -200,7 +208,7 @@ __global__ void __launch_bounds__(256, MANY ? 2 : 4) pages_score_kernel(const __
     const uint32_t first = part * unit;
     if (r.n_pages <= a.n_select || first >= r.n_pages) return;  // (all of the row's pages are taken without a score)
     SelQuery<T, HD, MANY> q;
-    q.load(a, row, head);
+    q.load(a, row, head, &s_query[threadIdx.x >> 5][0][0]);
     uint32_t *keys = a.keys + ((uint64_t)(row - row0) * a.pg.n_kv + head) * pitch;
     q.score(a, r, head, first, min(first + unit, r.n_pages), 16, [&](uint32_t p, uint32_t key) { keys[p] = key; });
 }
@@ -233,8 +241,10 @@ __device__ __forceinline__ void pick(const PagedSelectArgs &a, const uint32_t *k
     if (all) lo = hi = SEL_FORCED;
     while (!all && lo < hi) {
         const int shift = max(0, 32 - __clz(hi - lo) - 11);  // (hi - lo) >> shift is below 2048
+#pragma unroll 1
         for (uint32_t i = threadIdx.x; i < SEL_BINS; i += THREADS) s_hist[i] = 0u;
         __syncthreads();
+#pragma unroll 1
         for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
             const uint32_t k = keys[i];
             if (k >= lo && k <= hi) atomicAdd(s_hist + ((k - lo) >> shift), 1u);
@@ -271,6 +281,7 @@ __device__ __forceinline__ void pick(const PagedSelectArgs &a, const uint32_t *k
         gt = i < w1 && (all ? k >= lo : k > hi);
         eq = i < w1 && !all && k == lo;
     };
+#pragma unroll 1
     for (uint32_t i = w0; i < w1; i += 32) {
         bool gt, eq;
         kinds(i + lane, gt, eq);
@@ -278,6 +289,7 @@ __device__ __forceinline__ void pick(const PagedSelectArgs &a, const uint32_t *k
     }
     above = warps_before<NW>(above, s_parts[0]).x;
     equal = warps_before<NW>(equal, s_parts[1]).x;
+#pragma unroll 1
     for (uint32_t i = w0; i < w1; i += 32) {
         bool gt, eq;
         kinds(i + lane, gt, eq);
@@ -292,18 +304,20 @@ __device__ __forceinline__ void pick(const PagedSelectArgs &a, const uint32_t *k
 template <typename T, int HD, bool MANY>
 __global__ void __launch_bounds__(256) pages_score_pick_kernel(const __grid_constant__ PagedSelectArgs a) {
     extern __shared__ __align__(16) uint32_t held[];
+    __shared__ __align__(16) T s_query[8][MANY ? 16 : 8][HD];
     pdl_release();
     pdl_wait();
     const uint32_t head = blockIdx.x % a.pg.n_kv, row = blockIdx.x / a.pg.n_kv, warp = threadIdx.x >> 5;
     const SelRow r = sel_row(a, row);
     int32_t *out = a.selected + (uint64_t)blockIdx.x * a.n_select;
     if (r.n_pages <= a.n_select) {  // all of them
+#pragma unroll 1
         for (uint32_t i = threadIdx.x; i < a.n_select; i += 256) out[i] = i < r.n_pages ? (int32_t)i : -1;
         return;
     }
     uint32_t lo = 0xffffffffu, hi = 0;
     SelQuery<T, HD, MANY> q;
-    q.load(a, row, head);
+    q.load(a, row, head, &s_query[warp][0][0]);
     q.score(a, r, head, warp * 16, r.n_pages, 8 * 16, [&](uint32_t p, uint32_t key) {
         held[p] = key;
         if (key != SEL_FORCED) lo = min(lo, key), hi = max(hi, key);
@@ -319,6 +333,7 @@ __global__ void __launch_bounds__(THREADS) pages_pick_kernel(const __grid_consta
     const uint32_t n = sel_row(a, row).n_pages;
     int32_t *out = a.selected + ((uint64_t)row * a.pg.n_kv + head) * a.n_select;
     if (n <= a.n_select) {
+#pragma unroll 1
         for (uint32_t i = threadIdx.x; i < a.n_select; i += THREADS) out[i] = i < n ? (int32_t)i : -1;
         return;
     }
@@ -343,7 +358,7 @@ cudaError_t launch(PagedSelectArgs a, int sm_count, cudaStream_t st, uint32_t *l
     *launches = 1;
     // One kernel while a CTA per SM scores its own pages at once.
     if (pages <= SEL_FUSED && pairs <= (uint64_t)sm_count) return launch_pdl(pages_score_pick_kernel<T, HD, MANY>, dim3((uint32_t)pairs), dim3(256), pages * 4, st, a);
-    const uint32_t unit = pairs * pages >= 64ull * 32 * sm_count ? 64 : 16;  // (32 warps an SM, and all of them busy)
+    const uint32_t unit = pairs * pages >= 128ull * 32 * sm_count ? 128 : pairs * pages >= 64ull * 32 * sm_count ? 64 : 32;  // (up to 32 warps an SM)
     const uint32_t pitch = (pages + 7) / 8 * 8, units = (pages + unit - 1) / unit;
     const uint64_t fit = std::min<uint64_t>(PG_KEYS_BYTES / ((uint64_t)pitch * 4 * a.pg.n_kv), 0x7fffffffu / ((uint64_t)units * a.pg.n_kv));  // rows of a batch
     if (fit == 0) return cudaErrorInvalidConfiguration;
