@@ -32,6 +32,7 @@ constexpr int PG_SOFT = 512, PG_MMA_WARP = 16, PG_TMA_WARP = 17, PG_THREADS = 18
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
 constexpr uint32_t PG_LEAST = 2;        // tiles of a CTA: one for each stream
+constexpr uint32_t PG_START = 3;        // what the start and end of a piece cost, in tiles
 
 // mbarriers and small arrays, byte offsets
 constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 144, PB_S_FULL = 192, PB_P_FULL = 208, PB_O_FULL = 224, PB_Q_FULL = 240, PB_SLOT = 248, PB_ABORT = 252,
@@ -84,22 +85,23 @@ template <uint32_t MR>
 __device__ __forceinline__ PgSeq pg_seq(const PagedAttnArgs &a, uint32_t s) {
     PgSeq q{};
     const int32_t f0 = a.first[s], f1 = a.first[s + 1];
+    const uint32_t ctx = a.n_ctx[s], room = a.pg.stride * KV_PAGE;  // (all loads before the first decision)
     if (f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens) return q;
-    const uint32_t room = a.pg.stride * KV_PAGE;
     q.row0 = (uint32_t)f0;
     q.drafts = min((uint32_t)(f1 - f0), a.max_drafts);
-    q.ctx = min(a.n_ctx[s], room);
+    q.ctx = min(ctx, room);
     q.limit = min(q.ctx + q.drafts, room);
     q.n_pages = (q.limit + KV_PAGE - 1) / KV_PAGE;
     q.n_tiles = (q.n_pages + PG_PAGES - 1) / PG_PAGES;
     q.n_rt = (q.drafts * a.group + MR - 1) / MR;
     return q;
 }
-// Pieces in the order (tile of rows, sequence, head), so that CTAs half a round apart read the same keys at about the same time.  All of a
-// warp's lanes hold the same walk.
+// Pieces in the order (tile of rows, sequence, head), so that CTAs half a round apart read the same keys at about the same time.  A piece is
+// PG_START units and one for each of its tiles, so that a CTA with parts of two pieces has less of them (8 x 16 tokens at 8k, ragged: 63 k
+// clocks with one piece and 80 k with two before).  All of a warp's lanes hold the same walk.
 template <uint32_t MR>
 struct PgWalk {
-    uint32_t at, end, per;       // units (tiles) of this CTA, units a CTA (the launcher sees to it that all of them are below 2^31)
+    uint32_t at, end, per;       // units of this CTA, units a CTA (the launcher sees to it that all of them are below 2^31)
     uint32_t rt, seq, head, tile;
     PgSeq q;
 
@@ -108,9 +110,10 @@ struct PgWalk {
         auto load = [&](uint32_t s0) { return s0 + lane < a.n_units ? pg_seq<MR>(a, s0 + lane) : PgSeq{}; };
         const PgSeq front = load(0);  // (up to 32 sequences are read once)
         uint32_t total = 0;
+#pragma unroll 1
         for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) {
             const PgSeq x = s0 ? load(s0) : front;
-            total += (uint32_t)warp_sum_i((int)(x.n_tiles * x.n_rt)) * a.pg.n_kv;
+            total += (uint32_t)warp_sum_i((int)((x.n_tiles + PG_START) * x.n_rt)) * a.pg.n_kv;
         }
         per = max((total + gridDim.x - 1) / gridDim.x, PG_LEAST);
         at = min(total, blockIdx.x * per), end = min(total, at + per);
@@ -118,10 +121,12 @@ struct PgWalk {
         q = PgSeq{};
         if (at >= end) return;
         uint32_t before = 0;
+#pragma unroll 1
         for (rt = 0; rt < a.row_tiles; ++rt)
+#pragma unroll 1
             for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) {
                 const PgSeq x = s0 ? load(s0) : front;
-                const uint32_t mine = rt < x.n_rt ? x.n_tiles * a.pg.n_kv : 0;
+                const uint32_t mine = rt < x.n_rt ? (x.n_tiles + PG_START) * a.pg.n_kv : 0;
                 uint32_t sum = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -135,18 +140,23 @@ struct PgWalk {
                     const uint32_t off = at - (before + of(sum - mine));
                     seq = s0 + src;
                     q = PgSeq{of(x.row0), of(x.drafts), of(x.ctx), of(x.limit), of(x.n_pages), of(x.n_tiles), of(x.n_rt)};
-                    head = off / q.n_tiles, tile = off % q.n_tiles;
+                    head = off / (q.n_tiles + PG_START);
+                    begin(off % (q.n_tiles + PG_START));
                     return;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
         at = end;
     }
+    __device__ __forceinline__ void begin(uint32_t unit) {  // at unit `unit` of a piece
+        tile = unit > PG_START ? unit - PG_START : 0u;
+        at += unit < PG_START ? PG_START - unit : 0u;
+    }
     __device__ __forceinline__ bool more() const { return at < end; }
     __device__ __forceinline__ uint32_t last() const { return min(q.n_tiles, tile + (end - at)); }  // the present piece is tiles [tile, last())
     __device__ __forceinline__ void next(const PagedAttnArgs &a) {
         const uint32_t to = last();
-        at += to - tile;
+        at += to - tile + PG_START;
         tile = 0;
         if (at >= end || ++head < a.pg.n_kv) return;
         head = 0;
@@ -493,7 +503,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             }
             soft_sync();
             const bool whole = w.tile == 0 && end == w.q.n_tiles;
-            const uint32_t origin = w.at - w.tile, begin = blockIdx.x * w.per;  // of the whole piece and of this CTA, in units
+            const uint32_t origin = w.at - w.tile, begin = blockIdx.x * w.per;  // of the piece's first tile and of this CTA, in units
             float *part_out = a.partial + (2ull * blockIdx.x + (origin > begin ? 1 : 0)) * P::PART;  // a CTA has a part of two pieces at most
             // this thread's columns of its row: half of them, or (both streams have the same rows) a quarter of them of both outputs
             constexpr uint32_t COLS = WIDE ? HD / 2 : HD / 4;
@@ -507,6 +517,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             }
             const float norm = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // nothing seen: 0; a sum that is no number stays none
             const bool special = *odd != 0u;
+            const float gain = whole ? norm : 1.0f, g0 = f0 * gain, g1 = f1 * gain;
+            // 16 columns at a time, a thread per row -> four lanes a row: whole sectors, by way of the queries' place, which no product reads any
+            // more.  (One form for results and parts: instructions that are executed once are fetched from memory first.)
+            uint8_t *stage = smem + warp * 2048;
             if (ok && warm && (!WIDE || had[s]))
 #pragma unroll 1
                 for (uint32_t c = 0; c < COLS; c += 16) {
@@ -517,8 +531,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     float x[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        x[e] = f0 != 0.0f ? __uint_as_float(o0[e]) * f0 : 0.0f;  // (a stream without tiles has left nothing there)
-                        if (!WIDE && f1 != 0.0f) x[e] = fmaf(__uint_as_float(o1[e]), f1, x[e]);
+                        x[e] = f0 != 0.0f ? __uint_as_float(o0[e]) * g0 : 0.0f;  // (a stream without tiles has left nothing there)
+                        if (!WIDE && f1 != 0.0f) x[e] = fmaf(__uint_as_float(o1[e]), g1, x[e]);
                     }
                     if (special && live) {  // values that are no numbers, of drafted tokens that this row sees (their weights are above zero)
 #pragma unroll 1
@@ -535,35 +549,20 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                             }
                         }
                     }
-                    // a thread per row -> four (two) lanes a row: whole sectors, by way of the queries' place, which no product reads any more
-                    uint8_t *stage = smem + warp * 2048;
                     __syncwarp();
-                    if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            *reinterpret_cast<uint4 *>(stage + lane * 32 + ((e ^ (lane >> 2 & 1)) << 4)) =
-                                make_uint4(pack16<T>(x[8 * e] * norm, x[8 * e + 1] * norm), pack16<T>(x[8 * e + 2] * norm, x[8 * e + 3] * norm),
-                                           pack16<T>(x[8 * e + 4] * norm, x[8 * e + 5] * norm), pack16<T>(x[8 * e + 6] * norm, x[8 * e + 7] * norm));
-                        __syncwarp();
-#pragma unroll
-                        for (uint32_t k = 0; k < 2; ++k) {
-                            const uint32_t row = 16 * k + lane / 2, f = w.rt * MR + warp_row + row, t0 = f * magic >> 16;
-                            if (warp_row + row < n_rows)
-                                *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + t0) * a.out_stride + (w.head * a.group + f - t0 * a.group) * HD + col0 + c + 8 * (lane & 1)) =
-                                    *reinterpret_cast<const uint4 *>(stage + row * 32 + (((lane & 1) ^ (row >> 2 & 1)) << 4));
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<float4 *>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-                        __syncwarp();
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const uint32_t row = 8 * k + lane / 4, e = lane & 3;
-                            if (warp_row + row < n_rows)
-                                __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)(warp_row + row) * HD + col0 + c + 4 * e),
-                                       *reinterpret_cast<const float4 *>(stage + row * 64 + ((e ^ (row >> 1 & 3)) << 4)));
-                        }
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<float4 *>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t row = lane / 4; row < 32 && warp_row + row < n_rows; row += 8) {
+                        const uint32_t e = lane & 3, f = w.rt * MR + warp_row + row, t0 = f * magic >> 16;
+                        const float4 y = *reinterpret_cast<const float4 *>(stage + row * 64 + ((e ^ (row >> 1 & 3)) << 4));
+                        if (whole)
+                            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + t0) * a.out_stride + (w.head * a.group + f - t0 * a.group) * HD + col0 + c + 4 * e) =
+                                make_uint2(pack16<T>(y.x, y.y), pack16<T>(y.z, y.w));
+                        else
+                            __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)(warp_row + row) * HD + col0 + c + 4 * e), y);
                     }
                 }
             if (!whole && live && part == 0 && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
@@ -598,7 +597,7 @@ __global__ void __launch_bounds__(256) pages_merge_kernel(const __grid_constant_
     if (p.parts == 0 || row >= p.rows) return;
     float top = -INFINITY, total = 0.0f;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+#pragma unroll 4
     for (uint32_t k = 0; k < p.parts; ++k) {
         const float *at = a.partial + (k ? (p.slot & ~1u) + 2 * k : p.slot) * PART;
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(at + (uint64_t)MR * HD + 2 * row));
