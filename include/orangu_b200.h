@@ -236,7 +236,8 @@ int ob_pages_bounds(ob_pages *pages, uint32_t layer, uint32_t n_seq, const uint3
  * number counts as 0, magnitudes above 1e18 as 1e18): a page's score is the largest over the heads of
  * (dq * d) * sum_e max(c_e * largest_e, c_e * smallest_e), an upper bound of q.k up to the rounding of c.  The first keep_first and the
  * last keep_last pages are taken, then those with the largest scores, the first one of equals; a page that is not there scores lowest.
- * selected: [n_rows][n_head_kv][n_select], ascending, -1 behind the last.  At most 131072 pages a row (OB_ERR_CAPACITY). */
+ * selected: [n_rows][n_head_kv][n_select], ascending, -1 behind the last.  At most 131072 pages a row (OB_ERR_CAPACITY);
+ * n_select may be more than a row has. */
 int ob_pages_select(ob_pages *pages, const int8_t *codes, const float *scales, uint32_t n_rows, const void *q, uint64_t q_stride,
                     const int32_t *row_seq, const uint32_t *n_pos, uint32_t n_head, uint32_t max_pos, uint32_t n_select, uint32_t keep_first,
                     uint32_t keep_last, int32_t *selected, void *stream);

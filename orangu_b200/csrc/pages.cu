@@ -53,6 +53,7 @@ __device__ __forceinline__ void copy_page(const uint8_t *src, uint8_t *dst, uint
 
 // grid (pairs, layers x 2)
 __global__ void __launch_bounds__(MOVE_THREADS) pages_copy_kernel(const __grid_constant__ MoveArgs a, const int32_t *__restrict__ src, const int32_t *__restrict__ dst) {
+    ob::pdl_release();
     ob::pdl_wait();
     const int32_t s = src[blockIdx.x], d = dst[blockIdx.x];
     if ((uint32_t)s >= a.n_pages || (uint32_t)d >= a.n_pages || s == d) return;
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) pages_copy_kernel(const __grid_c
 // grid (children, layers x 2 + 1): the last row of CTAs writes the tables
 __global__ void __launch_bounds__(MOVE_THREADS) pages_fork_kernel(const __grid_constant__ MoveArgs a, uint32_t n_layer, const int32_t *__restrict__ parent,
                                                                   const int32_t *__restrict__ child, const uint32_t *__restrict__ n_pos, const int32_t *__restrict__ fresh) {
+    ob::pdl_release();
     ob::pdl_wait();
     const int32_t p = parent[blockIdx.x], c = child[blockIdx.x], f = fresh[blockIdx.x];
     if ((uint32_t)p >= a.n_seq || (uint32_t)c >= a.n_seq || p == c) return;
@@ -81,42 +83,53 @@ __global__ void __launch_bounds__(MOVE_THREADS) pages_fork_kernel(const __grid_c
     copy_page(pool + (uint64_t)s * a.page_bytes(), pool + (uint64_t)f * a.page_bytes(), (uint32_t)(a.page_bytes() / 16));
 }
 
-// grid (sequences, layers x 2, groups of heads): every word is read before the first is written.  A thread holds KEEP_WORDS of the
-// words (head, j, 16 bytes); `heads` of them a CTA so that they fit.
+// x / d for x below 65536 by the high half of a product.
+struct Divide {
+    uint32_t d, m;
+    __host__ __device__ explicit Divide(uint32_t by) : d(by), m(by > 1 ? 0xffffffffu / by + 1 : 0u) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return d > 1 ? __umulhi(x, m) : x; }
+};
+
+// grid (sequences, shares of the (layer, keys or values, head) pools): every word of a pool's head is read before the first is written.  A CTA
+// takes as many of them at a time as its threads hold words (KEEP_WORDS of 16 bytes each), so that a few positions a head fill it, too.
 constexpr uint32_t KEEP_WORDS = 4;
-__global__ void __launch_bounds__(MOVE_THREADS) pages_keep_kernel(const __grid_constant__ MoveArgs a, uint32_t most, const uint32_t *__restrict__ n_ctx, const int32_t *__restrict__ kept,
-                                                                  uint32_t kept_stride, const uint32_t *__restrict__ n_kept) {
-    __shared__ uint64_t s_from[64], s_to[64];  // bytes of head 0's row in a layer's pool; ~0: none
+__global__ void __launch_bounds__(MOVE_THREADS, 6) pages_keep_kernel(const __grid_constant__ MoveArgs a, uint32_t pools, const Divide kv, uint32_t most, const uint32_t *__restrict__ n_ctx,
+                                                                     const int32_t *__restrict__ kept, uint32_t kept_stride, const uint32_t *__restrict__ n_kept) {
+    __shared__ uint64_t s_from[64], s_to[64];  // bytes of head 0's row in a layer's pool; equal: nothing to do
+    ob::pdl_release();
     ob::pdl_wait();
-    const uint32_t n = min(n_kept[blockIdx.x], most), ctx = n_ctx[blockIdx.x];
-    if (n == 0) return;
-    const int32_t *table = a.tables + (uint64_t)blockIdx.x * a.stride;
-    if (threadIdx.x < 2 * n) {
-        const uint32_t j = threadIdx.x >> 1;
-        const int32_t i = threadIdx.x & 1 ? kept[(uint64_t)blockIdx.x * kept_stride + j] : (int32_t)j;
-        uint64_t at = ~0ull;
+    {
+        const uint32_t j = threadIdx.x >> 1, ctx = n_ctx[blockIdx.x];
+        const int32_t i = j < most && (threadIdx.x & 1) ? kept[(uint64_t)blockIdx.x * kept_stride + j] : (int32_t)j;
         const uint64_t x = (uint64_t)ctx + (uint32_t)i;
-        if ((uint32_t)i < 64 && x < (uint64_t)a.stride * KV_PAGE) {
-            const int32_t id = table[x / KV_PAGE];
+        uint64_t at = ~0ull;
+        if (j < most && (uint32_t)i < 64 && x < (uint64_t)a.stride * KV_PAGE) {
+            const int32_t id = a.tables[(uint64_t)blockIdx.x * a.stride + x / KV_PAGE];
             if ((uint32_t)id < a.n_pages) at = (uint64_t)id * a.page_bytes() + x % KV_PAGE * a.row_bytes;
         }
-        (threadIdx.x & 1 ? s_from : s_to)[j] = at;
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, at, 1);
+        if (at == ~0ull || other == ~0ull) at = 0;  // either is not there: both are the same place
+        if (j < 64) (threadIdx.x & 1 ? s_from : s_to)[j] = at;
     }
+    const uint32_t n = min(n_kept[blockIdx.x], most), shift = a.row_bytes == 128 ? 3 : 4, unit = n << shift;  // words of a pool's head
     __syncthreads();
-    uint8_t *pool = a.pool(blockIdx.y >> 1, blockIdx.y & 1);
-    const uint32_t row = a.row_bytes / 16, head_words = n * row, fit = max(1u, KEEP_WORDS * MOVE_THREADS / head_words);
-    for (uint32_t h0 = blockIdx.z * fit; h0 < a.n_kv; h0 += gridDim.z * fit) {
-        const uint32_t words = min(fit, a.n_kv - h0) * head_words;
+    if (n == 0) return;
+    const Divide by_n(n);
+    const uint32_t fit = KEEP_WORDS * MOVE_THREADS / unit, total = pools * a.n_kv;
+#pragma unroll 1
+    for (uint32_t p0 = blockIdx.y * fit; p0 < total; p0 += gridDim.y * fit) {
+        const uint32_t words = min(fit, total - p0) * unit;
         uint4 x[KEEP_WORDS];
         uint8_t *to[KEEP_WORDS];
 #pragma unroll
         for (uint32_t u = 0; u < KEEP_WORDS; ++u) {
-            const uint32_t i = u * MOVE_THREADS + threadIdx.x, h = h0 + i / head_words, j = i % head_words / row, c = i % row;
+            const uint32_t i = u * MOVE_THREADS + threadIdx.x, row = i >> shift, p = by_n(row), j = row - p * n;
             to[u] = nullptr;
-            if (i < words && s_from[j] != ~0ull && s_to[j] != ~0ull && s_from[j] != s_to[j]) {
-                const uint64_t off = (uint64_t)h * KV_PAGE * a.row_bytes + c * 16;
-                x[u] = *reinterpret_cast<const uint4 *>(pool + s_from[j] + off);
-                to[u] = pool + s_to[j] + off;
+            if (i < words && s_from[j] != s_to[j]) {
+                const uint32_t pool = kv(p0 + p), head = p0 + p - pool * a.n_kv;
+                uint8_t *base = a.pool(pool >> 1, pool & 1) + (uint64_t)head * KV_PAGE * a.row_bytes + ((i & ((1u << shift) - 1)) << 4);
+                x[u] = *reinterpret_cast<const uint4 *>(base + s_from[j]);
+                to[u] = base + s_to[j];
             }
         }
         __syncthreads();
@@ -128,77 +141,160 @@ __global__ void __launch_bounds__(MOVE_THREADS) pages_keep_kernel(const __grid_c
 
 // Bounds of a page's keys.  A warp per (page, head): 16 bytes a lane, HD / 8 lanes a row, the lanes' maxima and minima of f16 or bf16 pairs;
 // then the unit d = max(|hi|, |lo|) / 127 and the codes ceil(hi / d), floor(lo / d), so that a code times d is no tighter than the keys
-// (by more than the division's rounding).  Reading the keys bounds it.
+// (by more than the division's rounding).  Reading the keys is the bound to aim at; what was in the way were instructions, 640 a page and head
+// (4.3 TB/s for 4096 pages of 8 heads) before this form.
+// Two values in a word: plain words and instructions (through the types of the headers the compiler takes the halves apart: 1000
+// instructions a page instead of the few hundred there are).
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
-    using V = __half2;
-    static __device__ __forceinline__ float2 f(V v) { return __half22float2(v); }
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ float2 f(uint32_t v) {
+        float2 r;
+        asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(v));
+        return r;
+    }
 };
 template <> struct Pair<bf16> {
-    using V = __nv_bfloat162;
-    static __device__ __forceinline__ float2 f(V v) { return __bfloat1622float2(v); }
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ float2 f(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 };
+constexpr uint32_t SIGNS = 0x80008000u;
+constexpr uint32_t BOUND_DEPTH = 3;   // pages of a warp's ring: 96 KB a CTA with 128 entries a key
 constexpr float BOUND_MOST = 1e18f;  // what larger keys count as: the scores stay finite
 __device__ __forceinline__ float bounded(float v) { return v != v ? 0.0f : fminf(fmaxf(v, -BOUND_MOST), BOUND_MOST); }
 
+// grid (CTAs of a sequence, sequences): warp w of a sequence has head w % n_kv of every `step`th page from w / n_kv on; the next page's number
+// and keys are on their way while a page is done.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) pages_bounds_kernel(const __grid_constant__ PageView pg, const uint32_t *__restrict__ first_pos, const uint32_t *__restrict__ n_pos, int8_t *codes, float *scales) {
-    using V = typename Pair<T>::V;
+__global__ void __launch_bounds__(256) pages_bounds_kernel(const __grid_constant__ PageView pg, uint32_t step, const uint32_t *__restrict__ first_pos, const uint32_t *__restrict__ n_pos, int8_t *codes,
+                                                           float *scales) {
+    using P = Pair<T>;
     constexpr uint32_t LANES = HD / 8, STEP = 32 / LANES, ROWS = KV_PAGE / STEP;  // lanes a row, rows a load, loads
+    ob::pdl_release();
     ob::pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, unit = blockIdx.x * 8 + (threadIdx.x >> 5), seq = blockIdx.y, room = pg.stride * KV_PAGE;
-    const uint32_t from = first_pos[seq], to = min(n_pos[seq], room);
-    const uint32_t page = from / KV_PAGE + unit / pg.n_kv, head = unit % pg.n_kv;
-    if (from >= to || page >= (to + KV_PAGE - 1) / KV_PAGE) return;
-    const int32_t id = pg.tables[(uint64_t)seq * pg.stride + page];
-    if ((uint32_t)id >= pg.n_pages) return;
-    const uint32_t filled = min(to - page * KV_PAGE, (uint32_t)KV_PAGE);
-    const uint64_t at = (uint64_t)id * pg.n_kv + head;
-    const uint4 *k = reinterpret_cast<const uint4 *>(static_cast<const T *>(pg.k) + at * KV_PAGE * HD);
-    uint4 x[ROWS];
+    const uint32_t lane = threadIdx.x & 31, w = blockIdx.x * 8 + (threadIdx.x >> 5), seq = blockIdx.y, first = w / pg.n_kv, head = w - first * pg.n_kv;
+    const uint32_t from = first_pos[seq], to = min(n_pos[seq], pg.stride * KV_PAGE), end = (to + KV_PAGE - 1) / KV_PAGE;
+    if (from >= to || first >= step) return;
+    const int32_t *table = pg.tables + (uint64_t)seq * pg.stride;
+    auto page_of = [&](uint32_t p) {
+        const int32_t id = p < end ? table[p] : -1;
+        return (uint32_t)id < pg.n_pages ? id : -1;
+    };
+    extern __shared__ __align__(16) uint4 ring[];  // [warp][BOUND_DEPTH][page's keys of a head]
+    constexpr uint32_t WORDS = KV_PAGE * HD / 8;
+    uint4 *own = ring + (threadIdx.x >> 5) * BOUND_DEPTH * WORDS;
+    auto request = [&](uint32_t p, int32_t id, uint32_t slot) {
+        if (id >= 0) {
+            const uint4 *k = reinterpret_cast<const uint4 *>(static_cast<const T *>(pg.k) + ((uint64_t)id * pg.n_kv + head) * KV_PAGE * HD) + lane;
+            const uint32_t filled = min(to - p * KV_PAGE, (uint32_t)KV_PAGE), dst = smem_addr(own + slot * WORDS + lane);
 #pragma unroll
-    for (uint32_t i = 0; i < ROWS; ++i) {
-        const uint32_t row = i * STEP + lane / LANES;
-        x[i] = ob::ldg128_stream(k + (row < filled ? i * 32 + lane : lane % LANES));  // rows that are not filled: the first one again
-    }
-    V hi[4], lo[4];
+            for (uint32_t i = 0; i < ROWS; ++i) cp16(dst + i * 512, i * STEP + lane / LANES < filled ? k + i * 32 : k - lane / LANES * LANES, true);  // rows that are not filled: the first one again
+        }
+        cp_commit();
+    };
+    // From the exchange on the first LANES lanes have the largest keys, the next ones the smallest with their sign turned: floor(x) = -ceil(-x).
+    const bool low = lane / LANES & 1;
+    auto bound = [&](int32_t id, uint32_t slot) {
+        const uint4 *x = own + slot * WORDS + lane, x0 = x[0];
+        uint32_t hi[4] = {x0.x, x0.y, x0.z, x0.w}, lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) hi[e] = lo[e] = reinterpret_cast<const V *>(&x[0])[e];
+        for (int e = 0; e < 4; ++e) lo[e] = hi[e] ^ SIGNS;
 #pragma unroll
-    for (uint32_t i = 1; i < ROWS; ++i)
+        for (uint32_t i = 1; i < ROWS; ++i) {
+            const uint4 xi = x[i * 32];
+            const uint32_t v[4] = {xi.x, xi.y, xi.z, xi.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[e] = P::max(hi[e], v[e]), lo[e] = P::max(lo[e], v[e] ^ SIGNS);
+        }
+        if constexpr (STEP == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi[e] = P::max(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], 16));
+                lo[e] = P::max(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], 16));
+            }
+        }
+        float b[8], top = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const V v = reinterpret_cast<const V *>(&x[i])[e];
-            hi[e] = __hmax2(hi[e], v), lo[e] = __hmin2(lo[e], v);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, low ? hi[e] : lo[e], LANES);
+            const float2 f = P::f(P::max(low ? lo[e] : hi[e], got));
+            b[2 * e] = f.x, b[2 * e + 1] = f.y;
         }
 #pragma unroll
-    for (uint32_t o = LANES; o < 32; o <<= 1)
+        for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(b[e]));
+        if (__any_sync(0xffffffffu, !(top <= BOUND_MOST))) {
+            top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            hi[e] = __hmax2(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
-            lo[e] = __hmin2(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+            for (int e = 0; e < 8; ++e) {
+                b[e] = bounded(b[e]);
+                top = fmaxf(top, b[e]);
+            }
         }
-    float h[8], l[8], top = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float2 a = Pair<T>::f(hi[e]), b = Pair<T>::f(lo[e]);
-        h[2 * e] = bounded(a.x), h[2 * e + 1] = bounded(a.y), l[2 * e] = bounded(b.x), l[2 * e + 1] = bounded(b.y);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, fmaxf(fabsf(h[e]), fabsf(l[e])));
-    top = ob::warp_max(top);
-    const float d = __fdiv_rn(top, 127.0f), by = d > 0.0f ? d : 1.0f;
-    if (lane < 2 * LANES) {  // the first LANES lanes write the largest, the next ones the smallest
-        const bool low = lane >= LANES;
-        uint32_t w[2] = {0, 0};
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // (not negative: ordered as its bits are)
+        const float d = __fdiv_rn(top, 127.0f), by = d > 0.0f ? d : 1.0f;
+        // The quotient's next whole number by way of a product with about 1 / d, which is off by less than 2^-14 (127 times 2^-22 and 2^-24):
+        // where that may be on the other side of one, the division is done, but not for those near 127, whose code is 127 either way.
+        constexpr float MAGIC = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers, which are then the low bits
+        const float inverse = __frcp_rn(by);
+        float r[8];
+        bool near = !(by > 1e-37f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float c = low ? floorf(__fdiv_rn(l[e], by)) : ceilf(__fdiv_rn(h[e], by));
-            w[e / 4] |= ((uint32_t)(int)fminf(fmaxf(c, -127.0f), 127.0f) & 255u) << (e % 4 * 8);
+            const float q = b[e] * inverse;
+            near |= q < 126.9f && fabsf(q - ((q + MAGIC) - MAGIC)) < 2.5e-4f;
+            r[e] = fminf((q + 0.5f) + MAGIC, MAGIC + 127.0f);
         }
-        *reinterpret_cast<uint2 *>(codes + at * 2 * HD + lane * 8) = make_uint2(w[0], w[1]);
+        if (near) {
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {
+                float y = b[0];
+#pragma unroll
+                for (int k = 1; k < 8; ++k) y = e == k ? b[k] : y;
+                y = fminf(ceilf(__fdiv_rn(y, by)), 127.0f) + MAGIC;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = e == k ? y : r[k];
+            }
+        }
+        const uint64_t at = (uint64_t)id * pg.n_kv + head;
+        if (lane < 2 * LANES) {
+            uint32_t c[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t a = __byte_perm(__float_as_uint(r[4 * e]), __float_as_uint(r[4 * e + 1]), 0x0040), z = __byte_perm(__float_as_uint(r[4 * e + 2]), __float_as_uint(r[4 * e + 3]), 0x0040);
+                c[e] = __byte_perm(a, z, 0x5410);
+                if (low) c[e] = __vneg4(c[e]);
+            }
+            *reinterpret_cast<uint2 *>(codes + at * 2 * HD + lane * 8) = make_uint2(c[0], c[1]);
+        }
+        if (lane == 0) scales[at] = d;
+    };
+    uint32_t page = from / KV_PAGE + first, slot = 0;
+    int32_t id[BOUND_DEPTH];  // pages of this turn and the next ones
+#pragma unroll
+    for (uint32_t i = 0; i < BOUND_DEPTH; ++i) id[i] = page_of(page + i * step);
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < BOUND_DEPTH; ++i) request(page + i * step, id[i], i);
+#pragma unroll 1
+    for (; page < end; page += step) {
+        const int32_t after = page_of(page + BOUND_DEPTH * step);
+        cp_wait<BOUND_DEPTH - 2>();
+        __syncwarp();
+        request(page + (BOUND_DEPTH - 1) * step, id[BOUND_DEPTH - 1], slot == 0 ? BOUND_DEPTH - 1 : slot - 1);
+        if (id[0] >= 0) bound(id[0], slot);
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < BOUND_DEPTH; ++i) id[i] = id[i + 1];
+        id[BOUND_DEPTH - 1] = after;
+        slot = slot + 1 == BOUND_DEPTH ? 0 : slot + 1;
     }
-    if (lane == 0) scales[at] = d;
+    cp_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------------------------- checks
@@ -298,8 +394,11 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
             return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: no tensor map of the pages can be made (n_pages * n_head_kv * 16 rows have to be below 2^31)");
         }
     void *ws = nullptr;
-    cudaError_t e = cudaMalloc(&ws, PG_WORKSPACE);
-    if (e == cudaSuccess) {
+    cudaError_t e = cudaSuccess;
+    if (!ctx->page_workspaces.empty()) {  // one that a destroyed handle has left: its counters are zero again
+        ws = ctx->page_workspaces.back();
+        ctx->page_workspaces.pop_back();
+    } else if ((e = cudaMalloc(&ws, PG_WORKSPACE)) == cudaSuccess) {
         e = cudaMemsetAsync(ws, 0, PG_COUNTERS * 4, ctx->stream);
         if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // calls come on any stream
         if (e != cudaSuccess) cudaFree(ws);
@@ -318,7 +417,12 @@ void ob_pages_destroy(ob_pages *p) {
     if (!p) return;
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
-    cudaFree(p->workspace);
+    cudaDeviceSynchronize();
+    try {
+        p->ctx->page_workspaces.push_back(p->workspace);  // for the next handle; the context frees it
+    } catch (const std::bad_alloc &) {
+        cudaFree(p->workspace);
+    }
     delete p;
 }
 
@@ -363,7 +467,7 @@ int ob_pages_attention(ob_pages *p, uint32_t layer, uint32_t n_rows, const void 
     if (!row_seq && n_rows > p->d.n_seq) return bad(p, who, "more rows than tables");
     if (int rc = check_heads(p, who, n_head)) return rc;
     if (n_rows > (1u << 24)) return bad(p, who, "too many rows");
-    if (n_select == 0 || n_select > p->d.table_stride) return bad(p, who, "n_select has to be at least 1 and at most table_stride");
+    if (n_select == 0 || n_select > PG_SELECT_PAGES) return bad(p, who, "n_select has to be 1 to 131072");
     if (!std::isfinite(scale) || scale <= 0.0f) return bad(p, who, "scale has to be finite and above zero");
     if (int rc = check_rows(p, who, "q_stride", q_stride, n_head)) return rc;
     if (int rc = check_rows(p, who, "out_stride", out_stride, n_head)) return rc;
@@ -389,7 +493,7 @@ int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint3
     if (!row_seq && n_rows > p->d.n_seq) return bad(p, who, "more rows than tables");
     if (int rc = check_heads(p, who, n_head)) return rc;
     if (n_rows > (1u << 24)) return bad(p, who, "too many rows");
-    if (n_select == 0 || n_select > p->d.table_stride) return bad(p, who, "n_select has to be at least 1 and at most table_stride");
+    if (n_select == 0 || n_select > PG_SELECT_PAGES) return bad(p, who, "n_select has to be 1 to 131072");
     if ((uint64_t)keep_first + keep_last > n_select) return bad(p, who, "keep_first + keep_last is more than n_select");
     if (std::min<uint64_t>(((uint64_t)max_pos + KV_PAGE - 1) / KV_PAGE, p->d.table_stride) > PG_SELECT_PAGES)
         return fail(p->ctx, OB_ERR_CAPACITY, "pages_select: a row has more than " + std::to_string(PG_SELECT_PAGES) + " pages");
@@ -420,11 +524,19 @@ int ob_pages_bounds(ob_pages *p, uint32_t layer, uint32_t n_seq, const uint32_t 
     if (int rc = check_pointers(p, who, {{first_pos, "first_pos", 4}, {n_pos, "n_pos", 4}, {codes, "codes", 16}, {scales, "scales", 4}})) return rc;
     const PageView v = view(p, layer);
     const uint64_t pages = std::min<uint64_t>((uint64_t)(max_new - 1) / KV_PAGE + 2, p->d.table_stride);  // positions that do not begin a page touch one more
-    const uint64_t ctas = (pages * v.n_kv + 7) / 8;
-    if (ctas > 0x7fffffffull) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_bounds: too many pages");
-    const dim3 grid((uint32_t)ctas, n_seq);
+    // Warps for all places (two CTAs an SM with 128 entries, four with 64), each for several pages where there are that many.
+    const uint32_t bytes = 8 * BOUND_DEPTH * KV_PAGE * v.dim * 2;
+    const uint64_t warps = std::min<uint64_t>(pages, std::max<uint64_t>(1, 2048ull / v.dim * p->ctx->sm_count / ((uint64_t)n_seq * v.n_kv))) * v.n_kv;
+    const dim3 grid((uint32_t)((warps + 7) / 8), n_seq);
     auto kernel = v.is_bf16 ? (v.dim == 64 ? pages_bounds_kernel<bf16, 64> : pages_bounds_kernel<bf16, 128>) : (v.dim == 64 ? pages_bounds_kernel<__half, 64> : pages_bounds_kernel<__half, 128>);
-    return launched(p, who, ob::launch_pdl(kernel, grid, dim3(256), 0, stream_of(p, stream), v, first_pos, n_pos, codes, scales));
+    static PerDeviceOnce once;
+    if (cudaError_t e = once.run([] {
+            for (auto k : {pages_bounds_kernel<bf16, 64>, pages_bounds_kernel<bf16, 128>, pages_bounds_kernel<__half, 64>, pages_bounds_kernel<__half, 128>})
+                if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * BOUND_DEPTH * KV_PAGE * 128 * 2)) return e;
+            return cudaSuccess;
+        }))
+        return launched(p, who, e);
+    return launched(p, who, ob::launch_pdl(kernel, grid, dim3(256), bytes, stream_of(p, stream), v, (uint32_t)(warps / v.n_kv), first_pos, n_pos, codes, scales));
 }
 
 int ob_pages_copy(ob_pages *p, uint32_t n, const int32_t *src, const int32_t *dst, void *stream) {
@@ -458,9 +570,12 @@ int ob_pages_keep(ob_pages *p, uint32_t n_seq, const uint32_t *n_ctx, const int3
     if (kept_stride == 0 || kept_stride > PG_MAX_DRAFTS) return bad(p, who, "kept_stride has to be 1 to 64");
     if (n_seq == 0) return OB_OK;
     if (int rc = check_pointers(p, who, {{n_ctx, "n_ctx", 4}, {kept, "kept", 4}, {n_kept, "n_kept", 4}})) return rc;
-    // Heads are shared out over CTAs while there are few of them.
-    const uint32_t z = std::min(p->d.n_head_kv, std::max(1u, (uint32_t)(4ull * p->ctx->sm_count / ((uint64_t)n_seq * 2 * p->d.n_layer))));
-    return launched(p, who, ob::launch_pdl(pages_keep_kernel, dim3(n_seq, 2 * p->d.n_layer, z), dim3(MOVE_THREADS), 0, stream_of(p, stream), moves(p), kept_stride, n_ctx, kept, kept_stride, n_kept));
+    // About two turns a CTA where all of its places are taken (six an SM), one where they are not.
+    const uint64_t total = 2ull * p->d.n_layer * p->d.n_head_kv;
+    if (total > 65535) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_keep: n_layer * n_head_kv above 32767");
+    const uint64_t few = std::max<uint64_t>(1, 12ull * p->ctx->sm_count / n_seq), turns = (total * kept_stride * (p->d.head_dim / 8) + KEEP_WORDS * MOVE_THREADS - 1) / (KEEP_WORDS * MOVE_THREADS);
+    return launched(p, who, ob::launch_pdl(pages_keep_kernel, dim3(n_seq, (uint32_t)std::max<uint64_t>(1, std::min(few, turns))), dim3(MOVE_THREADS), 0, stream_of(p, stream), moves(p), 2 * p->d.n_layer,
+                                           Divide(p->d.n_head_kv), kept_stride, n_ctx, kept, kept_stride, n_kept));
 }
 
 }  // extern "C"

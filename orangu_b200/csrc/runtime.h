@@ -5,6 +5,7 @@
 
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "../../include/orangu_b200.h"
 #include "common.cuh"
@@ -27,6 +28,7 @@ struct ob_ctx {
     uint64_t launches = 0;
     float last_ms = 0.0f;
     Scratch sx, sy, sq, sd, ss, sh, shs, sdt, saux, saux2, saux3;
+    std::vector<void *> page_workspaces;  // of handles of cache pages that are gone (pages.cu)
 };
 
 struct ob_weight {

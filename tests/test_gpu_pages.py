@@ -342,11 +342,11 @@ def queries(made, rows, group, std=1.5):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("kv,group,held,n,keep", [
     (1, 1, [1], 1, (0, 0)), (2, 4, [400, 33, 160], 5, (1, 2)), (8, 4, [700], 12, (0, 1)), (1, 16, [333, 300, 16, 17], 4, (2, 2)), (2, 7, [1000, 20], 30, (3, 0)), (1, 3, [2000], 1, (0, 0)),
-    (2, 8, [500] * 9, 8, (1, 1))])
+    (2, 8, [500] * 9, 8, (1, 1)), (2, 4, [64, 3], 128, (1, 2)), (1, 12, [1500, 1400], 70, (5, 9))])
 def test_chosen_pages_and_their_attention(backend, kind, dim, kv, group, held, n, keep):
     import torch
 
-    made = Made(backend, kind, kv, dim, held, seed=n + dim, stride=max(-(-max(held) // PAGE), n))
+    made = Made(backend, kind, kv, dim, held, seed=n + dim)
     codes, scales, wc, ws = bounded(made, held)
     q = queries(made, len(held), group)
     chosen, want = choose(made, q, codes, scales, (wc, ws), held, n, *keep)
@@ -719,7 +719,7 @@ def test_refusals(backend):
         return L.ob_pages_select(h, *a.values())
 
     assert select() == 0 and select(n=0) == 0 and select(max_pos=0) == 0
-    for change, rc in ((dict(n=3), -1), (dict(heads=5), -1), (dict(n_select=0), -1), (dict(n_select=3), -1), (dict(first=2), -1), (dict(first=0xffffffff, last=1), -1), (dict(codes=p(codes) + 1), -1),
+    for change, rc in ((dict(n=3), -1), (dict(heads=5), -1), (dict(n_select=0), -1), (dict(n_select=131073), -1), (dict(first=2), -1), (dict(first=0xffffffff, last=1), -1), (dict(codes=p(codes) + 1), -1),
                        (dict(scales=None), -1), (dict(seq=host.data_ptr()), -1), (dict(chosen=None), -1), (dict(qs=4), -1)):
         assert select(**change) == rc, change
 
@@ -729,7 +729,7 @@ def test_refusals(backend):
         return L.ob_pages_attention(h, *a.values())
 
     assert attention() == 0 and attention(n=0) == 0
-    for change, rc in ((dict(layer=2), -1), (dict(n=3), -1), (dict(heads=0), -1), (dict(n_select=0), -1), (dict(n_select=3), -1), (dict(scale=0.0), -1), (dict(chosen=None), -1), (dict(os=100), -1)):
+    for change, rc in ((dict(layer=2), -1), (dict(n=3), -1), (dict(heads=0), -1), (dict(n_select=0), -1), (dict(n_select=131073), -1), (dict(scale=0.0), -1), (dict(chosen=None), -1), (dict(os=100), -1)):
         assert attention(**change) == rc, change
     i = p(lens)
     assert L.ob_pages_bounds(h, 0, 2, i, i, 4, p(codes), p(scales), st) == 0 and L.ob_pages_bounds(h, 0, 2, i, i, 0, p(codes), p(scales), st) == 0
