@@ -210,11 +210,41 @@ def test_tree_pages_that_are_not_there(backend):
     assert torch.equal(a, b) and (a[3:] == 0).all() and torch.isfinite(a).all()
 
 
-def test_tree_tokens_past_the_bound_and_odd_offsets_are_left_out(backend):
+@pytest.mark.parametrize("group,dim", [(2, 64), (8, 64), (3, 128), (16, 128)])
+def test_tree_of_many_sequences(backend, group, dim):
+    """More sequences than a warp has lanes, some of them without drafted tokens, some without context."""
+    r = np.random.default_rng(group)
+    drafts = [int(v) for v in r.integers(0, 6, 75)]
+    ctx = [0 if v < 20 else int(v) for v in r.integers(0, 400, 75)]
+    made = Made(backend, "bf16", 2, dim, [a + b for a, b in zip(ctx, drafts)], seed=dim + group)
+    run_tree(made, group, ctx, drafts)
+
+
+def test_handles_come_and_go(backend):
+    """A handle's workspace is used again by later ones: in the state that a new one has."""
+    import torch
+
+    from orangu_b200 import PagedCache
+
+    made = Made(backend, "f16", 2, 64, [2500, 900], seed=3)
+    first = {}
+    for turn in range(3):
+        for group, drafts in ((2, 4), (8, 20)):
+            made.r = np.random.default_rng(group)
+            out = run_tree(made, group, [2500 - drafts, 900 - drafts], [drafts, drafts])
+            if turn:
+                assert torch.equal(out, first[group])
+            first[group] = out
+        made.cache.close()
+        made.cache = PagedCache(backend, made.kd, made.vd, made.td)
+
+
+@pytest.mark.parametrize("group", [2, 8])
+def test_tree_tokens_past_the_bound_and_odd_offsets_are_left_out(backend, group):
     import torch
 
     made = Made(backend, "f16", 1, 64, [30, 30, 30, 30], seed=2)
-    q = torch.randn(12, 2, 64, device="cuda").half()
+    q = torch.randn(12, group, 64, device="cuda").half()
     st = torch.cuda.current_stream().cuda_stream
 
     def run(first, max_drafts):
@@ -415,6 +445,37 @@ def test_choice_among_many_pages(backend, rows, pages, n):
     n_pos = [pages * PAGE - int(v) for v in r.integers(0, 40, rows)]
     for std in (1.5, 1e-7, 60000.0):
         choose(made, queries(made, rows, group, std), torch.from_numpy(wc).cuda(), torch.from_numpy(ws).cuda(), (wc, ws), n_pos, n, 1 if n > 1 else 0, 0)
+
+
+def test_more_rows_than_the_workspace_holds_scores_for(backend):
+    """3000 rows of 8 heads and 700 pages are scored in two batches: the lists of the same rows in calls of their own."""
+    import torch
+
+    from orangu_b200 import PagedCache
+
+    r = np.random.default_rng(5)
+    rows, pages, kv, dim, n = 3000, 700, 8, 64, 24
+    x = torch.randn((1, pages, kv, PAGE, dim), device="cuda").half()
+    cache = PagedCache(backend, x, x.clone(), ints([r.permutation(pages)]))
+    st = torch.cuda.current_stream().cuda_stream
+    codes, scales = torch.zeros((pages, kv, 2, dim), dtype=torch.int8, device="cuda"), torch.zeros((pages, kv), device="cuda")
+    cache.bounds(ints([0]), ints([pages * PAGE]), codes, scales, max_new=pages * PAGE, stream=st)
+    q = torch.randn(rows, kv * 2, dim, device="cuda").half()
+    seq, n_pos = ints([0] * rows), ints(r.integers(1, pages * PAGE + 1, rows))
+    whole = torch.full((rows, kv, n), -9, dtype=torch.int32, device="cuda")
+    parts = torch.full_like(whole, -8)
+    cache.select(q, codes, scales, n_pos, whole, max_pos=pages * PAGE, keep_last=2, row_seq=seq, stream=st)
+    for a in range(0, rows, 700):
+        cache.select(q[a:a + 700], codes, scales, n_pos[a:a + 700], parts[a:a + 700], max_pos=pages * PAGE, keep_last=2, row_seq=seq[a:a + 700], stream=st)
+    out = torch.empty_like(q)
+    cache.attention(q, whole, n_pos, 0.125, out, row_seq=seq, stream=st)
+    torch.cuda.synchronize()
+    assert torch.equal(whole, parts)
+    k, v, table = float64(x[0]), float64(x[0]), cache._arrays[2].cpu().numpy()
+    some = [0, 1, 1333, 2998, 2999]
+    lists, lens = whole.cpu().numpy(), n_pos.cpu().numpy()
+    o, tol = plain.listed(float64(q)[some], k, v, table, lens[some], lists[some], 0.125, [0] * len(some), tolerance("f16", dim))
+    check(float64(out)[some], o, tol, "f16")
 
 
 def test_odd_queries_and_pages_that_are_not_there(backend):
