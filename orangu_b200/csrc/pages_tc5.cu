@@ -6,14 +6,23 @@
 // is cut leaves (maximum, sum, output) in fp32, and a second kernel, launched along, adds them up over all SMs (the last of a piece's
 // CTAs to arrive doing it alone took as long as all the rest: 181 us for 8 x 64 tokens of 4 heads a key/value head at 8192).
 //
-//   warps 0-15 softmax: eight warps per stream, two threads per row with 64 positions each.  Scores come from tensor memory, weights go back
-//              into the same columns: f16, or bf16 as value plus remainder.
-//   warp 16    issues the products: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
-//   warp 17    issues the TMA loads of pages, 16 rows x 64 columns each, straight from the cache into the swizzled operand tiles
+//   warps 0-7  softmax: four warps per stream, a thread per row.  Scores come from tensor memory, weights go back into the same
+//              columns: f16, or bf16 as value plus remainder.
+//   warps 8, 9 issue the products of a stream each: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
+//   warp 10    issues the TMA loads of pages, 16 rows x 64 columns each, straight from the cache into the swizzled operand tiles
 //
-// There are two streams of scores, so that one's softmax runs under the other's products.  Up to 128 rows (WIDE false) they are the even and the
-// odd tiles of the same rows, with an output each; above that they are two tiles of 128 rows that share keys and values.  Context
-// positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
+// There are two streams of scores.  Up to 128 rows (WIDE false) they are the even and the odd tiles of the same rows, with an output each;
+// above that they are two tiles of 128 rows that share keys and values.  A stream goes in steps of half a tile through two places for
+// scores: while one's weights are made, the other's are multiplied and its next scores come.  Whole tiles with one place a stream, 16 softmax
+// warps and one that issued all products took 25.6 us for one sequence of 512 positions and 48 rows a key/value head and 52 us for
+// eight of 4096 and 64, now 19.5 and 48; 300 to 320 us for four of 32,000 and 256 rows, as now.
+//
+// What bounds it (head dimension 128): up to 128 rows the bytes, 208 us for 32 sequences of 8192 with 64 rows (floor 166, 5.2 TB/s).  Above, the
+// chain of a step: 2080 clocks for two warps' 64 positions, of which the special function unit works 40 % and the tensor cores 40 %
+// (605 us for 32 sequences of 8192 with 512 rows, 0.9 PFLOP/s; floor 335).  A part of the powers of two on the fused multiply-adds,
+// 1/8 to 1/2 of them, took from 2 % less to 6 % more.
+//
+// Context positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
 // per thread.  There, values of positions that nobody has, or that are no numbers, are set to zero in shared memory (0 times them
 // would reach rows that do not see them); what rows do see of the latter is added at the end.  All waits are bounded.
 #include <algorithm>
@@ -28,18 +37,18 @@ namespace ob {
 namespace {
 
 constexpr uint32_t PG_ROWS = 128, PG_KEYS = 128, PG_PAGES = PG_KEYS / KV_PAGE, PG_BLOCK = PG_KEYS * 128;  // block: 128 rows of 64 columns
-constexpr int PG_SOFT = 512, PG_MMA_WARP = 16, PG_TMA_WARP = 17, PG_THREADS = 18 * 32;
+constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 11 * 32;
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
 constexpr uint32_t PG_LEAST = 2;        // tiles of a CTA: one for each stream
 constexpr uint32_t PG_START = 3;        // what the start and end of a piece cost, in tiles
 
 // mbarriers and small arrays, byte offsets
-constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 144, PB_S_FULL = 192, PB_P_FULL = 208, PB_O_FULL = 224, PB_Q_FULL = 240, PB_SLOT = 248, PB_ABORT = 252,
-                   PB_ODD = 256, PB_TOP = 264, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
+constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 144, PB_S_FULL = 192 /* [stream][place] */, PB_P_FULL = 224, PB_PV_DONE = 256, PB_O_FULL = 272, PB_Q_FULL = 288,
+                   PB_SLOT = 296, PB_ABORT = 300, PB_ODD = 304, PB_TOP = 312, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
 template <int HD, bool WIDE>
 struct PgPlan {
-    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, Q = WIDE || HD == 64 ? 2 * OPERAND : OPERAND;  // (32 KB at least: outputs leave by way of it)
+    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, Q = (WIDE ? 2 : 1) * OPERAND;  // (16 KB at least: outputs leave by way of it)
     static constexpr uint32_t FIT = (227 * 1024 - PB_BYTES - Q) / (2 * OPERAND), STAGES = FIT < 6 ? FIT : 6;
     static constexpr uint32_t K = Q, V = K + STAGES * OPERAND, BAR = V + STAGES * OPERAND, BYTES = BAR + PB_BYTES;
     static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
@@ -60,8 +69,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ void pair_sync(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 9, %0;" ::"n"(PG_SOFT) : "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PG_SOFT) : "memory"); }
 
 template <typename T> __device__ __forceinline__ uint32_t pack16(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
@@ -186,16 +194,19 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < ST; ++s) {
             mbar_init(bar + PB_K_FULL + 8 * s, 1);
-            mbar_init(bar + PB_K_EMPTY + 8 * s, 1);
+            mbar_init(bar + PB_K_EMPTY + 8 * s, WIDE ? 2 : 1);  // the streams that read a tile
             mbar_init(bar + PB_V_FULL + 8 * s, 1);
-            mbar_init(bar + PB_V_EMPTY + 8 * s, 1);
+            mbar_init(bar + PB_V_EMPTY + 8 * s, WIDE ? 2 : 1);
         }
         for (uint32_t s = 0; s < 2; ++s) {
-            mbar_init(bar + PB_S_FULL + 8 * s, 1);
-            mbar_init(bar + PB_P_FULL + 8 * s, 8);
+            for (uint32_t b = 0; b < 2; ++b) {
+                mbar_init(bar + PB_S_FULL + 16 * s + 8 * b, 1);
+                mbar_init(bar + PB_P_FULL + 16 * s + 8 * b, 4);
+            }
+            mbar_init(bar + PB_PV_DONE + 8 * s, 1);
             mbar_init(bar + PB_O_FULL + 8 * s, 1);
         }
-        mbar_init(bar + PB_Q_FULL, 16);
+        mbar_init(bar + PB_Q_FULL, 8);
         *abort = 0u;
         *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD) = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -210,8 +221,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_SLOT);
     PgWalk<MR> w;
     w.start(a);
-    // Tiles of a piece that a stream takes: all of them, or every other one.  With row tiles the second stream may have no rows.
-    auto has = [&](uint32_t s, uint32_t i, uint32_t rows) { return WIDE ? s == 0 || rows > PG_ROWS : (i & 1u) == s; };
+    // Steps of a stream in a piece: two for each of its tiles, which are all of them or every other one.  With two tiles of rows the second
+    // stream may have no rows.
+    auto steps_of = [&](uint32_t s, uint32_t tiles, uint32_t rows) { return WIDE ? (s == 0 || rows > PG_ROWS ? 2 * tiles : 0u) : (tiles + 1 - s) / 2 * 2; };
+    auto tile_of = [&](uint32_t s, uint32_t step) { return WIDE ? step / 2 : s + step / 2 * 2; };
 
     if (warp == PG_TMA_WARP) {
         uint32_t n = 0;  // tiles so far
@@ -245,83 +258,79 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 y = next;
             }
         }
-    } else if (warp == PG_MMA_WARP) {
+    } else if (warp >= PG_MMA_WARP) {
         constexpr uint32_t F16 = REMAINDER ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
-        const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
-        uint32_t n = 0, turn = 0, used0 = 0, used1 = 0;  // tiles and pieces so far, weights taken from each stream so far
+        const uint32_t id_s = umma_idesc_bf16(PG_KEYS / 2) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
+        const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
+        uint32_t n = 0, turn = 0, done = 0;  // tiles and pieces so far, steps of the stream so far
         bool ok = true;
-        const uint64_t q_desc = umma_desc_sw128(sbase), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
-        auto scores = [&](uint32_t s, uint32_t at) {
-            const uint32_t st = at % ST;
-            if (!mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / ST) & 1u, abort)) return false;
-            tc_fence_after();
-            const uint64_t qd = q_desc + ((WIDE ? s * OPERAND : 0u) >> 4), kd = k_desc + (st * OPERAND >> 4);
-#pragma unroll
-            for (uint32_t b = 0; b < HD / 16; ++b)
-                umma_bf16_warp(tmem + PG_TMEM_S + s * PG_KEYS, qd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
-            umma_commit_warp(bar + PB_S_FULL + 8 * s);
-            return true;
-        };
+        const uint64_t q_desc = umma_desc_sw128(sbase + (WIDE ? s * OPERAND : 0u)), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
         for (; w.more() && ok; w.next(a), ++turn) {
-            const uint32_t tiles = w.last() - w.tile, rows = w.q.drafts * a.group - w.rt * MR;
-            ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);
-            tc_fence_after();
-            if (WIDE) {
-                for (uint32_t s = 0; s < 2 && ok; ++s)
-                    if (has(s, 0, rows)) ok = scores(s, n);
-                if (ok) umma_commit_warp(bar + PB_K_EMPTY + 8 * (n % ST));
-            } else {
-                for (uint32_t s = 0; s < 2 && s < tiles && ok; ++s) {
-                    ok = scores(s, n + s);
-                    if (ok) umma_commit_warp(bar + PB_K_EMPTY + 8 * ((n + s) % ST));
+            const uint32_t tiles = w.last() - w.tile, steps = steps_of(s, tiles, w.q.drafts * a.group - w.rt * MR);
+            if (WIDE && steps == 0) {  // no rows: only says of every tile that it does not need it
+                for (uint32_t i = 0; i < tiles && ok; ++i) {
+                    const uint32_t st = (n + i) % ST, par = ((n + i) / ST) & 1u;
+                    ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, par, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, par, abort);
+                    if (ok && lane == 0) mbar_arrive(bar + PB_K_EMPTY + 8 * st), mbar_arrive(bar + PB_V_EMPTY + 8 * st);
+                    __syncwarp();
                 }
+                n += tiles;
+                continue;
             }
-            for (uint32_t i = 0; i < tiles && ok; ++i) {
-                const uint32_t st = (n + i) % ST;
-#pragma unroll
-                for (uint32_t s = 0; s < 2; ++s) {
-                    if (!ok || !has(s, i, rows)) continue;
-                    uint32_t &used = s ? used1 : used0;
-                    ok = mbar_wait_warp(bar + PB_P_FULL + 8 * s, used & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, ((n + i) / ST) & 1u, abort);
-                    ++used;
-                    if (!ok) continue;
+            ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);
+#pragma unroll 1
+            for (int step = -2; step < (int)steps && ok; ++step) {  // -2, -1: only the first scores
+                const uint32_t half = step & 1;
+                if (step >= 0) {
+                    const uint32_t at = n + tile_of(s, step), st = at % ST;
+                    ok = mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * half, done >> 1 & 1u, abort);
+                    ++done;
+                    if (ok && half == 0) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / ST) & 1u, abort);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t p = tmem + PG_TMEM_S + s * PG_KEYS, d = tmem + PG_TMEM_O + s * 128;
-                    const uint64_t vd = v_desc + (st * OPERAND >> 4);
-                    const uint32_t add = WIDE ? i : i >> 1;  // the stream's first product writes, the others add
+                    const uint32_t p = ts + half * 64;
+                    const uint64_t vd = v_desc + (st * OPERAND >> 4) + half * 4 * 128;
 #pragma unroll
-                    for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {
+                    for (uint32_t kk = 0; kk < PG_KEYS / 32; ++kk) {  // the stream's first product writes, the others add
                         if (REMAINDER) {  // 16 positions: eight columns of values, eight of remainders
-                            umma_bf16_ta_warp(d, p + kk * 16, vd + kk * 128, id_o, add || kk ? 1u : 0u);
-                            umma_bf16_ta_warp(d, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
-                        } else {  // 64 positions are the second half of their 64 columns
-                            umma_bf16_ta_warp(d, p + kk / 4 * 64 + 32 + kk % 4 * 8, vd + kk * 128, id_o, add || kk ? 1u : 0u);
+                            umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
+                            umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
+                        } else {
+                            umma_bf16_ta_warp(to, p + kk * 8, vd + kk * 128, id_o, step || kk ? 1u : 0u);
                         }
                     }
-                    const uint32_t step = WIDE ? 1 : 2;
-                    if (i + step >= tiles) {
-                        umma_commit_warp(bar + PB_O_FULL + 8 * s);
-                    } else {
-                        ok = scores(s, n + i + step);
-                        if (ok && !WIDE) umma_commit_warp(bar + PB_K_EMPTY + 8 * ((n + i + step) % ST));
-                    }
+                    umma_commit_warp(bar + PB_PV_DONE + 8 * s);
+                    if (half) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
                 }
-                if (!ok) break;
-                umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
-                if (WIDE && i + 1 < tiles) umma_commit_warp(bar + PB_K_EMPTY + 8 * ((n + i + 1) % ST));
+                const uint32_t next = step + 2;
+                if (next < steps) {
+                    const uint32_t at = n + tile_of(s, next), st = at % ST;
+                    if (half == 0) {
+                        ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / ST) & 1u, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    const uint64_t kd = k_desc + ((st * OPERAND + half * (PG_BLOCK / 2)) >> 4);
+#pragma unroll
+                    for (uint32_t b = 0; b < HD / 16; ++b)
+                        umma_bf16_warp(ts + half * 64, q_desc + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
+                    umma_commit_warp(bar + PB_S_FULL + 16 * s + 8 * half);
+                    if (half) umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
+                } else if (half) {
+                    umma_commit_warp(bar + PB_O_FULL + 8 * s);
+                }
             }
             n += tiles;
         }
     } else if (warp < PG_MMA_WARP) {
-        const uint32_t s = warp / 8, part = warp / 4 % 2, quad = warp % 4, r = quad * 32 + lane, pair = 1 + s * 4 + quad;
+        const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
         const uint32_t magic = (65536 + a.group - 1) / a.group;  // x / group = x magic / 65536 for x below 4096, group up to 16
         const float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
-        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * PG_KEYS + part * 64, to = lanes + PG_TMEM_O;
-        volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][half][row]: maxima; at the end [stream][sum, maximum][row]
-        const uint32_t own = (2 * s + part) * PG_ROWS, other = (2 * s + (part ^ 1u)) * PG_ROWS;
+        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * PG_KEYS, to = lanes + PG_TMEM_O;
+        volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][sum, maximum][row]
         volatile uint32_t *odd = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD);
         bool ok = true;
-        uint32_t used = 0, n = 0;   // tiles of scores taken, tiles of the CTA so far
+        uint32_t used = 0, n = 0;   // steps of the stream, tiles of the CTA so far
         bool said = false;          // a piece that others go on with has been written down
         uint32_t both[2] = {0, 0};  // pieces with tiles of either stream (WIDE false: every warp reads both outputs)
         for (; w.more(); w.next(a)) {
@@ -360,26 +369,26 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 return tile < end && p < w.q.n_pages && (uint32_t)table[p] < a.pg.n_pages;
             };
             // ---- the tiles
-            const uint32_t step = WIDE ? 1 : 2, first = WIDE ? 0 : s;
-            const bool mine = WIDE ? s == 0 || n_rows > PG_ROWS : s < tiles;  // this stream has tiles here
+            const uint32_t steps = steps_of(s, tiles, n_rows);
             float m = -INFINITY, l = 0.0f;
-            bool there = pages_of(w.tile + first);
-            for (uint32_t i = first; mine && i < tiles; i += step, ++used) {
-                ok = ok && mbar_wait_warp(bar + PB_S_FULL + 8 * s, used & 1u, abort);
-                const uint32_t valid = __ballot_sync(0xffffffffu, there) & 0xffu, x0 = (w.tile + i) * PG_KEYS;
-                there = pages_of(w.tile + i + step);
-                const bool masked = valid != 0xffu || x0 + PG_KEYS > w.q.ctx;
-                if (ok && x0 + PG_KEYS > w.q.ctx) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
-                if (!ok) {  // a wait was given up: nothing more is computed, but the other half's barriers are kept company
-                    if (warm) pair_sync(pair);
-                    continue;
+            bool there = pages_of(w.tile + tile_of(s, 0));
+            uint32_t valid = 0;
+            for (uint32_t step = 0; step < steps; ++step, ++used) {
+                const uint32_t i = tile_of(s, step), half = step & 1, x0 = (w.tile + i) * PG_KEYS;
+                const bool past = x0 + PG_KEYS > w.q.ctx;
+                ok = ok && mbar_wait_warp(bar + PB_S_FULL + 16 * s + 8 * half, used >> 1 & 1u, abort);
+                if (half == 0) {
+                    valid = __ballot_sync(0xffffffffu, there) & 0xffu;
+                    there = pages_of(w.tile + tile_of(s, step + 2));
+                    if (ok && past) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
                 }
-                if (x0 + PG_KEYS > w.q.ctx) {  // values of positions past the context
+                if (!ok) break;  // a wait was given up: nothing more is computed
+                if (half == 0 && past) {  // values of positions past the context
                     uint8_t *v = smem + P::V + (n + i) % ST * OPERAND;
                     const uint32_t from = w.q.ctx > x0 ? w.q.ctx - x0 : 0u;
                     bool bad = false;
 #pragma unroll 1
-                    for (uint32_t c = from * 8 + (warp % 8) * 32 + lane; c < PG_KEYS * 8; c += 256)
+                    for (uint32_t c = from * 8 + (warp % 4) * 32 + lane; c < PG_KEYS * 8; c += 128)
 #pragma unroll 1
                         for (uint32_t b = 0; b < NB; ++b) {
                             uint4 *at = reinterpret_cast<uint4 *>(v + b * PG_BLOCK) + c;
@@ -400,46 +409,70 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 if (warm) {
+                    const uint32_t tp = ts + half * 64;
                     tc_fence_after();
-                    uint64_t bits = ~0ull;  // what the row sees of this half of the tile
-                    if (masked) {
-                        const uint32_t k0 = x0 + part * 64;
-                        bits = k0 >= w.q.ctx ? 0ull : w.q.ctx - k0 >= 64 ? ~0ull : (1ull << (w.q.ctx - k0)) - 1;  // context
-                        if (k0 + 64 > w.q.ctx) {  // drafted token j at ctx + j
+                    uint32_t u[2][32];
+                    tmem_ld32(tp, u[0]);
+                    tmem_ld32(tp + 32, u[1]);
+                    tmem_ld_wait();
+                    if (valid != 0xffu || past) {
+                        const uint32_t k0 = x0 + half * 64;  // the step's first position
+                        uint64_t bits = k0 >= w.q.ctx ? 0ull : w.q.ctx - k0 >= 64 ? ~0ull : (1ull << (w.q.ctx - k0)) - 1;  // what the row sees: context,
+                        if (k0 + 64 > w.q.ctx) {                                                                          // drafted token j at ctx + j
                             const int shift = (int)(w.q.ctx - k0);  // above -64 where any of them is here
                             bits |= shift >= 0 ? seen << shift : shift > -64 ? seen >> -shift : 0ull;
                         }
 #pragma unroll
                         for (int p = 0; p < 4; ++p)
-                            if (!(valid >> (part * 4 + p) & 1)) bits &= ~(0xffffull << (16 * p));
+                            if (!(valid >> (half * 4 + p) & 1)) bits &= ~(0xffffull << (16 * p));
+#pragma unroll
+                        for (int e = 0; e < 64; ++e)
+                            if (!(bits >> e & 1)) u[e / 32][e % 32] = 0xff800000u;
                     }
-                    auto hide = [&](uint32_t(&u)[32], int c) {
-                        const uint32_t word = (uint32_t)(bits >> (c * 32));
+                    // weights against the maximum so far, which stays while no score is above it by more than the slack: then the output need not be
+                    // rescaled, and the new maximum is not waited for
+                    if (__any_sync(0xffffffffu, m == -INFINITY)) {  // a row that has seen nothing yet: its first maximum
+                        float top = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(word >> e & 1)) u[e] = 0xff800000u;
-                    };
-                    // The first 32 scores are read twice, for the maximum and for the weights: all 64 would not fit beside the rest.
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    uint32_t u[32];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        tmem_ld32(ts + 32 * c, u);
-                        tmem_ld_wait();
-                        if (masked) hide(u, c);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) top[e / 2 % 4] = max3(top[e / 2 % 4], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+                        for (int e = 0; e < 64; e += 2) top = max3(top, __uint_as_float(u[e / 32][e % 32]), __uint_as_float(u[e / 32][e % 32 + 1]));
+                        if (m == -INFINITY) m = top * scale2;
                     }
-                    const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
-                    xchg[own] = here;
-                    pair_sync(pair);
-                    const float now = fmaxf(here, xchg[other]);
-                    const bool grown = m > -INFINITY && now > m + PG_SLACK;
-                    if (__any_sync(0xffffffffu, grown)) {  // the product before this tile's scores is done: the output may be rescaled
+                    float sum0, sum1;
+#pragma unroll 1
+                    for (;;) {
+                        const float base = m == -INFINITY ? 0.0f : -m;  // (still nothing: weights of zero)
+                        float top[2] = {-INFINITY, -INFINITY};
+                        sum0 = sum1 = 0.0f;
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {  // 16 positions
+                            uint32_t v[16];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float x0 = __uint_as_float(u[g / 2][g % 2 * 16 + 2 * e]), x1 = __uint_as_float(u[g / 2][g % 2 * 16 + 2 * e + 1]);
+                                float e0, e1;
+                                top[e % 2] = max3(top[e % 2], x0, x1);
+                                fma2(e0, e1, x0, x1, scale2, base);
+                                e0 = pow2(e0), e1 = pow2(e1);
+                                add2(sum0, sum1, e0, e1);
+                                v[e] = pack16<T>(e0, e1);
+                                if constexpr (REMAINDER) v[8 + e] = pack16<T>(e0 - __uint_as_float(v[e] << 16), e1 - __uint_as_float(v[e] & 0xffff0000u));
+                            }
+                            if constexpr (REMAINDER) {
+                                tmem_st16(tp + 16 * g, v);
+                            } else {
+                                const uint32_t(&h)[8] = reinterpret_cast<const uint32_t(&)[8]>(v);
+                                tmem_st8(tp + 8 * g, h);
+                            }
+                        }
+                        const float now = fmaxf(top[0], top[1]) * scale2;
+                        const bool grown = now > m + PG_SLACK;
+                        if (!__any_sync(0xffffffffu, grown)) break;
+                        if (step > 0) ok = mbar_wait_warp(bar + PB_PV_DONE + 8 * s, (used - 1) & 1u, abort);  // the product before these scores
+                        tc_fence_after();
                         const float keep = grown ? pow2(m - now) : 1.0f;
                         if (grown) m = now, l *= keep;
 #pragma unroll 1
-                        for (uint32_t c = 16 * part; c < HD; c += 32) {
+                        for (uint32_t c = 0; c < HD; c += 16) {
                             uint32_t o[16];
                             tmem_ld16(to + s * 128 + c, o);
                             tmem_ld_wait();
@@ -448,42 +481,12 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                             tmem_st16(to + s * 128 + c, o);
                         }
                     }
-                    if (m == -INFINITY) m = now;
-                    const float base = m == -INFINITY ? 0.0f : -m;  // a row that has seen nothing yet keeps weights of zero
-                    float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-                    for (int c = 1; c >= 0; --c) {  // 32 positions
-                        if (c == 0) {
-                            tmem_ld32(ts, u);
-                            tmem_ld_wait();
-                            if (masked) hide(u, 0);
-                        }
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            uint32_t v[16];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                float e0, e1;
-                                fma2(e0, e1, __uint_as_float(u[16 * g + 2 * e]), __uint_as_float(u[16 * g + 2 * e + 1]), scale2, base);
-                                e0 = pow2(e0), e1 = pow2(e1);
-                                add2(sum0, sum1, e0, e1);
-                                v[e] = pack16<T>(e0, e1);
-                                if constexpr (REMAINDER) v[8 + e] = pack16<T>(e0 - __uint_as_float(v[e] << 16), e1 - __uint_as_float(v[e] & 0xffff0000u));
-                            }
-                            if constexpr (REMAINDER) {
-                                tmem_st16(ts + 32 * c + 16 * g, v);
-                            } else {
-                                const uint32_t(&h)[8] = reinterpret_cast<const uint32_t(&)[8]>(v);
-                                tmem_st8(ts + 32 + 16 * c + 8 * g, h);
-                            }
-                        }
-                    }
                     l += sum0 + sum1;
                     tmem_st_wait();
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar + PB_P_FULL + 8 * s);
+                if (lane == 0) mbar_arrive(bar + PB_P_FULL + 16 * s + 8 * half);
             }
             n += tiles;
             // ---- the piece is done: the streams' outputs and sums
@@ -495,20 +498,15 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     ++both[k];
                 }
             tc_fence_after();
-            if (part) xchg[own] = l;  // (both halves have read the last maxima: their products are done)
-            pair_sync(pair);
-            if (part == 0) {
-                l += xchg[other];
-                xchg[own] = l, xchg[other] = m;
-            }
+            xchg[2 * s * PG_ROWS] = l, xchg[(2 * s + 1) * PG_ROWS] = m;
             soft_sync();
             const bool whole = w.tile == 0 && end == w.q.n_tiles;
             const uint32_t origin = w.at - w.tile, begin = blockIdx.x * w.per;  // of the piece's first tile and of this CTA, in units
             float *part_out = a.partial + (2ull * blockIdx.x + (origin > begin ? 1 : 0)) * P::PART;  // a CTA has a part of two pieces at most
-            // this thread's columns of its row: half of them, or (both streams have the same rows) a quarter of them of both outputs
-            constexpr uint32_t COLS = WIDE ? HD / 2 : HD / 4;
-            const uint32_t col0 = (WIDE ? part : warp / 4) * COLS;
-            float f0 = 1.0f, f1 = 0.0f, sum = xchg[2 * s * PG_ROWS], peak = m;
+            // this thread's columns of its row: all of them, or (both streams have the same rows) half of them of both outputs
+            constexpr uint32_t COLS = WIDE ? HD : HD / 2;
+            const uint32_t col0 = WIDE ? 0u : s * COLS;
+            float f0 = 1.0f, f1 = 0.0f, sum = l, peak = m;
             if (!WIDE) {
                 const float m0 = xchg[PG_ROWS], m1 = had[1] ? xchg[3 * PG_ROWS] : -INFINITY;
                 peak = fmaxf(m0, m1);
@@ -565,7 +563,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                             __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)(warp_row + row) * HD + col0 + c + 4 * e), y);
                     }
                 }
-            if (!whole && live && part == 0 && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
+            if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
             if (!whole && origin >= begin && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
                 a.pieces[blockIdx.x] = PagePiece{(origin + w.q.n_tiles - 1) / w.per - blockIdx.x + 1, 2 * blockIdx.x + (origin > begin ? 1u : 0u), min(n_rows, MR), w.rt * MR, w.q.row0, w.head};
                 said = true;
