@@ -13,6 +13,7 @@
 // through the pieces that lie in its part.  A piece that is cut leaves (m, sum, output) in fp32 and the last of its CTAs to arrive -- a
 // counter tells, which goes back to zero by itself -- adds the parts up in order, so the result does not depend on who was last.
 #include <algorithm>
+#include <type_traits>
 
 #include "mixers_common.cuh"
 #include "pages.h"
@@ -433,23 +434,51 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
         __syncthreads();
         if (!s_last) continue;
         __threadfence();
-        for (uint32_t i = threadIdx.x; i < n_rows * VEC; i += PA_THREADS) {
-            const uint32_t r = i / VEC, c = i % VEC;
-            float top = -INFINITY, l = 0.0f;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-            for (uint32_t k = c0; k <= c1; ++k) {
-                const float *from_k = slot(k);
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from_k + PA_ROWS * HD + 2 * r));
-                const float4 y = __ldcg(reinterpret_cast<const float4 *>(from_k + r * HD + 4 * c));
-                if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-                const float higher = fmaxf(top, ml.x), f0 = top == -INFINITY ? 0.0f : pow2(top - higher), f1 = ml.x == -INFINITY ? 0.0f : pow2(ml.x - higher);
-                top = higher;
-                l = fmaf(ml.y, f1, l * f0);
-                x.x = fmaf(y.x, f1, x.x * f0), x.y = fmaf(y.y, f1, x.y * f0), x.z = fmaf(y.z, f1, x.z * f0), x.w = fmaf(y.w, f1, x.w * f0);
+        // 16 entries of parts are under way at once: a sequence of 32,000 positions, whose eight pieces have 55 parts each, takes 51 us for 16 rows of
+        // 128 and 43 us for 4, and with one row after the other 67 and 47 us
+        auto add_up = [&](auto rows) {
+            constexpr uint32_t MINE = decltype(rows)::value, APART = PA_THREADS / VEC, AHEAD = 16 / MINE;  // rows of a thread, from one to the next, parts
+            const uint32_t r0 = threadIdx.x / VEC, c = threadIdx.x % VEC;
+            float top[MINE], l[MINE];
+            float4 x[MINE];
+#pragma unroll
+            for (uint32_t j = 0; j < MINE; ++j) top[j] = -INFINITY, l[j] = 0.0f, x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (uint32_t k = c0; k <= c1; k += AHEAD) {
+                float2 ml[AHEAD][MINE];
+                float4 y[AHEAD][MINE];
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < MINE; ++j) {
+                        const uint32_t r = r0 + j * APART;
+                        const float *from_k = slot(k + i);
+                        ml[i][j] = make_float2(-INFINITY, 0.0f), y[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (k + i <= c1 && r < n_rows) {
+                            ml[i][j] = __ldcg(reinterpret_cast<const float2 *>(from_k + PA_ROWS * HD + 2 * r));
+                            y[i][j] = __ldcg(reinterpret_cast<const float4 *>(from_k + r * HD + 4 * c));
+                        }
+                    }
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < MINE; ++j) {
+                        const float2 ml1 = ml[i][j];
+                        const float4 y1 = y[i][j];
+                        const float higher = fmaxf(top[j], ml1.x), f0 = top[j] == -INFINITY ? 0.0f : pow2(top[j] - higher), f1 = ml1.x == -INFINITY ? 0.0f : pow2(ml1.x - higher);
+                        top[j] = higher;
+                        l[j] = fmaf(ml1.y, f1, l[j] * f0);
+                        x[j].x = fmaf(y1.x, f1, x[j].x * f0), x[j].y = fmaf(y1.y, f1, x[j].y * f0), x[j].z = fmaf(y1.z, f1, x[j].z * f0), x[j].w = fmaf(y1.w, f1, x[j].w * f0);
+                    }
             }
-            store(r, c, x, l);
-        }
+#pragma unroll
+            for (uint32_t j = 0; j < MINE; ++j)
+                if (r0 + j * APART < n_rows) store(r0 + j * APART, c, x[j], l[j]);
+        };
+        if (n_rows * VEC <= PA_THREADS)
+            add_up(std::integral_constant<uint32_t, 1>{});
+        else
+            add_up(std::integral_constant<uint32_t, PA_ROWS * VEC / PA_THREADS>{});
     }
 }
 
