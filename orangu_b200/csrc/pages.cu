@@ -378,7 +378,7 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     if (d.type != OB_TYPE_F16 && d.type != OB_TYPE_BF16) return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: pages are f16 (OB_TYPE_F16) or bfloat16 (OB_TYPE_BF16)");
     if (d.head_dim != 64 && d.head_dim != 128) return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: head_dim has to be 64 or 128");
     if (!d.n_layer || !d.n_pages || !d.n_head_kv || !d.n_seq || !d.table_stride) return fail(ctx, OB_ERR_INVALID, "pages_create: a size is zero");
-    if (d.n_layer > 16383 || d.n_head_kv > 4096 || d.n_pages > 0x7fffffffu || d.table_stride > (1u << 27) || d.n_seq > (1u << 24))
+    if (d.n_layer > 16383 || d.n_head_kv > 4096 || d.n_pages > 0x7fffffffu || d.table_stride > (1u << 26) || d.n_seq > (1u << 24))
         return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: a size is too large");
     const uint64_t elems = (uint64_t)d.n_pages * d.n_head_kv * KV_PAGE * d.head_dim;
     if (d.n_layer > 1 && (d.layer_stride < elems || d.layer_stride % 8)) return fail(ctx, OB_ERR_INVALID, "pages_create: layer_stride has to be a multiple of 8 and at least a layer's pages");
@@ -387,7 +387,12 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     if (!on_device(ctx, d.k) || !on_device(ctx, d.v) || !on_device(ctx, d.tables)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages and tables have to be memory of the context's device");
     ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, nullptr, {}};
     if (!p) return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
-    p->maps.resize(d.n_layer);
+    try {
+        p->maps.resize(d.n_layer);
+    } catch (const std::bad_alloc &) {
+        delete p;
+        return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
+    }
     for (uint32_t l = 0; l < d.n_layer; ++l)
         if (!make_page_maps(view(p, l), &p->maps[l])) {
             delete p;
@@ -449,8 +454,8 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx;
     use_workspace(p, a);
     if (max_drafts * a.group > PG_FEW_ROWS) {
-        // (the walk over all tiles counts them in 31 bits)
-        if ((uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + 7) / 8) * ((max_drafts * a.group + 127) / 128) >= (1ull << 31))
+        // (the walk over all pieces counts their tiles, and PG_START more for each, in 31 bits)
+        if ((uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + 7) / 8 + PG_START) * ((max_drafts * a.group + 127) / 128) >= (1ull << 31))
             return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tree: the tables of all sequences together have room for too many positions");
         return launched(p, who, launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, stream_of(p, stream)), 2);
     }

@@ -41,7 +41,6 @@ constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 11 
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
 constexpr uint32_t PG_LEAST = 2;        // tiles of a CTA: one for each stream
-constexpr uint32_t PG_START = 3;        // what the start and end of a piece cost, in tiles
 
 // mbarriers and small arrays, byte offsets
 constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 144, PB_S_FULL = 192 /* [stream][place] */, PB_P_FULL = 224, PB_PV_DONE = 256, PB_O_FULL = 272, PB_Q_FULL = 288,

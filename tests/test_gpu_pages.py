@@ -819,3 +819,22 @@ def test_refusals(backend):
         cache.attention(q, torch.zeros((6, 2, 2), dtype=torch.int32, device="cuda"), lens, 0.1, out)  # six rows, two tables
     with pytest.raises(OranguError):
         cache.copy(torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))  # host memory
+
+
+def test_a_walk_of_more_than_31_bits_is_refused(backend):
+    """Every (rows, sequence, head) piece counts as its tiles and three more: 2^22 sequences of one tile of 64 heads, in four tiles of 128 rows, are 2^32."""
+    import torch
+
+    from orangu_b200 import OranguError, PagedCache
+
+    n_seq, heads = 1 << 22, 64
+    k = torch.zeros((1, 1, heads, PAGE, 64), dtype=torch.float16, device="cuda")
+    cache = PagedCache(backend, k, k.clone(), torch.zeros((n_seq, 1), dtype=torch.int32, device="cuda"))
+    q = torch.zeros((1, heads * 16, 64), dtype=torch.float16, device="cuda")
+    first, ctx = torch.zeros(n_seq + 1, dtype=torch.int32, device="cuda"), torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 9.0)
+    with pytest.raises(OranguError, match="too many positions"):
+        cache.attention_tree(q, first, ctx, words([1]), 0.1, out, 32, 16)
+    cache.attention_tree(q, first[:1025], ctx[:1024], words([1]), 0.1, out, 32, 16)  # (no tokens: nothing is written)
+    torch.cuda.synchronize()
+    assert bool((out == 9.0).all())
