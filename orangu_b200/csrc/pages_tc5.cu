@@ -551,15 +551,22 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<float4 *>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
                     __syncwarp();
-#pragma unroll 1
-                    for (uint32_t row = lane / 4; row < 32 && warp_row + row < n_rows; row += 8) {
-                        const uint32_t e = lane & 3, f = w.rt * MR + warp_row + row, t0 = f * magic >> 16;
-                        const float4 y = *reinterpret_cast<const float4 *>(stage + row * 64 + ((e ^ (row >> 1 & 3)) << 4));
+                    float4 y[4];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const uint32_t row = lane / 4 + 8 * k;
+                        y[k] = *reinterpret_cast<const float4 *>(stage + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const uint32_t row = warp_row + lane / 4 + 8 * k, e = col0 + c + 4 * (lane & 3);
+                        if (row >= n_rows) break;
+                        const uint32_t f = w.rt * MR + row, t0 = f * magic >> 16;
                         if (whole)
-                            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + t0) * a.out_stride + (w.head * a.group + f - t0 * a.group) * HD + col0 + c + 4 * e) =
-                                make_uint2(pack16<T>(y.x, y.y), pack16<T>(y.z, y.w));
+                            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (uint64_t)(w.q.row0 + t0) * a.out_stride + (w.head * a.group + f - t0 * a.group) * HD + e) =
+                                make_uint2(pack16<T>(y[k].x, y[k].y), pack16<T>(y[k].z, y[k].w));
                         else
-                            __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)(warp_row + row) * HD + col0 + c + 4 * e), y);
+                            __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)row * HD + e), y[k]);
                     }
                 }
             if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
