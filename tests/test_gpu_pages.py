@@ -151,6 +151,21 @@ def test_tree_strides_layers_and_scales(backend):
     run_tree(made, 4, [30, 60], [10, 5], layer=2, scale=1e-6)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,drafts,order", [(4, 2, 1), (4, 16, 1), (4, 64, 1), (8, 40, -1), (2, 20, -1)])
+def test_tree_scores_that_grow_and_shrink_by_powers_of_two(backend, kind, dim, group, drafts, order):
+    """Keys twice (or half) as large every 64 positions: every step has a new maximum, far above the last one, for half of the rows at least."""
+    ctx = [64 * 12 + 5, 64 * 9]
+    made = Made(backend, kind, 2, dim, [c + drafts for c in ctx], seed=drafts + dim)
+    for s, c in enumerate(ctx):
+        for x in range(c + drafts):
+            page, slot, f = made.tables[s, x // PAGE], x % PAGE, 2.0 ** (min(order * (x // 64), 12) - (6 if order > 0 else -5))
+            made.kd[0, page, :, slot] *= f
+    made.k = float64(made.kd[0])  # (the smallest f16 keys have lost bits)
+    run_tree(made, group, ctx, [drafts] * 2)
+
+
 def test_tree_tokens_that_see_nothing_are_zero_and_others_do_not_notice(backend):
     made = Made(backend, "f16", 2, 64, [3, 20 + 4], seed=5)
     run_tree(made, 2, [0, 20], [3, 4], bits=[0, 0b111, 0b100, 0, 0b1111, 0b1, 0b1000])
