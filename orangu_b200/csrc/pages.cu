@@ -455,7 +455,7 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     use_workspace(p, a);
     if (max_drafts * a.group > PG_FEW_ROWS) {
         // (the walk over all pieces counts their tiles, and PG_START more for each, in 31 bits)
-        if ((uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + 7) / 8 + PG_START) * ((max_drafts * a.group + 127) / 128) >= (1ull << 31))
+        if ((uint64_t)n_seq * p->d.n_head_kv * (((uint64_t)p->d.table_stride + PG_PAGES - 1) / PG_PAGES + PG_START) * ((max_drafts * a.group + 127) / 128) >= (1ull << 31))
             return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tree: the tables of all sequences together have room for too many positions");
         return launched(p, who, launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, stream_of(p, stream)), 2);
     }

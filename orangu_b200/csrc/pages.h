@@ -12,7 +12,8 @@ namespace ob {
 constexpr uint32_t PG_MAX_DRAFTS = 64;   // drafted tokens of a sequence: a bit each
 constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
 constexpr uint32_t PG_FEW_ROWS = 16;     // drafted tokens times heads of a key/value head: up to here mma.sync tiles, above tcgen05 tiles
-constexpr uint32_t PG_START = 3;         // tcgen05: what the start and end of a piece cost, in tiles
+constexpr uint32_t PG_PAGES = 4;         // pages of a tile of the tcgen05 kernel
+constexpr uint32_t PG_START = 6;         // what the start and end of a piece cost there, in tiles
 constexpr size_t PG_WORKSPACE = 64u << 20;  // partial results of the splits, behind the counters
 constexpr uint32_t PG_COUNTERS = 4096;   // arrival counters, zero between launches
 struct alignas(32) PagePiece {  // rows whose parts several CTAs have left (pages_tc5.cu), for the kernel that adds them up

@@ -36,19 +36,21 @@ namespace ob {
 
 namespace {
 
-constexpr uint32_t PG_ROWS = 128, PG_KEYS = 128, PG_PAGES = PG_KEYS / KV_PAGE, PG_BLOCK = PG_KEYS * 128;  // block: 128 rows of 64 columns
+constexpr uint32_t PG_ROWS = 128, PG_KEYS = PG_PAGES * KV_PAGE, PG_BLOCK = PG_KEYS * 128, PG_QBLOCK = PG_ROWS * 128;  // a tile's positions; blocks of 64 columns
 constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 11 * 32;
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
-constexpr uint32_t PG_LEAST = 2;        // tiles of a CTA: one for each stream
+constexpr uint32_t PG_LEAST = 4;        // units of a CTA
 
 // mbarriers and small arrays, byte offsets
-constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = 48, PB_V_FULL = 96, PB_V_EMPTY = 144, PB_S_FULL = 192 /* [stream][place] */, PB_P_FULL = 224, PB_PV_DONE = 256, PB_O_FULL = 272, PB_Q_FULL = 288,
-                   PB_SLOT = 296, PB_ABORT = 300, PB_ODD = 304, PB_TOP = 312, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
+constexpr uint32_t PG_STAGES = 12;      // at most
+constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = PB_K_FULL + 8 * PG_STAGES, PB_V_FULL = PB_K_EMPTY + 8 * PG_STAGES, PB_V_EMPTY = PB_V_FULL + 8 * PG_STAGES, PB_S_FULL = PB_V_EMPTY + 8 * PG_STAGES /* [stream][place] */,
+                   PB_P_FULL = PB_S_FULL + 32, PB_PV_DONE = PB_P_FULL + 32, PB_O_FULL = PB_PV_DONE + 16, PB_Q_FULL = PB_O_FULL + 16, PB_SLOT = PB_Q_FULL + 8, PB_ABORT = PB_SLOT + 4, PB_ODD = PB_ABORT + 4,
+                   PB_TOP = PB_ODD + 8, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
 template <int HD, bool WIDE>
 struct PgPlan {
-    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, Q = (WIDE ? 2 : 1) * OPERAND;  // (16 KB at least: outputs leave by way of it)
-    static constexpr uint32_t FIT = (227 * 1024 - PB_BYTES - Q) / (2 * OPERAND), STAGES = FIT < 6 ? FIT : 6;
+    static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, ROWS = NB * PG_QBLOCK, Q = (WIDE ? 2 : 1) * ROWS;  // (16 KB at least: outputs leave by way of it)
+    static constexpr uint32_t FIT = (227 * 1024 - PB_BYTES - Q) / (2 * OPERAND), STAGES = FIT < PG_STAGES ? FIT : PG_STAGES;
     static constexpr uint32_t K = Q, V = K + STAGES * OPERAND, BAR = V + STAGES * OPERAND, BYTES = BAR + PB_BYTES;
     static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
     static constexpr uint64_t PART = (uint64_t)MR * (HD + 2);  // floats of a partial result
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1)
 pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
     using P = PgPlan<HD, WIDE>;
     constexpr bool REMAINDER = EXPONENT16<T> == 0x7f80u;
-    constexpr uint32_t ST = P::STAGES, OPERAND = P::OPERAND, NB = P::NB, MR = P::MR;
+    constexpr uint32_t ST = P::STAGES, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem);
     const uint32_t bar = sbase + P::BAR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -220,10 +222,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_SLOT);
     PgWalk<MR> w;
     w.start(a);
-    // Steps of a stream in a piece: two for each of its tiles, which are all of them or every other one.  With two tiles of rows the second
-    // stream may have no rows.
-    auto steps_of = [&](uint32_t s, uint32_t tiles, uint32_t rows) { return WIDE ? (s == 0 || rows > PG_ROWS ? 2 * tiles : 0u) : (tiles + 1 - s) / 2 * 2; };
-    auto tile_of = [&](uint32_t s, uint32_t step) { return WIDE ? step / 2 : s + step / 2 * 2; };
+    // Tiles of a stream in a piece: all of them or every other one.  With two tiles of rows the second stream may have no rows.
+    auto steps_of = [&](uint32_t s, uint32_t tiles, uint32_t rows) { return WIDE ? (s == 0 || rows > PG_ROWS ? tiles : 0u) : (tiles + 1 - s) / 2; };
+    auto tile_of = [&](uint32_t s, uint32_t step) { return WIDE ? step : s + 2 * step; };
 
     if (warp == PG_TMA_WARP) {
         uint32_t n = 0;  // tiles so far
@@ -232,8 +233,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         for (; w.more() && ok; w.next(a)) {
             const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
             const uint32_t end = w.last();
-            auto row_of = [&](uint32_t tile) {  // lanes 0-7: the first row of a page of the tile
-                const uint32_t p = tile * PG_PAGES + (lane & 7);
+            const uint32_t page = lane % PG_PAGES, box = lane / PG_PAGES, at = box * PG_BLOCK + page * (KV_PAGE * 128);  // a lane a copy
+            auto row_of = [&](uint32_t tile) {  // the first row of the lane's page of the tile
+                const uint32_t p = tile * PG_PAGES + page;
                 const int32_t id = tile < end && p < w.q.n_pages ? table[p] : -1;
                 return (uint32_t)id < a.pg.n_pages ? ((uint32_t)id * a.pg.n_kv + w.head) * KV_PAGE : nowhere;
             };
@@ -243,54 +245,45 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 if (n >= ST && !(ok = mbar_wait_warp(bar + PB_K_EMPTY + 8 * st, par, abort))) break;
                 if (lane == 0) mbar_expect_tx(bar + PB_K_FULL + 8 * st, OPERAND);
                 __syncwarp();
-                if (lane < PG_PAGES)
-                    for (uint32_t b = 0; b < NB; ++b)
-                        tma_load_2d(sbase + P::K + st * OPERAND + b * PG_BLOCK + lane * (KV_PAGE * 128), &tm_k, (int32_t)(b * 64), (int32_t)y, bar + PB_K_FULL + 8 * st);
+                if (box < NB) tma_load_2d(sbase + P::K + st * OPERAND + at, &tm_k, (int32_t)(box * 64), (int32_t)y, bar + PB_K_FULL + 8 * st);
                 __syncwarp();
                 if (n >= ST && !(ok = mbar_wait_warp(bar + PB_V_EMPTY + 8 * st, par, abort))) break;
                 if (lane == 0) mbar_expect_tx(bar + PB_V_FULL + 8 * st, OPERAND);
                 __syncwarp();
-                if (lane < PG_PAGES)
-                    for (uint32_t b = 0; b < NB; ++b)
-                        tma_load_2d(sbase + P::V + st * OPERAND + b * PG_BLOCK + lane * (KV_PAGE * 128), &tm_v, (int32_t)(b * 64), (int32_t)y, bar + PB_V_FULL + 8 * st);
+                if (box < NB) tma_load_2d(sbase + P::V + st * OPERAND + at, &tm_v, (int32_t)(box * 64), (int32_t)y, bar + PB_V_FULL + 8 * st);
                 __syncwarp();
                 y = next;
             }
         }
     } else if (warp >= PG_MMA_WARP) {
         constexpr uint32_t F16 = REMAINDER ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
-        const uint32_t id_s = umma_idesc_bf16(PG_KEYS / 2) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
-        const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
-        uint32_t n = 0, turn = 0, done = 0;  // tiles and pieces so far, steps of the stream so far
+        const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
+        const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
+        uint32_t n = 0, turn = 0, done = 0;  // tiles, pieces and tiles of the stream so far
         bool ok = true;
-        const uint64_t q_desc = umma_desc_sw128(sbase + (WIDE ? s * OPERAND : 0u)), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
+        const uint64_t q_desc = umma_desc_sw128(sbase + (WIDE ? s * ROWS : 0u)), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
         for (; w.more() && ok; w.next(a), ++turn) {
             const uint32_t tiles = w.last() - w.tile, steps = steps_of(s, tiles, w.q.drafts * a.group - w.rt * MR);
-            if (WIDE && steps == 0) {  // no rows: only says of every tile that it does not need it
+            ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);  // (of every piece: a phase that is not waited for could be taken for the next one)
+            if (WIDE && steps == 0)  // no rows: only says of every tile that it does not need it
                 for (uint32_t i = 0; i < tiles && ok; ++i) {
                     const uint32_t st = (n + i) % ST, par = ((n + i) / ST) & 1u;
                     ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, par, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, par, abort);
                     if (ok && lane == 0) mbar_arrive(bar + PB_K_EMPTY + 8 * st), mbar_arrive(bar + PB_V_EMPTY + 8 * st);
                     __syncwarp();
                 }
-                n += tiles;
-                continue;
-            }
-            ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);
 #pragma unroll 1
             for (int step = -2; step < (int)steps && ok; ++step) {  // -2, -1: only the first scores
-                const uint32_t half = step & 1;
+                const uint32_t place = (done + step) & 1u;
                 if (step >= 0) {
                     const uint32_t at = n + tile_of(s, step), st = at % ST;
-                    ok = mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * half, done >> 1 & 1u, abort);
-                    ++done;
-                    if (ok && half == 0) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / ST) & 1u, abort);
+                    ok = mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * place, (done + step) >> 1 & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / ST) & 1u, abort);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t p = ts + half * 64;
-                    const uint64_t vd = v_desc + (st * OPERAND >> 4) + half * 4 * 128;
+                    const uint32_t p = ts + place * PG_KEYS;
+                    const uint64_t vd = v_desc + (st * OPERAND >> 4);
 #pragma unroll
-                    for (uint32_t kk = 0; kk < PG_KEYS / 32; ++kk) {  // the stream's first product writes, the others add
+                    for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add
                         if (REMAINDER) {  // 16 positions: eight columns of values, eight of remainders
                             umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
                             umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
@@ -299,33 +292,31 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         }
                     }
                     umma_commit_warp(bar + PB_PV_DONE + 8 * s);
-                    if (half) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
+                    umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
                 }
                 const uint32_t next = step + 2;
                 if (next < steps) {
                     const uint32_t at = n + tile_of(s, next), st = at % ST;
-                    if (half == 0) {
-                        ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / ST) & 1u, abort);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    const uint64_t kd = k_desc + ((st * OPERAND + half * (PG_BLOCK / 2)) >> 4);
+                    ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / ST) & 1u, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t kd = k_desc + (st * OPERAND >> 4);
 #pragma unroll
                     for (uint32_t b = 0; b < HD / 16; ++b)
-                        umma_bf16_warp(ts + half * 64, q_desc + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
-                    umma_commit_warp(bar + PB_S_FULL + 16 * s + 8 * half);
-                    if (half) umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
-                } else if (half) {
+                        umma_bf16_warp(ts + place * PG_KEYS, q_desc + (b / 4) * (PG_QBLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
+                    umma_commit_warp(bar + PB_S_FULL + 16 * s + 8 * place);
+                    umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
+                } else if (next == steps + 1 && steps > 0) {
                     umma_commit_warp(bar + PB_O_FULL + 8 * s);
                 }
             }
-            n += tiles;
+            n += tiles, done += steps;
         }
     } else if (warp < PG_MMA_WARP) {
         const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
         const uint32_t magic = (65536 + a.group - 1) / a.group;  // x / group = x magic / 65536 for x below 4096, group up to 16
         const float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
-        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * PG_KEYS, to = lanes + PG_TMEM_O;
+        const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * 2 * PG_KEYS, to = lanes + PG_TMEM_O;
         volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][sum, maximum][row]
         volatile uint32_t *odd = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD);
         bool ok = true;
@@ -351,7 +342,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 #pragma unroll
                 for (uint32_t k = 0; k < BATCH; ++k) {
                     const uint32_t i = (t + k) * PG_SOFT + threadIdx.x, row = i / WORDS, c = i % WORDS;
-                    *reinterpret_cast<uint4 *>(smem + row / PG_ROWS * OPERAND + c / 8 * PG_BLOCK + row % PG_ROWS * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[k];
+                    *reinterpret_cast<uint4 *>(smem + row / PG_ROWS * ROWS + c / 8 * PG_QBLOCK + row % PG_ROWS * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[k];
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -363,26 +354,22 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 seen = a.visible[w.q.row0 + (w.rt * MR + f_row) / a.group];
                 if (w.q.limit - w.q.ctx < 64) seen &= (1ull << (w.q.limit - w.q.ctx)) - 1;
             }
-            auto pages_of = [&](uint32_t tile) {  // lanes 0-7: whether a page of the tile is there
-                const uint32_t p = tile * PG_PAGES + (lane & 7);
+            auto pages_of = [&](uint32_t tile) {  // whether the lane's page of the tile is there
+                const uint32_t p = tile * PG_PAGES + lane % PG_PAGES;
                 return tile < end && p < w.q.n_pages && (uint32_t)table[p] < a.pg.n_pages;
             };
             // ---- the tiles
             const uint32_t steps = steps_of(s, tiles, n_rows);
             float m = -INFINITY, l = 0.0f;
             bool there = pages_of(w.tile + tile_of(s, 0));
-            uint32_t valid = 0;
             for (uint32_t step = 0; step < steps; ++step, ++used) {
-                const uint32_t i = tile_of(s, step), half = step & 1, x0 = (w.tile + i) * PG_KEYS;
+                const uint32_t i = tile_of(s, step), place = used & 1, x0 = (w.tile + i) * PG_KEYS, valid = __ballot_sync(0xffffffffu, there) & ((1u << PG_PAGES) - 1);
                 const bool past = x0 + PG_KEYS > w.q.ctx;
-                ok = ok && mbar_wait_warp(bar + PB_S_FULL + 16 * s + 8 * half, used >> 1 & 1u, abort);
-                if (half == 0) {
-                    valid = __ballot_sync(0xffffffffu, there) & 0xffu;
-                    there = pages_of(w.tile + tile_of(s, step + 2));
-                    if (ok && past) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
-                }
+                there = pages_of(w.tile + tile_of(s, step + 1));
+                ok = ok && mbar_wait_warp(bar + PB_S_FULL + 16 * s + 8 * place, used >> 1 & 1u, abort);
+                if (ok && past) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
                 if (!ok) break;  // a wait was given up: nothing more is computed
-                if (half == 0 && past) {  // values of positions past the context
+                if (past) {  // values of positions past the context
                     uint8_t *v = smem + P::V + (n + i) % ST * OPERAND;
                     const uint32_t from = w.q.ctx > x0 ? w.q.ctx - x0 : 0u;
                     bool bad = false;
@@ -408,22 +395,21 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 if (warm) {
-                    const uint32_t tp = ts + half * 64;
+                    const uint32_t tp = ts + place * PG_KEYS;
                     tc_fence_after();
                     uint32_t u[2][32];
                     tmem_ld32(tp, u[0]);
                     tmem_ld32(tp + 32, u[1]);
                     tmem_ld_wait();
-                    if (valid != 0xffu || past) {
-                        const uint32_t k0 = x0 + half * 64;  // the step's first position
-                        uint64_t bits = k0 >= w.q.ctx ? 0ull : w.q.ctx - k0 >= 64 ? ~0ull : (1ull << (w.q.ctx - k0)) - 1;  // what the row sees: context,
-                        if (k0 + 64 > w.q.ctx) {                                                                          // drafted token j at ctx + j
-                            const int shift = (int)(w.q.ctx - k0);  // above -64 where any of them is here
+                    if (valid != (1u << PG_PAGES) - 1 || past) {
+                        uint64_t bits = x0 >= w.q.ctx ? 0ull : w.q.ctx - x0 >= 64 ? ~0ull : (1ull << (w.q.ctx - x0)) - 1;  // what the row sees: context,
+                        if (past) {                                                                                       // drafted token j at ctx + j
+                            const int shift = (int)(w.q.ctx - x0);  // above -64 where any of them is here
                             bits |= shift >= 0 ? seen << shift : shift > -64 ? seen >> -shift : 0ull;
                         }
 #pragma unroll
                         for (int p = 0; p < 4; ++p)
-                            if (!(valid >> (half * 4 + p) & 1)) bits &= ~(0xffffull << (16 * p));
+                            if (!(valid >> p & 1)) bits &= ~(0xffffull << (16 * p));
 #pragma unroll
                         for (int e = 0; e < 64; ++e)
                             if (!(bits >> e & 1)) u[e / 32][e % 32] = 0xff800000u;
@@ -485,7 +471,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar + PB_P_FULL + 16 * s + 8 * half);
+                if (lane == 0) mbar_arrive(bar + PB_P_FULL + 16 * s + 8 * place);
             }
             n += tiles;
             // ---- the piece is done: the streams' outputs and sums

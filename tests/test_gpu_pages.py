@@ -235,6 +235,17 @@ def test_tree_of_many_sequences(backend, group, dim):
     run_tree(made, group, ctx, drafts)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_tree_short_pieces_with_and_without_rows_for_the_second_stream(backend, kind, dim):
+    """Up to 512 rows a head in the call, but many sequences with 128 or fewer and contexts of a few tiles, several of them after one another in a CTA."""
+    drafts = [64, 1, 16, 17, 2, 33, 48, 49, 0, 8] * 5
+    ctx = [(37 * i) % 190 for i in range(len(drafts))]
+    made = Made(backend, kind, 8, dim, [c + d for c, d in zip(ctx, drafts)], seed=dim)
+    for _ in range(3):
+        run_tree(made, 8, ctx, drafts)
+
+
 def test_handles_come_and_go(backend):
     """A handle's workspace is used again by later ones: in the state that a new one has."""
     import torch
@@ -837,7 +848,7 @@ def test_refusals(backend):
 
 
 def test_a_walk_of_more_than_31_bits_is_refused(backend):
-    """Every (rows, sequence, head) piece counts as its tiles and three more: 2^22 sequences of one tile of 64 heads, in four tiles of 128 rows, are 2^32."""
+    """Every (rows, sequence, head) piece counts as its tiles and six more: 2^22 sequences of one tile of 64 heads, in four tiles of 128 rows, are 7 2^30."""
     import torch
 
     from orangu_b200 import OranguError, PagedCache
