@@ -1,7 +1,7 @@
 // Attention of drafted tokens on the fifth-generation tensor cores: the form of ob_pages_attention_tree for more rows (drafted token, query
 // head) a key/value head than the mma.sync kernel of pages_attention.cu keeps up with.  The mathematics is the same.
 //
-// The tiles of 128 positions of all (rows, sequence, key/value head) pieces are laid end to end and shared out evenly: every SM has one CTA with
+// The tiles of 64 positions of all (rows, sequence, key/value head) pieces are laid end to end and shared out evenly: every SM has one CTA with
 // the same number of tiles, whatever the lengths of the contexts, and walks through the pieces that lie in its part.  A piece that
 // is cut leaves (maximum, sum, output) in fp32, and a second kernel, launched along, adds them up over all SMs (the last of a piece's
 // CTAs to arrive doing it alone took as long as all the rest: 181 us for 8 x 64 tokens of 4 heads a key/value head at 8192).
@@ -9,18 +9,20 @@
 //   warps 0-7  softmax: four warps per stream, a thread per row.  Scores come from tensor memory, weights go back into the same
 //              columns: f16, or bf16 as value plus remainder.
 //   warps 8, 9 issue the products of a stream each: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
-//   warp 10    issues the TMA loads of pages, 16 rows x 64 columns each, straight from the cache into the swizzled operand tiles
+//   warps 10, 11 issue the TMA loads of keys and of values, pages of 16 rows x 64 columns each, straight from the cache into the swizzled operand
+//              tiles, each into a ring of its own
 //
 // There are two streams of scores.  Up to 128 rows (WIDE false) they are the even and the odd tiles of the same rows, with an output each;
-// above that they are two tiles of 128 rows that share keys and values.  A stream goes in steps of half a tile through two places for
-// scores: while one's weights are made, the other's are multiplied and its next scores come.  Whole tiles with one place a stream, 16 softmax
-// warps and one that issued all products took 25.6 us for one sequence of 512 positions and 48 rows a key/value head and 52 us for
-// eight of 4096 and 64, now 19.5 and 48; 300 to 320 us for four of 32,000 and 256 rows, as now.
+// above that they are two tiles of 128 rows that share keys and values.  A stream has two places for scores: while one's weights
+// are made, the other's are multiplied and its next scores come.  Tiles of 128 positions with one place a stream, 16 softmax warps and one that
+// issued all products took 25.6 us for one sequence of 512 positions and 48 rows a key/value head, 52 us for eight of 4096 and 64, now 17.4
+// and 43 to 46; with keys and values through one ring, in order, 32 sequences of 8192 with 128 rows took 218 to 233 us, now 200 (keys are wanted two
+// steps before their values: of one order only the values were ahead).
 //
-// What bounds it (head dimension 128): up to 128 rows the bytes, 208 us for 32 sequences of 8192 with 64 rows (floor 166, 5.2 TB/s).  Above, the
+// What bounds it (head dimension 128): up to 128 rows the bytes, 200 us for 32 sequences of 8192 with 128 rows (floor 167, 5.4 TB/s).  Above, the
 // chain of a step: 2080 clocks for two warps' 64 positions, of which the special function unit works 40 % and the tensor cores 40 %
-// (605 us for 32 sequences of 8192 with 512 rows, 0.9 PFLOP/s; floor 335).  A part of the powers of two on the fused multiply-adds,
-// 1/8 to 1/2 of them, took from 2 % less to 6 % more.
+// (613 us for 32 sequences of 8192 with 512 rows, 0.9 PFLOP/s; floor 335; without the weights 488, without the products 495).  A part of the
+// powers of two on the fused multiply-adds, 1/8 to 1/2 of them, took from 2 % less to 6 % more.
 //
 // Context positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
 // per thread.  There, values of positions that nobody has, or that are no numbers, are set to zero in shared memory (0 times them
@@ -37,7 +39,7 @@ namespace ob {
 namespace {
 
 constexpr uint32_t PG_ROWS = 128, PG_KEYS = PG_PAGES * KV_PAGE, PG_BLOCK = PG_KEYS * 128, PG_QBLOCK = PG_ROWS * 128;  // a tile's positions; blocks of 64 columns
-constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 11 * 32;
+constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 12 * 32;
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
 constexpr uint32_t PG_LEAST = 4;        // units of a CTA
@@ -50,11 +52,16 @@ constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = PB_K_FULL + 8 * PG_STAGES, PB_V_F
 template <int HD, bool WIDE>
 struct PgPlan {
     static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, ROWS = NB * PG_QBLOCK, Q = (WIDE ? 2 : 1) * ROWS;  // (16 KB at least: outputs leave by way of it)
-    static constexpr uint32_t FIT = (227 * 1024 - PB_BYTES - Q) / (2 * OPERAND), STAGES = FIT < PG_STAGES ? FIT : PG_STAGES;
-    static constexpr uint32_t K = Q, V = K + STAGES * OPERAND, BAR = V + STAGES * OPERAND, BYTES = BAR + PB_BYTES;
+    // Places of the two rings.  Values are wanted two steps after their keys: they get more.  Where the streams take every other tile, the numbers are
+    // even, so that a place is always the same stream's within a piece: waits go by the parity of a phase, and a stream that runs ahead must not ask
+    // for a place's next tile before the one before, the other stream's, has arrived.
+    // Where both streams take all tiles, two share a place: half the waits (32 sequences of 8192 with 512 rows, bf16: 720 us, and 773 with a place a tile).
+    static constexpr uint32_t G = WIDE ? 2 : 1, PLACE = G * OPERAND, FIT = (227 * 1024 - PB_BYTES - Q) / PLACE, EVEN = WIDE ? 1 : 2;
+    static constexpr uint32_t KST = std::min(FIT / 3 / EVEN * EVEN + WIDE, PG_STAGES), VST = std::min((FIT - KST) / EVEN * EVEN, PG_STAGES);
+    static constexpr uint32_t K = Q, V = K + KST * PLACE, BAR = V + VST * PLACE, BYTES = BAR + PB_BYTES;
     static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
     static constexpr uint64_t PART = (uint64_t)MR * (HD + 2);  // floats of a partial result
-    static_assert(STAGES >= 2 && BYTES <= 227 * 1024, "shared memory");
+    static_assert(KST >= 2 && VST >= 3 && PG_STAGES % 2 == 0 && (WIDE || (KST % 2 == 0 && VST % 2 == 0)) && BYTES <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b, float c) {
@@ -187,13 +194,13 @@ __global__ void __launch_bounds__(PG_THREADS, 1)
 pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
     using P = PgPlan<HD, WIDE>;
     constexpr bool REMAINDER = EXPONENT16<T> == 0x7f80u;
-    constexpr uint32_t ST = P::STAGES, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
+    constexpr uint32_t KST = P::KST, VST = P::VST, G = P::G, PLACE = P::PLACE, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem);
     const uint32_t bar = sbase + P::BAR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ABORT);
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < ST; ++s) {
+        for (uint32_t s = 0; s < PG_STAGES; ++s) {
             mbar_init(bar + PB_K_FULL + 8 * s, 1);
             mbar_init(bar + PB_K_EMPTY + 8 * s, WIDE ? 2 : 1);  // the streams that read a tile
             mbar_init(bar + PB_V_FULL + 8 * s, 1);
@@ -226,62 +233,62 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     auto steps_of = [&](uint32_t s, uint32_t tiles, uint32_t rows) { return WIDE ? (s == 0 || rows > PG_ROWS ? tiles : 0u) : (tiles + 1 - s) / 2; };
     auto tile_of = [&](uint32_t s, uint32_t step) { return WIDE ? step : s + 2 * step; };
 
-    if (warp == PG_TMA_WARP) {
-        uint32_t n = 0;  // tiles so far
+    if (warp >= PG_TMA_WARP) {
+        const bool values = warp > PG_TMA_WARP;
+        const CUtensorMap *map = values ? &tm_v : &tm_k;
+        const uint32_t ring = sbase + (values ? P::V : P::K), full = bar + (values ? PB_V_FULL : PB_K_FULL), empty = bar + (values ? PB_V_EMPTY : PB_K_EMPTY), places = values ? VST : KST;
+        uint32_t st = 0, par = 1;  // the tile's place, and the parity of its last use: a place that was not used yet is empty
         bool ok = true;
         const uint32_t nowhere = a.pg.n_pages * a.pg.n_kv * KV_PAGE;  // the row behind the pool: reads as zero
+        const uint32_t page = lane % (G * PG_PAGES), box = lane / (G * PG_PAGES), at = page / PG_PAGES * OPERAND + box * PG_BLOCK + page % PG_PAGES * (KV_PAGE * 128);  // a lane a copy
         for (; w.more() && ok; w.next(a)) {
             const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
             const uint32_t end = w.last();
-            const uint32_t page = lane % PG_PAGES, box = lane / PG_PAGES, at = box * PG_BLOCK + page * (KV_PAGE * 128);  // a lane a copy
-            auto row_of = [&](uint32_t tile) {  // the first row of the lane's page of the tile
+            auto row_of = [&](uint32_t tile) {  // the first row of the lane's page of the tiles from this one on
                 const uint32_t p = tile * PG_PAGES + page;
-                const int32_t id = tile < end && p < w.q.n_pages ? table[p] : -1;
+                const int32_t id = p < min(end * PG_PAGES, w.q.n_pages) ? table[p] : -1;
                 return (uint32_t)id < a.pg.n_pages ? ((uint32_t)id * a.pg.n_kv + w.head) * KV_PAGE : nowhere;
             };
             uint32_t y = row_of(w.tile);
-            for (uint32_t i = w.tile; i < end && ok; ++i, ++n) {
-                const uint32_t next = row_of(i + 1), st = n % ST, par = ((n / ST) & 1u) ^ 1u;
-                if (n >= ST && !(ok = mbar_wait_warp(bar + PB_K_EMPTY + 8 * st, par, abort))) break;
-                if (lane == 0) mbar_expect_tx(bar + PB_K_FULL + 8 * st, OPERAND);
+            for (uint32_t i = w.tile; i < end; i += G) {
+                const uint32_t next = row_of(i + G);
+                if (!(ok = mbar_wait_warp(empty + 8 * st, par, abort))) break;
+                if (lane == 0) mbar_expect_tx(full + 8 * st, PLACE);
                 __syncwarp();
-                if (box < NB) tma_load_2d(sbase + P::K + st * OPERAND + at, &tm_k, (int32_t)(box * 64), (int32_t)y, bar + PB_K_FULL + 8 * st);
-                __syncwarp();
-                if (n >= ST && !(ok = mbar_wait_warp(bar + PB_V_EMPTY + 8 * st, par, abort))) break;
-                if (lane == 0) mbar_expect_tx(bar + PB_V_FULL + 8 * st, OPERAND);
-                __syncwarp();
-                if (box < NB) tma_load_2d(sbase + P::V + st * OPERAND + at, &tm_v, (int32_t)(box * 64), (int32_t)y, bar + PB_V_FULL + 8 * st);
+                if (box < NB) tma_load_2d(ring + st * PLACE + at, map, (int32_t)(box * 64), (int32_t)y, full + 8 * st);
                 __syncwarp();
                 y = next;
+                if (++st == places) st = 0, par ^= 1;
             }
         }
     } else if (warp >= PG_MMA_WARP) {
         constexpr uint32_t F16 = REMAINDER ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
         const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
         const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
-        uint32_t n = 0, turn = 0, done = 0;  // tiles, pieces and tiles of the stream so far
+        uint32_t n = 0, turn = 0, done = 0;  // places, pieces and tiles of the stream so far
         bool ok = true;
         const uint64_t q_desc = umma_desc_sw128(sbase + (WIDE ? s * ROWS : 0u)), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
         for (; w.more() && ok; w.next(a), ++turn) {
             const uint32_t tiles = w.last() - w.tile, steps = steps_of(s, tiles, w.q.drafts * a.group - w.rt * MR);
             ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);  // (of every piece: a phase that is not waited for could be taken for the next one)
             if (WIDE && steps == 0)  // no rows: only says of every tile that it does not need it
-                for (uint32_t i = 0; i < tiles && ok; ++i) {
-                    const uint32_t st = (n + i) % ST, par = ((n + i) / ST) & 1u;
-                    ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, par, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, par, abort);
-                    if (ok && lane == 0) mbar_arrive(bar + PB_K_EMPTY + 8 * st), mbar_arrive(bar + PB_V_EMPTY + 8 * st);
+                for (uint32_t i = 0; i < (tiles + G - 1) / G && ok; ++i) {
+                    const uint32_t kt = (n + i) % KST, vt = (n + i) % VST;
+                    ok = mbar_wait_warp(bar + PB_K_FULL + 8 * kt, ((n + i) / KST) & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * vt, ((n + i) / VST) & 1u, abort);
+                    if (ok && lane == 0) mbar_arrive(bar + PB_K_EMPTY + 8 * kt), mbar_arrive(bar + PB_V_EMPTY + 8 * vt);
                     __syncwarp();
                 }
 #pragma unroll 1
             for (int step = -2; step < (int)steps && ok; ++step) {  // -2, -1: only the first scores
                 const uint32_t place = (done + step) & 1u;
                 if (step >= 0) {
-                    const uint32_t at = n + tile_of(s, step), st = at % ST;
-                    ok = mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * place, (done + step) >> 1 & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / ST) & 1u, abort);
+                    const uint32_t i = tile_of(s, step), at = n + i / G, st = at % VST;
+                    if (i % G == 0) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / VST) & 1u, abort);
+                    ok = ok && mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * place, (done + step) >> 1 & 1u, abort);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t p = ts + place * PG_KEYS;
-                    const uint64_t vd = v_desc + (st * OPERAND >> 4);
+                    const uint64_t vd = v_desc + ((st * PLACE + i % G * OPERAND) >> 4);
 #pragma unroll
                     for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add
                         if (REMAINDER) {  // 16 positions: eight columns of values, eight of remainders
@@ -292,25 +299,25 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         }
                     }
                     umma_commit_warp(bar + PB_PV_DONE + 8 * s);
-                    umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
+                    if (i % G == G - 1 || step + 1 == (int)steps) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
                 }
                 const uint32_t next = step + 2;
                 if (next < steps) {
-                    const uint32_t at = n + tile_of(s, next), st = at % ST;
-                    ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / ST) & 1u, abort);
+                    const uint32_t i = tile_of(s, next), at = n + i / G, st = at % KST;
+                    if (i % G == 0) ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / KST) & 1u, abort);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t kd = k_desc + (st * OPERAND >> 4);
+                    const uint64_t kd = k_desc + ((st * PLACE + i % G * OPERAND) >> 4);
 #pragma unroll
                     for (uint32_t b = 0; b < HD / 16; ++b)
                         umma_bf16_warp(ts + place * PG_KEYS, q_desc + (b / 4) * (PG_QBLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
                     umma_commit_warp(bar + PB_S_FULL + 16 * s + 8 * place);
-                    umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
+                    if (i % G == G - 1 || next + 1 == steps) umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
                 } else if (next == steps + 1 && steps > 0) {
                     umma_commit_warp(bar + PB_O_FULL + 8 * s);
                 }
             }
-            n += tiles, done += steps;
+            n += (tiles + G - 1) / G, done += steps;
         }
     } else if (warp < PG_MMA_WARP) {
         const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
@@ -320,7 +327,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][sum, maximum][row]
         volatile uint32_t *odd = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD);
         bool ok = true;
-        uint32_t used = 0, n = 0;   // steps of the stream, tiles of the CTA so far
+        uint32_t used = 0, n = 0;   // tiles of the stream, places so far
         bool said = false;          // a piece that others go on with has been written down
         uint32_t both[2] = {0, 0};  // pieces with tiles of either stream (WIDE false: every warp reads both outputs)
         for (; w.more(); w.next(a)) {
@@ -367,10 +374,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 const bool past = x0 + PG_KEYS > w.q.ctx;
                 there = pages_of(w.tile + tile_of(s, step + 1));
                 ok = ok && mbar_wait_warp(bar + PB_S_FULL + 16 * s + 8 * place, used >> 1 & 1u, abort);
-                if (ok && past) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i) % ST), ((n + i) / ST) & 1u, abort);
+                if (ok && past) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * ((n + i / G) % VST), ((n + i / G) / VST) & 1u, abort);
                 if (!ok) break;  // a wait was given up: nothing more is computed
                 if (past) {  // values of positions past the context
-                    uint8_t *v = smem + P::V + (n + i) % ST * OPERAND;
+                    uint8_t *v = smem + P::V + (n + i / G) % VST * PLACE + i % G * OPERAND;
                     const uint32_t from = w.q.ctx > x0 ? w.q.ctx - x0 : 0u;
                     bool bad = false;
 #pragma unroll 1
@@ -473,7 +480,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar + PB_P_FULL + 16 * s + 8 * place);
             }
-            n += tiles;
+            n += (tiles + G - 1) / G;
             // ---- the piece is done: the streams' outputs and sums
             const bool had[2] = {true, WIDE ? n_rows > PG_ROWS : tiles > 1};
 #pragma unroll
