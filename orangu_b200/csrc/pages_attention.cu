@@ -10,7 +10,7 @@
 // The sum of the weights is one more product, with ones, of the same rounded weights.
 //
 // The pages of all (sequence, key/value head) pieces, laid end to end, are shared out evenly over the CTAs, whatever the lengths; a CTA walks
-// through the pieces that lie in its part.  A piece that is cut leaves (m, sum, output) in fp32 and the last of its CTAs to arrive -- a
+// through the pieces that lie in its part, or has a part of one piece only where there are CTAs enough for that.  A piece that is cut leaves (m, sum, output) in fp32 and the last of its CTAs to arrive -- a
 // counter tells, which goes back to zero by itself -- adds the parts up in order, so the result does not depend on who was last.
 #include <algorithm>
 #include <type_traits>
@@ -60,7 +60,11 @@ struct PaShape {
     static_assert(PA_WARPS * PA_ROWS * (PITCH + 2) * 4 <= RINGS, "the warps' results meet in the rings");
 };
 
-constexpr uint32_t PA_LEAST = 2 * PA_WARPS;  // pages of a CTA
+// Pages of a CTA.  Adding up the parts of a piece of n pages takes as long as some of them, so that there are not many more parts than the
+// square root of n; and a piece that begins in the middle of a CTA's share costs that CTA a second start and end, so that shares are up to
+// 1 / PA_MORE larger where no piece has to.  One sequence, 16 rows of 128, in a graph: 14.2 -> 9.9 us of 512 positions, 17.8 -> 13.3 of 2048,
+// 26.2 -> 20.6 of 8192; 8 sequences of 2048 21.7 -> 18.2 us.  (Half of it for lists, whose rows are few: 128 pages 8.5 us, 9.2 without the half.)
+constexpr uint32_t PA_LEAST = 2 * PA_WARPS, PA_MORE = 4;
 
 // A sequence (tree) or row (list) as the walk sees it.
 struct PaUnit {
@@ -78,20 +82,33 @@ __device__ __forceinline__ PaUnit pa_tree_unit(const PagedAttnArgs &a, uint32_t 
     u.n_pages = (u.limit + KV_PAGE - 1) / KV_PAGE;
     return u;
 }
-// Pieces in the order (unit, head); every warp holds the same walk.
+// Pieces in the order (unit, head); every warp holds the same walk.  Where the grid has a CTA for every `per` pages of every piece, a piece begins a new
+// CTA (`apart`): none has the end of one and the start of the next.
 template <bool TREE>
 struct PaWalk {
-    uint64_t at, end, per;  // pages of this CTA, pages a CTA
+    uint64_t at, end, per;  // pages of this CTA, pages a CTA; with `apart`, every piece counts as a multiple of `per`
     uint32_t unit, head, page;
+    bool apart;
     PaUnit u;
 
     __device__ __forceinline__ void start(const PagedAttnArgs &a) {
         const uint32_t lane = threadIdx.x & 31;
+        const uint64_t pieces = (uint64_t)a.n_units * a.pg.n_kv;
+        apart = false;
         if constexpr (!TREE) {
-            const uint64_t total = (uint64_t)a.n_units * a.pg.n_kv * a.n_list;
-            share(total);
-            const uint64_t item = at / a.n_list;
-            page = (uint32_t)(at % a.n_list);
+            share(pieces * a.n_list, pieces);
+            uint32_t parts = 1;
+            if (pieces <= gridDim.x)  // (then everything fits 32 bits)
+                for (uint32_t more = 0; more < 2 && !apart; ++more) {
+                    const uint32_t each = (uint32_t)per + more * ((uint32_t)per / PA_MORE + 1);
+                    parts = (a.n_list + each - 1) / each;
+                    apart = (uint32_t)pieces * parts <= gridDim.x;
+                    if (apart) per = each;
+                }
+            const uint64_t total = apart ? pieces * parts * per : pieces * a.n_list;
+            at = min(total, blockIdx.x * per), end = min(total, at + per);
+            const uint64_t item = apart ? blockIdx.x / parts : at / a.n_list;
+            page = apart ? blockIdx.x % parts * (uint32_t)per : (uint32_t)(at % a.n_list);
             unit = (uint32_t)(item / a.pg.n_kv), head = (uint32_t)(item % a.pg.n_kv);
             u.n_pages = a.n_list;
         } else {
@@ -99,7 +116,19 @@ struct PaWalk {
             const PaUnit front = load(0);  // (up to 32 sequences are read once)
             uint64_t total = 0;
             for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) total += (uint32_t)warp_sum_i((int)(s0 ? load(s0) : front).n_pages);
-            share(total * a.pg.n_kv);
+            total *= a.pg.n_kv;
+            share(total, pieces);
+            uint32_t each = 1;
+            if (pieces <= gridDim.x)
+                for (uint32_t more = 0; more < 2 && !apart; ++more) {
+                    each = (uint32_t)per + more * ((uint32_t)per / PA_MORE + 1);  // (about a piece's pages at most: 32 bits)
+                    uint64_t parts = 0;
+                    for (uint32_t s0 = 0; s0 < a.n_units; s0 += 32) parts += (uint32_t)warp_sum_i((int)(((s0 ? load(s0) : front).n_pages + each - 1) / each));
+                    parts *= a.pg.n_kv;
+                    apart = parts <= gridDim.x;
+                    if (apart) per = each, total = parts * per;
+                }
+            at = min(total, blockIdx.x * per), end = min(total, at + per);
             uint64_t before = 0;
             unit = head = page = 0, u = PaUnit{};
             for (uint32_t s0 = 0; at < end; s0 += 32) {
@@ -108,7 +137,8 @@ struct PaWalk {
                     break;
                 }
                 const PaUnit x = s0 ? load(s0) : front;
-                uint32_t sum = x.n_pages;
+                const uint32_t span = apart ? (x.n_pages + each - 1) / each * each : x.n_pages;
+                uint32_t sum = span;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -120,22 +150,23 @@ struct PaWalk {
                     auto of = [&](uint32_t v) { return __shfl_sync(0xffffffffu, v, src); };
                     unit = s0 + src;
                     u = PaUnit{of(x.row0), of(x.drafts), of(x.ctx), of(x.limit), of(x.n_pages)};
-                    const uint32_t off = (uint32_t)(at - (before + of(sum - x.n_pages)) * a.pg.n_kv);
-                    head = off / u.n_pages, page = off % u.n_pages;
+                    const uint32_t off = (uint32_t)(at - (before + of(sum - span)) * a.pg.n_kv), length = of(span);
+                    head = off / length, page = off % length;
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
         }
     }
-    __device__ __forceinline__ void share(uint64_t total) {
-        per = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)PA_LEAST);
-        at = min(total, blockIdx.x * per), end = min(total, at + per);
+    __device__ __forceinline__ void share(uint64_t total, uint64_t pieces) {
+        const float piece = (float)total / (float)pieces;  // pages of a piece, about
+        const uint64_t even = total >> 32 ? (total + gridDim.x - 1) / gridDim.x : total ? ((uint32_t)total - 1) / gridDim.x + 1 : 0;
+        per = max(even, (uint64_t)max(PA_LEAST, (uint32_t)sqrtf(TREE ? piece : 0.5f * piece)));
     }
     __device__ __forceinline__ bool more() const { return at < end; }
     __device__ __forceinline__ uint32_t last() const { return (uint32_t)min((uint64_t)u.n_pages, page + (end - at)); }  // the present piece is pages [page, last())
     __device__ __forceinline__ void next(const PagedAttnArgs &a) {
-        at += last() - page;
+        at = apart ? end : at + (last() - page);
         page = 0;
         if (at >= end || ++head < a.pg.n_kv) return;
         head = 0;
@@ -490,7 +521,7 @@ cudaError_t launch(PagedAttnArgs a, int sm_count, cudaStream_t st) {
     if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::RINGS); })) return e;
     const uint64_t pages = TREE ? (std::min(a.max_ctx, a.pg.stride * KV_PAGE) + a.max_drafts + KV_PAGE - 1) / KV_PAGE : a.n_list;  // (tree: about, of a sequence)
     const uint64_t most = std::min<uint64_t>({(uint64_t)sm_count * PA_CTAS, PG_COUNTERS, PG_PARTIAL / (2 * S::PART * 4)});
-    const uint64_t grid = std::min(most, std::max<uint64_t>(1, (a.n_units * pages * a.pg.n_kv + PA_LEAST - 1) / PA_LEAST));
+    const uint64_t grid = std::min(most, std::max<uint64_t>(1, a.n_units * ((pages + PA_LEAST - 1) / PA_LEAST) * a.pg.n_kv));
     return launch_pdl(kernel, dim3((uint32_t)grid), dim3(PA_THREADS), S::RINGS, st, a);
 }
 
