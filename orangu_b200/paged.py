@@ -13,29 +13,35 @@ from . import capi
 from .backend import CudaBackend
 
 _PAGE = 16
-_INT = ("int32", "uint32")
+
+
+class _Kinds(dict):
+    """dtype -> whether it is one of the named ones."""
+
+    def __init__(self, *names):
+        self.names = names
+
+    def __missing__(self, dtype):
+        ok = self[dtype] = str(dtype).replace("torch.", "") in self.names
+        return ok
+
+
+_INT, _INT32, _INT8, _WORDS, _FLOAT = _Kinds("int32", "uint32"), _Kinds("int32"), _Kinds("int8"), _Kinds("int64", "uint64"), _Kinds("float32")
 
 
 def _stream(stream):
     return 1 if stream == 0 else stream  # to the C ABI null is the context's stream; 1 is what the runtime calls the legacy default stream
 
 
-_known = {}  # (dtype, accepted names) -> whether it is one of them
-
-
-def _array(name, a, shape, dtypes):
+def _array(name, a, shape, kinds):
     """Address of a contiguous array of that shape."""
+    if a.shape == shape and kinds[a.dtype] and a.is_contiguous():
+        return a.data_ptr()
     if a.shape != shape:
         raise ValueError(f"{name} is {list(a.shape)}, expected {list(shape)}")
-    dtype = a.dtype
-    ok = _known.get((dtype, dtypes))
-    if ok is None:
-        ok = _known[dtype, dtypes] = str(dtype).replace("torch.", "") in dtypes
-    if not ok:
-        raise ValueError(f"{name} is {dtype}, expected {dtypes[0]}")
-    if not a.is_contiguous():
-        raise ValueError(f"{name} is not contiguous")
-    return a.data_ptr()
+    if not kinds[a.dtype]:
+        raise ValueError(f"{name} is {a.dtype}, expected {kinds.names[0]}")
+    raise ValueError(f"{name} is not contiguous")
 
 
 class PagedCache:
@@ -56,8 +62,8 @@ class PagedCache:
         self.backend, self._lib, self._arrays = backend, backend._lib, (k, v, tables)
         self.n_layer, self.n_pages, self.n_head_kv, _, self.head_dim = shape
         self.n_seq, self.table_stride = tuple(tables.shape)
-        d = capi.PagesDesc(_array("k", k, shape, (name,)), _array("v", v, shape, (name,)), self.n_pages * self.n_head_kv * _PAGE * self.head_dim, types[name],
-                           self.n_layer, self.n_pages, self.n_head_kv, self.head_dim, self.n_seq, self.table_stride, _array("tables", tables, tuple(tables.shape), ("int32",)))
+        d = capi.PagesDesc(_array("k", k, shape, _Kinds(name)), _array("v", v, shape, _Kinds(name)), self.n_pages * self.n_head_kv * _PAGE * self.head_dim, types[name],
+                           self.n_layer, self.n_pages, self.n_head_kv, self.head_dim, self.n_seq, self.table_stride, _array("tables", tables, tuple(tables.shape), _INT32))
         h = C.c_void_p()
         capi.check(backend._h, self._lib.ob_pages_create(backend._h, C.byref(d), C.byref(h)))
         self._h = h
@@ -102,11 +108,11 @@ class PagedCache:
             raise ValueError(f"out is {list(out.shape)}, expected {list(q.shape)}")
         self._check(self._lib.ob_pages_attention_tree(
             self._h, layer, n_seq, qp, q_stride, n, _array("first_token", first_token, (n_seq + 1,), _INT), _array("n_ctx", n_ctx, (n_seq,), _INT),
-            _array("visible", visible, (n,), ("int64", "uint64")), heads, max_drafts, max_context, scale, op, o_stride, _stream(stream)))
+            _array("visible", visible, (n,), _WORDS), heads, max_drafts, max_context, scale, op, o_stride, _stream(stream)))
 
     def _bounds(self, codes, scales):
         pages = (self.n_pages, self.n_head_kv)
-        return _array("codes", codes, pages + (2, self.head_dim), ("int8",)), _array("scales", scales, pages, ("float32",))
+        return _array("codes", codes, pages + (2, self.head_dim), _INT8), _array("scales", scales, pages, _FLOAT)
 
     def bounds(self, first_pos, n_pos, codes, scales, max_new: int, layer: int = 0, stream=None):
         """8-bit bounds of the keys of the pages that hold positions first_pos[s] .. n_pos[s] - 1 (at most ``max_new`` a sequence): codes [pages, kv heads, 2,
@@ -123,7 +129,7 @@ class PagedCache:
         n_select = selected.shape[-1]
         self._check(self._lib.ob_pages_select(
             self._h, cp, sp, n, qp, q_stride, _array("row_seq", row_seq, (n,), _INT) if row_seq is not None else None, _array("n_pos", n_pos, (n,), _INT), heads, max_pos,
-            n_select, keep_first, keep_last, _array("selected", selected, (n, self.n_head_kv, n_select), ("int32",)), _stream(stream)))
+            n_select, keep_first, keep_last, _array("selected", selected, (n, self.n_head_kv, n_select), _INT32), _stream(stream)))
 
     def attention(self, q, selected, n_pos, scale: float, out, row_seq=None, layer: int = 0, stream=None):
         """Attention of every row over the positions below n_pos[row] of the pages in ``selected`` (numbers within the row's sequence)."""
@@ -134,12 +140,12 @@ class PagedCache:
         n_select = selected.shape[-1]
         self._check(self._lib.ob_pages_attention(
             self._h, layer, n, qp, q_stride, _array("row_seq", row_seq, (n,), _INT) if row_seq is not None else None, _array("n_pos", n_pos, (n,), _INT), heads,
-            _array("selected", selected, (n, self.n_head_kv, n_select), ("int32",)), n_select, scale, op, o_stride, _stream(stream)))
+            _array("selected", selected, (n, self.n_head_kv, n_select), _INT32), n_select, scale, op, o_stride, _stream(stream)))
 
     def copy(self, src, dst, stream=None):
         """Page dst[i] of every layer becomes a copy of page src[i]; no page is written by one pair and in another."""
         n = src.shape[0]
-        self._check(self._lib.ob_pages_copy(self._h, n, _array("src", src, (n,), ("int32",)), _array("dst", dst, (n,), ("int32",)), _stream(stream)))
+        self._check(self._lib.ob_pages_copy(self._h, n, _array("src", src, (n,), _INT32), _array("dst", dst, (n,), _INT32), _stream(stream)))
 
     def fork(self, parent, child, n_pos, fresh, stream=None):
         """Sequence child[i] goes on from the first n_pos[i] positions of parent[i]: it shares the full pages; a last one that is not full is copied to page
@@ -151,5 +157,5 @@ class PagedCache:
     def keep(self, n_ctx, kept, n_kept, stream=None):
         """In all layers, position n_ctx[s] + kept[s, j] goes to n_ctx[s] + j for j < n_kept[s]: the accepted path of a tree of drafts moves together."""
         n_seq, width = kept.shape
-        self._check(self._lib.ob_pages_keep(self._h, n_seq, _array("n_ctx", n_ctx, (n_seq,), _INT), _array("kept", kept, (n_seq, width), ("int32",)), width,
+        self._check(self._lib.ob_pages_keep(self._h, n_seq, _array("n_ctx", n_ctx, (n_seq,), _INT), _array("kept", kept, (n_seq, width), _INT32), width,
                                             _array("n_kept", n_kept, (n_seq,), _INT), _stream(stream)))
