@@ -11,7 +11,10 @@ namespace ob {
 
 constexpr uint32_t PG_MAX_DRAFTS = 64;   // drafted tokens of a sequence: a bit each
 constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
-constexpr uint32_t PG_FEW_ROWS = 16;     // drafted tokens times heads of a key/value head: up to here mma.sync tiles, above tcgen05 tiles
+// Drafted tokens times heads of a key/value head: up to here mma.sync tiles of 16 rows, above tcgen05 tiles of 128.  Both at 16 rows, head
+// dimension 128: 16.4 and 17.4 us for one sequence of 512, 43.0 and 48.1 for 32 of 1024, 190.5 and 189.5 for 32 of 8192; 64: 14.3 and 15.4, 30.7 and
+// 39.9, 119 and 146.  More rows would read all pages once per 16.
+constexpr uint32_t PG_FEW_ROWS = 16;
 constexpr uint32_t PG_PAGES = 4;         // pages of a tile of the tcgen05 kernel
 constexpr uint32_t PG_START = 6;         // what the start and end of a piece cost there, in tiles
 constexpr size_t PG_WORKSPACE = 64u << 20;  // partial results of the splits, behind the counters
