@@ -9,8 +9,9 @@
 // from memory straight into the fragments (a lane's 16 bytes serve two steps; the order of the terms inside a step is free), and the
 // heads as columns: a page's best head is two exchanges away.  Nor do the queries need shared memory: four lanes hold a head's codes just
 // where the fragments want them.  What bounds the scores is the reading of the codes, 2 dim + 4 bytes a page; with eight pages as columns and
-// the heads as rows, four times as many instructions did (51 us for 64 rows of 6 to 24 k positions, 8 heads of 128; now 27 us for the 120 MB, 4.4 TB/s,
-// of which the start of the only wave of warps is a fifth, and 8 for the choice).
+// the heads as rows, four times as many instructions did (51 us for 64 rows of 6 to 24 k positions, 8 heads of 128; now 27 us for the 120 MB, and
+// 8 for the choice).  With rows half as long the two take 29 us instead of 36: starts, chains of loads and the rounds of the choice are the larger part.  Rings of
+// cp.async in shared memory, codes brought to the L2 cache ahead, the first codes before the queries and fewer warps with more registers all took 35 to 38.
 //
 // Scores are kept as 32-bit words in their order.  Many of them are made by a kernel of their own, a warp per 128 pages (fewer where there are few), neighbouring warps
 // the heads of the same pages, whose codes lie together; few of them in the CTA that picks.  A CTA per (row, head) then picks: counts in
