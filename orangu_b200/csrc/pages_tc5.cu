@@ -632,7 +632,7 @@ cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStre
 
 bool make_page_maps(const PageView &pg, PageMaps *out) {
     const uint64_t rows = (uint64_t)pg.n_pages * pg.n_kv * KV_PAGE;
-    if (rows + PG_KEYS > 0x7fffffffull) return false;  // coordinates have 31 bits
+    if (rows + 128 > 0x7fffffffull) return false;  // coordinates have 31 bits, and a row behind the pool is asked for
     const CUtensorMapDataType type = pg.is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap tm[2];
     if (!make_map_2d(&tm[0], type, 2, pg.k, pg.dim, rows, (uint64_t)pg.dim * 2, 64, KV_PAGE, CU_TENSOR_MAP_SWIZZLE_128B) ||
