@@ -1,0 +1,73 @@
+"""Operators over the pages of a caller's cache at the edges of what they allow: equal scores, numbers that are none, long contexts, large tables, calls that
+are captured first and replayed with other lengths, handles that outlive their context."""
+import numpy as np
+import pytest
+
+import pages_plain as plain
+from gpu_common import backend  # noqa: F401
+from test_gpu_pages import PAGE, ints
+
+pytestmark = pytest.mark.gpu
+
+
+def current():
+    import torch
+
+    return torch.cuda.current_stream().cuda_stream
+
+
+# ------------------------------------------------------------------------------------------- equal scores
+class Bounds:
+    """Bounds of `pages` pages for a choice alone; no keys have to be there for it."""
+
+    def __init__(self, be, rows, pages, kv, dim, seed, kind="f16"):
+        import torch
+
+        from orangu_b200 import PagedCache
+
+        self.r, self.kind, self.kv, self.dim = np.random.default_rng(seed), kind, kv, dim
+        x = torch.zeros((1, pages, kv, PAGE, dim), dtype=torch.float16 if kind == "f16" else torch.bfloat16, device="cuda")
+        self.tables = np.stack([self.r.permutation(pages) for _ in range(rows)])
+        self.cache = PagedCache(be, x, x.clone(), ints(self.tables))
+        hi = self.r.integers(-127, 128, (pages, kv, 1, dim))
+        self.codes = np.concatenate([hi, np.minimum(hi, self.r.integers(-127, 128, hi.shape))], 2).astype(np.int8)
+        self.scales = (self.r.random((pages, kv)) * 0.01 + 0.01).astype(np.float32)
+
+    def choose(self, group, n_pos, n, keep_first, keep_last, zero=(), rounds=1):
+        """Lists of random queries, those of the rows in `zero` all zero: equal scores."""
+        import torch
+
+        rows = len(n_pos)
+        qv, qb = plain.bits16((rows, self.kv * group, self.dim), self.r, self.kind, 1.5)
+        for row in zero:
+            qv[row], qb[row] = 0.0, 0
+        q = torch.from_numpy(qb.view(np.int16)).cuda().view(torch.float16 if self.kind == "f16" else torch.bfloat16)
+        codes, scales, lens = torch.from_numpy(self.codes).cuda(), torch.from_numpy(self.scales).cuda(), ints(n_pos)
+        want = plain.select(qv, self.codes, self.scales, self.tables, n_pos, n, keep_first, keep_last, list(range(rows)), self.kv)
+        for _ in range(rounds):
+            chosen = torch.full((rows, self.kv, n), -7, dtype=torch.int32, device="cuda")
+            self.cache.select(q, codes, scales, lens, chosen, max_pos=max(n_pos), keep_first=keep_first, keep_last=keep_last, stream=current())
+            torch.cuda.synchronize()
+            assert (chosen.cpu().numpy() == want).all()
+
+
+# (one kernel; two, 256 threads; two, 1024 threads)
+@pytest.mark.parametrize("rows,pages,n", [(3, 3, 1), (2, 40, 7), (4, 500, 64), (160, 12, 5), (2, 700, 100), (1, 4500, 128)])
+@pytest.mark.parametrize("keep", [(0, 0), (1, 2)])
+def test_rows_of_zeros_among_others(backend, rows, pages, n, keep):
+    """Padded rows of a batch: all of their scores are equal, their lists the first pages."""
+    b = Bounds(backend, rows, pages, 2, 64, seed=rows + pages)
+    n = max(n, sum(keep))
+    n_pos = [pages * PAGE - int(v) for v in b.r.integers(0, 16, rows)]
+    for zero in (range(rows), range(0, rows, 2)):
+        b.choose(4, n_pos, n, *keep, zero=zero, rounds=20)
+    b.scales[:] = 0.0  # bounds of a cache of zeros
+    b.choose(4, n_pos, n, *keep)
+
+
+@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("group", [9, 16])
+def test_many_heads_scored_by_a_kernel_of_their_own(backend, kind, dim, group):
+    """More than eight query heads a key/value head, rows of more pages than one CTA scores for itself."""
+    b = Bounds(backend, 3, 900, 2, dim, seed=group + dim, kind=kind)
+    b.choose(group, [900 * PAGE, 600 * PAGE - 3, 40], 30, 1, 2, zero=[1])
