@@ -521,8 +521,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     float x[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        x[e] = f0 != 0.0f ? __uint_as_float(o0[e]) * g0 : 0.0f;  // (a stream without tiles has left nothing there)
-                        if (!WIDE && f1 != 0.0f) x[e] = fmaf(__uint_as_float(o1[e]), g1, x[e]);
+                        x[e] = __uint_as_float(o0[e]) * g0;
+                        if (!WIDE && had[1]) x[e] = fmaf(__uint_as_float(o1[e]), g1, x[e]);  // (a stream without tiles has left nothing there)
                     }
                     if (special && live) {  // values that are no numbers, of drafted tokens that this row sees (their weights are above zero)
 #pragma unroll 1

@@ -5,7 +5,7 @@ import pytest
 
 import pages_plain as plain
 from gpu_common import backend  # noqa: F401
-from test_gpu_pages import PAGE, ints
+from test_gpu_pages import PAGE, Made, ints, random_tree, words
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,51 @@ def test_many_heads_scored_by_a_kernel_of_their_own(backend, kind, dim, group):
     """More than eight query heads a key/value head, rows of more pages than one CTA scores for itself."""
     b = Bounds(backend, 3, 900, 2, dim, seed=group + dim, kind=kind)
     b.choose(group, [900 * PAGE, 600 * PAGE - 3, 40], 30, 1, 2, zero=[1])
+
+
+# ------------------------------------------------------------------------------------------- rows that are no numbers
+FORMS = [(4, 3), (4, 20), (8, 40)]  # group, drafted tokens: up to 16 rows a key/value head, up to 128, more
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("group,drafts", FORMS)
+@pytest.mark.parametrize("ctx", [[9, 21], [100] * 40, [0, 3000]])  # pieces of one tile, whole ones of several, cut ones
+def test_a_query_that_is_no_number_has_no_result_and_no_neighbours(backend, kind, group, drafts, ctx):
+    import torch
+
+    made = Made(backend, kind, 2, 64, [c + drafts for c in ctx], seed=drafts)
+    n = drafts * len(ctx)
+    q = torch.randn(n, 2 * group, 64, device="cuda").to(made.kd.dtype)
+    bits = words([b for _ in ctx for b in random_tree(made.r, drafts)])
+    first, lens = ints([drafts * i for i in range(len(ctx) + 1)]), ints(ctx)
+
+    def run():
+        out = torch.full_like(q, 5.0)
+        made.cache.attention_tree(q, first, lens, bits, 0.125, out, max_drafts=drafts, max_context=max(ctx), stream=current())
+        torch.cuda.synchronize()
+        return out
+
+    clean = run()
+    odd = [0, drafts // 2, n - 1]
+    others = [t for t in range(n) if t not in odd]
+    q[odd, :, 5] = float("nan")
+    out = run()
+    assert torch.isnan(out[odd]).all() and torch.isfinite(clean).all()
+    assert torch.equal(out[others], clean[others])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("group,drafts", FORMS)
+def test_a_token_that_sees_only_a_key_that_is_no_number_has_no_result(backend, kind, group, drafts):
+    import torch
+
+    made = Made(backend, kind, 2, 64, [drafts], seed=drafts)
+    made.kd[0, int(made.tables[0, 0]), :, 1, 7] = float("nan")  # drafted token 1
+    bits = [1 << i if i != 1 else 1 for i in range(drafts)]     # every token sees itself, and
+    bits[2] = 0b10                                              # one sees token 1 alone
+    q = torch.randn(drafts, 2 * group, 64, device="cuda").to(made.kd.dtype)
+    out = torch.full_like(q, 5.0)
+    made.cache.attention_tree(q, ints([0, drafts]), ints([0]), words(bits), 0.125, out, max_drafts=drafts, max_context=0, stream=current())
+    torch.cuda.synchronize()
+    assert torch.isnan(out[2]).all()
+    assert torch.isfinite(out[[t for t in range(drafts) if t != 2]]).all()
