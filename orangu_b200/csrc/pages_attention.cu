@@ -6,8 +6,8 @@
 // in one pass with the running maximum m_r and sum.  A CTA has the (up to 16) rows of one key/value head and a stretch of the sequence's
 // pages, which its four warps take in turn, each through a ring of its own: no barrier until the end.  Both products are mma.sync m16n8k16
 // (f16 or bf16, fp32 accumulators): the bytes of the cache are the bound, and 16 rows fill its tile where a tcgen05 tile needs 128.
-// Weights of bf16 caches enter as value and remainder, since 8 bits of weight would be the largest error of the result; f16 has 11.
-// The sum of the weights is one more product, with ones, of the same rounded weights.
+// Weights enter as value and remainder of the cache's type, since 8 or 11 bits of weight alone would be the largest error of the result: f16 ones
+// are off by 2^-22 then, bf16 ones by 2^-16.  The sum of the weights is one more product, with ones, of the same rounded weights.
 //
 // The pages of all (sequence, key/value head) pieces, laid end to end, are shared out evenly over the CTAs, whatever the lengths; a CTA walks
 // through the pieces that lie in its part, or has a part of one piece only where there are CTAs enough for that.  A piece that is cut leaves (m, sum, output) in fp32 and the last of its CTAs to arrive -- a
@@ -191,7 +191,6 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
     using H = Half2<T>;
     using S = PaShape<HD>;
     constexpr int DEPTH = S::DEPTH, KS = HD / 16, CHUNKS = HD / 8;
-    constexpr bool REMAINDER = H::ONES == 0x3f803f80u;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t s_last;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -356,13 +355,11 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
                     const float e0 = pow2(fmaf(s[n][2 * h], scale2, off)), e1 = pow2(fmaf(s[n][2 * h + 1], scale2, off));
                     const uint32_t u = H::pack(e0, e1);
                     w[2 * n + h] = u;
-                    if constexpr (REMAINDER) {
-                        const float2 r = H::unpack(u);
-                        rest[2 * n + h] = H::pack(e0 - r.x, e1 - r.y);
-                    }
+                    const float2 r = H::unpack(u);
+                    rest[2 * n + h] = H::pack(e0 - r.x, e1 - r.y);
                 }
             H::mma(sum, w, H::ONES, H::ONES);
-            if constexpr (REMAINDER) H::mma(sum, rest, H::ONES, H::ONES);
+            H::mma(sum, rest, H::ONES, H::ONES);
             bool odd = false;  // a drafted token's value is not finite: 0 times it would reach rows that do not see the token
             if (drafted) {
 #pragma unroll 1
@@ -381,10 +378,8 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
                     ldsm4t(f, vs + v_row * HD * 2 + (((n + v_half) ^ (v_row & 7)) << 4));
                     H::mma(o[n], w, f[0], f[1]);
                     H::mma(o[n + 1], w, f[2], f[3]);
-                    if constexpr (REMAINDER) {
-                        H::mma(o[n], rest, f[0], f[1]);
-                        H::mma(o[n + 1], rest, f[2], f[3]);
-                    }
+                    H::mma(o[n], rest, f[0], f[1]);
+                    H::mma(o[n + 1], rest, f[2], f[3]);
                 }
             } else {  // term by term, those that a row sees
 #pragma unroll 1
@@ -393,11 +388,8 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float2 p = H::unpack(__shfl_sync(0xffffffffu, j < 8 ? w[h] : w[2 + h], src));
-                        float x = j & 1 ? p.y : p.x;
-                        if constexpr (REMAINDER) {
-                            const float2 r = H::unpack(__shfl_sync(0xffffffffu, j < 8 ? rest[h] : rest[2 + h], src));
-                            x += j & 1 ? r.y : r.x;
-                        }
+                        const float2 r = H::unpack(__shfl_sync(0xffffffffu, j < 8 ? rest[h] : rest[2 + h], src));
+                        const float x = j & 1 ? p.y + r.y : p.x + r.x;
                         const bool see = !(__shfl_sync(0xffffffffu, hidden, src) >> ((j >> 3) * 4 + 2 * h + (j & 1)) & 1);
 #pragma unroll
                         for (int n = 0; n < HD / 8; ++n) {

@@ -7,7 +7,7 @@
 // CTAs to arrive doing it alone took as long as all the rest: 181 us for 8 x 64 tokens of 4 heads a key/value head at 8192).
 //
 //   warps 0-7  softmax: four warps per stream, a thread per row.  Scores come from tensor memory, weights go back into the same
-//              columns: f16, or bf16 as value plus remainder.
+//              columns, as value and remainder of the cache's type: one of 8 or 11 bits alone would be the largest error of the result.
 //   warps 8, 9 issue the products of a stream each: scores = queries (shared memory) x keys, output += weights (tensor memory) x values
 //   warps 10, 11 issue the TMA loads of keys and of values, pages of 16 rows x 64 columns each, straight from the cache into the swizzled operand
 //              tiles, each into a ring of its own
@@ -88,6 +88,8 @@ template <> __device__ __forceinline__ uint32_t pack16<bf16>(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ float2 unpack16(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
+__device__ __forceinline__ float2 unpack16(uint32_t u, bf16) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 __device__ __forceinline__ float from16(__half v) { return __half2float(v); }
 __device__ __forceinline__ float from16(bf16 v) { return __bfloat162float(v); }
 template <typename T> constexpr uint32_t EXPONENT16 = 0x7c00u;
@@ -193,7 +195,6 @@ template <typename T, int HD, bool WIDE>
 __global__ void __launch_bounds__(PG_THREADS, 1)
 pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
     using P = PgPlan<HD, WIDE>;
-    constexpr bool REMAINDER = EXPONENT16<T> == 0x7f80u;
     constexpr uint32_t KST = P::KST, VST = P::VST, G = P::G, PLACE = P::PLACE, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem);
@@ -262,7 +263,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             }
         }
     } else if (warp >= PG_MMA_WARP) {
-        constexpr uint32_t F16 = REMAINDER ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
+        constexpr uint32_t F16 = EXPONENT16<T> == EXPONENT16<bf16> ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
         const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
         const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
         uint32_t n = 0, turn = 0, done = 0;  // places, pieces and tiles of the stream so far
@@ -290,13 +291,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     const uint32_t p = ts + place * PG_KEYS;
                     const uint64_t vd = v_desc + ((st * PLACE + i % G * OPERAND) >> 4);
 #pragma unroll
-                    for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add
-                        if (REMAINDER) {  // 16 positions: eight columns of values, eight of remainders
-                            umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
-                            umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
-                        } else {
-                            umma_bf16_ta_warp(to, p + kk * 8, vd + kk * 128, id_o, step || kk ? 1u : 0u);
-                        }
+                    for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add; 16 positions: eight columns of values, eight of remainders
+                        umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
+                        umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
                     }
                     umma_commit_warp(bar + PB_PV_DONE + 8 * s);
                     if (i % G == G - 1 || step + 1 == (int)steps) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
@@ -447,14 +444,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                                 e0 = pow2(e0), e1 = pow2(e1);
                                 add2(sum0, sum1, e0, e1);
                                 v[e] = pack16<T>(e0, e1);
-                                if constexpr (REMAINDER) v[8 + e] = pack16<T>(e0 - __uint_as_float(v[e] << 16), e1 - __uint_as_float(v[e] & 0xffff0000u));
+                                const float2 r = unpack16(v[e], T());
+                                v[8 + e] = pack16<T>(e0 - r.x, e1 - r.y);
                             }
-                            if constexpr (REMAINDER) {
-                                tmem_st16(tp + 16 * g, v);
-                            } else {
-                                const uint32_t(&h)[8] = reinterpret_cast<const uint32_t(&)[8]>(v);
-                                tmem_st8(tp + 8 * g, h);
-                            }
+                            tmem_st16(tp + 16 * g, v);
                         }
                         const float now = fmaxf(top[0], top[1]) * scale2;
                         const bool grown = now > m + PG_SLACK;

@@ -5,7 +5,7 @@ import pytest
 
 import pages_plain as plain
 from gpu_common import backend  # noqa: F401
-from test_gpu_pages import PAGE, Made, ints, random_tree, words
+from test_gpu_pages import PAGE, Made, check, float64, ints, random_tree, words
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +119,41 @@ def test_a_token_that_sees_only_a_key_that_is_no_number_has_no_result(backend, k
     torch.cuda.synchronize()
     assert torch.isnan(out[2]).all()
     assert torch.isfinite(out[[t for t in range(drafts) if t != 2]]).all()
+
+
+# ------------------------------------------------------------------------------------------- weights
+def fine(kind, v, score):
+    """Bound of an output's error but for its own rounding, where the products of queries and keys are exact: weights go in as value and remainder (f16 2^-22,
+    bf16 2^-16), in numerator and denominator.  A score's product with the scale's power of two has three roundings; 2^-20 covers 2^x and the online
+    sums."""
+    return v * (2 * (2.0 ** -22 if kind == "f16" else 2.0 ** -16) + 4 * 2.0 ** -24 * 1.5 * score + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("group,drafts", FORMS)
+@pytest.mark.parametrize("ctx", [300, 2000])
+def test_weights_have_more_bits_than_the_cache(backend, kind, group, drafts, ctx):
+    """Keys and queries of -1, 0 and 1: scores are exact, and what is left is the weights'."""
+    import torch
+
+    made = Made(backend, kind, 1, 64, [ctx + drafts], seed=ctx)
+    signs = lambda *s: made.r.integers(-1, 2, s).astype(np.float64)  # noqa: E731
+    made.k[:] = signs(*made.k.shape)
+    made.kd.copy_(torch.from_numpy(made.k)[None])
+    q = signs(drafts, group, 64)
+    qd = torch.from_numpy(q).cuda().to(made.kd.dtype)
+    out = torch.empty_like(qd)
+    bits = [(2 << i) - 1 for i in range(drafts)]
+    made.cache.attention_tree(qd, ints([0, drafts]), ints([ctx]), words(bits), 0.125, out, max_drafts=drafts, max_context=ctx, stream=current())
+    torch.cuda.synchronize()
+    want = np.zeros(q.shape)
+    tol = plain.tree(q, made.k, made.v, made.tables, [0, drafts], [ctx], bits, 0.125, want, lambda v, qk, n: fine(kind, v, qk))
+    check(float64(out), want, tol, kind)
+    # the same positions as a list of pages
+    pages = -(-ctx // PAGE)
+    lists = ints(np.arange(pages)[None, None])
+    row = torch.empty_like(qd[:1])
+    made.cache.attention(qd[:1], lists, ints([ctx]), 0.125, row, stream=current())
+    torch.cuda.synchronize()
+    o, tol = plain.listed(q[:1], made.k, made.v, made.tables, [ctx], lists.cpu().numpy(), 0.125, [0], lambda v, qk, n: fine(kind, v, qk))
+    check(float64(row), o, tol, kind)
