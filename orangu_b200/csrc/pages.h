@@ -2,6 +2,7 @@
 // pages.cu hand to the kernels of pages_attention.cu, pages_tc5.cu and pages_select.cu.
 #pragma once
 
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -15,6 +16,13 @@ constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
 // dimension 128: 16.4 and 17.4 us for one sequence of 512, 43.0 and 48.1 for 32 of 1024, 190.5 and 189.5 for 32 of 8192; 64: 14.3 and 15.4, 30.7 and
 // 39.9, 119 and 146.  More rows would read all pages once per 16.
 constexpr uint32_t PG_FEW_ROWS = 16;
+constexpr float PG_SLACK = 8.0f;         // growth of a row's maximum (powers of two) that is put up with before its output is rescaled
+// Weights are made 2^PG_RAISE times as large, in numerator and denominator alike.  An f16 weight has steps of 2^-24 at best: of the running maximum's
+// weight as 1, those below 2^-25 would vanish and those below 2^-14 lose bits, raised they are off by 2^-32.  (131,000 positions of 2^-21 behind one of 1:
+// the result was off by 31 to 129 half steps of f16, now by 0.4 to 2; the rest is the sums'.)  With the slack the largest is 2^15, of f16's 2^16.  bf16
+// has the range of fp32.
+template <typename T> constexpr float PG_RAISE = 0.0f;
+template <> inline constexpr float PG_RAISE<__half> = 7.0f;
 constexpr uint32_t PG_PAGES = 4;         // pages of a tile of the tcgen05 kernel
 constexpr uint32_t PG_START = 6;         // what the start and end of a piece cost there, in tiles
 constexpr size_t PG_WORKSPACE = 64u << 20;  // partial results of the splits, behind the counters

@@ -7,7 +7,8 @@
 // pages, which its four warps take in turn, each through a ring of its own: no barrier until the end.  Both products are mma.sync m16n8k16
 // (f16 or bf16, fp32 accumulators): the bytes of the cache are the bound, and 16 rows fill its tile where a tcgen05 tile needs 128.
 // Weights enter as value and remainder of the cache's type, since 8 or 11 bits of weight alone would be the largest error of the result: f16 ones
-// are off by 2^-22 then, bf16 ones by 2^-16.  The sum of the weights is one more product, with ones, of the same rounded weights.
+// are off by 2^-22 then, bf16 ones by 2^-16.  The sum of the weights is one more product, with ones, of the same rounded weights (that of
+// pages_tc5.cu is of the weights before their rounding: the difference is 2^-32 of the largest a position at most, PG_RAISE).
 //
 // The pages of all (sequence, key/value head) pieces, laid end to end, are shared out evenly over the CTAs, whatever the lengths; a CTA walks
 // through the pieces that lie in its part, or has a part of one piece only where there are CTAs enough for that.  A piece that is cut leaves (m, sum, output) in fp32 and the last of its CTAs to arrive -- a
@@ -48,7 +49,6 @@ template <> struct Half2<bf16> {
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_bf16(c, a, b0, b1); }
 };
 
-constexpr float PA_SLACK = 8.0f;  // growth of the maximum (powers of two) that is put up with before the output is rescaled
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, PA_CTAS = 3;  // CTAs an SM: one's start and end under another's pages
 constexpr int PA_ROWS = 16;
 
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                 now[h] = x * scale2;
-                grown |= now[h] > m[h] + PA_SLACK;  // (the first time, too)
+                grown |= now[h] > m[h] + PG_SLACK;  // (the first time, too)
             }
             if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float off = m[h] == -INFINITY ? 0.0f : -m[h];
+                    const float off = m[h] == -INFINITY ? 0.0f : PG_RAISE<T> - m[h];
                     const float e0 = pow2(fmaf(s[n][2 * h], scale2, off)), e1 = pow2(fmaf(s[n][2 * h + 1], scale2, off));
                     const uint32_t u = H::pack(e0, e1);
                     w[2 * n + h] = u;

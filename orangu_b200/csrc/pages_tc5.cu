@@ -41,7 +41,6 @@ namespace {
 constexpr uint32_t PG_ROWS = 128, PG_KEYS = PG_PAGES * KV_PAGE, PG_BLOCK = PG_KEYS * 128, PG_QBLOCK = PG_ROWS * 128;  // a tile's positions; blocks of 64 columns
 constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 12 * 32;
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
-constexpr float PG_SLACK = 8.0f;        // growth of the maximum (powers of two) that is put up with
 constexpr uint32_t PG_LEAST = 4;        // units of a CTA
 
 // mbarriers and small arrays, byte offsets
@@ -429,7 +428,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     float sum0, sum1;
 #pragma unroll 1
                     for (;;) {
-                        const float base = m == -INFINITY ? 0.0f : -m;  // (still nothing: weights of zero)
+                        const float base = m == -INFINITY ? 0.0f : PG_RAISE<T> - m;  // (still nothing: weights of zero)
                         float top[2] = {-INFINITY, -INFINITY};
                         sum0 = sum1 = 0.0f;
 #pragma unroll
