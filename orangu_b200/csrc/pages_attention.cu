@@ -152,8 +152,9 @@ struct PaWalk {
                     auto of = [&](uint32_t v) { return __shfl_sync(0xffffffffu, v, src); };
                     unit = s0 + src;
                     u = PaUnit{of(x.row0), of(x.drafts), of(x.ctx), of(x.limit), of(x.n_pages)};
-                    const uint32_t off = (uint32_t)(at - (before + of(sum - span)) * a.pg.n_kv), length = of(span);
-                    head = off / length, page = off % length;
+                    const uint64_t off = at - (before + of(sum - span)) * a.pg.n_kv;  // pages of all heads: up to 2^38
+                    const uint32_t length = of(span);
+                    head = off >> 32 ? (uint32_t)(off / length) : (uint32_t)off / length, page = (uint32_t)(off - (uint64_t)head * length);
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);

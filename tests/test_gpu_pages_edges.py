@@ -5,7 +5,7 @@ import pytest
 
 import pages_plain as plain
 from gpu_common import backend  # noqa: F401
-from test_gpu_pages import PAGE, Made, check, float64, ints, random_tree, words
+from test_gpu_pages import PAGE, Made, check, device16, float64, ints, random_tree, tolerance, words
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,36 @@ def test_many_small_weights_behind_a_large_one(backend, kind, group, drafts, pow
     chain = n / (4 if rows <= 16 else 2 if rows <= 128 else 1) / 16 * 2 * (17 / 4 + 1) * 2.0 ** -23
     lost = chain * ((rest + abs(first_value)) / (rest + 1) + abs(want))  # in the numerator and in the denominator
     check(float64(out), np.full(out.shape, want), np.full(out.shape[:2], fine(kind, 1.0, n, score) + lost), kind)
+
+
+# ------------------------------------------------------------------------------------------- large tables
+def test_a_table_whose_pages_times_heads_pass_32_bits(backend):
+    """2^26 places of a table, most of them empty, and 72 heads: 4.8 10^9 pages in a walk."""
+    import torch
+
+    from orangu_b200 import PagedCache
+
+    stride, kv, dim = 1 << 26, 72, 64
+    r = np.random.default_rng(1)
+    k, kb = plain.bits16((5, kv, PAGE, dim), r, "f16")
+    v, vb = plain.bits16((5, kv, PAGE, dim), r, "f16")
+    places = {0: 2, 7: 4, (1 << 25) + 3: 0, (1 << 26) - 2: 3, (1 << 26) - 1: 1}
+    table = torch.full((1, stride), -1, dtype=torch.int32, device="cuda")
+    for at, page in places.items():
+        table[0, at] = page
+    cache = PagedCache(backend, device16(kb[None], "f16"), device16(vb[None], "f16"), table)
+    q, qb = plain.bits16((2, kv, dim), r, "f16", 1.5)
+    out = torch.full((2, kv, dim), 9.0, dtype=torch.float16, device="cuda")
+    ctx = stride * PAGE - 2  # the last two positions are the drafted ones
+    for _ in range(2):       # (the counters are zero again)
+        out.fill_(9.0)
+        cache.attention_tree(device16(qb, "f16"), ints([0, 2]), ints([ctx]), words([1, 3]), 0.125, out, max_drafts=2, max_context=ctx, stream=current())
+        torch.cuda.synchronize()
+        flat = lambda x: np.concatenate([x[p].transpose(1, 0, 2) for p in places.values()])  # noqa: E731  [positions, kv, dim]
+        want, tol = np.zeros(q.shape), np.zeros(q.shape[:2])
+        for t in range(2):
+            seen = np.ones(len(places) * PAGE, bool)
+            seen[len(seen) - 2:] = [True, t == 1]
+            o, big, qk, n = plain.attend(q[t], flat(k), flat(v), seen, 0.125)
+            want[t], tol[t] = o, tolerance("f16", dim)(big, qk, n)
+        check(float64(out), want, tol, "f16")
