@@ -207,8 +207,9 @@ typedef struct ob_pages_desc {
     uint32_t n_seq, table_stride; /* tables: [n_seq][table_stride] */
     int32_t *tables;
 } ob_pages_desc;
-/* The description is copied; the memory it names stays the caller's and has to outlive the handle's calls.  Destroy waits for the device; what was
- * captured with the handle must not be replayed after it.  n_pages * n_head_kv * 16 has to be
+/* The description is copied; the memory it names stays the caller's and has to outlive the handle's calls.  Destroy waits for the device (which ends a capture
+ * of one of its streams: not while there is one); what was captured with the handle must not be replayed after it.  Workspaces of destroyed handles
+ * are kept for later ones and freed with the context.  A handle may be destroyed after its context; calls on it are refused then.  n_pages * n_head_kv * 16 has to be
  * below 2^31 - 128, n_layer at most 16383, n_head_kv 4096, n_seq 2^24, table_stride 2^26 (OB_ERR_UNSUPPORTED). */
 int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out);
 void ob_pages_destroy(ob_pages *pages);

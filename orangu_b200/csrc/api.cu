@@ -105,7 +105,7 @@ void ob_destroy(ob_ctx *ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Scratch *s : {&ctx->sx, &ctx->sy, &ctx->sq, &ctx->sd, &ctx->ss, &ctx->sh, &ctx->shs, &ctx->sdt, &ctx->saux, &ctx->saux2, &ctx->saux3})
         if (s->p) cudaFree(s->p);
-    for (void *w : ctx->page_workspaces) cudaFree(w);
+    close_pages(ctx);
     cudaEventDestroy(ctx->ev0);
     cudaEventDestroy(ctx->ev1);
     cudaStreamDestroy(ctx->stream);

@@ -15,7 +15,7 @@
 using namespace obrt;
 
 struct ob_pages {
-    ob_ctx *ctx;
+    ob_ctx *ctx;           // null once the context is gone
     ob_pages_desc d;
     uint64_t layer_bytes;  // from a layer's pages to the next one's
     uint8_t *workspace;    // PG_COUNTERS words that are zero between launches, as many PagePiece, then partial results
@@ -369,6 +369,13 @@ int launched(ob_pages *p, const char *who, cudaError_t e, uint32_t kernels = 1) 
 
 }  // namespace
 
+void obrt::close_pages(ob_ctx *ctx) {
+    for (ob_pages *p : ctx->pages) p->ctx = nullptr;  // the handles are their owners' to destroy
+    ctx->pages.clear();
+    for (void *w : ctx->page_workspaces) cudaFree(w);  // (waits for the device)
+    ctx->page_workspaces.clear(), ctx->free_page_workspaces.clear();
+}
+
 extern "C" {
 
 int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
@@ -389,8 +396,11 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     if (!on_device(ctx, d.k) || !on_device(ctx, d.v) || !on_device(ctx, d.tables)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages and tables have to be memory of the context's device");
     ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, nullptr, {}};
     if (!p) return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
-    try {
+    try {  // (all that could throw, before there is anything on the device)
         p->maps.resize(d.n_layer);
+        ctx->pages.reserve(ctx->pages.size() + 1);
+        ctx->page_workspaces.reserve(ctx->page_workspaces.size() + 1);
+        ctx->free_page_workspaces.reserve(ctx->page_workspaces.size() + 1);
     } catch (const std::bad_alloc &) {
         delete p;
         return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
@@ -402,13 +412,16 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
         }
     void *ws = nullptr;
     cudaError_t e = cudaSuccess;
-    if (!ctx->page_workspaces.empty()) {  // one that a destroyed handle has left: its counters are zero again
-        ws = ctx->page_workspaces.back();
-        ctx->page_workspaces.pop_back();
+    if (!ctx->free_page_workspaces.empty()) {  // one that a destroyed handle has left
+        ws = ctx->free_page_workspaces.back();
+        ctx->free_page_workspaces.pop_back();
     } else if ((e = cudaMalloc(&ws, PG_WORKSPACE)) == cudaSuccess) {
+        ctx->page_workspaces.push_back(ws);
+    }
+    if (e == cudaSuccess) {
         e = cudaMemsetAsync(ws, 0, PG_COUNTERS * 4, ctx->stream);
         if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // calls come on any stream
-        if (e != cudaSuccess) cudaFree(ws);
+        if (e != cudaSuccess) ctx->free_page_workspaces.push_back(ws);
     }
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -416,19 +429,23 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
         return fail(ctx, e == cudaErrorMemoryAllocation ? OB_ERR_OOM : OB_ERR_CUDA, std::string("pages_create: ") + cudaGetErrorString(e));
     }
     p->workspace = static_cast<uint8_t *>(ws);
+    ctx->pages.push_back(p);
     *out = p;
     return OB_OK;
 }
 
 void ob_pages_destroy(ob_pages *p) {
     if (!p) return;
-    std::lock_guard<std::mutex> g(p->ctx->mu);
-    Bind b(p->ctx);
-    cudaDeviceSynchronize();
-    try {
-        p->ctx->page_workspaces.push_back(p->workspace);  // for the next handle; the context frees it
-    } catch (const std::bad_alloc &) {
-        cudaFree(p->workspace);
+    if (ob_ctx *ctx = p->ctx) {
+        std::lock_guard<std::mutex> g(ctx->mu);
+        Bind b(ctx);
+        ctx->pages.erase(std::find(ctx->pages.begin(), ctx->pages.end(), p));
+        // For the next handle, unless the device cannot be waited for (while a stream of it is captured): kernels may be using it still then, and it
+        // only goes with the context.
+        if (cudaDeviceSynchronize() == cudaSuccess)
+            ctx->free_page_workspaces.push_back(p->workspace);  // (there is room: ob_pages_create)
+        else
+            cudaGetLastError();
     }
     delete p;
 }
@@ -436,7 +453,7 @@ void ob_pages_destroy(ob_pages *p) {
 int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const void *q, uint64_t q_stride, uint32_t n_tokens, const int32_t *first_token, const uint32_t *n_ctx,
                             const uint64_t *visible, uint32_t n_head, uint32_t max_drafts, uint32_t max_ctx, float scale, void *out, uint64_t out_stride, void *stream) {
     const char *who = "pages_attention_tree";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
@@ -467,7 +484,7 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
 int ob_pages_attention(ob_pages *p, uint32_t layer, uint32_t n_rows, const void *q, uint64_t q_stride, const int32_t *row_seq, const uint32_t *n_pos, uint32_t n_head,
                        const int32_t *selected, uint32_t n_select, float scale, void *out, uint64_t out_stride, void *stream) {
     const char *who = "pages_attention";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
@@ -494,7 +511,7 @@ int ob_pages_attention(ob_pages *p, uint32_t layer, uint32_t n_rows, const void 
 int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint32_t n_rows, const void *q, uint64_t q_stride, const int32_t *row_seq, const uint32_t *n_pos, uint32_t n_head,
                     uint32_t max_pos, uint32_t n_select, uint32_t keep_first, uint32_t keep_last, int32_t *selected, void *stream) {
     const char *who = "pages_select";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (!row_seq && n_rows > p->d.n_seq) return bad(p, who, "more rows than tables");
@@ -521,7 +538,7 @@ int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint3
 
 int ob_pages_bounds(ob_pages *p, uint32_t layer, uint32_t n_seq, const uint32_t *first_pos, const uint32_t *n_pos, uint32_t max_new, int8_t *codes, float *scales, void *stream) {
     const char *who = "pages_bounds";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
@@ -548,7 +565,7 @@ int ob_pages_bounds(ob_pages *p, uint32_t layer, uint32_t n_seq, const uint32_t 
 
 int ob_pages_copy(ob_pages *p, uint32_t n, const int32_t *src, const int32_t *dst, void *stream) {
     const char *who = "pages_copy";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (n > 0x7fffffffu) return bad(p, who, "too many pages");
@@ -559,7 +576,7 @@ int ob_pages_copy(ob_pages *p, uint32_t n, const int32_t *src, const int32_t *ds
 
 int ob_pages_fork(ob_pages *p, uint32_t n, const int32_t *parent, const int32_t *child, const uint32_t *n_pos, const int32_t *fresh, void *stream) {
     const char *who = "pages_fork";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (n > 0x7fffffffu) return bad(p, who, "too many sequences");
@@ -570,7 +587,7 @@ int ob_pages_fork(ob_pages *p, uint32_t n, const int32_t *parent, const int32_t 
 
 int ob_pages_keep(ob_pages *p, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept, void *stream) {
     const char *who = "pages_keep";
-    if (!p) return bad(p, who, "null argument");
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
     if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");

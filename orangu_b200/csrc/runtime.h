@@ -28,7 +28,9 @@ struct ob_ctx {
     uint64_t launches = 0;
     float last_ms = 0.0f;
     Scratch sx, sy, sq, sd, ss, sh, shs, sdt, saux, saux2, saux3;
-    std::vector<void *> page_workspaces;  // of handles of cache pages that are gone (pages.cu)
+    // Cache pages of callers (pages.cu): handles that are open, all workspaces that were made for handles, and those that no handle uses.
+    std::vector<ob_pages *> pages;
+    std::vector<void *> page_workspaces, free_page_workspaces;
 };
 
 struct ob_weight {
@@ -65,6 +67,8 @@ struct Bind {  // makes the context's device current for the scope of a call
         if (prev >= 0) cudaSetDevice(prev);
     }
 };
+
+void close_pages(ob_ctx *ctx);  // before the context goes: its handles of cache pages refuse every call from then on
 
 // Uploads (a slice of) a GGUF matrix and re-lays it for the kernels; see DevWeight.
 int make_weight(ob_ctx *ctx, const uint8_t *raw, uint64_t row_bytes, uint32_t type, uint32_t in_dim, uint32_t out_dim, uint32_t row0,

@@ -70,8 +70,7 @@ class PagedCache:
 
     def close(self):
         if self._h:
-            if self.backend._h:
-                self._lib.ob_pages_destroy(self._h)
+            self._lib.ob_pages_destroy(self._h)  # (after the backend's close(), too: the handle knows)
             self._h = None
 
     def __del__(self):

@@ -225,3 +225,74 @@ def test_a_table_whose_pages_times_heads_pass_32_bits(backend):
             o, big, qk, n = plain.attend(q[t], flat(k), flat(v), seen, 0.125)
             want[t], tol[t] = o, tolerance("f16", dim)(big, qk, n)
         check(float64(out), want, tol, "f16")
+
+
+# ------------------------------------------------------------------------------------------- handles and their context
+def free_bytes():
+    import torch
+
+    torch.cuda.synchronize()
+    return torch.cuda.mem_get_info()[0]
+
+
+def tiny_cache(be):
+    import torch
+
+    from orangu_b200 import PagedCache
+
+    k = torch.zeros((1, 2, 1, PAGE, 64), dtype=torch.float16, device="cuda")
+    return PagedCache(be, k, k.clone(), ints([[0, 1]]))
+
+
+def test_a_handle_outlives_its_context():
+    import torch
+
+    from orangu_b200 import CudaBackend, OranguError
+
+    be = CudaBackend.init(0)
+    cache, lib = tiny_cache(be), be._lib
+    q, out = torch.zeros((1, 1, 64), dtype=torch.float16, device="cuda"), torch.full((1, 1, 64), 9.0, dtype=torch.float16, device="cuda")
+    lens, i = ints([5]), ints([0])
+    calls = [lambda: cache.attention_tree(q, ints([0, 1]), lens, words([1]), 0.1, out, 1, 5), lambda: cache.attention(q, ints([[[0]]]), lens, 0.1, out), lambda: cache.copy(i, ints([1])),
+             lambda: cache.keep(lens, ints([[0]]), i), lambda: cache.fork(i, i, lens, i)]
+    before = free_bytes()
+    be.close()
+    assert free_bytes() - before >= 64 << 20  # the workspace of a handle that is open goes with the context
+    for call in calls:
+        with pytest.raises(OranguError):
+            call()
+    torch.cuda.synchronize()
+    assert (out == 9.0).all()
+    cache.close()
+    cache.close()
+    lib.ob_pages_destroy(None)
+
+
+def test_a_workspace_that_may_be_in_use_is_not_given_away():
+    """While a stream is captured the device cannot be waited for: the destroyed handle's workspace stays out of use, and later ones are reused as ever."""
+    import ctypes as C
+
+    import torch
+
+    from orangu_b200 import CudaBackend
+
+    be = CudaBackend.init(0)
+    one, two = tiny_cache(be), tiny_cache(be)
+    rt = C.CDLL([line.split()[-1] for line in open("/proc/self/maps") if "libcudart" in line][0])
+    stream = torch.cuda.Stream()
+    graph = C.c_void_p()
+    torch.cuda.synchronize()
+    assert rt.cudaStreamBeginCapture(C.c_void_p(stream.cuda_stream), 2) == 0
+    one.close()
+    rt.cudaStreamEndCapture(C.c_void_p(stream.cuda_stream), C.byref(graph))
+    rt.cudaGetLastError()
+    two.close()
+    was = free_bytes()
+    three = tiny_cache(be)  # takes what `two` left
+    assert was - free_bytes() < 32 << 20
+    four = tiny_cache(be)
+    assert was - free_bytes() >= 64 << 20
+    three.close(), four.close()
+    was = free_bytes()
+    be.close()
+    assert free_bytes() - was >= 3 * 64 << 20  # the first one's, too
