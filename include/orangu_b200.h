@@ -213,6 +213,12 @@ typedef struct ob_pages_desc {
  * below 2^31 - 128, n_layer at most 16383, n_head_kv 4096, n_seq 2^24, table_stride 2^26 (OB_ERR_UNSUPPORTED). */
 int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out);
 void ob_pages_destroy(ob_pages *pages);
+/* Waits for `stream`, on which the handle was used.  Every wait inside the kernels is bounded: OB_ERR_CUDA when ob_pages_attention_tree, called or replayed
+ * from a capture, gave one up since this was last asked, and its output is not valid.  (Never seen; a call returns before its kernels run and cannot
+ * say so itself.)  ob_synchronize reports it, too, for all of a context's handles, but waits for the context's stream only. */
+int ob_pages_synchronize(ob_pages *pages, void *stream);
+/* Diagnostic: runs a warp whose wait does run out on `stream`, for the next ob_pages_synchronize (and ob_synchronize) to report. */
+int ob_pages_wait_selftest(ob_pages *pages, void *stream);
 
 /* Attention of drafted tokens.  Sequence s has n_ctx[s] positions that all of its drafted tokens see, and drafted tokens first_token[s] ..
  * first_token[s + 1] - 1 of the packed n_tokens (first_token: [n_seq + 1], ascending; no more than max_drafts <= 64 each, those past it

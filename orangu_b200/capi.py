@@ -131,6 +131,8 @@ SIGNATURES = {
     "ob_attention_decode_static": (_i32, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _f32, _vp, _vp]),
     "ob_pages_create": (_i32, [_vp, C.POINTER(PagesDesc), _PP]),
     "ob_pages_destroy": (None, [_vp]),
+    "ob_pages_synchronize": (_i32, [_vp, _vp]),
+    "ob_pages_wait_selftest": (_i32, [_vp, _vp]),
     "ob_pages_attention_tree": (_i32, [_vp, _u32, _u32, _vp, _u64, _u32, _vp, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _u64, _vp]),
     "ob_pages_bounds": (_i32, [_vp, _u32, _u32, _vp, _vp, _u32, _vp, _vp, _vp]),
     "ob_pages_select": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp]),

@@ -21,7 +21,6 @@
 #include <vector>
 
 
-#include "pages.h"
 #include "runtime.h"
 
 static thread_local std::string g_init_error;
@@ -135,7 +134,7 @@ int ob_synchronize(ob_ctx *ctx) {
     Bind b(ctx);
     OB_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
     if (quantized_built() && gemm_tc5_take_status()) return fail(ctx, OB_ERR_CUDA, "a tensor-core product gave up a bounded wait (pipeline barrier); its output is not valid");
-    if (pages_take_status()) return fail(ctx, OB_ERR_CUDA, "attention of drafted tokens gave up a bounded wait (pipeline barrier); its output is not valid");
+    if (pages_gave_up(ctx)) return fail(ctx, OB_ERR_CUDA, "attention of drafted tokens gave up a bounded wait (pipeline barrier); its output is not valid");
     return OB_OK;
 }
 

@@ -18,7 +18,8 @@ struct ob_pages {
     ob_ctx *ctx;           // null once the context is gone
     ob_pages_desc d;
     uint64_t layer_bytes;  // from a layer's pages to the next one's
-    uint8_t *workspace;    // PG_COUNTERS words that are zero between launches, as many PagePiece, then partial results
+    PageWorkspace ws;      // PG_COUNTERS words that are zero between launches, as many PagePiece, then partial results
+    uint32_t untold;       // who was not told of a wait that was given up: SYNCHRONIZE, PAGES_SYNCHRONIZE
     std::vector<PageMaps> maps;  // of every layer
 };
 
@@ -353,9 +354,19 @@ MoveArgs moves(const ob_pages *p) {
     return MoveArgs{static_cast<uint8_t *>(d.k), static_cast<uint8_t *>(d.v), p->layer_bytes, d.n_pages, d.n_head_kv, d.head_dim * 2, d.tables, d.n_seq, d.table_stride};
 }
 void use_workspace(const ob_pages *p, PagedAttnArgs &a) {
-    a.counters = reinterpret_cast<uint32_t *>(p->workspace);
-    a.pieces = reinterpret_cast<PagePiece *>(p->workspace + PG_COUNTERS * 4);
-    a.partial = reinterpret_cast<float *>(p->workspace + PG_COUNTERS * (4 + sizeof(PagePiece)));
+    a.counters = reinterpret_cast<uint32_t *>(p->ws.mem);
+    a.pieces = reinterpret_cast<PagePiece *>(p->ws.mem + PG_COUNTERS * 4);
+    a.partial = reinterpret_cast<float *>(p->ws.mem + PG_COUNTERS * (4 + sizeof(PagePiece)));
+    a.status = p->ws.status;
+}
+// Whether a wait was given up since `who` was last told.
+constexpr uint32_t SYNCHRONIZE = 1, PAGES_SYNCHRONIZE = 2;
+bool take_status(ob_pages *p, uint32_t who) {
+    volatile uint32_t *word = p->ws.status;
+    if (*word) *word = 0, p->untold = SYNCHRONIZE | PAGES_SYNCHRONIZE;
+    const bool mine = p->untold & who;
+    p->untold &= ~who;
+    return mine;
 }
 cudaStream_t stream_of(const ob_pages *p, void *stream) { return stream ? static_cast<cudaStream_t>(stream) : p->ctx->stream; }
 int launched(ob_pages *p, const char *who, cudaError_t e, uint32_t kernels = 1) {
@@ -369,10 +380,16 @@ int launched(ob_pages *p, const char *who, cudaError_t e, uint32_t kernels = 1) 
 
 }  // namespace
 
+bool obrt::pages_gave_up(ob_ctx *ctx) {
+    std::lock_guard<std::mutex> l(ctx->pages_mu);
+    bool any = false;
+    for (ob_pages *p : ctx->pages) any |= take_status(p, SYNCHRONIZE);
+    return any;
+}
 void obrt::close_pages(ob_ctx *ctx) {
     for (ob_pages *p : ctx->pages) p->ctx = nullptr;  // the handles are their owners' to destroy
     ctx->pages.clear();
-    for (void *w : ctx->page_workspaces) cudaFree(w);  // (waits for the device)
+    for (const PageWorkspace &w : ctx->page_workspaces) cudaFree(w.mem), cudaFreeHost(w.status);  // (the first waits for the device)
     ctx->page_workspaces.clear(), ctx->free_page_workspaces.clear();
 }
 
@@ -394,9 +411,10 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     if (!d.k || !d.v || !d.tables) return fail(ctx, OB_ERR_INVALID, "pages_create: null argument");
     if (!aligned(d.k, 16) || !aligned(d.v, 16) || !aligned(d.tables, 4)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages have to be aligned to 16 bytes, tables to 4");
     if (!on_device(ctx, d.k) || !on_device(ctx, d.v) || !on_device(ctx, d.tables)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages and tables have to be memory of the context's device");
-    ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, nullptr, {}};
+    ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, {}, 0, {}};
     if (!p) return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
     try {  // (all that could throw, before there is anything on the device)
+        std::lock_guard<std::mutex> l(ctx->pages_mu);
         p->maps.resize(d.n_layer);
         ctx->pages.reserve(ctx->pages.size() + 1);
         ctx->page_workspaces.reserve(ctx->page_workspaces.size() + 1);
@@ -410,16 +428,20 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
             delete p;
             return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: no tensor map of the pages can be made (n_pages * n_head_kv * 16 rows have to be below 2^31)");
         }
-    void *ws = nullptr;
+    PageWorkspace ws{};
     cudaError_t e = cudaSuccess;
     if (!ctx->free_page_workspaces.empty()) {  // one that a destroyed handle has left
         ws = ctx->free_page_workspaces.back();
         ctx->free_page_workspaces.pop_back();
-    } else if ((e = cudaMalloc(&ws, PG_WORKSPACE)) == cudaSuccess) {
-        ctx->page_workspaces.push_back(ws);
+    } else {
+        e = cudaMalloc(&ws.mem, PG_WORKSPACE);
+        if (e == cudaSuccess) e = cudaHostAlloc(&ws.status, sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);  // (one address on both sides)
+        if (e == cudaSuccess) ctx->page_workspaces.push_back(ws);
+        else cudaFree(ws.mem), ws = {};
     }
     if (e == cudaSuccess) {
-        e = cudaMemsetAsync(ws, 0, PG_COUNTERS * 4, ctx->stream);
+        *ws.status = 0;
+        e = cudaMemsetAsync(ws.mem, 0, PG_COUNTERS * 4, ctx->stream);
         if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // calls come on any stream
         if (e != cudaSuccess) ctx->free_page_workspaces.push_back(ws);
     }
@@ -428,8 +450,11 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
         delete p;
         return fail(ctx, e == cudaErrorMemoryAllocation ? OB_ERR_OOM : OB_ERR_CUDA, std::string("pages_create: ") + cudaGetErrorString(e));
     }
-    p->workspace = static_cast<uint8_t *>(ws);
-    ctx->pages.push_back(p);
+    p->ws = ws;
+    {
+        std::lock_guard<std::mutex> l(ctx->pages_mu);
+        ctx->pages.push_back(p);
+    }
     *out = p;
     return OB_OK;
 }
@@ -439,15 +464,42 @@ void ob_pages_destroy(ob_pages *p) {
     if (ob_ctx *ctx = p->ctx) {
         std::lock_guard<std::mutex> g(ctx->mu);
         Bind b(ctx);
-        ctx->pages.erase(std::find(ctx->pages.begin(), ctx->pages.end(), p));
+        {
+            std::lock_guard<std::mutex> l(ctx->pages_mu);
+            ctx->pages.erase(std::find(ctx->pages.begin(), ctx->pages.end(), p));
+        }
         // For the next handle, unless the device cannot be waited for (while a stream of it is captured): kernels may be using it still then, and it
         // only goes with the context.
         if (cudaDeviceSynchronize() == cudaSuccess)
-            ctx->free_page_workspaces.push_back(p->workspace);  // (there is room: ob_pages_create)
+            ctx->free_page_workspaces.push_back(p->ws);  // (there is room: ob_pages_create)
         else
             cudaGetLastError();
     }
     delete p;
+}
+
+int ob_pages_synchronize(ob_pages *p, void *stream) {
+    const char *who = "pages_synchronize";
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
+    ob_ctx *ctx = p->ctx;
+    Bind b(ctx);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(stream_of(p, stream), &capture);
+    if (e == cudaSuccess && capture == cudaStreamCaptureStatusNone) e = cudaStreamSynchronize(stream_of(p, stream));  // (others may launch meanwhile)
+    std::lock_guard<std::mutex> g(ctx->mu);
+    if (e != cudaSuccess) return launched(p, who, e);
+    if (capture != cudaStreamCaptureStatusNone) return bad(p, who, "the stream is being captured");
+    std::lock_guard<std::mutex> l(ctx->pages_mu);
+    if (take_status(p, PAGES_SYNCHRONIZE)) return fail(ctx, OB_ERR_CUDA, "pages_synchronize: attention of drafted tokens gave up a bounded wait (pipeline barrier); its output is not valid");
+    return OB_OK;
+}
+
+int ob_pages_wait_selftest(ob_pages *p, void *stream) {
+    const char *who = "pages_wait_selftest";
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
+    std::lock_guard<std::mutex> g(p->ctx->mu);
+    Bind b(p->ctx);
+    return launched(p, who, launch_pages_wait_selftest(p->ws.status, stream_of(p, stream)));
 }
 
 int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const void *q, uint64_t q_stride, uint32_t n_tokens, const int32_t *first_token, const uint32_t *n_ctx,
@@ -530,7 +582,7 @@ int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint3
     a.pg = view(p, 0);
     a.codes = codes, a.scales = scales, a.q = q, a.q_stride = q_stride, a.group = n_head / p->d.n_head_kv, a.n_rows = n_rows, a.n_pos = n_pos, a.row_seq = row_seq;
     a.max_pos = max_pos, a.n_select = n_select, a.keep_first = keep_first, a.keep_last = keep_last, a.selected = selected;
-    a.keys = reinterpret_cast<uint32_t *>(p->workspace + PG_COUNTERS * (4 + sizeof(PagePiece)));
+    a.keys = reinterpret_cast<uint32_t *>(p->ws.mem + PG_COUNTERS * (4 + sizeof(PagePiece)));
     uint32_t kernels = 0;
     const cudaError_t e = launch_pages_select(a, p->ctx->sm_count, stream_of(p, stream), &kernels);
     return launched(p, who, e, kernels);

@@ -63,6 +63,7 @@ struct PagedAttnArgs {
     uint32_t *counters;
     PagePiece *pieces;
     float *partial;
+    uint32_t *status;  // pinned host memory: 1 when a bounded wait ran out and the outputs are not valid
     // filled in by the launcher
     uint32_t row_tiles;
 };
@@ -75,7 +76,7 @@ struct alignas(64) PageMaps {
 };
 bool make_page_maps(const PageView &pg, PageMaps *out);  // false: the pool has too many rows for them
 cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st);
-int pages_take_status();  // 1 when a bounded wait of that kernel ran out since the last call
+cudaError_t launch_pages_wait_selftest(uint32_t *status, cudaStream_t st);  // a warp whose wait runs out, and then ends as that kernel does
 
 struct PagedSelectArgs {
     PageView pg;

@@ -94,6 +94,16 @@ __device__ __forceinline__ float from16(bf16 v) { return __bfloat162float(v); }
 template <typename T> constexpr uint32_t EXPONENT16 = 0x7c00u;
 template <> constexpr uint32_t EXPONENT16<bf16> = 0x7f80u;
 
+// The end of a warp that gave up a wait, or found that another had: the word that the host reads (ob_pages_synchronize), and time for copies that
+// are still in flight to land before the shared memory goes away.
+__device__ __forceinline__ void gave_up(uint32_t *status) {
+    if ((threadIdx.x & 31) == 0) {
+        *reinterpret_cast<volatile uint32_t *>(status) = 1u;
+        __threadfence_system();
+    }
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+}
+
 // A sequence as the walk sees it.
 struct PgSeq {
     uint32_t row0, drafts, ctx, limit, n_pages, n_tiles, n_rt;  // n_rt: tiles of rows
@@ -566,9 +576,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         if (threadIdx.x == 0 && !said) a.pieces[blockIdx.x].parts = 0;
     }
     __syncwarp();
-    if (*abort) {  // let copies that are still in flight land before the shared memory goes away
-        for (int i = 0; i < 200; ++i) __nanosleep(1000);
-    }
+    if (*abort) gave_up(a.status);
     tc_fence_before();
     __syncthreads();
     if (warp == PG_MMA_WARP) tmem_dealloc(tmem, PG_TMEM_COLS);
@@ -603,6 +611,19 @@ __global__ void __launch_bounds__(256) pages_merge_kernel(const __grid_constant_
         make_uint2(pack16<T>(x.x * g, x.y * g), pack16<T>(x.z * g, x.w * g));
 }
 
+// A barrier that nothing arrives at, waited for with a short limit.
+__global__ void __launch_bounds__(32) pages_wait_selftest_kernel(uint32_t *status) {
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ uint32_t abort;
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&bar), 1);
+        abort = 0u;
+    }
+    __syncwarp();
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), 0u, &abort, 256));
+    if (!ok && *reinterpret_cast<volatile uint32_t *>(&abort)) gave_up(status);
+}
+
 template <typename T, int HD, bool WIDE>
 cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStream_t st) {
     using P = PgPlan<HD, WIDE>;
@@ -614,7 +635,6 @@ cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStre
     static_assert(sizeof(PageMaps) == 2 * sizeof(CUtensorMap), "two maps");
     CUtensorMap tm[2];
     memcpy(tm, &maps, sizeof(tm));
-    g_tc5_launched.store(true, std::memory_order_relaxed);
     if (cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(PG_THREADS), P::BYTES, st, tm[0], tm[1], a)) return e;
     const uint32_t rows = std::min(P::MR, a.max_drafts * a.group), per = 256 / (HD / 4);
     return launch_pdl(pages_merge_kernel<T, HD, P::MR>, dim3(ctas, (rows + per - 1) / per), dim3(256), 0, st, a);
@@ -644,15 +664,9 @@ cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, 
     return wide ? launch<__half, 128, true>(a, maps, sm_count, st) : launch<__half, 128, false>(a, maps, sm_count, st);
 }
 
-int pages_take_status() {
-    if (!g_tc5_launched.load()) return 0;  // (it stays set: replays of captured calls leave no trace on the host)
-    uint32_t v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_tc5_status, 4) != cudaSuccess) return 0;
-    if (v) {
-        const uint32_t z = 0;
-        cudaMemcpyToSymbol(g_tc5_status, &z, 4);
-    }
-    return (int)v;
+cudaError_t launch_pages_wait_selftest(uint32_t *status, cudaStream_t st) {
+    pages_wait_selftest_kernel<<<1, 32, 0, st>>>(status);
+    return cudaGetLastError();
 }
 
 }  // namespace ob

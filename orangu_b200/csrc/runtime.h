@@ -18,6 +18,11 @@ struct Scratch {  // grow-only device buffer
     size_t cap = 0;
 };
 
+struct PageWorkspace {  // of a handle of cache pages (pages.cu)
+    uint8_t *mem;      // on the device
+    uint32_t *status;  // pinned: set by a kernel that gave up a wait
+};
+
 struct ob_ctx {
     int device = 0;
     int sm_count = 0;
@@ -29,8 +34,9 @@ struct ob_ctx {
     float last_ms = 0.0f;
     Scratch sx, sy, sq, sd, ss, sh, shs, sdt, saux, saux2, saux3;
     // Cache pages of callers (pages.cu): handles that are open, all workspaces that were made for handles, and those that no handle uses.
+    std::mutex pages_mu;  // of the list and what its handles have not been told; taken for moments, after `mu` where both are
     std::vector<ob_pages *> pages;
-    std::vector<void *> page_workspaces, free_page_workspaces;
+    std::vector<PageWorkspace> page_workspaces, free_page_workspaces;
 };
 
 struct ob_weight {
@@ -68,7 +74,8 @@ struct Bind {  // makes the context's device current for the scope of a call
     }
 };
 
-void close_pages(ob_ctx *ctx);  // before the context goes: its handles of cache pages refuse every call from then on
+bool pages_gave_up(ob_ctx *ctx);  // whether a call on one of the context's handles of cache pages gave up a wait since this was last asked
+void close_pages(ob_ctx *ctx);    // before the context goes: its handles of cache pages refuse every call from then on
 
 // Uploads (a slice of) a GGUF matrix and re-lays it for the kernels; see DevWeight.
 int make_weight(ob_ctx *ctx, const uint8_t *raw, uint64_t row_bytes, uint32_t type, uint32_t in_dim, uint32_t out_dim, uint32_t row0,

@@ -83,6 +83,11 @@ class PagedCache:
         if rc:
             capi.check(self.backend._h, rc)
 
+    def synchronize(self, stream=None):
+        """Waits for ``stream``.  Raises OranguError if a wait inside a kernel of attention_tree ran out since this was last asked: its output is not
+        valid then."""
+        self._check(self._lib.ob_pages_synchronize(self._h, _stream(stream)))
+
     def _rows(self, name, a):
         """Address, rows, heads and row stride of queries or outputs [rows, heads, head_dim], rows any multiple of eight entries apart."""
         shape = a.shape

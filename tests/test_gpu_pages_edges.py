@@ -296,3 +296,48 @@ def test_a_workspace_that_may_be_in_use_is_not_given_away():
     was = free_bytes()
     be.close()
     assert free_bytes() - was >= 3 * 64 << 20  # the first one's, too
+
+
+def test_a_wait_that_ran_out_is_reported_by_its_handle(backend):
+    """The word that a kernel leaves when it gives up a wait is the handle's own: seen on the caller's stream, once, whoever else synchronizes."""
+    import torch
+
+    from orangu_b200 import CudaBackend, OranguError, capi
+
+    other = CudaBackend.init(0)
+    a, b, elsewhere = tiny_cache(backend), tiny_cache(backend), tiny_cache(other)
+    stream = torch.cuda.Stream()
+    st = stream.cuda_stream
+    for used in (st, 0):
+        capi.check(backend._h, backend._lib.ob_pages_wait_selftest(a._h, used or 1))
+        torch.cuda.synchronize()
+        for c in (b, elsewhere):
+            c.synchronize(used)
+        other.synchronize()
+        with pytest.raises(OranguError, match="gave up a bounded wait"):
+            a.synchronize(used)
+        a.synchronize(used)  # said once,
+        with pytest.raises(OranguError, match="gave up a bounded wait"):
+            backend.synchronize()  # and once for all handles of the context
+        backend.synchronize()
+    # replays leave no trace on the host but that word
+    q, out = torch.ones((20, 4, 64), dtype=torch.float16, device="cuda"), torch.empty((20, 4, 64), dtype=torch.float16, device="cuda")
+    first, ctx, bits = ints([0, 20]), ints([5]), words([1] * 20)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        a.attention_tree(q, first, ctx, bits, 0.1, out, 20, 5, stream=st)
+        capi.check(backend._h, backend._lib.ob_pages_wait_selftest(a._h, st))
+        with pytest.raises(OranguError, match="captured"):
+            a.synchronize(st)  # and the capture goes on
+    a.synchronize(st)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(OranguError, match="gave up a bounded wait"):
+            a.synchronize(st)
+    assert (out[0] == 0).all()  # (a cache of zeros)
+    a.close()
+    c = tiny_cache(backend)  # the workspace that `a` left: the word is clear
+    c.synchronize(st)
+    backend.synchronize()
+    other.close()
