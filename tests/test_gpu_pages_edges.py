@@ -5,7 +5,7 @@ import pytest
 
 import pages_plain as plain
 from gpu_common import backend  # noqa: F401
-from test_gpu_pages import PAGE, Made, check, device16, float64, ints, random_tree, tolerance, words
+from test_gpu_pages import PAGE, Made, check, device16, float64, ints, random_tree, run_tree, tolerance, words
 
 pytestmark = pytest.mark.gpu
 
@@ -341,3 +341,138 @@ def test_a_wait_that_ran_out_is_reported_by_its_handle(backend):
     c.synchronize(st)
     backend.synchronize()
     other.close()
+
+
+# ------------------------------------------------------------------------------------------- captures
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("group,drafts", [(4, 4), (4, 30), (8, 40)])
+def test_a_replay_goes_by_the_lengths_tables_and_masks_of_its_time(backend, kind, group, drafts):
+    """One captured round (bounds, choice in one kernel and in two, attention over lists and of trees, kept positions) replayed with everything on the device
+    rewritten: contexts beyond the captured bound, sequences without drafted tokens or without context, tables in another order."""
+    import torch
+
+    from orangu_b200 import PagedCache
+
+    kv, dim, seqs, stride = 2, 64, 4, 700
+    r = np.random.default_rng(drafts)
+    dtype = torch.float16 if kind == "f16" else torch.bfloat16
+    k = torch.randn((2, seqs * stride, kv, PAGE, dim), device="cuda").to(dtype)
+    v = torch.randn_like(k)
+    n = seqs * drafts
+
+    def inputs(lens, counts, seed):
+        g = np.random.default_rng(seed)
+        first = np.concatenate([[0], np.cumsum(counts)])
+        bits = [int(g.integers(0, 1 << 62)) for _ in range(n)]
+        return dict(tables=ints(g.permutation(seqs * stride).reshape(seqs, stride)), first=ints(first), lens=ints(lens), bits=words(bits), held=ints([a + b for a, b in zip(lens, counts)]),
+                    zeros=ints([0] * seqs), kept=ints(np.sort(g.integers(0, max(counts), (seqs, 3)), -1)), n_kept=ints([min(3, c) for c in counts]),
+                    q=torch.randn((n, kv * group, dim), device="cuda").to(dtype))
+
+    sets = [inputs([100, 60, 30, 17], [drafts] * seqs, 1), inputs([9000, 0, 5000, 16], [drafts, 1, 0, drafts // 2], 2), inputs([0, 11000, 1, 10000], [0, drafts, drafts, 2], 3),
+            inputs([100, 60, 30, 17], [drafts] * seqs, 1)]
+    live = {a: b.clone() for a, b in sets[0].items()}
+    pool = [k.clone(), v.clone()]
+    cache = PagedCache(backend, pool[0], pool[1], live["tables"])
+
+    def outputs():
+        return dict(tree=torch.zeros((n, kv * group, dim), dtype=dtype, device="cuda"), row=torch.zeros((seqs, kv * group, dim), dtype=dtype, device="cuda"),
+                    few=torch.zeros((seqs, kv, 20), dtype=torch.int32, device="cuda"), many=torch.zeros((seqs, kv, 30), dtype=torch.int32, device="cuda"),
+                    codes=torch.zeros((k.shape[1], kv, 2, dim), dtype=torch.int8, device="cuda"), scales=torch.zeros((k.shape[1], kv), device="cuda"))
+
+    def once(c, s, o, bound):
+        st = current()
+        for layer in range(2):
+            c.bounds(s["zeros"], s["lens"], o["codes"], o["scales"], max_new=stride * PAGE, layer=layer, stream=st)
+            c.select(s["q"][:seqs], o["codes"], o["scales"], s["lens"], o["few"], max_pos=512 * PAGE, keep_last=1, stream=st)
+            c.select(s["q"][:seqs], o["codes"], o["scales"], s["lens"], o["many"], max_pos=stride * PAGE, keep_first=1, stream=st)
+            c.attention(s["q"][:seqs], o["many"], s["lens"], 0.125, o["row"], layer=layer, stream=st)
+            c.attention_tree(s["q"], s["first"], s["lens"], s["bits"], 0.125, o["tree"], max_drafts=drafts, max_context=bound, layer=layer, stream=st)
+        c.keep(s["lens"], s["kept"], s["n_kept"], stream=st)
+
+    got = outputs()
+    once(cache, live, got, 100)  # (a first one that is not captured)
+    pool[0].copy_(k), pool[1].copy_(v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        once(cache, live, got, 100)
+    for s in sets:
+        for name, x in s.items():
+            live[name].copy_(x)
+        for x in got.values():
+            x.zero_()
+        pool[0].copy_(k), pool[1].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = [k.clone(), v.clone()]
+        direct, want = PagedCache(backend, fresh[0], fresh[1], s["tables"]), outputs()
+        once(direct, s, want, 100)  # (the bound shares out the work: the same one for the same sums)
+        torch.cuda.synchronize()
+        for name in got:
+            assert torch.equal(got[name], want[name]), name
+        assert torch.equal(pool[0], fresh[0]) and torch.equal(pool[1], fresh[1])
+        cache.synchronize()
+        direct.close()
+
+
+def test_the_first_calls_of_a_process_are_captured():
+    """Kernels that were never launched before, in a capture that allows nothing unsafe."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = """
+import torch
+from orangu_b200 import CudaBackend, PagedCache
+be = CudaBackend.init(0)
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+k = torch.randn((1, 6, 1, 16, 64), device="cuda").half()
+cache = PagedCache(be, k, k.clone(), ints([[0, 1, 2], [3, 4, 5]]))
+q = torch.randn((8, 4, 64), device="cuda").half()
+out, row, codes, scales = torch.zeros_like(q), torch.zeros_like(q[:2]), torch.zeros((6, 1, 2, 64), dtype=torch.int8, device="cuda"), torch.zeros((6, 1), device="cuda")
+few, lens, first, bits = ints([[[0, 0]]] * 2), ints([33, 20]), ints([0, 4, 8]), torch.ones(8, dtype=torch.int64, device="cuda")
+zeros, kept, src, dst = ints([0, 0]), ints([[1], [0]]), ints([0]), ints([5])
+wide, wide_out = torch.randn((20, 16, 64), device="cuda").half(), torch.zeros((20, 16, 64), dtype=torch.float16, device="cuda")
+wide_first, wide_bits = ints([0, 10, 20]), torch.ones(20, dtype=torch.int64, device="cuda")
+
+def once():
+    st = torch.cuda.current_stream().cuda_stream
+    cache.bounds(zeros, lens, codes, scales, max_new=48, stream=st)
+    cache.select(q[:2], codes, scales, lens, few, max_pos=48, stream=st)
+    cache.attention(q[:2], few, lens, 0.1, row, stream=st)
+    cache.attention_tree(q, first, lens, bits, 0.1, out, 4, 33, stream=st)
+    cache.attention_tree(wide, wide_first, lens, wide_bits, 0.1, wide_out, 10, 33, stream=st)
+    cache.keep(lens, kept, ints_one, stream=st)
+    cache.fork(zeros[:1], src_one, lens[:1], dst, stream=st)
+    cache.copy(src, dst, stream=st)
+
+ints_one, src_one = ints([1, 1]), ints([1])
+state = [x.clone() for x in cache._arrays]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    once()
+g.replay()
+torch.cuda.synchronize()
+a = [x.clone() for x in (out, wide_out, row, few, codes, scales) + cache._arrays]
+for x, y in zip(cache._arrays, state):
+    x.copy_(y)
+for x in (out, wide_out, row, few, codes, scales):
+    x.zero_()
+once()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(a, (out, wide_out, row, few, codes, scales) + cache._arrays)) and bool(out.any()) and bool(wide_out.any())
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(here), timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------- long contexts
+@pytest.mark.parametrize("kind,dim,group,drafts", [("f16", 128, 4, 4), ("bf16", 64, 2, 7), ("f16", 64, 4, 17), ("bf16", 128, 4, 16), ("f16", 128, 8, 17), ("bf16", 64, 16, 9)])
+def test_trees_over_seventy_thousand_positions(backend, kind, dim, group, drafts):
+    ctx = [70_001, 3, 20_000]
+    counts = [drafts, 1, 2]
+    made = Made(backend, kind, 1, dim, [a + b for a, b in zip(ctx, counts)], seed=dim + drafts)
+    run_tree(made, group, ctx, counts)
