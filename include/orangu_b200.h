@@ -33,7 +33,9 @@ extern "C" {
  * 3: ob_model_desc gained tp_presliced.
  * 5: the layered descriptions gained softmax attention over cached keys and values, sequential blocks and mixtures of experts.
  * 6: they gained state-space and time-mixing layers, two mixers in a block, normed inputs, and kept tokens, sinks, soft caps, shared
- *    keys and values of attention. */
+ *    keys and values of attention.
+ * The entry points ob_pages_* came within 7: they change no struct and no function that was there, and a host that does not find them at link or load
+ * time has an older library. */
 #define OB_ABI_VERSION 7u
 
 typedef enum ob_status {
@@ -232,7 +234,7 @@ int ob_pages_attention_tree(ob_pages *pages, uint32_t layer, uint32_t n_seq, con
                             uint32_t max_ctx, float scale, void *out, uint64_t out_stride, void *stream);
 
 /* Bounds of the keys of one layer's pages, for ob_pages_select.  For the pages that hold positions first_pos[s] .. n_pos[s] - 1 (no more
- * than max_new of them a sequence), per page and key/value head, over those of its positions that are below n_pos[s]: the unit
+ * than max_new of them a sequence; at most 65535 sequences a call), per page and key/value head, over those of its positions that are below n_pos[s]: the unit
  * d = max |k| / 127 in scales [n_pages][n_head_kv], and codes [n_pages][n_head_kv][2][head_dim] with ceil(largest / d), then
  * floor(smallest / d).  A key that is no number does not count, and magnitudes above 1e18 count as 1e18.  After a step that appends a
  * token, call it with the token's position. */
@@ -255,7 +257,8 @@ int ob_pages_attention(ob_pages *pages, uint32_t layer, uint32_t n_rows, const v
                        const uint32_t *n_pos, uint32_t n_head, const int32_t *selected, uint32_t n_select, float scale, void *out,
                        uint64_t out_stride, void *stream);
 
-/* Page dst[i] of every layer becomes a copy of page src[i].  A page that one pair writes may be in no other pair. */
+/* Page dst[i] of every layer becomes a copy of page src[i].  A page that one pair writes may be in no other pair.  Tables and bounds are not touched:
+ * who moves a page also renames it in the tables and moves its codes and scales, or makes them again (ob_pages_bounds). */
 int ob_pages_copy(ob_pages *pages, uint32_t n, const int32_t *src, const int32_t *dst, void *stream);
 /* Sequence child[i] goes on from the first n_pos[i] positions of sequence parent[i]: its table names the parent's full pages, and
  * page fresh[i], with the contents copied, for a last one that is not full.  Which sequences hold a page is for the caller to count.  A
@@ -263,7 +266,8 @@ int ob_pages_copy(ob_pages *pages, uint32_t n, const int32_t *src, const int32_t
 int ob_pages_fork(ob_pages *pages, uint32_t n, const int32_t *parent, const int32_t *child, const uint32_t *n_pos, const int32_t *fresh, void *stream);
 /* The accepted ones of a tree of drafted tokens move together behind their context: in all layers the key and value at position n_ctx[s] + j
  * become those that were at n_ctx[s] + kept[s][j], for j < n_kept[s] (at most kept_stride <= 64; kept: [n_seq][kept_stride], numbers below 64 in any
- * order).  All of a sequence's are read before the first is written; those whose place or source is not there are left out. */
+ * order).  All of a sequence's are read before the first is written; those whose place or source is not there are left out.  It
+ * writes to the pages that hold positions n_ctx[s] and on: where a fork shares one of them, copy it first.  n_layer * n_head_kv is at most 32767. */
 int ob_pages_keep(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept, void *stream);
 
 /* sampling::apply_repeat_penalty + argmax (E/sampling.rs:336-359); last index wins ties.

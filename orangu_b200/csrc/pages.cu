@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) pages_copy_kernel(const __grid_c
     copy_page(pool + (uint64_t)s * a.page_bytes(), pool + (uint64_t)d * a.page_bytes(), (uint32_t)(a.page_bytes() / 16));
 }
 
-// grid (children, layers x 2 + 1): the last row of CTAs writes the tables.  Eight children at 1000 positions: 4.2 us in a graph, a launch and two reads that
+// grid (children, layers x 2 + 1): the last row of CTAs writes the tables.  Eight children at 1000 positions: 3.0 us in a graph, a launch and two reads that
 // depend on each other.
 __global__ void __launch_bounds__(MOVE_THREADS) pages_fork_kernel(const __grid_constant__ MoveArgs a, uint32_t n_layer, const int32_t *__restrict__ parent,
                                                                   const int32_t *__restrict__ child, const uint32_t *__restrict__ n_pos, const int32_t *__restrict__ fresh) {

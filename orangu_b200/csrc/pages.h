@@ -13,8 +13,8 @@ namespace ob {
 constexpr uint32_t PG_MAX_DRAFTS = 64;   // drafted tokens of a sequence: a bit each
 constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
 // Drafted tokens times heads of a key/value head: up to here mma.sync tiles of 16 rows, above tcgen05 tiles of 128.  Both at 16 rows, head
-// dimension 128: 16.4 and 17.4 us for one sequence of 512, 43.0 and 48.1 for 32 of 1024, 190.5 and 189.5 for 32 of 8192; 64: 14.3 and 15.4, 30.7 and
-// 39.9, 119 and 146.  More rows would read all pages once per 16.
+// dimension 128: 16.4 and 18.4 us for one sequence of 512, 45.1 and 51.2 for 32 of 1024, 195 and 223 for 32 of 8192; 64: 14.3 and 16.4, 30.7 and
+// 43.0, 119 and 166.  More rows would read all pages once per 16.
 constexpr uint32_t PG_FEW_ROWS = 16;
 constexpr float PG_SLACK = 8.0f;         // growth of a row's maximum (powers of two) that is put up with before its output is rescaled
 // Weights are made 2^PG_RAISE times as large, in numerator and denominator alike.  An f16 weight has steps of 2^-24 at best: of the running maximum's

@@ -14,7 +14,7 @@
 // through the pieces that lie in its part, or has a part of one piece only where there are CTAs enough for that.  A piece that is cut leaves (m, sum, output) in fp32 and the last of its CTAs to arrive -- a
 // counter tells, which goes back to zero by itself -- adds the parts up in order, so the result does not depend on who was last.
 //
-// 32 sequences of 8192, 16 rows a head of 128: 190 us, 5.7 TB/s.  64 rows over 64 listed pages of random places, 8 heads of 128: 49 us, 5.4 TB/s.
+// 32 sequences of 8192, 16 rows a head of 128: 195 us, 5.5 TB/s.  64 rows over 64 listed pages of random places, 8 heads of 128: 49 us, 5.4 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_attention_kernel(co
         if (!s_last) continue;
         __threadfence();
         // 16 entries of parts are under way at once: a sequence of 32,000 positions, whose eight pieces have 55 parts each, takes 51 us for 16 rows of
-        // 128 and 43 us for 4, and with one row after the other 67 and 47 us
+        // 128 and 49 us for 4; with one row after the other 16 rows took 67 us
         auto add_up = [&](auto rows) {
             constexpr uint32_t MINE = decltype(rows)::value, APART = PA_THREADS / VEC, AHEAD = 16 / MINE;  // rows of a thread, from one to the next, parts
             const uint32_t r0 = threadIdx.x / VEC, c = threadIdx.x % VEC;

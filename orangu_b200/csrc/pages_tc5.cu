@@ -15,14 +15,14 @@
 // There are two streams of scores.  Up to 128 rows (WIDE false) they are the even and the odd tiles of the same rows, with an output each;
 // above that they are two tiles of 128 rows that share keys and values.  A stream has two places for scores: while one's weights
 // are made, the other's are multiplied and its next scores come.  Tiles of 128 positions with one place a stream, 16 softmax warps and one that
-// issued all products took 25.6 us for one sequence of 512 positions and 48 rows a key/value head, 52 us for eight of 4096 and 64, now 17.4
-// and 43 to 46; with keys and values through one ring, in order, 32 sequences of 8192 with 128 rows took 218 to 233 us, now 200 (keys are wanted two
-// steps before their values: of one order only the values were ahead).
+// issued all products took 25.6 us for one sequence of 512 positions and 48 rows a key/value head, 52 us for eight of 4096 and 64, and this form 17.4
+// and 43 to 46 (then without remainders of f16 weights, now 18.4 and 47); with keys and values through one ring, in order, 32 sequences of 8192 with 128
+// rows took 230 us over bfloat16 pages, with a ring each 216 (keys are wanted two steps before their values: of one order only the values were ahead).
 //
-// What bounds it (head dimension 128): up to 128 rows the bytes, 200 us for 32 sequences of 8192 with 128 rows (floor 167, 5.4 TB/s).  Above, the
-// chain of a step: 2080 clocks for two warps' 64 positions, of which the special function unit works 40 % and the tensor cores 40 %
-// (613 us for 32 sequences of 8192 with 512 rows, 0.9 PFLOP/s; floor 335; without the weights 488, without the products 495).  A part of the
-// powers of two on the fused multiply-adds, 1/8 to 1/2 of them, took from 2 % less to 6 % more.
+// What bounds it (head dimension 128): up to 128 rows the bytes, 217 to 240 us for 32 sequences of 8192 with 128 rows (floor 167, 4.6 to 5 TB/s).  Above,
+// the chain of a step (scores, weights and their remainders, two products): the tensor cores work 54 % of the time and the special function unit 36 %; 727 us
+// for 32 sequences of 8192 with 512 rows in a call of its own, 855 in a loop, where the clocks fall under the power limit (floor 335).  A part of the powers of
+// two on the fused multiply-adds, 1/8 to 1/2 of them, took from 2 % less to 6 % more.
 //
 // Context positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
 // per thread.  There, values of positions that nobody has, or that are no numbers, are set to zero in shared memory (0 times them
