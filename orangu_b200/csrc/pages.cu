@@ -368,6 +368,12 @@ bool take_status(ob_pages *p, uint32_t who) {
     p->untold &= ~who;
     return mine;
 }
+// The state that a new handle's workspace has, before any stream's next work.
+cudaError_t clear(const ob_ctx *ctx, const PageWorkspace &ws) {
+    *ws.status = 0;
+    const cudaError_t e = cudaMemsetAsync(ws.mem, 0, PG_COUNTERS * 4, ctx->stream);
+    return e == cudaSuccess ? cudaStreamSynchronize(ctx->stream) : e;
+}
 cudaStream_t stream_of(const ob_pages *p, void *stream) { return stream ? static_cast<cudaStream_t>(stream) : p->ctx->stream; }
 int launched(ob_pages *p, const char *who, cudaError_t e, uint32_t kernels = 1) {
     if (e != cudaSuccess) {
@@ -436,16 +442,11 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     } else {
         e = cudaMalloc(&ws.mem, PG_WORKSPACE);
         if (e == cudaSuccess) e = cudaHostAlloc(&ws.status, sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);  // (one address on both sides)
+        if (e == cudaSuccess) e = clear(ctx, ws);
         if (e == cudaSuccess) ctx->page_workspaces.push_back(ws);
-        else cudaFree(ws.mem), ws = {};
-    }
-    if (e == cudaSuccess) {
-        *ws.status = 0;
-        e = cudaMemsetAsync(ws.mem, 0, PG_COUNTERS * 4, ctx->stream);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // calls come on any stream
-        if (e != cudaSuccess) ctx->free_page_workspaces.push_back(ws);
     }
     if (e != cudaSuccess) {
+        cudaFree(ws.mem), cudaFreeHost(ws.status);
         cudaGetLastError();
         delete p;
         return fail(ctx, e == cudaErrorMemoryAllocation ? OB_ERR_OOM : OB_ERR_CUDA, std::string("pages_create: ") + cudaGetErrorString(e));
@@ -470,7 +471,7 @@ void ob_pages_destroy(ob_pages *p) {
         }
         // For the next handle, unless the device cannot be waited for (while a stream of it is captured): kernels may be using it still then, and it
         // only goes with the context.
-        if (cudaDeviceSynchronize() == cudaSuccess)
+        if (cudaDeviceSynchronize() == cudaSuccess && clear(ctx, p->ws) == cudaSuccess)
             ctx->free_page_workspaces.push_back(p->ws);  // (there is room: ob_pages_create)
         else
             cudaGetLastError();
