@@ -18,7 +18,7 @@ def build(tmp_path, *flags):
 def test_lists_with_a_warp_held_up(tmp_path):
     r, exe = build(tmp_path)
     assert r.returncode == 0, r.stderr
-    r = subprocess.run([exe], capture_output=True, text=True)  # (ends itself after a minute)
+    r = subprocess.run([exe], capture_output=True, text=True)  # (ends itself after four minutes)
     assert r.returncode == 0, f"{r.returncode}: {r.stdout}"
 
 
