@@ -34,7 +34,7 @@ extern "C" {
  * 5: the layered descriptions gained softmax attention over cached keys and values, sequential blocks and mixtures of experts.
  * 6: they gained state-space and time-mixing layers, two mixers in a block, normed inputs, and kept tokens, sinks, soft caps, shared
  *    keys and values of attention.
- * The entry points ob_pages_* came within 7: they change no struct and no function that was there, and a host that does not find them at link or load
+ * The entry points ob_pages_* and ob_drafts_verify came within 7: they change no struct and no function that was there, and a host that does not find them at link or load
  * time has an older library. */
 #define OB_ABI_VERSION 7u
 
@@ -199,11 +199,13 @@ int ob_attention_decode_static(ob_ctx *ctx, const float *q_dev, const void *k_pa
  * handles of the same pages may be used side by side.  Numbers in device memory are not known to the host: where the text below gives
  * them a range, what lies outside is left out, never followed.  Products accumulate in fp32, softmax statistics are fp32. */
 #define OB_TYPE_F16 1u /* with OB_TYPE_BF16 below: types of pages; neither is a type of weights here */
+#define OB_TYPE_Q4_PAGES 256u /* pages in 4 bits, [layer][page][n_head_kv][9 * head_dim] bytes, for keys and for values: written by ob_pages_store, read by
+                               * ob_pages_load and ob_pages_attention_tokens; copied, forked and kept like the others */
 typedef struct ob_pages ob_pages;
 typedef struct ob_pages_desc {
     void *k, *v;            /* aligned to 16 bytes */
-    uint64_t layer_stride;  /* elements from a layer's pages to the next one's, a multiple of 8; unused with one layer */
-    uint32_t type;          /* OB_TYPE_F16 or OB_TYPE_BF16 */
+    uint64_t layer_stride;  /* elements from a layer's pages to the next one's, a multiple of 8 (4-bit pages: bytes, a multiple of 16); unused with one layer */
+    uint32_t type;          /* OB_TYPE_F16, OB_TYPE_BF16 or OB_TYPE_Q4_PAGES */
     uint32_t n_layer, n_pages, n_head_kv;
     uint32_t head_dim;      /* 64 or 128 */
     uint32_t n_seq, table_stride; /* tables: [n_seq][table_stride] */
@@ -269,6 +271,58 @@ int ob_pages_fork(ob_pages *pages, uint32_t n, const int32_t *parent, const int3
  * order).  All of a sequence's are read before the first is written; those whose place or source is not there are left out.  It
  * writes to the pages that hold positions n_ctx[s] and on: where a fork shares one of them, copy it first.  n_layer * n_head_kv is at most 32767. */
 int ob_pages_keep(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept, void *stream);
+
+/* 4-bit pages.  Of 32 neighbouring entries x of a position's key or value, m is the one of largest magnitude (of equal ones the negative one), and their
+ * unit is d = -m / 8, made larger to 7 significant bits and to a multiple of 2^-24; an entry is kept as c = x / d rounded to the nearest whole number (ties to
+ * even) from -8 to 7, and stands for c * d, which is an f16 number exactly.  No number counts as 0, magnitudes above 7168 as 7168.
+ *
+ * Store: rows first_token[s] + j of k and v, [n_tokens][n_head_kv][head_dim] f16 or bfloat16 (k_stride, v_stride elements apart, multiples of 8), become
+ * positions n_ctx[s] + j of sequence s, j < first_token[s + 1] - first_token[s] and < max_tokens.  Load: the other way, rounded to the rows' type.  Positions that are
+ * not there are left out, and rows of no sequence left as they were.  No page that two sequences share may be written for both.  At most 65535 sequences
+ * a call; other pages than 4-bit ones are refused (OB_ERR_UNSUPPORTED). */
+int ob_pages_store(ob_pages *pages, uint32_t layer, uint32_t n_seq, const void *k, const void *v, uint32_t type, uint64_t k_stride, uint64_t v_stride,
+                   uint32_t n_tokens, const int32_t *first_token, const uint32_t *n_ctx, uint32_t max_tokens, void *stream);
+int ob_pages_load(ob_pages *pages, uint32_t layer, uint32_t n_seq, void *k, void *v, uint32_t type, uint64_t k_stride, uint64_t v_stride,
+                  uint32_t n_tokens, const int32_t *first_token, const uint32_t *n_ctx, uint32_t max_tokens, void *stream);
+
+/* Attention of the newest tokens of each sequence, whose keys and values are in the pages already: of single tokens, of parts of prompts, of
+ * drafts.  As ob_pages_attention_tree, over pages of any type, with these differences.  q_type: the type of q and out, f16 or bfloat16 over 4-bit pages, the pages' own
+ * otherwise.  visible may be NULL: token j of a sequence sees the context, the tokens before it and itself, and there may be any number of
+ * tokens; with bits no more than 64 a sequence.  mass, if not NULL, [n_seq][n_head_kv][mass_stride] with mass_stride at least table_stride * 16 (at most 65535
+ * sequences): to mass[s][h][x] of each position x < n_ctx[s] that is there the weights are added that it gets from all tokens and the query heads of h, and
+ * those of the new positions are set to theirs.  Tokens past max_tokens of a sequence have no outputs, and neither weights nor places.  n_tokens * n_head is at most
+ * 2^21 with masses (OB_ERR_CAPACITY). */
+int ob_pages_attention_tokens(ob_pages *pages, uint32_t layer, uint32_t n_seq, const void *q, uint32_t q_type, uint64_t q_stride, uint32_t n_tokens,
+                              const int32_t *first_token, const uint32_t *n_ctx, const uint64_t *visible, uint32_t n_head, uint32_t max_tokens,
+                              uint32_t max_ctx, float scale, void *out, uint64_t out_stride, float *mass, uint64_t mass_stride, void *stream);
+
+/* Caches are cut down to n_keep positions, in all layers.  Of a sequence with more, per layer and key/value head, the first keep_first and the last keep_last
+ * positions stay, and of the others those with the largest masses ([n_layer][n_seq][n_head_kv][mass_stride]; the first one of equals, what is no number counts
+ * as the smallest).  Keys, values and masses of what stays move together in order, from position 0 on; kept [n_layer][n_seq][n_head_kv][n_keep] says
+ * which positions they were, ascending, -1 behind the last; n_left[s] = min(n_pos[s], n_keep) (not the memory of n_pos).  What lies behind is left as it was.
+ * A position moves only where both its place and its source are there.  max_pos: about the largest n_pos; results do not depend on its being right.  It
+ * writes to the sequence's pages: where a fork shares one of them, copy it first.  The heads of a position are no longer of one token then: a
+ * sequence's new keys are rotated by the token's own number, not by where they lie. */
+int ob_pages_evict(ob_pages *pages, uint32_t n_seq, const uint32_t *n_pos, float *mass, uint64_t mass_stride, uint32_t max_pos, uint32_t n_keep,
+                   uint32_t keep_first, uint32_t keep_last, int32_t *kept, uint32_t *n_left, void *stream);
+/* ob_pages_keep for the masses of all layers: call both. */
+int ob_pages_keep_mass(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept,
+                       float *mass, uint64_t mass_stride, void *stream);
+
+/* Verification of drafted tokens by probabilities.  Sequence s has nodes first_token[s] .. first_token[s + 1] - 1 of the packed n_tokens (at most 64, those
+ * past it are left out), as ob_pages_attention_tokens had them: node 0 is its last certain token, node i the drafted token tokens[i] that continues node
+ * parent[i] < i (numbers within the sequence; the root's entries of both are not read).  Row i of target, [n_tokens][n_vocab] f32, f16 or bfloat16, target_stride elements apart:
+ * the target's probabilities of what follows node i; draft: those that node i's children were drawn from independently, or NULL (each was certain).
+ * uniform: [n_tokens] numbers from [0, 1).  From node 0 on the children of the present node are tried in ascending order; c = 0 and T = 1 at first:
+ *   with draft     child x is accepted where uniform[x] T q(x) < p(x) - c q(x); if not, c becomes c + T and T the sum of max(p - c q, 0)
+ *   without        where uniform[x] T < p(x); if not, T becomes T - p(x) and p(x) zero
+ * until no child of the present node is accepted.  next_token[s] is then the first v at which the sum of max(p - c q, 0) (without draft: p) exceeds uniform[0] times all of
+ * it; if all of it is zero, the same of the target's row, and -1 if that is zero, too.  kept [n_seq][kept_stride <= 64]: 0 and the accepted nodes, -1 behind
+ * them, as ob_pages_keep takes them, n_kept how many (at most kept_stride).  A probability that is not a positive finite number counts as zero; a node whose
+ * parent or token is out of range is never accepted.  A sequence without nodes: n_kept 0, next_token -1.  Sums are in 64 bits. */
+int ob_drafts_verify(ob_ctx *ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t n_vocab, uint32_t type, const void *target, uint64_t target_stride, const void *draft,
+                     uint64_t draft_stride, const int32_t *tokens, const int32_t *parent, const int32_t *first_token, const float *uniform, int32_t *kept,
+                     uint32_t kept_stride, uint32_t *n_kept, int32_t *next_token, void *stream);
 
 /* sampling::apply_repeat_penalty + argmax (E/sampling.rs:336-359); last index wins ties.
  * recent may be NULL; penalty 1.0 disables it. */

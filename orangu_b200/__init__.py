@@ -12,7 +12,7 @@ from .fenipel import FenipelModel  # noqa: F401
 from .filorax import FiloraxModel  # noqa: F401
 from .nenodra import NenodraModel  # noqa: F401
 from .senuvik import SenuvikModel  # noqa: F401
-from .paged import PagedCache  # noqa: F401
+from .paged import PagedCache, verify_drafts  # noqa: F401
 from .registry import load_model  # noqa: F401
 from .scheduler import SlotPool, SlotGuard  # noqa: F401
 

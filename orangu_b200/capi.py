@@ -37,7 +37,7 @@ class ModelDesc(C.Structure):
         ("rope_freqs", C.c_void_p), ("tp_presliced", C.c_uint32), ("rope_neox", C.c_uint32)]
 
 
-TYPE_F16, TYPE_BF16 = 1, 30
+TYPE_F16, TYPE_BF16, TYPE_Q4_PAGES = 1, 30, 256
 MIXER_LATENT_ATTENTION, MIXER_RETENTION, MIXER_ATTENTION, MIXER_STATE_SPACE, MIXER_TIME_MIXING = 1, 2, 3, 4, 5
 FF_CLAMPED_GLU, FF_RELU2, FF_EXPERTS, FF_GELU_GLU = 0, 1, 2, 3
 ROUTER_SIGMOID, ROUTER_SOFTMAX, ROUTER_SOFTMAX_ALL = 0, 1, 2
@@ -140,6 +140,12 @@ SIGNATURES = {
     "ob_pages_copy": (_i32, [_vp, _u32, _vp, _vp, _vp]),
     "ob_pages_fork": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp, _vp]),
     "ob_pages_keep": (_i32, [_vp, _u32, _vp, _vp, _u32, _vp, _vp]),
+    "ob_pages_store": (_i32, [_vp, _u32, _u32, _vp, _vp, _u32, _u64, _u64, _u32, _vp, _vp, _u32, _vp]),
+    "ob_pages_load": (_i32, [_vp, _u32, _u32, _vp, _vp, _u32, _u64, _u64, _u32, _vp, _vp, _u32, _vp]),
+    "ob_pages_attention_tokens": (_i32, [_vp, _u32, _u32, _vp, _u32, _u64, _u32, _vp, _vp, _vp, _u32, _u32, _u32, _f32, _vp, _u64, _vp, _u64, _vp]),
+    "ob_pages_evict": (_i32, [_vp, _u32, _vp, _vp, _u64, _u32, _u32, _u32, _u32, _vp, _vp, _vp]),
+    "ob_pages_keep_mass": (_i32, [_vp, _u32, _vp, _vp, _u32, _vp, _vp, _u64, _vp]),
+    "ob_drafts_verify": (_i32, [_vp, _u32, _u32, _u32, _u32, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _vp, _vp]),
     "ob_argmax": (_i32, [_vp, _vp, _u32, _vp, _u32, _u32, _f32, _vp]),
     "ob_model_create": (_i32, [_vp, C.POINTER(ModelDesc), _PP]),
     "ob_layered_model_create": (_i32, [_vp, C.POINTER(LayeredDesc), _PP]),

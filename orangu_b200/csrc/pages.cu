@@ -1,5 +1,6 @@
 // Operators over the pages of a cache that the caller holds: the entry points ob_pages_* (checks, handle, workspace), and the kernels that
-// move pages and positions or bound the keys of a page.  Attention is in pages_attention.cu, the choice of pages in pages_select.cu.
+// move pages and positions or bound the keys of a page.  Attention is in pages_attention.cu, pages_tc5.cu and pages_q4.cu, the choice of pages in pages_select.cu;
+// 4-bit pages are written and read in pages_store.cu, weights added up in pages_mass.cu, caches cut in pages_evict.cu.  Verification of drafts: drafts.cu.
 //
 // What moves data is bound by its bytes: whole 16-byte words, several in flight per thread, one launch for all layers, keys and
 // values.
@@ -8,6 +9,7 @@
 #include <new>
 #include <vector>
 
+#include "drafts.h"
 #include "mixers_common.cuh"
 #include "pages.h"
 #include "runtime.h"
@@ -339,6 +341,11 @@ int check_heads(ob_pages *p, const char *who, uint32_t n_head) {
     return OB_OK;
 }
 
+bool is_q4(const ob_pages *p) { return p->d.type == OB_TYPE_Q4_PAGES; }
+int refuse_q4(ob_pages *p, const char *who) { return is_q4(p) ? fail(p->ctx, OB_ERR_UNSUPPORTED, std::string(who) + ": not over 4-bit pages") : OB_OK; }
+// Bytes of 16 positions of one head, keys or values.
+uint32_t block_bytes(const ob_pages_desc &d) { return d.type == OB_TYPE_Q4_PAGES ? 9 * d.head_dim : KV_PAGE * d.head_dim * 2; }
+
 PageView view(const ob_pages *p, uint32_t layer) {
     const ob_pages_desc &d = p->d;
     PageView v{};
@@ -351,7 +358,10 @@ PageView view(const ob_pages *p, uint32_t layer) {
 }
 MoveArgs moves(const ob_pages *p) {
     const ob_pages_desc &d = p->d;
-    return MoveArgs{static_cast<uint8_t *>(d.k), static_cast<uint8_t *>(d.v), p->layer_bytes, d.n_pages, d.n_head_kv, d.head_dim * 2, d.tables, d.n_seq, d.table_stride};
+    return MoveArgs{static_cast<uint8_t *>(d.k), static_cast<uint8_t *>(d.v), p->layer_bytes, d.n_pages, d.n_head_kv, block_bytes(d) / KV_PAGE, d.tables, d.n_seq, d.table_stride};
+}
+PagedKeepArgs keeps(const ob_pages *p, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept) {
+    return PagedKeepArgs{view(p, 0), p->layer_bytes, n_ctx, kept, kept_stride, n_kept};
 }
 void use_workspace(const ob_pages *p, PagedAttnArgs &a) {
     a.counters = reinterpret_cast<uint32_t *>(p->ws.mem);
@@ -407,17 +417,20 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
     const ob_pages_desc &d = *desc;
     std::lock_guard<std::mutex> g(ctx->mu);
     Bind b(ctx);
-    if (d.type != OB_TYPE_F16 && d.type != OB_TYPE_BF16) return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: pages are f16 (OB_TYPE_F16) or bfloat16 (OB_TYPE_BF16)");
+    if (d.type != OB_TYPE_F16 && d.type != OB_TYPE_BF16 && d.type != OB_TYPE_Q4_PAGES) return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: pages are f16 (OB_TYPE_F16), bfloat16 (OB_TYPE_BF16) or 4 bits (OB_TYPE_Q4_PAGES)");
     if (d.head_dim != 64 && d.head_dim != 128) return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: head_dim has to be 64 or 128");
     if (!d.n_layer || !d.n_pages || !d.n_head_kv || !d.n_seq || !d.table_stride) return fail(ctx, OB_ERR_INVALID, "pages_create: a size is zero");
     if (d.n_layer > 16383 || d.n_head_kv > 4096 || d.n_pages > 0x7fffffffu || d.table_stride > (1u << 26) || d.n_seq > (1u << 24))
         return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: a size is too large");
-    const uint64_t elems = (uint64_t)d.n_pages * d.n_head_kv * KV_PAGE * d.head_dim;
-    if (d.n_layer > 1 && (d.layer_stride < elems || d.layer_stride % 8)) return fail(ctx, OB_ERR_INVALID, "pages_create: layer_stride has to be a multiple of 8 and at least a layer's pages");
+    const bool q4 = d.type == OB_TYPE_Q4_PAGES;
+    const uint64_t bytes = (uint64_t)d.n_pages * d.n_head_kv * block_bytes(d), elems = q4 ? bytes : bytes / 2;
+    if (d.n_layer > 1 && (d.layer_stride < elems || d.layer_stride % (q4 ? 16 : 8)))
+        return fail(ctx, OB_ERR_INVALID, q4 ? "pages_create: layer_stride has to be a multiple of 16 and at least a layer's pages" : "pages_create: layer_stride has to be a multiple of 8 and at least a layer's pages");
+    if (q4 && (uint64_t)d.n_pages * d.n_head_kv * KV_PAGE >= (1ull << 31) - 128) return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: n_pages * n_head_kv * 16 has to be below 2^31 - 128");
     if (!d.k || !d.v || !d.tables) return fail(ctx, OB_ERR_INVALID, "pages_create: null argument");
     if (!aligned(d.k, 16) || !aligned(d.v, 16) || !aligned(d.tables, 4)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages have to be aligned to 16 bytes, tables to 4");
     if (!on_device(ctx, d.k) || !on_device(ctx, d.v) || !on_device(ctx, d.tables)) return fail(ctx, OB_ERR_INVALID, "pages_create: pages and tables have to be memory of the context's device");
-    ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * 2 : 0, {}, 0, {}};
+    ob_pages *p = new (std::nothrow) ob_pages{ctx, d, d.n_layer > 1 ? d.layer_stride * (q4 ? 1 : 2) : 0, {}, 0, {}};
     if (!p) return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
     try {  // (all that could throw, before there is anything on the device)
         std::lock_guard<std::mutex> l(ctx->pages_mu);
@@ -429,7 +442,7 @@ int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out) {
         delete p;
         return fail(ctx, OB_ERR_OOM, "pages_create: out of memory");
     }
-    for (uint32_t l = 0; l < d.n_layer; ++l)
+    for (uint32_t l = 0; l < d.n_layer && !q4; ++l)
         if (!make_page_maps(view(p, l), &p->maps[l])) {
             delete p;
             return fail(ctx, OB_ERR_UNSUPPORTED, "pages_create: no tensor map of the pages can be made (n_pages * n_head_kv * 16 rows have to be below 2^31)");
@@ -509,6 +522,7 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
+    if (int rc = refuse_q4(p, who)) return rc;
     if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
     if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");
     if (int rc = check_heads(p, who, n_head)) return rc;
@@ -523,7 +537,7 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     a.pg = view(p, layer);
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.group = n_head / p->d.n_head_kv, a.n_units = n_seq, a.scale = scale;
-    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx;
+    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx, a.block = max_drafts, a.blocks = 1;
     use_workspace(p, a);
     if (max_drafts * a.group > PG_FEW_ROWS) {
         // (the walk over all pieces counts their tiles, and PG_START more for each, in 31 bits)
@@ -540,6 +554,7 @@ int ob_pages_attention(ob_pages *p, uint32_t layer, uint32_t n_rows, const void 
     if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
+    if (int rc = refuse_q4(p, who)) return rc;
     if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
     if (!row_seq && n_rows > p->d.n_seq) return bad(p, who, "more rows than tables");
     if (int rc = check_heads(p, who, n_head)) return rc;
@@ -567,6 +582,7 @@ int ob_pages_select(ob_pages *p, const int8_t *codes, const float *scales, uint3
     if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
+    if (int rc = refuse_q4(p, who)) return rc;
     if (!row_seq && n_rows > p->d.n_seq) return bad(p, who, "more rows than tables");
     if (int rc = check_heads(p, who, n_head)) return rc;
     if (n_rows > (1u << 24)) return bad(p, who, "too many rows");
@@ -594,6 +610,7 @@ int ob_pages_bounds(ob_pages *p, uint32_t layer, uint32_t n_seq, const uint32_t 
     if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
     std::lock_guard<std::mutex> g(p->ctx->mu);
     Bind b(p->ctx);
+    if (int rc = refuse_q4(p, who)) return rc;
     if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
     if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");
     if (n_seq > 65535) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_bounds: more than 65535 sequences");
@@ -650,9 +667,162 @@ int ob_pages_keep(ob_pages *p, uint32_t n_seq, const uint32_t *n_ctx, const int3
     // About two turns a CTA where all of its places are taken (six an SM), one where they are not.
     const uint64_t total = 2ull * p->d.n_layer * p->d.n_head_kv;
     if (total > 65535) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_keep: n_layer * n_head_kv above 32767");
+    if (is_q4(p)) return launched(p, who, launch_pages_keep_q4(keeps(p, n_ctx, kept, kept_stride, n_kept), n_seq, p->d.n_layer, stream_of(p, stream)));
     const uint64_t few = std::max<uint64_t>(1, 12ull * p->ctx->sm_count / n_seq), turns = (total * kept_stride * (p->d.head_dim / 8) + KEEP_WORDS * MOVE_THREADS - 1) / (KEEP_WORDS * MOVE_THREADS);
     return launched(p, who, ob::launch_pdl(pages_keep_kernel, dim3(n_seq, (uint32_t)std::max<uint64_t>(1, std::min(few, turns))), dim3(MOVE_THREADS), 0, stream_of(p, stream), moves(p), 2 * p->d.n_layer,
                                            Divide(p->d.n_head_kv), kept_stride, n_ctx, kept, kept_stride, n_kept));
+}
+
+int ob_pages_attention_tokens(ob_pages *p, uint32_t layer, uint32_t n_seq, const void *q, uint32_t q_type, uint64_t q_stride, uint32_t n_tokens, const int32_t *first_token, const uint32_t *n_ctx,
+                              const uint64_t *visible, uint32_t n_head, uint32_t max_tokens, uint32_t max_ctx, float scale, void *out, uint64_t out_stride, float *mass, uint64_t mass_stride,
+                              void *stream) {
+    const char *who = "pages_attention_tokens";
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
+    std::lock_guard<std::mutex> g(p->ctx->mu);
+    Bind b(p->ctx);
+    const bool q4 = is_q4(p);
+    if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
+    if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");
+    if (int rc = check_heads(p, who, n_head)) return rc;
+    if (q4 ? q_type != OB_TYPE_F16 && q_type != OB_TYPE_BF16 : q_type != p->d.type) return bad(p, who, q4 ? "queries have to be f16 or bfloat16" : "queries have to be of the pages' type");
+    if (visible && max_tokens > PG_MAX_DRAFTS) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_attention_tokens: more than 64 tokens of a sequence with bits");
+    if (n_tokens > 0x7fffffffu || max_tokens > 0x7fffffffu) return bad(p, who, "too many tokens");
+    if (!std::isfinite(scale) || scale <= 0.0f) return bad(p, who, "scale has to be finite and above zero");
+    if (int rc = check_rows(p, who, "q_stride", q_stride, n_head)) return rc;
+    if (int rc = check_rows(p, who, "out_stride", out_stride, n_head)) return rc;
+    if (mass && mass_stride < (uint64_t)p->d.table_stride * KV_PAGE) return bad(p, who, "mass_stride has to be at least the positions of a table");
+    if (mass && n_seq > 65535) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_attention_tokens: more than 65535 sequences with masses");
+    if (mass && (uint64_t)n_tokens * n_head > PG_STATS / sizeof(float2)) return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tokens: n_tokens * n_head above 2^21 with masses");
+    max_tokens = std::min(max_tokens, n_tokens);
+    if (n_seq == 0 || max_tokens == 0) return OB_OK;
+    if (int rc = check_pointers(p, who, {{q, "q", 16}, {first_token, "first_token", 4}, {n_ctx, "n_ctx", 4}, {out, "out", 16}})) return rc;
+    if (visible)
+        if (int rc = check_pointers(p, who, {{visible, "visible", 8}})) return rc;
+    if (mass)
+        if (int rc = check_pointers(p, who, {{mass, "mass", 4}})) return rc;
+    PagedAttnArgs a{};
+    a.pg = view(p, layer);
+    a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+    a.group = n_head / p->d.n_head_kv, a.scale = scale;
+    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_tokens, a.max_ctx = max_ctx;
+    use_workspace(p, a);
+    if (mass) a.stats = reinterpret_cast<float2 *>(p->ws.mem + PG_WORKSPACE - PG_STATS);
+    a.block = q4 ? std::max(1u, PG_FEW_ROWS / a.group) : PG_MAX_DRAFTS;
+    a.block = std::min(a.block, max_tokens);
+    a.blocks = (max_tokens + a.block - 1) / a.block;
+    const uint64_t units = (uint64_t)n_seq * a.blocks;
+    const bool wide = !q4 && a.block * a.group > PG_FEW_ROWS;
+    // (a walk over all pieces counts their pages or tiles, and PG_START more for each, in 31 bits)
+    if (units >= (1ull << 24) || (wide && units * p->d.n_head_kv * (((uint64_t)p->d.table_stride + PG_PAGES - 1) / PG_PAGES + PG_START) * ((a.block * a.group + 127) / 128) >= (1ull << 31)))
+        return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tokens: too many tokens, or the tables of all sequences together have room for too many positions");
+    a.n_units = (uint32_t)units;
+    const cudaStream_t st = stream_of(p, stream);
+    const cudaError_t e = q4 ? launch_pages_q4_attention(a, q_type == OB_TYPE_BF16, p->ctx->sm_count, st)
+                        : wide ? launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, st)
+                               : launch_pages_attention(a, true, p->ctx->sm_count, st);
+    if (int rc = launched(p, who, e, wide ? 2 : 1)) return rc;
+    if (!mass) return OB_OK;
+    return launched(p, who, launch_pages_mass(a, q_type == OB_TYPE_BF16, q4, n_seq, mass, mass_stride, st));
+}
+
+namespace {
+int move_rows(ob_pages *p, const char *who, bool load, uint32_t layer, uint32_t n_seq, const void *k, const void *v, uint32_t type, uint64_t k_stride, uint64_t v_stride, uint32_t n_tokens,
+                     const int32_t *first_token, const uint32_t *n_ctx, uint32_t max_tokens, void *stream) {
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
+    std::lock_guard<std::mutex> g(p->ctx->mu);
+    Bind b(p->ctx);
+    if (!is_q4(p)) return fail(p->ctx, OB_ERR_UNSUPPORTED, std::string(who) + ": over 4-bit pages only");
+    if (layer >= p->d.n_layer) return bad(p, who, "no such layer");
+    if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");
+    if (n_seq > 65535) return fail(p->ctx, OB_ERR_UNSUPPORTED, std::string(who) + ": more than 65535 sequences");
+    if (type != OB_TYPE_F16 && type != OB_TYPE_BF16) return bad(p, who, "rows have to be f16 or bfloat16");
+    if (n_tokens > 0x7fffffffu) return bad(p, who, "too many tokens");
+    if (int rc = check_rows(p, who, "k_stride", k_stride, p->d.n_head_kv)) return rc;
+    if (int rc = check_rows(p, who, "v_stride", v_stride, p->d.n_head_kv)) return rc;
+    max_tokens = std::min(max_tokens, n_tokens);
+    if (n_seq == 0 || max_tokens == 0) return OB_OK;
+    if ((uint64_t)max_tokens * p->d.n_head_kv * 2 * (p->d.head_dim / 8) / 256 >= 0x7fffffffull) return fail(p->ctx, OB_ERR_CAPACITY, std::string(who) + ": too many tokens");
+    if (int rc = check_pointers(p, who, {{k, "k", 16}, {v, "v", 16}, {first_token, "first_token", 4}, {n_ctx, "n_ctx", 4}})) return rc;
+    PagedMoveArgs a{};
+    a.pg = view(p, layer);
+    a.k = k, a.v = v, a.k_stride = k_stride, a.v_stride = v_stride;
+    a.first = first_token, a.n_ctx = n_ctx, a.n_seq = n_seq, a.n_tokens = n_tokens, a.max_tokens = max_tokens;
+    return launched(p, who, launch_pages_store(a, type == OB_TYPE_BF16, load, stream_of(p, stream)));
+}
+}  // namespace
+int ob_pages_store(ob_pages *p, uint32_t layer, uint32_t n_seq, const void *k, const void *v, uint32_t type, uint64_t k_stride, uint64_t v_stride, uint32_t n_tokens, const int32_t *first_token,
+                   const uint32_t *n_ctx, uint32_t max_tokens, void *stream) {
+    return move_rows(p, "pages_store", false, layer, n_seq, k, v, type, k_stride, v_stride, n_tokens, first_token, n_ctx, max_tokens, stream);
+}
+int ob_pages_load(ob_pages *p, uint32_t layer, uint32_t n_seq, void *k, void *v, uint32_t type, uint64_t k_stride, uint64_t v_stride, uint32_t n_tokens, const int32_t *first_token,
+                  const uint32_t *n_ctx, uint32_t max_tokens, void *stream) {
+    return move_rows(p, "pages_load", true, layer, n_seq, k, v, type, k_stride, v_stride, n_tokens, first_token, n_ctx, max_tokens, stream);
+}
+
+int ob_pages_evict(ob_pages *p, uint32_t n_seq, const uint32_t *n_pos, float *mass, uint64_t mass_stride, uint32_t max_pos, uint32_t n_keep, uint32_t keep_first, uint32_t keep_last, int32_t *kept,
+                   uint32_t *n_left, void *stream) {
+    const char *who = "pages_evict";
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
+    std::lock_guard<std::mutex> g(p->ctx->mu);
+    Bind b(p->ctx);
+    if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");
+    if (n_keep == 0) return bad(p, who, "n_keep is zero");
+    if ((uint64_t)keep_first + keep_last > n_keep) return bad(p, who, "keep_first + keep_last is more than n_keep");
+    if (mass_stride < (uint64_t)p->d.table_stride * KV_PAGE) return bad(p, who, "mass_stride has to be at least the positions of a table");
+    if ((uint64_t)p->d.n_layer * n_seq * p->d.n_head_kv > 0x7fffffffull) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_evict: n_layer * n_seq * n_head_kv above 2^31");
+    if (n_seq == 0) return OB_OK;
+    if (int rc = check_pointers(p, who, {{n_pos, "n_pos", 4}, {mass, "mass", 4}, {kept, "kept", 4}, {n_left, "n_left", 4}})) return rc;
+    if (n_left == n_pos) return bad(p, who, "n_left may not be n_pos");
+    PagedEvictArgs a{};
+    a.pg = view(p, 0), a.layer_bytes = p->layer_bytes, a.n_seq = n_seq, a.n_pos = n_pos, a.mass = mass, a.mass_stride = mass_stride;
+    a.n_keep = n_keep, a.keep_first = keep_first, a.keep_last = keep_last, a.kept = kept, a.n_left = n_left;
+    return launched(p, who, launch_pages_evict(a, p->d.n_layer, max_pos, is_q4(p), stream_of(p, stream)), 2);
+}
+
+int ob_pages_keep_mass(ob_pages *p, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept, float *mass, uint64_t mass_stride, void *stream) {
+    const char *who = "pages_keep_mass";
+    if (!p || !p->ctx) return bad(p, who, "no handle, or its context is gone");
+    std::lock_guard<std::mutex> g(p->ctx->mu);
+    Bind b(p->ctx);
+    if (n_seq > p->d.n_seq) return bad(p, who, "more sequences than tables");
+    if (kept_stride == 0 || kept_stride > PG_MAX_DRAFTS) return bad(p, who, "kept_stride has to be 1 to 64");
+    if (mass_stride < (uint64_t)p->d.table_stride * KV_PAGE) return bad(p, who, "mass_stride has to be at least the positions of a table");
+    if ((uint64_t)p->d.n_layer * p->d.n_head_kv > 32767) return fail(p->ctx, OB_ERR_UNSUPPORTED, "pages_keep_mass: n_layer * n_head_kv above 32767");
+    if (n_seq == 0) return OB_OK;
+    if (int rc = check_pointers(p, who, {{n_ctx, "n_ctx", 4}, {kept, "kept", 4}, {n_kept, "n_kept", 4}, {mass, "mass", 4}})) return rc;
+    return launched(p, who, launch_pages_keep_mass(keeps(p, n_ctx, kept, kept_stride, n_kept), n_seq, p->d.n_layer, mass, mass_stride, stream_of(p, stream)));
+}
+
+int ob_drafts_verify(ob_ctx *ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t n_vocab, uint32_t type, const void *target, uint64_t target_stride, const void *draft, uint64_t draft_stride,
+                     const int32_t *tokens, const int32_t *parent, const int32_t *first_token, const float *uniform, int32_t *kept, uint32_t kept_stride, uint32_t *n_kept, int32_t *next_token,
+                     void *stream) {
+    auto invalid = [&](const std::string &what) { return fail(ctx, OB_ERR_INVALID, "drafts_verify: " + what); };
+    if (!ctx) return fail(nullptr, OB_ERR_INVALID, "drafts_verify: no context");
+    std::lock_guard<std::mutex> g(ctx->mu);
+    Bind b(ctx);
+    if (type != OB_TYPE_F32 && type != OB_TYPE_F16 && type != OB_TYPE_BF16) return fail(ctx, OB_ERR_UNSUPPORTED, "drafts_verify: probabilities are f32, f16 or bfloat16");
+    if (n_vocab == 0 || n_vocab > 0x7fffffffu) return invalid("n_vocab has to be 1 to 2^31 - 1");
+    if (n_tokens > 0x7fffffffu) return invalid("too many tokens");
+    if (target_stride < n_vocab || (draft && draft_stride < n_vocab)) return invalid("a stride is below n_vocab");
+    if (kept_stride == 0 || kept_stride > DRAFTS_MOST) return invalid("kept_stride has to be 1 to 64");
+    if (n_seq > (1u << 24)) return invalid("too many sequences");
+    if (n_seq == 0) return OB_OK;
+    const size_t size = type == OB_TYPE_F32 ? 4 : 2;
+    const Named list[] = {{target, "target", size}, {draft, "draft", size}, {tokens, "tokens", 4}, {parent, "parent", 4}, {first_token, "first_token", 4}, {uniform, "uniform", 4}, {kept, "kept", 4}, {n_kept, "n_kept", 4}, {next_token, "next_token", 4}};
+    for (const Named &n : list) {
+        if (!n.p && n.p == draft && &n == list + 1) continue;
+        if (!n.p) return invalid(std::string(n.name) + " is null");
+        if (!aligned(n.p, n.align)) return invalid(std::string(n.name) + " is not aligned to " + std::to_string(n.align) + " bytes");
+        if (!on_device(ctx, n.p)) return invalid(std::string(n.name) + " is not memory of the context's device");
+    }
+    DraftsVerifyArgs a{target, draft, target_stride, draft_stride, n_vocab, n_tokens, tokens, parent, first_token, uniform, kept, kept_stride, n_kept, next_token};
+    const cudaError_t e = launch_drafts_verify(a, n_seq, type == OB_TYPE_F32 ? 0 : type == OB_TYPE_F16 ? 1 : 2, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(ctx, OB_ERR_CUDA, std::string("drafts_verify: ") + cudaGetErrorString(e));
+    }
+    ++ctx->launches;
+    return OB_OK;
 }
 
 }  // extern "C"

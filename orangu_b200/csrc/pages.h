@@ -1,5 +1,5 @@
 // Operators over the pages of a cache that the caller holds (include/orangu_b200.h, ob_pages_*): what the entry points of
-// pages.cu hand to the kernels of pages_attention.cu, pages_tc5.cu and pages_select.cu.
+// pages.cu hand to the kernels of pages_attention.cu, pages_tc5.cu, pages_select.cu, pages_q4.cu, pages_store.cu, pages_mass.cu and pages_evict.cu.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -32,10 +32,12 @@ struct alignas(32) PagePiece {  // rows whose parts several CTAs have left (page
     uint32_t rows, row, token0, head;  // rows row .. row + rows - 1 of the sequence that begins at token0
 };
 constexpr size_t PG_PARTIAL = PG_WORKSPACE - PG_COUNTERS * (4 + sizeof(PagePiece));
+constexpr size_t PG_STATS = 16u << 20;      // of these, at the end: a maximum and the inverse of a sum per (token, head), where weights are added up per position
+constexpr size_t PG_PARTS = PG_PARTIAL - PG_STATS;
 
 // One layer's pages and the tables of the sequences.
 struct PageView {
-    const void *k, *v;  // [n_pages][n_kv][KV_PAGE][dim], f16 or bf16
+    const void *k, *v;  // [n_pages][n_kv][KV_PAGE][dim], f16 or bf16, or [n_pages][n_kv] blocks in 4 bits (pages_q4.cuh)
     bool is_bf16;
     uint32_t n_pages, n_kv, dim;
     const int32_t *tables;
@@ -53,7 +55,9 @@ struct PagedAttnArgs {
     const int32_t *first;     // [n_units + 1]
     const uint32_t *n_ctx;    // [n_units]
     const uint64_t *visible;  // [n_tokens]
-    uint32_t n_tokens, max_drafts, max_ctx;
+    uint32_t n_tokens, max_drafts, max_ctx;  // visible may be null: a token sees those before it and itself
+    uint32_t block, blocks;   // tokens of a unit, units of a sequence (n_units: all of them); several with visible == null (or in 4-bit pages)
+    float2 *stats;            // [n_tokens][n_kv * group] or null: a row's maximum and the inverse of its sum, so that a weight is 2^(score - maximum) times that
     // list
     const int32_t *list;      // [n_units][n_kv][n_list]
     const uint32_t *n_pos;    // [n_units]
@@ -77,6 +81,45 @@ struct alignas(64) PageMaps {
 bool make_page_maps(const PageView &pg, PageMaps *out);  // false: the pool has too many rows for them
 cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st);
 cudaError_t launch_pages_wait_selftest(uint32_t *status, cudaStream_t st);  // a warp whose wait runs out, and then ends as that kernel does
+
+// 4-bit pages, any number of rows: blocks of tokens that have at most PG_FEW_ROWS.
+cudaError_t launch_pages_q4_attention(const PagedAttnArgs &a, bool q_bf16, int sm_count, cudaStream_t st);
+// After an attention with `stats`, whose units are of n_seq sequences: [n_seq][n_kv][mass_stride].
+cudaError_t launch_pages_mass(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, cudaStream_t st);
+
+struct PagedMoveArgs {  // rows into 4-bit pages, or out of them
+    PageView pg;
+    const void *k, *v;  // [n_tokens][n_kv][dim], strides in elements
+    uint64_t k_stride, v_stride;
+    const int32_t *first;
+    const uint32_t *n_ctx;
+    uint32_t n_seq, n_tokens, max_tokens;
+};
+cudaError_t launch_pages_store(const PagedMoveArgs &a, bool is_bf16, bool load, cudaStream_t st);
+
+struct PagedEvictArgs {
+    PageView pg;             // of layer 0
+    uint64_t layer_bytes;
+    uint32_t n_seq;
+    const uint32_t *n_pos;
+    float *mass;             // [n_layer][n_seq][n_kv][mass_stride]
+    uint64_t mass_stride;
+    uint32_t n_keep, keep_first, keep_last;
+    int32_t *kept;           // [n_layer][n_seq][n_kv][n_keep]
+    uint32_t *n_left;
+};
+cudaError_t launch_pages_evict(const PagedEvictArgs &a, uint32_t n_layer, uint32_t max_pos, bool q4, cudaStream_t st);
+
+struct PagedKeepArgs {
+    PageView pg;             // of layer 0
+    uint64_t layer_bytes;
+    const uint32_t *n_ctx;
+    const int32_t *kept;
+    uint32_t kept_stride;
+    const uint32_t *n_kept;
+};
+cudaError_t launch_pages_keep_q4(const PagedKeepArgs &a, uint32_t n_seq, uint32_t n_layer, cudaStream_t st);
+cudaError_t launch_pages_keep_mass(const PagedKeepArgs &a, uint32_t n_seq, uint32_t n_layer, float *mass, uint64_t stride, cudaStream_t st);
 
 struct PagedSelectArgs {
     PageView pg;

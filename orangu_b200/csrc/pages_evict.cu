@@ -1,0 +1,224 @@
+// Cutting a cache down (ob_pages_evict): per layer, sequence and key/value head the first and the last positions stay, and of the others those with the
+// most weight; what stays moves together, in order.  And the accepted positions of drafts in 4-bit pages, and of masses (ob_pages_keep).
+//
+// The choice is that of pages_select.cu, by counts in equal parts of the masses' range: a CTA per (layer, sequence, head), the words of its masses in shared
+// memory where they fit.  The move goes to places that are never behind their sources (kept[j] >= j), so that a CTA that goes through a head's list
+// in order may read ahead as far as it likes, and has only to have read a batch before it writes it: one barrier a batch, no copy in between.
+#include <algorithm>
+
+#include "mixers_common.cuh"
+#include "pages.h"
+#include "pages_pick.cuh"
+#include "pages_q4.cuh"
+
+namespace ob {
+
+namespace {
+
+constexpr uint32_t EV_HELD = 32768;  // words of masses in shared memory at most
+constexpr uint32_t EV_THREADS = 256, EV_DEEP = 4;  // pieces of a thread in flight
+
+// Larger masses have larger words; what is no number has the smallest.
+__device__ __forceinline__ uint32_t mass_word(float s) {
+    if (s != s) return 0u;
+    const uint32_t u = __float_as_uint(s + 0.0f);  // (-0 is 0)
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+struct MassWords {
+    const float *mass;
+    uint32_t first, last;  // places below `first` and from `last` on are taken
+    __device__ __forceinline__ uint32_t operator[](uint32_t i) const { return i < first || i >= last ? SEL_FORCED : mass_word(__ldcg(mass + i)); }
+};
+
+// grid (layers x sequences x heads)
+template <uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) pages_evict_choose_kernel(const __grid_constant__ PagedEvictArgs a, uint32_t held) {
+    extern __shared__ __align__(16) uint32_t s_words[];
+    pdl_release();
+    pdl_wait();
+    const uint32_t seq = blockIdx.x / a.pg.n_kv % a.n_seq;
+    const uint32_t n = min(a.n_pos[seq], a.pg.stride * KV_PAGE);
+    int32_t *out = a.kept + (uint64_t)blockIdx.x * a.n_keep;
+    if (blockIdx.x % a.pg.n_kv == 0 && blockIdx.x / a.pg.n_kv < a.n_seq && threadIdx.x == 0) a.n_left[seq] = min(n, a.n_keep);
+    if (n <= a.n_keep) {
+        for (uint32_t i = threadIdx.x; i < a.n_keep; i += THREADS) out[i] = i < n ? (int32_t)i : -1;
+        return;
+    }
+    const MassWords words{a.mass + (uint64_t)blockIdx.x * a.mass_stride, a.keep_first, n - a.keep_last};
+    uint32_t lo = 0xffffffffu, hi = 0;
+    const bool fits = n <= held;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        const uint32_t w = words[i];
+        if (fits) s_words[i] = w;
+        if (w != SEL_FORCED) lo = min(lo, w), hi = max(hi, w);
+    }
+    const uint32_t want = a.n_keep - a.keep_first - a.keep_last;
+    if (fits) pick<THREADS>(want, s_words, n, lo, hi, out);
+    else pick<THREADS>(want, words, n, lo, hi, out);
+}
+
+// One position's key or value of a head, in pieces that a thread moves.
+template <int HD>
+struct Row16 {
+    static constexpr uint32_t PIECES = HD / 8, BLOCK = KV_PAGE * HD * 2;
+    using Word = uint4;
+    static __device__ __forceinline__ Word load(const uint8_t *block, bool, uint32_t p, uint32_t i) { return *reinterpret_cast<const uint4 *>(block + p * HD * 2 + i * 16); }
+    static __device__ __forceinline__ void store(uint8_t *block, bool, uint32_t p, uint32_t i, Word x) { *reinterpret_cast<uint4 *>(block + p * HD * 2 + i * 16) = x; }
+};
+template <int HD>
+struct Row4 {  // pairs of words, then units
+    using B = Q4Block<HD>;
+    static constexpr uint32_t PAIRS = HD / 16, PIECES = PAIRS + B::GROUPS, BLOCK = B::BYTES;
+    using Word = uint2;
+    static __device__ __forceinline__ Word load(const uint8_t *block, bool value, uint32_t p, uint32_t i) {
+        if (i < PAIRS) return *reinterpret_cast<const uint2 *>(block + B::word(value, p, 2 * i));
+        return make_uint2(*reinterpret_cast<const uint16_t *>(block + B::unit(value, p, i - PAIRS)), 0u);
+    }
+    static __device__ __forceinline__ void store(uint8_t *block, bool value, uint32_t p, uint32_t i, Word x) {
+        if (i < PAIRS) *reinterpret_cast<uint2 *>(block + B::word(value, p, 2 * i)) = x;
+        else *reinterpret_cast<uint16_t *>(block + B::unit(value, p, i - PAIRS)) = (uint16_t)x.x;
+    }
+};
+
+// grid (layers x sequences x heads, 3): keys, values, masses.
+template <typename R>
+__global__ void __launch_bounds__(EV_THREADS) pages_evict_move_kernel(const __grid_constant__ PagedEvictArgs a) {
+    pdl_release();
+    pdl_wait();
+    const uint32_t head = blockIdx.x % a.pg.n_kv, seq = blockIdx.x / a.pg.n_kv % a.n_seq, layer = blockIdx.x / a.pg.n_kv / a.n_seq;
+    const uint32_t n = min(a.n_pos[seq], a.pg.stride * KV_PAGE);
+    if (n <= a.n_keep) return;
+    const int32_t *kept = a.kept + (uint64_t)blockIdx.x * a.n_keep;
+    if (blockIdx.y == 2) {
+        float *mass = a.mass + (uint64_t)blockIdx.x * a.mass_stride;
+#pragma unroll 1
+        for (uint32_t j0 = a.keep_first; j0 < a.n_keep; j0 += EV_DEEP * EV_THREADS) {
+            float x[EV_DEEP];
+#pragma unroll
+            for (uint32_t u = 0; u < EV_DEEP; ++u) {
+                const uint32_t j = j0 + u * EV_THREADS + threadIdx.x;
+                if (j < a.n_keep) x[u] = mass[kept[j]];
+            }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t u = 0; u < EV_DEEP; ++u) {
+                const uint32_t j = j0 + u * EV_THREADS + threadIdx.x;
+                if (j < a.n_keep) mass[j] = x[u];
+            }
+        }
+        return;
+    }
+    const bool value = blockIdx.y;
+    uint8_t *pool = static_cast<uint8_t *>(const_cast<void *>(value ? a.pg.v : a.pg.k)) + layer * a.layer_bytes + (uint64_t)head * R::BLOCK;
+    const int32_t *table = a.pg.tables + (uint64_t)seq * a.pg.stride;
+    constexpr uint32_t ROWS = EV_DEEP * EV_THREADS / R::PIECES;  // positions of a batch
+    const uint64_t page_bytes = (uint64_t)a.pg.n_kv * R::BLOCK;
+#pragma unroll 1
+    for (uint32_t j0 = a.keep_first; j0 < a.n_keep; j0 += ROWS) {
+        typename R::Word x[EV_DEEP];
+        uint8_t *to[EV_DEEP];
+        const uint32_t rows = min(ROWS, a.n_keep - j0);
+#pragma unroll
+        for (uint32_t u = 0; u < EV_DEEP; ++u) {
+            const uint32_t i = u * EV_THREADS + threadIdx.x, r = i / R::PIECES, piece = i - r * R::PIECES, j = j0 + r;
+            to[u] = nullptr;
+            if (r >= rows) continue;
+            const uint32_t src = (uint32_t)kept[j];
+            if (src == j) continue;
+            const int32_t ps = table[src / KV_PAGE], pd = table[j / KV_PAGE];
+            if ((uint32_t)ps >= a.pg.n_pages || (uint32_t)pd >= a.pg.n_pages) continue;
+            x[u] = R::load(pool + (uint32_t)ps * page_bytes, value, src % KV_PAGE, piece);
+            to[u] = pool + (uint32_t)pd * page_bytes;
+        }
+        __syncthreads();  // a batch has been read before it is written; what the next one reads lies behind it
+#pragma unroll
+        for (uint32_t u = 0; u < EV_DEEP; ++u) {
+            const uint32_t i = u * EV_THREADS + threadIdx.x, r = i / R::PIECES;
+            if (to[u]) R::store(to[u], value, (j0 + r) % KV_PAGE, i - r * R::PIECES, x[u]);
+        }
+    }
+}
+
+// Place of position x of a sequence, and of head 0 of its page: bytes, or all ones.
+__device__ __forceinline__ bool kept_places(const PagedKeepArgs &a, uint32_t seq, uint32_t j, uint32_t &from, uint32_t &to) {
+    const uint32_t n = min(a.n_kept[seq], a.kept_stride);
+    if (j >= n) return false;
+    const int32_t i = a.kept[(uint64_t)seq * a.kept_stride + j];
+    const uint64_t ctx = a.n_ctx[seq], x = ctx + (uint32_t)i, y = ctx + j, room = (uint64_t)a.pg.stride * KV_PAGE;
+    if ((uint32_t)i >= 64 || (uint32_t)i == j || x >= room || y >= room) return false;
+    const int32_t *table = a.pg.tables + (uint64_t)seq * a.pg.stride;
+    if ((uint32_t)table[x / KV_PAGE] >= a.pg.n_pages || (uint32_t)table[y / KV_PAGE] >= a.pg.n_pages) return false;
+    from = (uint32_t)x, to = (uint32_t)y;
+    return true;
+}
+
+// grid (sequences, layers x 2 x heads): all of a head's positions are read before the first is written.
+template <int HD>
+__global__ void __launch_bounds__(256) pages_keep_q4_kernel(const __grid_constant__ PagedKeepArgs a) {
+    using R = Row4<HD>;
+    pdl_release();
+    pdl_wait();
+    const uint32_t head = blockIdx.y % a.pg.n_kv, pool = blockIdx.y / a.pg.n_kv;
+    const bool value = pool & 1;
+    uint8_t *base = static_cast<uint8_t *>(const_cast<void *>(value ? a.pg.v : a.pg.k)) + (pool >> 1) * a.layer_bytes + (uint64_t)head * R::BLOCK;
+    const uint64_t page_bytes = (uint64_t)a.pg.n_kv * R::BLOCK;
+    const int32_t *table = a.pg.tables + (uint64_t)blockIdx.x * a.pg.stride;
+    constexpr uint32_t TURNS = (64 * R::PIECES + 255) / 256;
+    uint2 x[TURNS];
+    uint32_t to[TURNS];
+#pragma unroll
+    for (uint32_t u = 0; u < TURNS; ++u) {
+        const uint32_t i = u * 256 + threadIdx.x, j = i / R::PIECES;
+        uint32_t from;
+        if (!kept_places(a, blockIdx.x, j, from, to[u])) {
+            to[u] = 0xffffffffu;
+            continue;
+        }
+        x[u] = R::load(base + (uint32_t)table[from / KV_PAGE] * page_bytes, value, from % KV_PAGE, i - j * R::PIECES);
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t u = 0; u < TURNS; ++u) {
+        const uint32_t i = u * 256 + threadIdx.x;
+        if (to[u] != 0xffffffffu) R::store(base + (uint32_t)table[to[u] / KV_PAGE] * page_bytes, value, to[u] % KV_PAGE, i % R::PIECES, x[u]);
+    }
+}
+
+// grid (sequences, layers x heads), a thread a position.
+__global__ void __launch_bounds__(64) pages_keep_mass_kernel(const __grid_constant__ PagedKeepArgs a, float *mass, uint64_t stride, uint32_t n_seq) {
+    pdl_release();
+    pdl_wait();
+    const uint32_t layer = blockIdx.y / a.pg.n_kv, head = blockIdx.y % a.pg.n_kv;
+    float *row = mass + (((uint64_t)layer * n_seq + blockIdx.x) * a.pg.n_kv + head) * stride;
+    uint32_t from, to;
+    const bool moves = kept_places(a, blockIdx.x, threadIdx.x, from, to);
+    const float x = moves ? row[from] : 0.0f;
+    __syncthreads();
+    if (moves) row[to] = x;
+}
+
+}  // namespace
+
+cudaError_t launch_pages_evict(const PagedEvictArgs &a, uint32_t n_layer, uint32_t max_pos, bool q4, cudaStream_t st) {
+    static PerDeviceOnce once;
+    if (cudaError_t e = once.run([] {
+            if (cudaError_t e = cudaFuncSetAttribute(pages_evict_choose_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_HELD * 4)) return e;
+            return cudaFuncSetAttribute(pages_evict_choose_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_HELD * 4);
+        }))
+        return e;
+    const uint32_t pairs = n_layer * a.n_seq * a.pg.n_kv, held = std::min({std::max(max_pos, 1u), a.pg.stride * KV_PAGE, EV_HELD});
+    if (cudaError_t e = max_pos <= 4096 ? launch_pdl(pages_evict_choose_kernel<256>, dim3(pairs), dim3(256), (size_t)held * 4, st, a, held)
+                                        : launch_pdl(pages_evict_choose_kernel<1024>, dim3(pairs), dim3(1024), (size_t)held * 4, st, a, held))
+        return e;
+    auto kernel = q4 ? (a.pg.dim == 64 ? pages_evict_move_kernel<Row4<64>> : pages_evict_move_kernel<Row4<128>>) : (a.pg.dim == 64 ? pages_evict_move_kernel<Row16<64>> : pages_evict_move_kernel<Row16<128>>);
+    return launch_pdl(kernel, dim3(pairs, 3), dim3(EV_THREADS), 0, st, a);
+}
+cudaError_t launch_pages_keep_q4(const PagedKeepArgs &a, uint32_t n_seq, uint32_t n_layer, cudaStream_t st) {
+    return launch_pdl(a.pg.dim == 64 ? pages_keep_q4_kernel<64> : pages_keep_q4_kernel<128>, dim3(n_seq, 2 * n_layer * a.pg.n_kv), dim3(256), 0, st, a);
+}
+cudaError_t launch_pages_keep_mass(const PagedKeepArgs &a, uint32_t n_seq, uint32_t n_layer, float *mass, uint64_t stride, cudaStream_t st) {
+    return launch_pdl(pages_keep_mass_kernel, dim3(n_seq, n_layer * a.pg.n_kv), dim3(64), 0, st, a, mass, stride, n_seq);
+}
+
+}  // namespace ob

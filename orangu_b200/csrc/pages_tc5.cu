@@ -109,14 +109,17 @@ struct PgSeq {
     uint32_t row0, drafts, ctx, limit, n_pages, n_tiles, n_rt;  // n_rt: tiles of rows
 };
 template <uint32_t MR>
-__device__ __forceinline__ PgSeq pg_seq(const PagedAttnArgs &a, uint32_t s) {
+__device__ __forceinline__ PgSeq pg_seq(const PagedAttnArgs &a, uint32_t unit) {
     PgSeq q{};
+    const uint32_t s = a.blocks > 1 ? unit / a.blocks : unit, skip = (unit - s * a.blocks) * a.block;  // (more than one block: all that is before it is context)
     const int32_t f0 = a.first[s], f1 = a.first[s + 1];
     const uint32_t ctx = a.n_ctx[s], room = a.pg.stride * KV_PAGE;  // (all loads before the first decision)
     if (f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens) return q;
-    q.row0 = (uint32_t)f0;
-    q.drafts = min((uint32_t)(f1 - f0), a.max_drafts);
-    q.ctx = min(ctx, room);
+    const uint32_t n = min((uint32_t)(f1 - f0), a.max_drafts);
+    if (skip >= n) return q;
+    q.row0 = (uint32_t)f0 + skip;
+    q.drafts = min(n - skip, a.block);
+    q.ctx = min(min(ctx, room) + skip, room);
     q.limit = min(q.ctx + q.drafts, room);
     q.n_pages = (q.limit + KV_PAGE - 1) / KV_PAGE;
     q.n_tiles = (q.n_pages + PG_PAGES - 1) / PG_PAGES;
@@ -252,7 +255,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         const uint32_t nowhere = a.pg.n_pages * a.pg.n_kv * KV_PAGE;  // the row behind the pool: reads as zero
         const uint32_t page = lane % (G * PG_PAGES), box = lane / (G * PG_PAGES), at = page / PG_PAGES * OPERAND + box * PG_BLOCK + page % PG_PAGES * (KV_PAGE * 128);  // a lane a copy
         for (; w.more() && ok; w.next(a)) {
-            const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
+            const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
             const uint32_t end = w.last();
             auto row_of = [&](uint32_t tile) {  // the first row of the lane's page of the tiles from this one on
                 const uint32_t p = tile * PG_PAGES + page;
@@ -340,7 +343,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             const uint32_t end = w.last(), tiles = end - w.tile, n_rows = w.q.drafts * a.group - w.rt * MR;  // rows from this tile of rows on
             const uint32_t f_row = (WIDE ? s * PG_ROWS : 0u) + r, warp_row = (WIDE ? s * PG_ROWS : 0u) + quad * 32;
             const bool live = f_row < n_rows, warm = warp_row < n_rows;  // this row, any row of the warp
-            const int32_t *table = a.pg.tables + (uint64_t)w.seq * a.pg.stride;
+            const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
             // ---- the queries, 16 bytes a thread and turn
             constexpr uint32_t WORDS = HD / 8, TURNS = MR * WORDS / PG_SOFT, BATCH = TURNS < 8 ? TURNS : 8;  // (all of a batch's loads before its stores)
 #pragma unroll 1
@@ -364,7 +367,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             if (lane == 0) mbar_arrive(bar + PB_Q_FULL);
             uint64_t seen = 0;
             if (live && w.q.ctx < end * PG_KEYS) {
-                seen = a.visible[w.q.row0 + (w.rt * MR + f_row) / a.group];
+                const uint32_t token = (w.rt * MR + f_row) / a.group;
+                seen = a.visible ? a.visible[w.q.row0 + token] : (2ull << token) - 1;
                 if (w.q.limit - w.q.ctx < 64) seen &= (1ull << (w.q.limit - w.q.ctx)) - 1;
             }
             auto pages_of = [&](uint32_t tile) {  // whether the lane's page of the tile is there
@@ -564,6 +568,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                             __stcg(reinterpret_cast<float4 *>(part_out + (uint64_t)row * HD + e), y[k]);
                     }
                 }
+            if (whole && a.stats && live && (WIDE || s == 0)) {
+                const uint32_t f = w.rt * MR + f_row, t0 = f * magic >> 16;
+                a.stats[(uint64_t)(w.q.row0 + t0) * a.group * a.pg.n_kv + w.head * a.group + f - t0 * a.group] = make_float2(peak - PG_RAISE<T>, norm);
+            }
             if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
             if (!whole && origin >= begin && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
                 a.pieces[blockIdx.x] = PagePiece{(origin + w.q.n_tiles - 1) / w.per - blockIdx.x + 1, 2 * blockIdx.x + (origin > begin ? 1u : 0u), min(n_rows, MR), w.rt * MR, w.q.row0, w.head};
@@ -607,6 +615,7 @@ __global__ void __launch_bounds__(256) pages_merge_kernel(const __grid_constant_
     }
     const float g = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;
     const uint32_t f = p.row + row;
+    if (a.stats && c == 0) a.stats[(uint64_t)(p.token0 + f / a.group) * a.group * a.pg.n_kv + p.head * a.group + f % a.group] = make_float2(top - PG_RAISE<T>, g);
     *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (uint64_t)(p.token0 + f / a.group) * a.out_stride + (uint64_t)(p.head * a.group + f % a.group) * HD + 4 * c) =
         make_uint2(pack16<T>(x.x * g, x.y * g), pack16<T>(x.z * g, x.w * g));
 }
@@ -630,13 +639,14 @@ cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStre
     auto kernel = pages_tree_tc5_kernel<T, HD, WIDE>;
     static PerDeviceOnce once;
     if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES); })) return e;
-    a.row_tiles = (a.max_drafts * a.group + P::MR - 1) / P::MR;
-    const uint32_t ctas = std::min<uint32_t>({(uint32_t)sm_count, PG_COUNTERS, (uint32_t)(PG_PARTIAL / (2 * P::PART * 4))});
+    const uint32_t most = std::min(a.max_drafts, a.block);  // tokens of a unit
+    a.row_tiles = (most * a.group + P::MR - 1) / P::MR;
+    const uint32_t ctas = std::min<uint32_t>({(uint32_t)sm_count, PG_COUNTERS, (uint32_t)(PG_PARTS / (2 * P::PART * 4))});
     static_assert(sizeof(PageMaps) == 2 * sizeof(CUtensorMap), "two maps");
     CUtensorMap tm[2];
     memcpy(tm, &maps, sizeof(tm));
     if (cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(PG_THREADS), P::BYTES, st, tm[0], tm[1], a)) return e;
-    const uint32_t rows = std::min(P::MR, a.max_drafts * a.group), per = 256 / (HD / 4);
+    const uint32_t rows = std::min(P::MR, most * a.group), per = 256 / (HD / 4);
     return launch_pdl(pages_merge_kernel<T, HD, P::MR>, dim3(ctas, (rows + per - 1) / per), dim3(256), 0, st, a);
 }
 
@@ -655,7 +665,7 @@ bool make_page_maps(const PageView &pg, PageMaps *out) {
 }
 
 cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st) {
-    const bool wide = a.max_drafts * a.group > PG_ROWS;
+    const bool wide = std::min(a.max_drafts, a.block) * a.group > PG_ROWS;
     if (a.pg.is_bf16) {
         if (a.pg.dim == 64) return wide ? launch<bf16, 64, true>(a, maps, sm_count, st) : launch<bf16, 64, false>(a, maps, sm_count, st);
         return wide ? launch<bf16, 128, true>(a, maps, sm_count, st) : launch<bf16, 128, false>(a, maps, sm_count, st);
