@@ -707,22 +707,21 @@ int ob_pages_attention_tokens(ob_pages *p, uint32_t layer, uint32_t n_seq, const
     a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_tokens, a.max_ctx = max_ctx;
     use_workspace(p, a);
     if (mass) a.stats = reinterpret_cast<float2 *>(p->ws.mem + PG_WORKSPACE - PG_STATS);
-    a.block = q4 ? std::max(1u, PG_FEW_ROWS / a.group) : PG_MAX_DRAFTS;
-    a.block = std::min(a.block, max_tokens);
+    a.block = std::min(PG_MAX_DRAFTS, max_tokens);
     a.blocks = (max_tokens + a.block - 1) / a.block;
     const uint64_t units = (uint64_t)n_seq * a.blocks;
-    const bool wide = !q4 && a.block * a.group > PG_FEW_ROWS;
+    const bool wide = a.block * a.group > PG_FEW_ROWS;
     // (a walk over all pieces counts their pages or tiles, and PG_START more for each, in 31 bits)
     if (units >= (1ull << 24) || (wide && units * p->d.n_head_kv * (((uint64_t)p->d.table_stride + PG_PAGES - 1) / PG_PAGES + PG_START) * ((a.block * a.group + 127) / 128) >= (1ull << 31)))
         return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tokens: too many tokens, or the tables of all sequences together have room for too many positions");
     a.n_units = (uint32_t)units;
     const cudaStream_t st = stream_of(p, stream);
-    const cudaError_t e = q4 ? launch_pages_q4_attention(a, q_type == OB_TYPE_BF16, p->ctx->sm_count, st)
-                        : wide ? launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, st)
-                               : launch_pages_attention(a, true, p->ctx->sm_count, st);
+    const bool q_bf16 = q_type == OB_TYPE_BF16;
+    const cudaError_t e = q4 ? (wide ? launch_pages_q4_tc5(a, q_bf16, p->ctx->sm_count, st) : launch_pages_q4_attention(a, q_bf16, p->ctx->sm_count, st))
+                             : (wide ? launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, st) : launch_pages_attention(a, true, p->ctx->sm_count, st));
     if (int rc = launched(p, who, e, wide ? 2 : 1)) return rc;
     if (!mass) return OB_OK;
-    return launched(p, who, launch_pages_mass(a, q_type == OB_TYPE_BF16, q4, n_seq, mass, mass_stride, st));
+    return launched(p, who, launch_pages_mass(a, q_bf16, q4, n_seq, mass, mass_stride, st));
 }
 
 namespace {

@@ -56,7 +56,7 @@ struct PagedAttnArgs {
     const uint32_t *n_ctx;    // [n_units]
     const uint64_t *visible;  // [n_tokens]
     uint32_t n_tokens, max_drafts, max_ctx;  // visible may be null: a token sees those before it and itself
-    uint32_t block, blocks;   // tokens of a unit, units of a sequence (n_units: all of them); several with visible == null (or in 4-bit pages)
+    uint32_t block, blocks;   // tokens of a unit, units of a sequence (n_units: all of them); several with visible == null only
     float2 *stats;            // [n_tokens][n_kv * group] or null: a row's maximum and the inverse of its sum, so that a weight is 2^(score - maximum) times that
     // list
     const int32_t *list;      // [n_units][n_kv][n_list]
@@ -82,8 +82,9 @@ bool make_page_maps(const PageView &pg, PageMaps *out);  // false: the pool has 
 cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st);
 cudaError_t launch_pages_wait_selftest(uint32_t *status, cudaStream_t st);  // a warp whose wait runs out, and then ends as that kernel does
 
-// 4-bit pages, any number of rows: blocks of tokens that have at most PG_FEW_ROWS.
+// 4-bit pages: units of tokens that have at most PG_FEW_ROWS, and of up to PG_MAX_DRAFTS tokens.
 cudaError_t launch_pages_q4_attention(const PagedAttnArgs &a, bool q_bf16, int sm_count, cudaStream_t st);
+cudaError_t launch_pages_q4_tc5(const PagedAttnArgs &a, bool q_bf16, int sm_count, cudaStream_t st);
 // After an attention with `stats`, whose units are of n_seq sequences: [n_seq][n_kv][mass_stride].
 cudaError_t launch_pages_mass(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, cudaStream_t st);
 

@@ -32,6 +32,7 @@
 
 #include "mixers_common.cuh"
 #include "pages.h"
+#include "pages_q4.cuh"
 #include "tc5_common.cuh"
 
 namespace ob {
@@ -40,6 +41,7 @@ namespace {
 
 constexpr uint32_t PG_ROWS = 128, PG_KEYS = PG_PAGES * KV_PAGE, PG_BLOCK = PG_KEYS * 128, PG_QBLOCK = PG_ROWS * 128;  // a tile's positions; blocks of 64 columns
 constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 12 * 32;
+constexpr int P4_CODE_WARPS = 6, P4_THREADS = (PG_TMA_WARP + P4_CODE_WARPS) * 32;  // over 4-bit pages: three warps for keys, three for values
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr uint32_t PG_LEAST = 4;        // units of a CTA
 
@@ -48,7 +50,7 @@ constexpr uint32_t PG_STAGES = 12;      // at most
 constexpr uint32_t PB_K_FULL = 0, PB_K_EMPTY = PB_K_FULL + 8 * PG_STAGES, PB_V_FULL = PB_K_EMPTY + 8 * PG_STAGES, PB_V_EMPTY = PB_V_FULL + 8 * PG_STAGES, PB_S_FULL = PB_V_EMPTY + 8 * PG_STAGES /* [stream][place] */,
                    PB_P_FULL = PB_S_FULL + 32, PB_PV_DONE = PB_P_FULL + 32, PB_O_FULL = PB_PV_DONE + 16, PB_Q_FULL = PB_O_FULL + 16, PB_SLOT = PB_Q_FULL + 8, PB_ABORT = PB_SLOT + 4, PB_ODD = PB_ABORT + 4,
                    PB_TOP = PB_ODD + 8, PB_BYTES = PB_TOP + 4 * PG_ROWS * 4;
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, bool Q4 = false>
 struct PgPlan {
     static constexpr uint32_t NB = HD / 64, OPERAND = NB * PG_BLOCK, ROWS = NB * PG_QBLOCK, Q = (WIDE ? 2 : 1) * ROWS;  // (16 KB at least: outputs leave by way of it)
     // Places of the two rings.  Values are wanted two steps after their keys: they get more.  Where the streams take every other tile, the numbers are
@@ -56,11 +58,14 @@ struct PgPlan {
     // for a place's next tile before the one before, the other stream's, has arrived.
     // Where both streams take all tiles, two share a place: half the waits (32 sequences of 8192 with 512 rows, bf16: 720 us, and 773 with a place a tile).
     static constexpr uint32_t G = WIDE ? 2 : 1, PLACE = G * OPERAND, FIT = (227 * 1024 - PB_BYTES - Q) / PLACE, EVEN = WIDE ? 1 : 2;
-    static constexpr uint32_t KST = std::min(FIT / 3 / EVEN * EVEN + WIDE, PG_STAGES), VST = std::min((FIT - KST) / EVEN * EVEN, PG_STAGES);
+    // Over 4-bit pages a place is always made by the same of three warps (waits go by parity here, too: a warp that went on to places that others had
+    // made before could take an earlier phase for the one it waits for): multiples of three where they fit.
+    static constexpr uint32_t KST = Q4 ? (FIT >= 12 ? 6 : 2) : std::min(FIT / 3 / EVEN * EVEN + WIDE, PG_STAGES);
+    static constexpr uint32_t VST = Q4 ? (FIT >= 18 ? 12 : FIT >= 12 ? 6 : 3) : std::min((FIT - KST) / EVEN * EVEN, PG_STAGES);
     static constexpr uint32_t K = Q, V = K + KST * PLACE, BAR = V + VST * PLACE, BYTES = BAR + PB_BYTES;
     static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
     static constexpr uint64_t PART = (uint64_t)MR * (HD + 2);  // floats of a partial result
-    static_assert(KST >= 2 && VST >= 3 && PG_STAGES % 2 == 0 && (WIDE || (KST % 2 == 0 && VST % 2 == 0)) && BYTES <= 227 * 1024, "shared memory");
+    static_assert(KST >= 2 && VST >= 3 && KST + VST <= FIT && PG_STAGES % 2 == 0 && (WIDE || (KST % 2 == 0 && VST % 2 == 0)) && BYTES <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b, float c) {
@@ -203,10 +208,56 @@ struct PgWalk {
     }
 };
 
-template <typename T, int HD, bool WIDE>
-__global__ void __launch_bounds__(PG_THREADS, 1)
+// 4-bit pages (layout: pages_q4.cuh): the entries are f16 numbers exactly, so that the operand tiles are those of an f16 cache, made by warps instead of TMA.  A warp
+// takes a place's keys (or values) at a time: from memory into registers, and as f16 into the swizzled rows, in two halves (whole
+// ones take more registers than the softmax warps leave).
+template <int HD, bool VALUE>
+struct P4Tile {
+    using B = Q4Block<HD>;
+    static constexpr uint32_t QUADS = HD / 32, PARTS = HD / 64, EACH = PG_KEYS * QUADS / 32 / PARTS;  // 16 bytes of codes: 32 entries with one unit; a row's, a lane's at a time
+    uint4 code[EACH];
+    uint32_t unit[EACH];
+
+    // id: lane p < PG_PAGES has the number of the tile's page p, or -1 (its entries are zero).
+    __device__ __forceinline__ void load(const uint8_t *pool, uint32_t n_kv, uint32_t head, int32_t id, uint32_t part) {
+        const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const uint32_t at = (part * EACH + i) * 32 + lane, place = at / QUADS % KV_PAGE, quad = at % QUADS;
+            const int32_t page = __shfl_sync(0xffffffffu, id, at / QUADS / KV_PAGE);
+            const uint8_t *block = pool + ((uint64_t)max(page, 0) * n_kv + head) * B::BYTES;
+            code[i] = __ldg(reinterpret_cast<const uint4 *>(block) + at % (KV_PAGE * QUADS));
+            const uint32_t q = VALUE && HD == 128 && (place & 2) ? quad ^ 2 : quad, pos = position(place);
+            unit[i] = page < 0 ? 0u : __ldg(reinterpret_cast<const uint16_t *>(block + B::unit(VALUE, pos, q)));
+        }
+    }
+    static __device__ __forceinline__ uint32_t position(uint32_t place) { return VALUE ? (place & 3) << 1 | (place >> 2 & 1) | (place & 8) : place; }
+    __device__ __forceinline__ void store(uint8_t *operand, uint32_t part) const {
+        const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const uint32_t at = (part * EACH + i) * 32 + lane, place = at / QUADS % KV_PAGE, quad = at % QUADS;
+            const uint32_t q = VALUE && HD == 128 && (place & 2) ? quad ^ 2 : quad, row = at / QUADS / KV_PAGE * KV_PAGE + position(place);
+            const uint32_t d = unit[i] * 0x10001u, n = q4_offset(d);
+            // eight lanes have two rows and all four quads: of the second two the order of the words is another, so that no two are in one bank
+            constexpr uint32_t SWAP = HD == 128 ? (VALUE ? 1 : 2) : 0;
+            const bool other = SWAP && (q & 2);
+            const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t x = other ? w[e ^ SWAP] : w[e], c = 4 * q + (other ? e ^ SWAP : e);
+                *reinterpret_cast<uint4 *>(operand + c / 8 * PG_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                    make_uint4(q4_field(x, 0, d, n), q4_field(x, 1, d, n), q4_field(x, 2, d, n), q4_field(x, 3, d, n));
+            }
+        }
+    }
+};
+
+template <typename T, int HD, bool WIDE, bool Q4>
+__global__ void __launch_bounds__(Q4 ? P4_THREADS : PG_THREADS, 1)
 pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
-    using P = PgPlan<HD, WIDE>;
+    using P = PgPlan<HD, WIDE, Q4>;
+    using TP = typename std::conditional<Q4, __half, T>::type;  // of the operands
     constexpr uint32_t KST = P::KST, VST = P::VST, G = P::G, PLACE = P::PLACE, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem);
@@ -246,7 +297,49 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     auto steps_of = [&](uint32_t s, uint32_t tiles, uint32_t rows) { return WIDE ? (s == 0 || rows > PG_ROWS ? tiles : 0u) : (tiles + 1 - s) / 2; };
     auto tile_of = [&](uint32_t s, uint32_t step) { return WIDE ? step : s + 2 * step; };
 
-    if (warp >= PG_TMA_WARP) {
+    if (Q4 && warp >= PG_TMA_WARP) {
+        if constexpr (Q4) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+            constexpr uint32_t TURNS = P4_CODE_WARPS / 2;
+            auto make = [&](auto value) {
+                constexpr bool VALUE = decltype(value)::value;
+                const uint32_t full = bar + (VALUE ? PB_V_FULL : PB_K_FULL), empty = bar + (VALUE ? PB_V_EMPTY : PB_K_EMPTY), mine = (warp - PG_TMA_WARP) / 2;
+                constexpr uint32_t PLACES = VALUE ? VST : KST;
+                const uint8_t *pool = static_cast<const uint8_t *>(VALUE ? a.pg.v : a.pg.k);
+                uint8_t *ring = smem + (VALUE ? P::V : P::K);
+                uint32_t n = 0;  // places so far
+                bool ok = true;
+                for (; w.more() && ok; w.next(a)) {
+                    const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
+                    const uint32_t end = w.last(), places = (end - w.tile + G - 1) / G;
+                    for (uint32_t k = 0; k < places && ok; ++k) {
+                        const uint32_t at = n + k, st = at % PLACES;
+                        if (st % TURNS != mine) continue;
+#pragma unroll 1
+                        for (uint32_t h = 0; h < G; ++h) {
+                            const uint32_t tile = w.tile + k * G + h, p = tile * PG_PAGES + lane % PG_PAGES;
+                            int32_t id = tile < end && p < w.q.n_pages ? table[p] : -1;
+                            if ((uint32_t)id >= a.pg.n_pages) id = -1;
+                            P4Tile<HD, VALUE> x;
+#pragma unroll 1
+                            for (uint32_t part = 0; part < x.PARTS; ++part) {
+                                x.load(pool, a.pg.n_kv, w.head, id, part);
+                                if (h == 0 && part == 0) ok = mbar_wait_warp(empty + 8 * st, ((at / PLACES) & 1u) ^ 1u, abort);  // (a place that was not used yet is empty)
+                                if (!ok) break;
+                                x.store(ring + st * PLACE + h * OPERAND, part);
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (ok && lane == 0) mbar_arrive(full + 8 * st);
+                    }
+                    n += places;
+                }
+            };
+            if ((warp - PG_TMA_WARP) & 1) make(std::true_type{});
+            else make(std::false_type{});
+        }
+    } else if (warp >= PG_TMA_WARP) {
         const bool values = warp > PG_TMA_WARP;
         const CUtensorMap *map = values ? &tm_v : &tm_k;
         const uint32_t ring = sbase + (values ? P::V : P::K), full = bar + (values ? PB_V_FULL : PB_K_FULL), empty = bar + (values ? PB_V_EMPTY : PB_K_EMPTY), places = values ? VST : KST;
@@ -275,7 +368,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             }
         }
     } else if (warp >= PG_MMA_WARP) {
-        constexpr uint32_t F16 = EXPONENT16<T> == EXPONENT16<bf16> ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
+        if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        constexpr uint32_t F16 = EXPONENT16<TP> == EXPONENT16<bf16> ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
         const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
         const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
         uint32_t n = 0, turn = 0, done = 0;  // places, pieces and tiles of the stream so far
@@ -329,11 +423,13 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             n += (tiles + G - 1) / G, done += steps;
         }
     } else if (warp < PG_MMA_WARP) {
+        if constexpr (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
         const uint32_t magic = (65536 + a.group - 1) / a.group;  // x / group = x magic / 65536 for x below 4096, group up to 16
-        const float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
+        float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
+        constexpr bool FACTORS = !std::is_same<T, TP>::value;
         const uint32_t lanes = tmem + ((quad * 32) << 16), ts = lanes + PG_TMEM_S + s * 2 * PG_KEYS, to = lanes + PG_TMEM_O;
-        volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][sum, maximum][row]
+        volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + r;  // [stream][sum, maximum][row]; before, in a sum's place, its thread's factor of the scores
         volatile uint32_t *odd = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + PB_ODD);
         bool ok = true;
         uint32_t used = 0, n = 0;   // tiles of the stream, places so far
@@ -358,6 +454,26 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 #pragma unroll
                 for (uint32_t k = 0; k < BATCH; ++k) {
                     const uint32_t i = (t + k) * PG_SOFT + threadIdx.x, row = i / WORDS, c = i % WORDS;
+                    if constexpr (FACTORS) {  // bfloat16 queries become f16 ones after a power of two per row has been taken out (pages_q4.cu)
+                        uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w}, top = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7fffu, u[e] >> 16 & 0x7fffu));
+#pragma unroll
+                        for (uint32_t o = 1; o < WORDS; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int e = top == 0 || top >= 0x7f80u ? 0 : max(-112, min(112, 14 - ((int)(top >> 7) - 127)));
+                        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float2 f = unpack16(u[x], T());
+                            u[x] = pack16<TP>(f.x * up, f.y * up);
+                        }
+                        v[k] = make_uint4(u[0], u[1], u[2], u[3]);
+                        if (c == 0) {
+                            volatile float *factor = reinterpret_cast<volatile float *>(smem + P::BAR + PB_TOP) + row % PG_ROWS;
+                            factor[row / PG_ROWS * 2 * PG_ROWS] = __uint_as_float((uint32_t)(127 - e) << 23);
+                            if (!WIDE) factor[2 * PG_ROWS] = __uint_as_float((uint32_t)(127 - e) << 23);
+                        }
+                    }
                     *reinterpret_cast<uint4 *>(smem + row / PG_ROWS * ROWS + c / 8 * PG_QBLOCK + row % PG_ROWS * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[k];
                 }
             }
@@ -365,6 +481,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar + PB_Q_FULL);
+            if constexpr (FACTORS) {
+                soft_sync();
+                scale2 = a.scale * 1.4426950408889634f * xchg[2 * s * PG_ROWS];
+            }
             uint64_t seen = 0;
             if (live && w.q.ctx < end * PG_KEYS) {
                 const uint32_t token = (w.rt * MR + f_row) / a.group;
@@ -402,8 +522,8 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                                 bool here = false;
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    if ((u[e] & EXPONENT16<T>) == EXPONENT16<T>) u[e] &= 0xffff0000u, here = true;
-                                    if ((u[e] >> 16 & EXPONENT16<T>) == EXPONENT16<T>) u[e] &= 0xffffu, here = true;
+                                    if ((u[e] & EXPONENT16<TP>) == EXPONENT16<TP>) u[e] &= 0xffff0000u, here = true;
+                                    if ((u[e] >> 16 & EXPONENT16<TP>) == EXPONENT16<TP>) u[e] &= 0xffffu, here = true;
                                 }
                                 if (here) *at = make_uint4(u[0], u[1], u[2], u[3]), bad = true;
                             }
@@ -442,7 +562,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     float sum0, sum1;
 #pragma unroll 1
                     for (;;) {
-                        const float base = m == -INFINITY ? 0.0f : PG_RAISE<T> - m;  // (still nothing: weights of zero)
+                        const float base = m == -INFINITY ? 0.0f : PG_RAISE<TP> - m;  // (still nothing: weights of zero)
                         float top[2] = {-INFINITY, -INFINITY};
                         sum0 = sum1 = 0.0f;
 #pragma unroll
@@ -456,9 +576,9 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                                 fma2(e0, e1, x0, x1, scale2, base);
                                 e0 = pow2(e0), e1 = pow2(e1);
                                 add2(sum0, sum1, e0, e1);
-                                v[e] = pack16<T>(e0, e1);
-                                const float2 r = unpack16(v[e], T());
-                                v[8 + e] = pack16<T>(e0 - r.x, e1 - r.y);
+                                v[e] = pack16<TP>(e0, e1);
+                                const float2 r = unpack16(v[e], TP());
+                                v[8 + e] = pack16<TP>(e0 - r.x, e1 - r.y);
                             }
                             tmem_st16(tp + 16 * g, v);
                         }
@@ -530,7 +650,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         x[e] = __uint_as_float(o0[e]) * g0;
                         if (!WIDE && had[1]) x[e] = fmaf(__uint_as_float(o1[e]), g1, x[e]);  // (a stream without tiles has left nothing there)
                     }
-                    if (special && live) {  // values that are no numbers, of drafted tokens that this row sees (their weights are above zero)
+                    if (!Q4 && special && live) {  // values that are no numbers, of drafted tokens that this row sees (their weights are above zero)
 #pragma unroll 1
                         for (uint32_t j = 0; j < w.q.limit - w.q.ctx; ++j) {
                             const uint32_t pos = w.q.ctx + j;
@@ -570,7 +690,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 }
             if (whole && a.stats && live && (WIDE || s == 0)) {
                 const uint32_t f = w.rt * MR + f_row, t0 = f * magic >> 16;
-                a.stats[(uint64_t)(w.q.row0 + t0) * a.group * a.pg.n_kv + w.head * a.group + f - t0 * a.group] = make_float2(peak - PG_RAISE<T>, norm);
+                a.stats[(uint64_t)(w.q.row0 + t0) * a.group * a.pg.n_kv + w.head * a.group + f - t0 * a.group] = make_float2(peak - PG_RAISE<TP>, norm);
             }
             if (!whole && live && (WIDE || s == 0)) __stcg(reinterpret_cast<float2 *>(part_out + (uint64_t)MR * HD + 2 * f_row), make_float2(peak, sum));
             if (!whole && origin >= begin && threadIdx.x == 0) {  // the piece begins here and goes on in other CTAs (one piece at most)
@@ -591,7 +711,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 }
 
 // grid (CTAs of the kernel above, rows / ROWS): the parts of the piece that began in a CTA, four columns a thread.
-template <typename T, int HD, uint32_t MR>
+template <typename T, int HD, uint32_t MR, bool Q4>
 __global__ void __launch_bounds__(256) pages_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr uint32_t VEC = HD / 4, ROWS = 256 / VEC;
     constexpr uint64_t PART = (uint64_t)MR * (HD + 2);
@@ -615,7 +735,7 @@ __global__ void __launch_bounds__(256) pages_merge_kernel(const __grid_constant_
     }
     const float g = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;
     const uint32_t f = p.row + row;
-    if (a.stats && c == 0) a.stats[(uint64_t)(p.token0 + f / a.group) * a.group * a.pg.n_kv + p.head * a.group + f % a.group] = make_float2(top - PG_RAISE<T>, g);
+    if (a.stats && c == 0) a.stats[(uint64_t)(p.token0 + f / a.group) * a.group * a.pg.n_kv + p.head * a.group + f % a.group] = make_float2(top - PG_RAISE<typename std::conditional<Q4, __half, T>::type>, g);
     *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (uint64_t)(p.token0 + f / a.group) * a.out_stride + (uint64_t)(p.head * a.group + f % a.group) * HD + 4 * c) =
         make_uint2(pack16<T>(x.x * g, x.y * g), pack16<T>(x.z * g, x.w * g));
 }
@@ -633,10 +753,10 @@ __global__ void __launch_bounds__(32) pages_wait_selftest_kernel(uint32_t *statu
     if (!ok && *reinterpret_cast<volatile uint32_t *>(&abort)) gave_up(status);
 }
 
-template <typename T, int HD, bool WIDE>
+template <typename T, int HD, bool WIDE, bool Q4>
 cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStream_t st) {
-    using P = PgPlan<HD, WIDE>;
-    auto kernel = pages_tree_tc5_kernel<T, HD, WIDE>;
+    using P = PgPlan<HD, WIDE, Q4>;
+    auto kernel = pages_tree_tc5_kernel<T, HD, WIDE, Q4>;
     static PerDeviceOnce once;
     if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES); })) return e;
     const uint32_t most = std::min(a.max_drafts, a.block);  // tokens of a unit
@@ -645,9 +765,9 @@ cudaError_t launch(PagedAttnArgs a, const PageMaps &maps, int sm_count, cudaStre
     static_assert(sizeof(PageMaps) == 2 * sizeof(CUtensorMap), "two maps");
     CUtensorMap tm[2];
     memcpy(tm, &maps, sizeof(tm));
-    if (cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(PG_THREADS), P::BYTES, st, tm[0], tm[1], a)) return e;
+    if (cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(Q4 ? P4_THREADS : PG_THREADS), P::BYTES, st, tm[0], tm[1], a)) return e;
     const uint32_t rows = std::min(P::MR, most * a.group), per = 256 / (HD / 4);
-    return launch_pdl(pages_merge_kernel<T, HD, P::MR>, dim3(ctas, (rows + per - 1) / per), dim3(256), 0, st, a);
+    return launch_pdl(pages_merge_kernel<T, HD, P::MR, Q4>, dim3(ctas, (rows + per - 1) / per), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -664,15 +784,18 @@ bool make_page_maps(const PageView &pg, PageMaps *out) {
     return true;
 }
 
-cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st) {
+template <bool Q4>
+static cudaError_t launch_type(const PagedAttnArgs &a, bool is_bf16, const PageMaps &maps, int sm_count, cudaStream_t st) {
     const bool wide = std::min(a.max_drafts, a.block) * a.group > PG_ROWS;
-    if (a.pg.is_bf16) {
-        if (a.pg.dim == 64) return wide ? launch<bf16, 64, true>(a, maps, sm_count, st) : launch<bf16, 64, false>(a, maps, sm_count, st);
-        return wide ? launch<bf16, 128, true>(a, maps, sm_count, st) : launch<bf16, 128, false>(a, maps, sm_count, st);
+    if (is_bf16) {
+        if (a.pg.dim == 64) return wide ? launch<bf16, 64, true, Q4>(a, maps, sm_count, st) : launch<bf16, 64, false, Q4>(a, maps, sm_count, st);
+        return wide ? launch<bf16, 128, true, Q4>(a, maps, sm_count, st) : launch<bf16, 128, false, Q4>(a, maps, sm_count, st);
     }
-    if (a.pg.dim == 64) return wide ? launch<__half, 64, true>(a, maps, sm_count, st) : launch<__half, 64, false>(a, maps, sm_count, st);
-    return wide ? launch<__half, 128, true>(a, maps, sm_count, st) : launch<__half, 128, false>(a, maps, sm_count, st);
+    if (a.pg.dim == 64) return wide ? launch<__half, 64, true, Q4>(a, maps, sm_count, st) : launch<__half, 64, false, Q4>(a, maps, sm_count, st);
+    return wide ? launch<__half, 128, true, Q4>(a, maps, sm_count, st) : launch<__half, 128, false, Q4>(a, maps, sm_count, st);
 }
+cudaError_t launch_pages_tree_tc5(const PagedAttnArgs &a, const PageMaps &maps, int sm_count, cudaStream_t st) { return launch_type<false>(a, a.pg.is_bf16, maps, sm_count, st); }
+cudaError_t launch_pages_q4_tc5(const PagedAttnArgs &a, bool q_bf16, int sm_count, cudaStream_t st) { return launch_type<true>(a, q_bf16, PageMaps{}, sm_count, st); }
 
 cudaError_t launch_pages_wait_selftest(uint32_t *status, cudaStream_t st) {
     pages_wait_selftest_kernel<<<1, 32, 0, st>>>(status);

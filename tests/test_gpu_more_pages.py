@@ -91,7 +91,7 @@ class Held:
                 for p in (self.kd, self.vd)]
 
 
-def run_tokens(made, group, ctx, counts, bits=None, weighed=False, extra=0, strides=(0, 0), max_tokens=None, max_context=None, layer=0, q_kind=None, q_std=1.5, scale=None, compare=True):
+def run_tokens(made, group, ctx, counts, bits=None, weighed=False, extra=0, strides=(0, 0), max_tokens=None, max_context=None, layer=0, q_kind=None, q_std=1.5, scale=None, compare=True, heads_of_kv=None):
     """Calls attention_tokens and compares; `extra` rows behind the last token, `strides` entries between rows."""
     import torch
 
@@ -111,13 +111,20 @@ def run_tokens(made, group, ctx, counts, bits=None, weighed=False, extra=0, stri
     made.cache.attention_tokens(qd, ints(first), ints(ctx), scale, out, max_tokens=max(list(counts) + [1]) if max_tokens is None else max_tokens,
                                 max_context=max(list(ctx) + [0]) if max_context is None else max_context, visible=words(bits + [0] * extra) if bits is not None else None, mass=md, layer=layer,
                                 stream=current())
-    torch.cuda.synchronize()
+    made.cache.synchronize(current())  # (says so if a wait inside a kernel was given up)
     if not compare:
         return out, md
     want = np.full((n, heads, dim), 7.0)
     mass64 = mass.astype(np.float64) if weighed else None
-    tol, mass_tol = more.attend_tokens(q, made.k[layer], made.v[layer], made.there, first, ctx, bits, scale, want, mass64, weight_error(dim))
-    got = float64(out)
+    if heads_of_kv is not None:  # of heads apart only, by way of a cache that has those alone
+        heads_of = np.concatenate([np.arange(h * group, (h + 1) * group) for h in heads_of_kv])
+        pick = lambda x: [s[:, list(heads_of_kv)] for s in x]  # noqa: E731
+        got, want, k, v, q = float64(out)[:, heads_of], want[:, heads_of], pick(made.k[layer]), pick(made.v[layer]), q[:, heads_of]
+        mass64 = mass64[:, list(heads_of_kv)] if weighed else None
+        md = md[:, list(heads_of_kv)] if weighed else None
+    else:
+        got, k, v = float64(out), made.k[layer], made.v[layer]
+    tol, mass_tol = more.attend_tokens(q, k, v, made.there, first, ctx, bits, scale, want, mass64, weight_error(dim))
     assert np.isfinite(got).all()
     off = np.abs(got - want) - (tol[..., None] + U[kind] * (np.abs(want) + tol[..., None]) + 2.0 ** -25)
     assert off.max(initial=-1.0) <= 0, f"{off.max()} over the bound at {np.unravel_index(off.argmax(), off.shape)}"
@@ -235,6 +242,14 @@ def test_parts_of_prompts(backend, pages, kind, dim, group, ctx, counts):
     made = Held(backend, pages, kind, 2, dim, [a + b for a, b in zip(ctx, counts)], seed=dim + group)
     run_tokens(made, group, ctx, counts, None, weighed=True)
     run_tokens(made, group, ctx, counts, None, strides=(24, 8), extra=1)
+
+
+@pytest.mark.parametrize("dim,group,counts", [(128, 8, [64, 40]), (64, 8, [64, 1]), (128, 4, [32, 20]), (64, 2, [60, 64]), (128, 16, [70, 9])])
+def test_many_tiles_with_many_rows(backend, dim, group, counts):
+    """More than twice as many tiles a CTA as its rings have places, in pieces of odd and even numbers of tiles."""
+    ctx = [9000, 4100]
+    made = Held(backend, "q4", "bf16", 8, dim, [a + b for a, b in zip(ctx, counts)], seed=dim + group)
+    run_tokens(made, group, ctx, counts, None, weighed=group == 2, heads_of_kv=(0, 7))
 
 
 @pytest.mark.parametrize("pages,kind,dim,group,counts", [("q4", "f16", 128, 4, [1, 1, 1]), ("q4", "bf16", 64, 4, [4, 1, 2]), ("bf16", "bf16", 128, 8, [1, 2, 1]), ("q4", "bf16", 128, 2, [20, 3, 40])])
