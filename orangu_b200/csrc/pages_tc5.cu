@@ -41,7 +41,7 @@ namespace {
 
 constexpr uint32_t PG_ROWS = 128, PG_KEYS = PG_PAGES * KV_PAGE, PG_BLOCK = PG_KEYS * 128, PG_QBLOCK = PG_ROWS * 128;  // a tile's positions; blocks of 64 columns
 constexpr int PG_SOFT = 256, PG_MMA_WARP = 8, PG_TMA_WARP = 10, PG_THREADS = 12 * 32;
-constexpr int P4_CODE_WARPS = 6, P4_THREADS = (PG_TMA_WARP + P4_CODE_WARPS) * 32;  // over 4-bit pages: three warps for keys, three for values
+constexpr int P4_TURNS = 2, P4_CODE_WARPS = 2 * P4_TURNS, P4_AHEAD = 2, P4_THREADS = 16 * 32;  // over 4-bit pages: warps for keys and for values; their tiles under way; whole warpgroups
 constexpr uint32_t PG_TMEM_S = 0, PG_TMEM_O = 256, PG_TMEM_COLS = 512;
 constexpr uint32_t PG_LEAST = 4;        // units of a CTA
 
@@ -57,12 +57,13 @@ struct PgPlan {
     // even, so that a place is always the same stream's within a piece: waits go by the parity of a phase, and a stream that runs ahead must not ask
     // for a place's next tile before the one before, the other stream's, has arrived.
     // Where both streams take all tiles, two share a place: half the waits (32 sequences of 8192 with 512 rows, bf16: 720 us, and 773 with a place a tile).
-    static constexpr uint32_t G = WIDE ? 2 : 1, PLACE = G * OPERAND, FIT = (227 * 1024 - PB_BYTES - Q) / PLACE, EVEN = WIDE ? 1 : 2;
-    // Over 4-bit pages a place is always made by the same of three warps (waits go by parity here, too: a warp that went on to places that others had
-    // made before could take an earlier phase for the one it waits for): multiples of three where they fit.
-    static constexpr uint32_t KST = Q4 ? (FIT >= 12 ? 6 : 2) : std::min(FIT / 3 / EVEN * EVEN + WIDE, PG_STAGES);
-    static constexpr uint32_t VST = Q4 ? (FIT >= 18 ? 12 : FIT >= 12 ? 6 : 3) : std::min((FIT - KST) / EVEN * EVEN, PG_STAGES);
-    static constexpr uint32_t K = Q, V = K + KST * PLACE, BAR = V + VST * PLACE, BYTES = BAR + PB_BYTES;
+    static constexpr uint32_t P4_CODES = Q4 ? P4_CODE_WARPS * P4_AHEAD * PG_PAGES * Q4Block<HD>::BYTES : 0;  // codes on their way
+    static constexpr uint32_t G = WIDE && !Q4 ? 2 : 1, PLACE = G * OPERAND, FIT = (227 * 1024 - PB_BYTES - Q - P4_CODES) / PLACE, EVEN = WIDE ? 1 : 2;
+    // Over 4-bit pages a place is always made by the same warp (waits go by parity here, too: a warp that went on to places that others had made
+    // before could take an earlier phase for the one it waits for): multiples of P4_TURNS.
+    static constexpr uint32_t KST = Q4 ? (FIT >= 20 ? 8 : FIT >= 8 ? 4 : 2) : std::min(FIT / 3 / EVEN * EVEN + WIDE, PG_STAGES);
+    static constexpr uint32_t VST = Q4 ? (FIT >= 20 ? 12 : 4) : std::min((FIT - KST) / EVEN * EVEN, PG_STAGES);
+    static constexpr uint32_t K = Q, V = K + KST * PLACE, CODES = V + VST * PLACE, BAR = CODES + P4_CODES, BYTES = BAR + PB_BYTES;
     static constexpr uint32_t MR = WIDE ? 2 * PG_ROWS : PG_ROWS;
     static constexpr uint64_t PART = (uint64_t)MR * (HD + 2);  // floats of a partial result
     static_assert(KST >= 2 && VST >= 3 && KST + VST <= FIT && PG_STAGES % 2 == 0 && (WIDE || (KST % 2 == 0 && VST % 2 == 0)) && BYTES <= 227 * 1024, "shared memory");
@@ -209,40 +210,37 @@ struct PgWalk {
 };
 
 // 4-bit pages (layout: pages_q4.cuh): the entries are f16 numbers exactly, so that the operand tiles are those of an f16 cache, made by warps instead of TMA.  A warp
-// takes a place's keys (or values) at a time: from memory into registers, and as f16 into the swizzled rows, in two halves (whole
-// ones take more registers than the softmax warps leave).
+// has a tile's keys (or values) at a time: codes and units come by cp.async into places of its own, a tile ahead, and go as f16 into the swizzled rows.
 template <int HD, bool VALUE>
 struct P4Tile {
     using B = Q4Block<HD>;
-    static constexpr uint32_t QUADS = HD / 32, PARTS = HD / 64, EACH = PG_KEYS * QUADS / 32 / PARTS;  // 16 bytes of codes: 32 entries with one unit; a row's, a lane's at a time
-    uint4 code[EACH];
-    uint32_t unit[EACH];
+    static constexpr uint32_t QUADS = HD / 32, EACH = PG_KEYS * QUADS / 32, WORDS = B::BYTES / 16, BYTES = PG_PAGES * B::BYTES;  // 16 bytes of codes: 32 entries with one unit; a row's, a lane's
 
-    // id: lane p < PG_PAGES has the number of the tile's page p, or -1 (its entries are zero).
-    __device__ __forceinline__ void load(const uint8_t *pool, uint32_t n_kv, uint32_t head, int32_t id, uint32_t part) {
+    // id: lane p < PG_PAGES has the number of the tile's page p, or -1 (zeros: its entries are zero).
+    static __device__ __forceinline__ void request(uint32_t dst, const uint8_t *pool, uint32_t n_kv, uint32_t head, int32_t id) {
         const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i) {
-            const uint32_t at = (part * EACH + i) * 32 + lane, place = at / QUADS % KV_PAGE, quad = at % QUADS;
-            const int32_t page = __shfl_sync(0xffffffffu, id, at / QUADS / KV_PAGE);
+        for (uint32_t p = 0; p < PG_PAGES; ++p) {
+            const int32_t page = __shfl_sync(0xffffffffu, id, p);
             const uint8_t *block = pool + ((uint64_t)max(page, 0) * n_kv + head) * B::BYTES;
-            code[i] = __ldg(reinterpret_cast<const uint4 *>(block) + at % (KV_PAGE * QUADS));
-            const uint32_t q = VALUE && HD == 128 && (place & 2) ? quad ^ 2 : quad, pos = position(place);
-            unit[i] = page < 0 ? 0u : __ldg(reinterpret_cast<const uint16_t *>(block + B::unit(VALUE, pos, q)));
+#pragma unroll
+            for (uint32_t c = lane; c < WORDS; c += 32) cp16(dst + p * B::BYTES + c * 16, block + c * 16, page >= 0);
         }
     }
-    static __device__ __forceinline__ uint32_t position(uint32_t place) { return VALUE ? (place & 3) << 1 | (place >> 2 & 1) | (place & 8) : place; }
-    __device__ __forceinline__ void store(uint8_t *operand, uint32_t part) const {
-        const uint32_t lane = threadIdx.x & 31;
-#pragma unroll
+    static __device__ __forceinline__ void make(const uint8_t *src, uint8_t *operand) {
+        uint32_t lane = threadIdx.x & 31;
+        asm volatile("" : "+r"(lane));  // (places are worked out where they are used)
+#pragma unroll 1
         for (uint32_t i = 0; i < EACH; ++i) {
-            const uint32_t at = (part * EACH + i) * 32 + lane, place = at / QUADS % KV_PAGE, quad = at % QUADS;
-            const uint32_t q = VALUE && HD == 128 && (place & 2) ? quad ^ 2 : quad, row = at / QUADS / KV_PAGE * KV_PAGE + position(place);
-            const uint32_t d = unit[i] * 0x10001u, n = q4_offset(d);
+            const uint32_t at = i * 32 + lane, page = at / QUADS / KV_PAGE, place = at / QUADS % KV_PAGE, quad = at % QUADS;
+            const uint32_t pos = VALUE ? (place & 3) << 1 | (place >> 2 & 1) | (place & 8) : place, q = VALUE && HD == 128 && (place & 2) ? quad ^ 2 : quad, row = page * KV_PAGE + pos;
+            const uint8_t *block = src + page * B::BYTES;
+            const uint4 code = reinterpret_cast<const uint4 *>(block)[at % (KV_PAGE * QUADS)];
+            const uint32_t d = *reinterpret_cast<const uint16_t *>(block + B::unit(VALUE, pos, q)) * 0x10001u, n = q4_offset(d);
             // eight lanes have two rows and all four quads: of the second two the order of the words is another, so that no two are in one bank
             constexpr uint32_t SWAP = HD == 128 ? (VALUE ? 1 : 2) : 0;
             const bool other = SWAP && (q & 2);
-            const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+            const uint32_t w[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
                 const uint32_t x = other ? w[e ^ SWAP] : w[e], c = 4 * q + (other ? e ^ SWAP : e);
@@ -299,45 +297,54 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 
     if (Q4 && warp >= PG_TMA_WARP) {
         if constexpr (Q4) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-            constexpr uint32_t TURNS = P4_CODE_WARPS / 2;
-            auto make = [&](auto value) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+            auto make = [&](auto value, uint32_t mine) {
                 constexpr bool VALUE = decltype(value)::value;
-                const uint32_t full = bar + (VALUE ? PB_V_FULL : PB_K_FULL), empty = bar + (VALUE ? PB_V_EMPTY : PB_K_EMPTY), mine = (warp - PG_TMA_WARP) / 2;
+                using Tile = P4Tile<HD, VALUE>;
                 constexpr uint32_t PLACES = VALUE ? VST : KST;
+                static_assert(PLACES % P4_TURNS == 0 && G == 1, "a place is always the same warp's");
+                const uint32_t full = bar + (VALUE ? PB_V_FULL : PB_K_FULL), empty = bar + (VALUE ? PB_V_EMPTY : PB_K_EMPTY);
                 const uint8_t *pool = static_cast<const uint8_t *>(VALUE ? a.pg.v : a.pg.k);
-                uint8_t *ring = smem + (VALUE ? P::V : P::K);
-                uint32_t n = 0;  // places so far
-                bool ok = true;
-                for (; w.more() && ok; w.next(a)) {
-                    const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
-                    const uint32_t end = w.last(), places = (end - w.tile + G - 1) / G;
-                    for (uint32_t k = 0; k < places && ok; ++k) {
-                        const uint32_t at = n + k, st = at % PLACES;
-                        if (st % TURNS != mine) continue;
-#pragma unroll 1
-                        for (uint32_t h = 0; h < G; ++h) {
-                            const uint32_t tile = w.tile + k * G + h, p = tile * PG_PAGES + lane % PG_PAGES;
-                            int32_t id = tile < end && p < w.q.n_pages ? table[p] : -1;
-                            if ((uint32_t)id >= a.pg.n_pages) id = -1;
-                            P4Tile<HD, VALUE> x;
-#pragma unroll 1
-                            for (uint32_t part = 0; part < x.PARTS; ++part) {
-                                x.load(pool, a.pg.n_kv, w.head, id, part);
-                                if (h == 0 && part == 0) ok = mbar_wait_warp(empty + 8 * st, ((at / PLACES) & 1u) ^ 1u, abort);  // (a place that was not used yet is empty)
-                                if (!ok) break;
-                                x.store(ring + st * PLACE + h * OPERAND, part);
-                            }
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (ok && lane == 0) mbar_arrive(full + 8 * st);
+                uint8_t *own = smem + P::CODES + (warp - PG_TMA_WARP) * P4_AHEAD * Tile::BYTES;
+                // The warp's next tile: number `at` of all tiles, those of its places.
+                uint32_t at = mine, before = 0;  // tiles of the pieces before
+                auto request = [&](uint32_t slot) {
+                    for (; w.more() && at - before >= w.last() - w.tile; w.next(a)) before += w.last() - w.tile;
+                    if (w.more()) {
+                        const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
+                        const uint32_t p = (w.tile + at - before) * PG_PAGES + lane % PG_PAGES;
+                        int32_t id = p < w.q.n_pages ? table[p] : -1;
+                        if ((uint32_t)id >= a.pg.n_pages) id = -1;
+                        Tile::request(smem_addr(own) + slot * Tile::BYTES, pool, a.pg.n_kv, w.head, id);
                     }
-                    n += places;
+                    cp_commit();
+                    const bool any = w.more();
+                    at += P4_TURNS;
+                    return any;
+                };
+                bool ok = true;
+                uint32_t end = ~0u;  // the first of the warp's tiles that there is not
+#pragma unroll 1
+                for (uint32_t n = mine, slot = 0; ok; slot = slot + 1 == P4_AHEAD ? 0 : slot + 1) {
+                    if (!request(slot)) end = min(end, at - P4_TURNS);
+                    if (at < mine + P4_AHEAD * P4_TURNS) continue;  // (the first ones are only asked for)
+                    if (n >= end) break;
+                    cp_wait<P4_AHEAD - 1>();
+                    __syncwarp();
+                    const uint32_t st = n % PLACES, from = slot + 1 == P4_AHEAD ? 0 : slot + 1;
+                    ok = mbar_wait_warp(empty + 8 * st, ((n / PLACES) & 1u) ^ 1u, abort);  // (a place that was not used yet is empty)
+                    if (!ok) break;
+                    Tile::make(own + from * Tile::BYTES, smem + (VALUE ? P::V : P::K) + st * PLACE);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();  // (all of the warp's rows are written, and its codes read)
+                    if (lane == 0) mbar_arrive(full + 8 * st);
+                    n += P4_TURNS;
                 }
+                cp_wait<0>();
             };
-            if ((warp - PG_TMA_WARP) & 1) make(std::true_type{});
-            else make(std::false_type{});
+            const uint32_t role = warp - PG_TMA_WARP;  // (two warps only fill their warpgroup)
+            if (role < P4_CODE_WARPS && (role & 1)) make(std::true_type{}, role / 2);
+            else if (role < P4_CODE_WARPS) make(std::false_type{}, role / 2);
         }
     } else if (warp >= PG_TMA_WARP) {
         const bool values = warp > PG_TMA_WARP;
@@ -368,7 +375,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             }
         }
     } else if (warp >= PG_MMA_WARP) {
-        if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         constexpr uint32_t F16 = EXPONENT16<TP> == EXPONENT16<bf16> ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
         const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
         const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
@@ -423,7 +430,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             n += (tiles + G - 1) / G, done += steps;
         }
     } else if (warp < PG_MMA_WARP) {
-        if constexpr (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        if constexpr (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");  // 256 threads x 152 and 256 x 104 are the 512 x 128 of the launch
         const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
         const uint32_t magic = (65536 + a.group - 1) / a.group;  // x / group = x magic / 65536 for x below 4096, group up to 16
         float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
