@@ -19,6 +19,6 @@ struct DraftsVerifyArgs {
     uint32_t *n_kept;
     int32_t *next;
 };
-cudaError_t launch_drafts_verify(const DraftsVerifyArgs &a, uint32_t n_seq, uint32_t type, cudaStream_t st);  // type: 0 f32, 1 f16, 2 bf16
+cudaError_t launch_drafts_verify(const DraftsVerifyArgs &a, uint32_t n_seq, uint32_t type, int sm_count, cudaStream_t st);  // type: 0 f32, 1 f16, 2 bf16
 
 }  // namespace ob

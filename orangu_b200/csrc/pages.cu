@@ -721,7 +721,7 @@ int ob_pages_attention_tokens(ob_pages *p, uint32_t layer, uint32_t n_seq, const
                              : (wide ? launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, st) : launch_pages_attention(a, true, p->ctx->sm_count, st));
     if (int rc = launched(p, who, e, wide ? 2 : 1)) return rc;
     if (!mass) return OB_OK;
-    return launched(p, who, launch_pages_mass(a, q_bf16, q4, n_seq, mass, mass_stride, st));
+    return launched(p, who, launch_pages_mass(a, q_bf16, q4, n_seq, mass, mass_stride, p->ctx->sm_count, st));
 }
 
 namespace {
@@ -740,13 +740,13 @@ int move_rows(ob_pages *p, const char *who, bool load, uint32_t layer, uint32_t 
     if (int rc = check_rows(p, who, "v_stride", v_stride, p->d.n_head_kv)) return rc;
     max_tokens = std::min(max_tokens, n_tokens);
     if (n_seq == 0 || max_tokens == 0) return OB_OK;
-    if ((uint64_t)max_tokens * p->d.n_head_kv * 2 * (p->d.head_dim / 8) / 256 >= 0x7fffffffull) return fail(p->ctx, OB_ERR_CAPACITY, std::string(who) + ": too many tokens");
+    if ((uint64_t)max_tokens * p->d.n_head_kv * 2 > (1ull << 30)) return fail(p->ctx, OB_ERR_CAPACITY, std::string(who) + ": too many tokens");
     if (int rc = check_pointers(p, who, {{k, "k", 16}, {v, "v", 16}, {first_token, "first_token", 4}, {n_ctx, "n_ctx", 4}})) return rc;
     PagedMoveArgs a{};
     a.pg = view(p, layer);
     a.k = k, a.v = v, a.k_stride = k_stride, a.v_stride = v_stride;
     a.first = first_token, a.n_ctx = n_ctx, a.n_seq = n_seq, a.n_tokens = n_tokens, a.max_tokens = max_tokens;
-    return launched(p, who, launch_pages_store(a, type == OB_TYPE_BF16, load, stream_of(p, stream)));
+    return launched(p, who, launch_pages_store(a, type == OB_TYPE_BF16, load, p->ctx->sm_count, stream_of(p, stream)));
 }
 }  // namespace
 int ob_pages_store(ob_pages *p, uint32_t layer, uint32_t n_seq, const void *k, const void *v, uint32_t type, uint64_t k_stride, uint64_t v_stride, uint32_t n_tokens, const int32_t *first_token,
@@ -815,7 +815,7 @@ int ob_drafts_verify(ob_ctx *ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t n_
         if (!on_device(ctx, n.p)) return invalid(std::string(n.name) + " is not memory of the context's device");
     }
     DraftsVerifyArgs a{target, draft, target_stride, draft_stride, n_vocab, n_tokens, tokens, parent, first_token, uniform, kept, kept_stride, n_kept, next_token};
-    const cudaError_t e = launch_drafts_verify(a, n_seq, type == OB_TYPE_F32 ? 0 : type == OB_TYPE_F16 ? 1 : 2, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    const cudaError_t e = launch_drafts_verify(a, n_seq, type == OB_TYPE_F32 ? 0 : type == OB_TYPE_F16 ? 1 : 2, ctx->sm_count, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(ctx, OB_ERR_CUDA, std::string("drafts_verify: ") + cudaGetErrorString(e));

@@ -86,7 +86,7 @@ cudaError_t launch_pages_wait_selftest(uint32_t *status, cudaStream_t st);  // a
 cudaError_t launch_pages_q4_attention(const PagedAttnArgs &a, bool q_bf16, int sm_count, cudaStream_t st);
 cudaError_t launch_pages_q4_tc5(const PagedAttnArgs &a, bool q_bf16, int sm_count, cudaStream_t st);
 // After an attention with `stats`, whose units are of n_seq sequences: [n_seq][n_kv][mass_stride].
-cudaError_t launch_pages_mass(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, cudaStream_t st);
+cudaError_t launch_pages_mass(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, int sm_count, cudaStream_t st);
 
 struct PagedMoveArgs {  // rows into 4-bit pages, or out of them
     PageView pg;
@@ -96,7 +96,7 @@ struct PagedMoveArgs {  // rows into 4-bit pages, or out of them
     const uint32_t *n_ctx;
     uint32_t n_seq, n_tokens, max_tokens;
 };
-cudaError_t launch_pages_store(const PagedMoveArgs &a, bool is_bf16, bool load, cudaStream_t st);
+cudaError_t launch_pages_store(const PagedMoveArgs &a, bool is_bf16, bool load, int sm_count, cudaStream_t st);
 
 struct PagedEvictArgs {
     PageView pg;             // of layer 0

@@ -5,8 +5,13 @@
 // so that m itself is -8 d or a little less.  No number counts as 0, and magnitudes above 7168 as 7168, which keeps d an f16 number and every entry c d one, too.
 // The quotient comes from a product with about 1 / d; where that lies near the middle between two codes the division is done.
 //
-// Half a warp has a key's or value's 128 entries, eight a lane (a quarter 64).
+// Half a warp has a key's or value's 128 entries, eight a lane (a quarter 64), and the same head of several tokens, so that where a row lies is worked
+// out once for keys and values of all heads and the loads of two rows are under way at once.  The arithmetic is the larger part: about 100 instructions for eight
+// entries.  Maxima are taken two at a time in the rows' type; codes are whole numbers in the low bits of a sum with 1.5 2^23, put together as
+// one number of base 16 by fused multiply-adds.
 #include <algorithm>
+#include <numeric>
+#include <type_traits>
 
 #include "mixers_common.cuh"
 #include "pages.h"
@@ -27,100 +32,185 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, bf16) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Where position n_ctx[seq] + j lies, if row j of the sequence is to be moved: page, position within it, row.
-struct PgPlace {
-    bool there;
-    uint32_t page, p;
-    uint64_t row;
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {  // no number if either is none
+        uint32_t d;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
 };
-__device__ __forceinline__ PgPlace place(const PagedMoveArgs &a, uint32_t seq, uint32_t j) {
+template <> struct Pair<bf16> {
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+};
+constexpr uint32_t SIGNS = 0x80008000u;
+
+// The rows of a group of lanes: one head's keys or values of tokens j, j + step, ...
+struct PgRows {
+    uint32_t head, j, step, count, room;
+    bool value;
+    int32_t first;
+    uint32_t ctx;
+    const int32_t *table;
+};
+template <uint32_t ROWS>
+__device__ __forceinline__ PgRows rows_of(const PagedMoveArgs &a, uint32_t group) {
+    PgRows r;
+    const uint32_t per = 2 * a.pg.n_kv, i = blockIdx.x * ROWS + group, part = i % per, seq = blockIdx.y;
+    r.j = i / per, r.step = gridDim.x * ROWS / per;  // (the grid is made so that there is no remainder)
+    r.value = part >= a.pg.n_kv, r.head = r.value ? part - a.pg.n_kv : part;
     const int32_t f0 = a.first[seq], f1 = a.first[seq + 1];
-    const uint64_t x = (uint64_t)a.n_ctx[seq] + j;
-    PgPlace at{false, 0, (uint32_t)x % KV_PAGE, (uint64_t)(uint32_t)f0 + j};
-    if (f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens || j >= (uint32_t)(f1 - f0) || j >= a.max_tokens || x >= (uint64_t)a.pg.stride * KV_PAGE) return at;
-    const int32_t id = a.pg.tables[(uint64_t)seq * a.pg.stride + x / KV_PAGE];
-    at.there = (uint32_t)id < a.pg.n_pages;
-    at.page = (uint32_t)id;
-    return at;
+    r.ctx = a.n_ctx[seq], r.first = f0, r.room = a.pg.stride * KV_PAGE;
+    r.count = f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens || r.ctx >= r.room ? 0u : min(min((uint32_t)(f1 - f0), a.max_tokens), r.room - r.ctx);
+    r.table = a.pg.tables + (uint64_t)seq * a.pg.stride;
+    return r;
+}
+__device__ __forceinline__ int32_t page_of(const PagedMoveArgs &a, const PgRows &r, uint32_t j) {
+    const int32_t id = j < r.count ? r.table[(r.ctx + j) / KV_PAGE] : -1;
+    return (uint32_t)id < a.pg.n_pages ? id : -1;
 }
 
-// grid (rows of all heads, keys and values / rows of a CTA, sequences).
+constexpr uint32_t ST_DEEP = 2;  // rows of a lane under way
+
+// grid (groups of lanes: (token, head, keys or values), sequences)
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) pages_store_kernel(const __grid_constant__ PagedMoveArgs a) {
     using B = Q4Block<HD>;
     constexpr uint32_t LANES = HD / 8, ROWS = 256 / LANES;
     pdl_release();
     pdl_wait();
-    const uint32_t seq = blockIdx.y, w = threadIdx.x % LANES, per = 2 * a.pg.n_kv;
-    const uint64_t i = (uint64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
-    const uint32_t j = (uint32_t)(i / per), part = (uint32_t)(i % per), value = part / a.pg.n_kv, head = part % a.pg.n_kv;
-    const PgPlace at = place(a, seq, j);
-    const T *src = static_cast<const T *>(value ? a.v : a.k) + at.row * (value ? a.v_stride : a.k_stride) + (uint64_t)head * HD + w * 8;
-    const uint4 u = at.there ? *reinterpret_cast<const uint4 *>(src) : make_uint4(0, 0, 0, 0);
-    const uint32_t word[4] = {u.x, u.y, u.z, u.w};
-    float x[8], most = 0.0f, least = 0.0f;  // (a group whose entries all have one sign: the other end stays zero)
+    const uint32_t w = threadIdx.x % LANES;
+    const PgRows r = rows_of<ROWS>(a, threadIdx.x / LANES);
+    const T *src = static_cast<const T *>(r.value ? a.v : a.k) + (uint64_t)(uint32_t)r.first * (r.value ? a.v_stride : a.k_stride) + (uint64_t)r.head * HD + w * 8;
+    const uint64_t stride = r.value ? a.v_stride : a.k_stride;
+    uint8_t *pool = static_cast<uint8_t *>(const_cast<void *>(r.value ? a.pg.v : a.pg.k)) + (uint64_t)r.head * B::BYTES;
+    const uint64_t page_bytes = (uint64_t)a.pg.n_kv * B::BYTES;
+    constexpr uint32_t lanes = 0xffffffffu;  // (a warp's groups go on as long as one of them has rows)
+    for (uint32_t j0 = r.j; __any_sync(lanes, j0 < r.count); j0 += ST_DEEP * r.step) {
+        uint4 u[ST_DEEP];
+        int32_t id[ST_DEEP];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float2 f = as_float2(word[e], T());
-        x[2 * e] = f.x, x[2 * e + 1] = f.y;
-    }
+        for (uint32_t k = 0; k < ST_DEEP; ++k) {
+            const uint32_t j = j0 + k * r.step;
+            u[k] = make_uint4(0, 0, 0, 0);
+            if (j < r.count) u[k] = ldg128_stream(src + j * stride);
+            id[k] = page_of(a, r, j);
+        }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -Q4_LARGEST), Q4_LARGEST);
-        most = fmaxf(most, x[e]), least = fminf(least, x[e]);
-    }
+        for (uint32_t k = 0; k < ST_DEEP; ++k) {
+            const uint32_t word[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+            uint32_t hi = Pair<T>::max(Pair<T>::max(word[0], word[1]), Pair<T>::max(word[2], word[3]));
+            uint32_t lo = Pair<T>::max(Pair<T>::max(word[0] ^ SIGNS, word[1] ^ SIGNS), Pair<T>::max(word[2] ^ SIGNS, word[3] ^ SIGNS));
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-    }
-    const float eighth = fmaxf(most, -least) * 0.125f;
-    // up to 7 significant bits; below 2^-18 to a multiple of 2^-24, the steps of f16 (a magnitude below 64 2^-24: its whole number of them)
-    float d = __uint_as_float((__float_as_uint(eighth) + 0x1ffffu) & ~0x1ffffu);
-    if (eighth < 0x1p-18f) d = ceilf(eighth * 0x1p24f) * 0x1p-24f;
-    if (most > -least) d = -d;
-    const float by = d != 0.0f ? d : 1.0f, inverse = __frcp_rn(by);
-    uint32_t out = 0;
+            for (int o = 1; o < 4; o <<= 1) {
+                hi = Pair<T>::max(hi, __shfl_xor_sync(lanes, hi, o));
+                lo = Pair<T>::max(lo, __shfl_xor_sync(lanes, lo, o));
+            }
+            const float2 hi2 = as_float2(hi, T()), lo2 = as_float2(lo, T());
+            float most = fmaxf(hi2.x, hi2.y), least = fmaxf(lo2.x, lo2.y), x[8];  // the largest, and the smallest with its sign turned
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float t = x[e] * inverse;  // off by less than 2^-20 (8 times 2^-23)
-        const float near = rintf(t);
-        if (fabsf(t - near) > 0.4999f) t = __fdiv_rn(x[e], by);
-        const int c = max(-8, min(7, (int)rintf(t)));
-        out |= (uint32_t)(c + 8) << (4 * (e >> 1) + 16 * (e & 1));
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = as_float2(word[e], T());
+                x[2 * e] = f.x, x[2 * e + 1] = f.y;
+            }
+            const bool odd = !(fmaxf(most, least) <= Q4_LARGEST) || hi2.x != hi2.x || hi2.y != hi2.y;  // no numbers, or too large ones, in these 32
+            if (__any_sync(lanes, odd)) {
+                most = least = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -Q4_LARGEST), Q4_LARGEST);
+                    most = fmaxf(most, x[e]), least = fmaxf(least, -x[e]);
+                }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    most = fmaxf(most, __shfl_xor_sync(lanes, most, o));
+                    least = fmaxf(least, __shfl_xor_sync(lanes, least, o));
+                }
+            }
+            const float eighth = fmaxf(most, least) * 0.125f;
+            // up to 7 significant bits; below 2^-18 to a multiple of 2^-24, the steps of f16
+            float d = __uint_as_float((__float_as_uint(eighth) + 0x1ffffu) & ~0x1ffffu);
+            if (eighth < 0x1p-18f) d = ceilf(eighth * 0x1p24f) * 0x1p-24f;
+            if (most > least) d = -d;
+            const float by = d != 0.0f ? d : 1.0f, inverse = __frcp_rn(by);
+            constexpr float MAGIC = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers, ties to even
+            float c[8], off = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float t = fmaf(x[e], inverse, MAGIC) - MAGIC;
+                off = fmaxf(off, fabsf(fmaf(x[e], inverse, -t)));  // (off by 8 times 2^-24 and a rounding)
+                c[e] = fminf(t, 7.0f);
+            }
+            if (off > 0.5f - 0x1p-19f) {  // next to the middle between two codes
+#pragma unroll
+                for (int e = 0; e < 8; ++e) c[e] = fmaxf(-8.0f, fminf(rintf(__fdiv_rn(x[e], by)), 7.0f));
+            }
+            // c + 8 in base 16: even entries in the low half, odd ones in the high half
+            constexpr float EIGHTS = 8.0f * 0x1111;
+            const float low = fmaf(fmaf(fmaf(c[6], 16.0f, c[4]), 16.0f, c[2]), 16.0f, c[0]) + (EIGHTS + MAGIC), high = fmaf(fmaf(fmaf(c[7], 16.0f, c[5]), 16.0f, c[3]), 16.0f, c[1]) + (EIGHTS + MAGIC);
+            if (id[k] < 0) continue;
+            const uint32_t p = (r.ctx + j0 + k * r.step) % KV_PAGE;
+            uint8_t *block = pool + (uint32_t)id[k] * page_bytes;
+            *reinterpret_cast<uint32_t *>(block + B::word(r.value, p, w)) = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+            if (w % 4 == 0) *reinterpret_cast<__half *>(block + B::unit(r.value, p, w / 4)) = __float2half_rn(d);
+        }
     }
-    if (!at.there) return;
-    uint8_t *block = static_cast<uint8_t *>(const_cast<void *>(value ? a.pg.v : a.pg.k)) + ((uint64_t)at.page * a.pg.n_kv + head) * B::BYTES;
-    *reinterpret_cast<uint32_t *>(block + B::word(value, at.p, w)) = out;
-    if (w % 4 == 0) *reinterpret_cast<__half *>(block + B::unit(value, at.p, w / 4)) = __float2half_rn(d);
 }
 
+constexpr uint32_t LD_DEEP = 4;
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) pages_load_kernel(const __grid_constant__ PagedMoveArgs a) {
     using B = Q4Block<HD>;
     constexpr uint32_t LANES = HD / 8, ROWS = 256 / LANES;
     pdl_release();
     pdl_wait();
-    const uint32_t seq = blockIdx.y, w = threadIdx.x % LANES, per = 2 * a.pg.n_kv;
-    const uint64_t i = (uint64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
-    const uint32_t j = (uint32_t)(i / per), part = (uint32_t)(i % per), value = part / a.pg.n_kv, head = part % a.pg.n_kv;
-    const PgPlace at = place(a, seq, j);
-    if (!at.there) return;
-    const uint8_t *block = static_cast<const uint8_t *>(value ? a.pg.v : a.pg.k) + ((uint64_t)at.page * a.pg.n_kv + head) * B::BYTES;
-    const uint32_t code = *reinterpret_cast<const uint32_t *>(block + B::word(value, at.p, w));
-    const float d = __half2float(*reinterpret_cast<const __half *>(block + B::unit(value, at.p, w / 4)));
-    uint32_t u[4];
+    const uint32_t w = threadIdx.x % LANES;
+    const PgRows r = rows_of<ROWS>(a, threadIdx.x / LANES);
+    T *dst = static_cast<T *>(const_cast<void *>(r.value ? a.v : a.k)) + (uint64_t)(uint32_t)r.first * (r.value ? a.v_stride : a.k_stride) + (uint64_t)r.head * HD + w * 8;
+    const uint64_t stride = r.value ? a.v_stride : a.k_stride;
+    const uint8_t *pool = static_cast<const uint8_t *>(r.value ? a.pg.v : a.pg.k) + (uint64_t)r.head * B::BYTES;
+    const uint64_t page_bytes = (uint64_t)a.pg.n_kv * B::BYTES;
+    for (uint32_t j0 = r.j; j0 < r.count; j0 += LD_DEEP * r.step) {
+        uint32_t code[LD_DEEP], unit[LD_DEEP];
+        int32_t id[LD_DEEP];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = pack2((float)((int)(code >> (4 * e) & 15u) - 8) * d, (float)((int)(code >> (4 * e + 16) & 15u) - 8) * d, T());
-    T *dst = static_cast<T *>(const_cast<void *>(value ? a.v : a.k)) + at.row * (value ? a.v_stride : a.k_stride) + (uint64_t)head * HD + w * 8;
-    *reinterpret_cast<uint4 *>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+        for (uint32_t k = 0; k < LD_DEEP; ++k) id[k] = page_of(a, r, j0 + k * r.step);
+#pragma unroll
+        for (uint32_t k = 0; k < LD_DEEP; ++k) {
+            const uint32_t p = (r.ctx + j0 + k * r.step) % KV_PAGE;
+            const uint8_t *block = pool + (uint32_t)max(id[k], 0) * page_bytes;
+            code[k] = unit[k] = 0;
+            if (id[k] >= 0) code[k] = *reinterpret_cast<const uint32_t *>(block + B::word(r.value, p, w)), unit[k] = *reinterpret_cast<const uint16_t *>(block + B::unit(r.value, p, w / 4));
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < LD_DEEP; ++k) {
+            if (id[k] < 0) continue;
+            const uint32_t d = unit[k] * 0x10001u, n = q4_offset(d);
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u[e] = q4_field(code[k], e, d, n);
+                if constexpr (!std::is_same<T, __half>::value) {
+                    const float2 f = as_float2(u[e], __half());
+                    u[e] = pack2(f.x, f.y, T());
+                }
+            }
+            __stcs(reinterpret_cast<uint4 *>(dst + (j0 + k * r.step) * stride), make_uint4(u[0], u[1], u[2], u[3]));
+        }
+    }
 }
 
 }  // namespace
 
-cudaError_t launch_pages_store(const PagedMoveArgs &a, bool is_bf16, bool load, cudaStream_t st) {
-    const uint32_t rows = 256 / (a.pg.dim / 8);
-    const dim3 grid((uint32_t)(((uint64_t)a.max_tokens * 2 * a.pg.n_kv + rows - 1) / rows), a.n_seq);
+cudaError_t launch_pages_store(const PagedMoveArgs &a, bool is_bf16, bool load, int sm_count, cudaStream_t st) {
+    // Whole rounds of (head, keys or values), and CTAs for all places (eight an SM); fewer where there are few tokens.
+    const uint32_t rows = 256 / (a.pg.dim / 8), per = 2 * a.pg.n_kv, round = per / std::gcd(per, rows);
+    const uint64_t all = ((uint64_t)a.max_tokens * per + rows - 1) / rows, most = std::max<uint64_t>(1, 8ull * sm_count / a.n_seq);
+    const dim3 grid((uint32_t)((std::min(all, most) + round - 1) / round * round), a.n_seq);
     auto pick = [&](auto k64, auto k128) { return launch_pdl(a.pg.dim == 64 ? k64 : k128, grid, dim3(256), 0, st, a); };
     if (load) return is_bf16 ? pick(pages_load_kernel<bf16, 64>, pages_load_kernel<bf16, 128>) : pick(pages_load_kernel<__half, 64>, pages_load_kernel<__half, 128>);
     return is_bf16 ? pick(pages_store_kernel<bf16, 64>, pages_store_kernel<bf16, 128>) : pick(pages_store_kernel<__half, 64>, pages_store_kernel<__half, 128>);
