@@ -70,6 +70,7 @@ struct PagedAttnArgs {
     uint32_t *status;  // pinned host memory: 1 when a bounded wait ran out and the outputs are not valid
     // filled in by the launcher
     uint32_t row_tiles;
+    uint32_t apart;    // shares of this many pages and more are even, whatever pieces begin in their middle
 };
 // With `tree`, max_drafts * group is at most PG_FEW_ROWS.
 cudaError_t launch_pages_attention(const PagedAttnArgs &a, bool tree, int sm_count, cudaStream_t st);

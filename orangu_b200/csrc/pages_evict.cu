@@ -67,17 +67,25 @@ struct Row16 {
     static __device__ __forceinline__ void store(uint8_t *block, bool, uint32_t p, uint32_t i, Word x) { *reinterpret_cast<uint4 *>(block + p * HD * 2 + i * 16) = x; }
 };
 template <int HD>
-struct Row4 {  // pairs of words, then units
+struct Row4 {  // eight entries each, then units
     using B = Q4Block<HD>;
-    static constexpr uint32_t PAIRS = HD / 16, PIECES = PAIRS + B::GROUPS, BLOCK = B::BYTES;
-    using Word = uint2;
+    static constexpr uint32_t EIGHTS = HD / 8, PIECES = EIGHTS + B::GROUPS, BLOCK = B::BYTES;
+    using Word = uint32_t;
     static __device__ __forceinline__ Word load(const uint8_t *block, bool value, uint32_t p, uint32_t i) {
-        if (i < PAIRS) return *reinterpret_cast<const uint2 *>(block + B::word(value, p, 2 * i));
-        return make_uint2(*reinterpret_cast<const uint16_t *>(block + B::unit(value, p, i - PAIRS)), 0u);
+        if (i >= EIGHTS) return *reinterpret_cast<const uint16_t *>(block + B::unit(value, p, i - EIGHTS));
+        if (!value) return *reinterpret_cast<const uint32_t *>(block + B::key(p, i));
+        const uint16_t *at = reinterpret_cast<const uint16_t *>(block + B::value(p, i));
+        return at[0] | (uint32_t)at[2] << 16;
     }
     static __device__ __forceinline__ void store(uint8_t *block, bool value, uint32_t p, uint32_t i, Word x) {
-        if (i < PAIRS) *reinterpret_cast<uint2 *>(block + B::word(value, p, 2 * i)) = x;
-        else *reinterpret_cast<uint16_t *>(block + B::unit(value, p, i - PAIRS)) = (uint16_t)x.x;
+        if (i >= EIGHTS) {
+            *reinterpret_cast<uint16_t *>(block + B::unit(value, p, i - EIGHTS)) = (uint16_t)x;
+        } else if (!value) {
+            *reinterpret_cast<uint32_t *>(block + B::key(p, i)) = x;
+        } else {
+            uint16_t *at = reinterpret_cast<uint16_t *>(block + B::value(p, i));
+            at[0] = (uint16_t)x, at[2] = (uint16_t)(x >> 16);
+        }
     }
 };
 
@@ -165,7 +173,7 @@ __global__ void __launch_bounds__(256) pages_keep_q4_kernel(const __grid_constan
     const uint64_t page_bytes = (uint64_t)a.pg.n_kv * R::BLOCK;
     const int32_t *table = a.pg.tables + (uint64_t)blockIdx.x * a.pg.stride;
     constexpr uint32_t TURNS = (64 * R::PIECES + 255) / 256;
-    uint2 x[TURNS];
+    typename R::Word x[TURNS];
     uint32_t to[TURNS];
 #pragma unroll
     for (uint32_t u = 0; u < TURNS; ++u) {

@@ -4,8 +4,10 @@
 // Both products are mma.sync m16n8k16 with the page's side as its 16 rows: scores^T = keys x queries^T (16 positions x 8 rows), then
 // output^T += values^T x weights^T (16 dimensions x 8 rows), whose weights come out of the scores' registers by one exchange of 8 x 8 halves.  Up to 8
 // rows are half the products that 16 rows on the other side would be.  The order of a product's terms is free: a lane takes 16 neighbouring bytes of a key and
-// 8 of a value.  Queries are f16; bfloat16 ones become that after a power of two per row has been taken out (their 8 bits fit, and what
-// falls below 2^-24 of 2^14 is less than 2^-38 of the row's largest).  Weights enter as value and remainder, raised by 2^7, as over f16 pages.
+// of two values.  Queries are f16; bfloat16 ones become that after a power of two per row has been taken out (their 8 bits fit, and what
+// falls below 2^-24 of 2^14 is less than 2^-38 of the row's largest).  Weights are f16 numbers raised by 2^7, as over f16 pages: where the output is f16, as value and
+// remainder; where it is bfloat16 their value alone, which is off by 2^-12 at most, an eighth of what the output's own rounding is (64 sequences of 4 to 16 k, 4 rows of
+// 128: 165 us, and 183 with remainders).
 //
 // 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, so that its arithmetic comes close to its bytes: of an SM's 472 issue slots
 // in the time that 2304 bytes take at 6.5 TB/s, about 180 make the entries, 24 are products, 30 reads of shared memory.
@@ -18,10 +20,12 @@ namespace ob {
 
 namespace {
 
+constexpr uint32_t P4_APART = 64;
+
 template <int HD>
 struct P4Shape {
     static constexpr uint32_t BLOCK = Q4Block<HD>::BYTES, SLOT = 2 * BLOCK;
-    static constexpr int DEPTH = HD == 128 ? 6 : 8;
+    static constexpr int DEPTH = HD == 128 ? 4 : 5;
     static constexpr int RINGS = PA_WARPS * DEPTH * SLOT;
     static_assert(PaResult<HD>::BYTES <= RINGS && SLOT % 16 == 0, "the warps' results meet in the rings");
 };
@@ -38,8 +42,7 @@ __device__ __forceinline__ uint32_t lds16(uint32_t at) {
 }
 template <int N> __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t at) {
     if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
-    else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
-    else v[0] = lds32(at);
+    else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of 8 x 8 halves, two of a row a lane
     uint32_t r;
@@ -49,11 +52,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of 8 x 8 halves
 
 // NT: columns of eight rows.
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 3) pages_q4_attention_kernel(const __grid_constant__ PagedAttnArgs a) {
     using F = Half2<__half>;
     using S = P4Shape<HD>;
     using B = Q4Block<HD>;
-    constexpr int DEPTH = S::DEPTH, KW = HD / 32, VW = HD / 64, MT = HD / 16;  // words of a lane: a key's row, a value's row; tiles of dimensions
+    constexpr bool REST = std::is_same<T, __half>::value;  // weights with their remainders
+    constexpr int DEPTH = S::DEPTH, KW = HD / 32, MT = HD / 16;  // words of a lane: of a key, of two values; tiles of dimensions
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t s_last;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -63,7 +67,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
     const float scale2 = a.scale * 1.4426950408889634f;
     // this lane's places in a block
     const uint32_t k_at = g * B::ROW + t * (HD / 8), k_unit = B::CODES + 2 * (g * B::GROUPS + t * (HD / 4) / Q4_GROUP);
-    const uint32_t v_at = t * B::ROW + (HD == 128 ? (g ^ (t & 2 ? 4 : 0)) * 8 : g * 4), v_unit = B::CODES + 2 * (g * (HD / 8) / Q4_GROUP * KV_PAGE + 2 * t);
+    const uint32_t v_at = t * HD + 8 * B::eight(t, g * (HD / 64)), v_unit = B::CODES + 2 * (g * (HD / 8) / Q4_GROUP * KV_PAGE + 2 * t);
     PaWalk<true> wk;
     wk.start(a);
     for (; wk.more(); wk.next(a)) {
@@ -84,25 +88,31 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
         auto number = [&](uint32_t step) { return __shfl_sync(0xffffffffu, step / 32 != block ? id_next : id_now, step & 31); };  // steps [32 block, 32 block + 64)
 
         const uint32_t base = smem_addr(smem) + warp * DEPTH * S::SLOT;
-        auto request = [&](uint32_t step) {  // copies of a step's keys and values
+        // copies of a step's keys and values, 16 bytes a lane and turn; in the turn that has the end of the keys and the start of the values the lanes go apart
+        constexpr uint32_t WORDS = S::BLOCK / 16, KEY_TURNS = WORDS / 32, ODD = WORDS % 32;
+        static_assert(ODD <= 16, "the second turn of the values begins behind the lanes that had the keys' end");
+        const uint8_t *k_base = static_cast<const uint8_t *>(a.pg.k) + (uint64_t)head * S::BLOCK + lane * 16, *v_base = static_cast<const uint8_t *>(a.pg.v) + (uint64_t)head * S::BLOCK + lane * 16;
+        const uint64_t page_bytes = (uint64_t)a.pg.n_kv * S::BLOCK;
+        auto request = [&](uint32_t step, uint32_t place) {
             if (step < n_steps) {
                 const int32_t id = number(step);
                 if (id >= 0) {
-                    const uint64_t off = ((uint64_t)id * a.pg.n_kv + head) * S::BLOCK;
-                    const uint8_t *k = static_cast<const uint8_t *>(a.pg.k) + off, *v = static_cast<const uint8_t *>(a.pg.v) + off;
-                    const uint32_t dst = base + step % DEPTH * S::SLOT;
-                    constexpr uint32_t WORDS = S::BLOCK / 16;
+                    const uint64_t off = (uint32_t)id * page_bytes;
+                    const uint8_t *k = k_base + off, *v = v_base + off;
+                    const uint32_t dst = base + place + lane * 16;
 #pragma unroll
-                    for (uint32_t i = 0; i < (2 * WORDS + 31) / 32; ++i) {
-                        const uint32_t c = i * 32 + lane;
-                        if (c < 2 * WORDS) cp16(dst + c * 16, c < WORDS ? k + c * 16 : v + (c - WORDS) * 16, true);
+                    for (uint32_t i = 0; i < KEY_TURNS; ++i) {
+                        cp16(dst + i * 512, k + i * 512, true);
+                        cp16(dst + S::BLOCK + i * 512, v + i * 512, true);
                     }
+                    if (lane < ODD) cp16(dst + KEY_TURNS * 512, k + KEY_TURNS * 512, true);
+                    else if (lane < 2 * ODD) cp16(dst + S::BLOCK + KEY_TURNS * 512 - ODD * 16, v + KEY_TURNS * 512 - ODD * 16, true);
                 }
             }
             cp_commit();
         };
 #pragma unroll 1
-        for (int i = 0; i < DEPTH - 1; ++i) request(i);
+        for (int i = 0; i < DEPTH - 1; ++i) request(i, i * S::SLOT);
 
         // ---- queries as B fragments: lane (g, t) has entries t HD / 4 .. of row g of each set of eight
         uint32_t q[NT][HD / 8];
@@ -137,16 +147,18 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
             fac[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t) * scale2, fac[n][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4) * scale2;
         }
 
-        float o[MT][NT][4], sum[NT][2], m[NT][2];
+        float o[MT][NT][4], sum[NT][2], m[NT][2], off[NT][2];  // off: what is added to a score's exponent
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            sum[n][0] = sum[n][1] = 0.0f, m[n][0] = m[n][1] = -INFINITY;
+            sum[n][0] = sum[n][1] = off[n][0] = off[n][1] = 0.0f, m[n][0] = m[n][1] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
         }
 
+        uint32_t place = 0, ahead = (DEPTH - 1) * S::SLOT;  // of this step, of the one that is asked for
+        int32_t id = number(0);
 #pragma unroll 1
         for (uint32_t step = 0; step < n_steps; ++step) {
             cp_wait<DEPTH - 2>();
@@ -156,9 +168,14 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
                 id_now = id_next;
                 id_next = look(32 * (block + 1) + lane);
             }
-            request(step + DEPTH - 1);
-            if (number(step) < 0) continue;
-            const uint32_t ks = base + step % DEPTH * S::SLOT, vs = ks + S::BLOCK, pos0 = (from + step * PA_WARPS) * KV_PAGE;
+            request(step + DEPTH - 1, ahead);
+            const int32_t now = id;
+            const uint32_t ks = base + place;
+            id = number(step + 1);
+            ahead = place;
+            place = place == (DEPTH - 1) * S::SLOT ? 0 : place + S::SLOT;
+            if (now < 0) continue;
+            const uint32_t vs = ks + S::BLOCK, pos0 = (from + step * PA_WARPS) * KV_PAGE;
 
             // ---- scores of positions g and g + 8 (rows) for rows 2 t, 2 t + 1 of each set
             float s[NT][4];
@@ -211,23 +228,25 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                         const float top = fmaxf(m[n][c], x), keep = m[n][c] == -INFINITY ? 0.0f : pow2(m[n][c] - top);
-                        m[n][c] = top;
+                        m[n][c] = top, off[n][c] = top == -INFINITY ? 0.0f : PG_RAISE<__half> - top;
                         sum[n][c] *= keep;
 #pragma unroll
                         for (int i = 0; i < MT; ++i) o[i][n][c] *= keep, o[i][n][2 + c] *= keep;
                     }
             }
-            uint32_t w[NT][2], rest[NT][2];
+            uint32_t w[NT][2], rest[NT][2];  // (REST)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float off0 = m[n][0] == -INFINITY ? 0.0f : PG_RAISE<__half> - m[n][0], off1 = m[n][1] == -INFINITY ? 0.0f : PG_RAISE<__half> - m[n][1];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float e0 = pow2(fmaf(s[n][2 * h], fac[n][0], off0)), e1 = pow2(fmaf(s[n][2 * h + 1], fac[n][1], off1));
+                    const float e0 = pow2(fmaf(s[n][2 * h], fac[n][0], off[n][0])), e1 = pow2(fmaf(s[n][2 * h + 1], fac[n][1], off[n][1]));
                     sum[n][0] += e0, sum[n][1] += e1;
                     const uint32_t u = F::pack(e0, e1);
-                    const float2 r = F::unpack(u);
-                    w[n][h] = transposed(u), rest[n][h] = transposed(F::pack(e0 - r.x, e1 - r.y));
+                    w[n][h] = transposed(u);
+                    if constexpr (REST) {
+                        const float2 r = F::unpack(u);
+                        rest[n][h] = transposed(F::pack(e0 - r.x, e1 - r.y));
+                    }
                 }
             }
             // ---- outputs of the lane's dimensions: positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9
@@ -238,23 +257,20 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
                 u1 &= (x + 8 < limit ? 0xffffu : 0u) | (x + 9 < limit ? 0xffff0000u : 0u);
             }
             const uint32_t n0 = q4_offset(u0), n1 = q4_offset(u1);
-            uint32_t v[4][VW];
+            uint32_t v0[KW], v1[KW];
+            lds_words(v0, vs + v_at);
+            lds_words(v1, vs + v_at + 4 * HD);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lds_words(v[i], vs + v_at + 4 * i * B::ROW);
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                const uint32_t x0 = __byte_perm(v[0][i], v[1][i], 0x5410), y0 = __byte_perm(v[0][i], v[1][i], 0x7632);
-                const uint32_t x1 = __byte_perm(v[2][i], v[3][i], 0x5410), y1 = __byte_perm(v[2][i], v[3][i], 0x7632);
+            for (int i = 0; i < KW; i += 2)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t f[4] = {q4_field(x0, j, u0, n0), q4_field(y0, j, u0, n0), q4_field(x1, j, u1, n1), q4_field(y1, j, u1, n1)};
+                    const uint32_t f[4] = {q4_field(v0[i], j, u0, n0), q4_field(v0[i + 1], j, u0, n0), q4_field(v1[i], j, u1, n1), q4_field(v1[i + 1], j, u1, n1)};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        F::mma(o[4 * i + j][n], f, w[n][0], w[n][1]);
-                        F::mma(o[4 * i + j][n], f, rest[n][0], rest[n][1]);
+                        F::mma(o[2 * i + j][n], f, w[n][0], w[n][1]);
+                        if constexpr (REST) F::mma(o[2 * i + j][n], f, rest[n][0], rest[n][1]);
                     }
                 }
-            }
         }
         cp_wait<0>();
         __syncthreads();
@@ -275,19 +291,20 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) pages_q4_attention_kernel
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
                 if (g == 0) sml[2 * r] = m[n][c], sml[2 * r + 1] = l;
             }
-        pa_finish<T, HD, true>(a, wk, so, sml, row0, n_rows, head, to, PG_RAISE<__half>, s_last);
+        pa_finish<T, HD, true, NT == 1 ? 8 : 16>(a, wk, so, sml, row0, n_rows, head, to, PG_RAISE<__half>, s_last);
     }
 }
 
 template <typename T, int HD, int NT>
-cudaError_t launch(const PagedAttnArgs &a, int sm_count, cudaStream_t st) {
+cudaError_t launch(PagedAttnArgs a, int sm_count, cudaStream_t st) {
     using S = P4Shape<HD>;
     auto kernel = pages_q4_attention_kernel<T, HD, NT>;
     static PerDeviceOnce once;
     if (cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::RINGS); })) return e;
     const uint64_t pages = (std::min<uint64_t>(a.max_ctx, (uint64_t)a.pg.stride * KV_PAGE) + a.max_drafts + KV_PAGE - 1) / KV_PAGE;  // about, of a sequence
-    const uint64_t most = std::min<uint64_t>({(uint64_t)sm_count * PA_CTAS, PG_COUNTERS, PG_PARTS / (2 * PaResult<HD>::PART * 4)});
+    const uint64_t most = std::min<uint64_t>({(uint64_t)sm_count * (NT == 1 ? 4 : 3), PG_COUNTERS, PG_PARTS / (2 * PaResult<HD>::PART * 4)});
     const uint64_t grid = std::min(most, std::max<uint64_t>(1, a.n_units * ((pages + PA_LEAST - 1) / PA_LEAST) * a.pg.n_kv));
+    a.apart = P4_APART;
     return launch_pdl(kernel, dim3((uint32_t)grid), dim3(PA_THREADS), S::RINGS, st, a);
 }
 template <typename T>

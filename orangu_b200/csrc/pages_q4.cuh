@@ -5,12 +5,13 @@
 // 72 d is one, too (10 bits, at most 64512), which is what makes an entry one fused multiply-add of its code: 64 + (c + 8) is the f16 number 0x5400 | (c + 8) << 4,
 // and (64 + c + 8) d - 72 d = c d is not rounded.
 //
-// A word of 32 bits is eight entries e0 .. e7 in order: nibble j of the low half is e_2j, nibble j of the high half e_2j+1, so that a mask takes
-// two neighbours at a time.  A block (page, head) is 9 HD bytes, HD / 2 a position and then the units:
+// Eight entries e0 .. e7 are two halves of 16 bits: nibble j of the first is e_2j, nibble j of the second e_2j+1.  As one word, a mask takes two neighbours at a
+// time.  A block (page, head) is 9 HD bytes, HD / 2 a position and then the units:
 //
 //   keys    position p's words in order at p HD / 2; units [position][32 entries]
-//   values  position p at slot(p) HD / 2, slot = p / 2 % 4 + p % 2 * 4 + p / 8 * 8; units [32 entries][position].  With HD = 128 the two halves of every other
-//           pair of slots are exchanged.  Four lanes then read four positions two apart, eight lanes the dimensions, without bank conflicts.
+//   values  positions 2 r and 2 r + 1 lie together, HD bytes: for each eight entries the first halves of both in a word, then the second ones, so that a mask takes
+//           the same entry of two positions; units [32 entries][position].  The places of the eights are exchanged by a mask that depends on r, so that four lanes with
+//           four pairs of positions and eight lanes with an eighth of the dimensions each read without bank conflicts.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -27,22 +28,27 @@ template <int HD>
 struct Q4Block {
     static constexpr uint32_t ROW = HD / 2, CODES = KV_PAGE * ROW, GROUPS = HD / Q4_GROUP, BYTES = CODES + KV_PAGE * GROUPS * 2;
     static_assert(BYTES == 9 * HD, "9 bits for two entries");
-    static __host__ __device__ __forceinline__ uint32_t slot(uint32_t p) { return (p >> 1 & 3) | (p & 1) << 2 | (p & 8); }
-    // Byte of word w (eight entries) of a position, and of the unit of group g.
-    static __host__ __device__ __forceinline__ uint32_t word(bool value, uint32_t p, uint32_t w) {
-        if (!value) return p * ROW + 4 * w;
-        const uint32_t s = slot(p);
-        return s * ROW + 4 * (HD == 128 && (s & 2) ? w ^ 8 : w);
-    }
+    // Byte of a key's entries 8 w .. 8 w + 7 (a word); of a value's (two halves, four bytes apart); and of the unit of group g.
+    static __host__ __device__ __forceinline__ uint32_t key(uint32_t p, uint32_t w) { return p * ROW + 4 * w; }
+    static __host__ __device__ __forceinline__ uint32_t eight(uint32_t r, uint32_t w) { return w ^ (HD == 128 ? (r & 3) << 2 : (r & 2) << 1); }  // place of eight w in pair r, and back
+    static __host__ __device__ __forceinline__ uint32_t value(uint32_t p, uint32_t w) { return (p >> 1) * HD + 8 * eight(p >> 1, w) + 2 * (p & 1); }
     static __host__ __device__ __forceinline__ uint32_t unit(bool value, uint32_t p, uint32_t g) { return CODES + 2 * (value ? g * KV_PAGE + p : p * GROUPS + g); }
 };
 
-// Field j of a word: the entries whose nibbles are j of both halves, times their units.  d: the units, n: -72 times them.
+// Field j of a word: the entries whose nibbles are j of both halves, times their units.  d: the units, n: -72 times them.  Nibbles 1 and 3 (after a shift by 8 for
+// both 2 and 3) are taken where they make 64 + c + 8; 0 and 2 where they make 1024 + c + 8, from which 1032 is taken first: that costs a fused
+// multiply-add more and a shift less, of which an SM does half as many.
 __device__ __forceinline__ uint32_t q4_field(uint32_t w, int j, uint32_t d, uint32_t n) {
-    const uint32_t x = j == 0 ? w << 4 : w >> (4 * j - 4);
+    const uint32_t x = j < 2 ? w : w >> 8;
     uint32_t u, r;
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(u) : "r"(x));  // (x & mask) | 64
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(d), "r"(n));
+    if (j & 1) {
+        asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(u) : "r"(x));  // (x & mask) | 64
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(d), "r"(n));
+    } else {
+        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(u) : "r"(x));  // (x & mask) | 1024
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(u) : "r"(u), "r"(0x64086408u));
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(d));
+    }
     return r;
 }
 __device__ __forceinline__ uint32_t q4_offset(uint32_t d) {  // -72 d, exact

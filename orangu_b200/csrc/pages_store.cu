@@ -155,7 +155,12 @@ __global__ void __launch_bounds__(256) pages_store_kernel(const __grid_constant_
             if (id[k] < 0) continue;
             const uint32_t p = (r.ctx + j0 + k * r.step) % KV_PAGE;
             uint8_t *block = pool + (uint32_t)id[k] * page_bytes;
-            *reinterpret_cast<uint32_t *>(block + B::word(r.value, p, w)) = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+            if (r.value) {
+                uint16_t *at = reinterpret_cast<uint16_t *>(block + B::value(p, w));
+                at[0] = (uint16_t)__float_as_uint(low), at[2] = (uint16_t)__float_as_uint(high);
+            } else {
+                *reinterpret_cast<uint32_t *>(block + B::key(p, w)) = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+            }
             if (w % 4 == 0) *reinterpret_cast<__half *>(block + B::unit(r.value, p, w / 4)) = __float2half_rn(d);
         }
     }
@@ -184,7 +189,14 @@ __global__ void __launch_bounds__(256) pages_load_kernel(const __grid_constant__
             const uint32_t p = (r.ctx + j0 + k * r.step) % KV_PAGE;
             const uint8_t *block = pool + (uint32_t)max(id[k], 0) * page_bytes;
             code[k] = unit[k] = 0;
-            if (id[k] >= 0) code[k] = *reinterpret_cast<const uint32_t *>(block + B::word(r.value, p, w)), unit[k] = *reinterpret_cast<const uint16_t *>(block + B::unit(r.value, p, w / 4));
+            if (id[k] < 0) continue;
+            if (r.value) {
+                const uint16_t *at = reinterpret_cast<const uint16_t *>(block + B::value(p, w));
+                code[k] = at[0] | (uint32_t)at[2] << 16;
+            } else {
+                code[k] = *reinterpret_cast<const uint32_t *>(block + B::key(p, w));
+            }
+            unit[k] = *reinterpret_cast<const uint16_t *>(block + B::unit(r.value, p, w / 4));
         }
 #pragma unroll
         for (uint32_t k = 0; k < LD_DEEP; ++k) {

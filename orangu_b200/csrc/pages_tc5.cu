@@ -227,25 +227,37 @@ struct P4Tile {
             for (uint32_t c = lane; c < WORDS; c += 32) cp16(dst + p * B::BYTES + c * 16, block + c * 16, page >= 0);
         }
     }
+    static __device__ __forceinline__ void put(uint8_t *operand, uint32_t row, uint32_t c, uint32_t x, uint32_t d, uint32_t n) {  // eight entries
+        *reinterpret_cast<uint4 *>(operand + c / 8 * PG_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+            make_uint4(q4_field(x, 0, d, n), q4_field(x, 1, d, n), q4_field(x, 2, d, n), q4_field(x, 3, d, n));
+    }
     static __device__ __forceinline__ void make(const uint8_t *src, uint8_t *operand) {
         uint32_t lane = threadIdx.x & 31;
         asm volatile("" : "+r"(lane));  // (places are worked out where they are used)
 #pragma unroll 1
         for (uint32_t i = 0; i < EACH; ++i) {
-            const uint32_t at = i * 32 + lane, page = at / QUADS / KV_PAGE, place = at / QUADS % KV_PAGE, quad = at % QUADS;
-            const uint32_t pos = VALUE ? (place & 3) << 1 | (place >> 2 & 1) | (place & 8) : place, q = VALUE && HD == 128 && (place & 2) ? quad ^ 2 : quad, row = page * KV_PAGE + pos;
+            const uint32_t at = i * 32 + lane, page = at / (QUADS * KV_PAGE), in_page = at % (QUADS * KV_PAGE);
             const uint8_t *block = src + page * B::BYTES;
-            const uint4 code = reinterpret_cast<const uint4 *>(block)[at % (KV_PAGE * QUADS)];
-            const uint32_t d = *reinterpret_cast<const uint16_t *>(block + B::unit(VALUE, pos, q)) * 0x10001u, n = q4_offset(d);
-            // eight lanes have two rows and all four quads: of the second two the order of the words is another, so that no two are in one bank
-            constexpr uint32_t SWAP = HD == 128 ? (VALUE ? 1 : 2) : 0;
-            const bool other = SWAP && (q & 2);
-            const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+            const uint4 code = reinterpret_cast<const uint4 *>(block)[in_page];
+            // eight lanes write two rows, or one: those of the second block of columns (head dimension 64: of the second row) have another order, so that no two
+            // are in one bank
+            if constexpr (VALUE) {
+                const uint32_t r = in_page / (2 * QUADS), w = B::eight(r, 2 * (in_page % (2 * QUADS))), row = page * KV_PAGE + 2 * r;
+                const bool other = HD == 128 ? (w & 8) != 0 : (r & 1) != 0;
+                const uint32_t u = *reinterpret_cast<const uint32_t *>(block + B::unit(true, 2 * r, w / 4));
+                const uint32_t d0 = __byte_perm(u, u, 0x1010), d1 = __byte_perm(u, u, 0x3232), n0 = q4_offset(d0), n1 = q4_offset(d1);
+                const uint32_t x0 = other ? code.z : code.x, y0 = other ? code.w : code.y, x1 = other ? code.x : code.z, y1 = other ? code.y : code.w, w0 = other ? w + 1 : w, w1 = other ? w : w + 1;
+                put(operand, row, w0, __byte_perm(x0, y0, 0x5410), d0, n0);
+                put(operand, row + 1, w0, __byte_perm(x0, y0, 0x7632), d1, n1);
+                put(operand, row, w1, __byte_perm(x1, y1, 0x5410), d0, n0);
+                put(operand, row + 1, w1, __byte_perm(x1, y1, 0x7632), d1, n1);
+            } else {
+                const uint32_t pos = in_page / QUADS, q = in_page % QUADS, row = page * KV_PAGE + pos;
+                const bool other = HD == 128 && (q & 2);
+                const uint32_t d = *reinterpret_cast<const uint16_t *>(block + B::unit(false, pos, q)) * 0x10001u, n = q4_offset(d);
+                const uint32_t w[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-                const uint32_t x = other ? w[e ^ SWAP] : w[e], c = 4 * q + (other ? e ^ SWAP : e);
-                *reinterpret_cast<uint4 *>(operand + c / 8 * PG_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-                    make_uint4(q4_field(x, 0, d, n), q4_field(x, 1, d, n), q4_field(x, 2, d, n), q4_field(x, 3, d, n));
+                for (uint32_t e = 0; e < 4; ++e) put(operand, row, 4 * q + (other ? e ^ 2 : e), other ? w[e ^ 2] : w[e], d, n);
             }
         }
     }
@@ -256,6 +268,7 @@ __global__ void __launch_bounds__(Q4 ? P4_THREADS : PG_THREADS, 1)
 pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
     using P = PgPlan<HD, WIDE, Q4>;
     using TP = typename std::conditional<Q4, __half, T>::type;  // of the operands
+    constexpr bool REST = !Q4 || std::is_same<T, __half>::value;  // weights with their remainders; f16 ones for bfloat16 outputs without (pages_q4.cu)
     constexpr uint32_t KST = P::KST, VST = P::VST, G = P::G, PLACE = P::PLACE, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem);
@@ -406,7 +419,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 #pragma unroll
                     for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add; 16 positions: eight columns of values, eight of remainders
                         umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
-                        umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
+                        if constexpr (REST) umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
                     }
                     umma_commit_warp(bar + PB_PV_DONE + 8 * s);
                     if (i % G == G - 1 || step + 1 == (int)steps) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
@@ -574,7 +587,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         sum0 = sum1 = 0.0f;
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {  // 16 positions
-                            uint32_t v[16];
+                            uint32_t v[REST ? 16 : 8];
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 const float x0 = __uint_as_float(u[g / 2][g % 2 * 16 + 2 * e]), x1 = __uint_as_float(u[g / 2][g % 2 * 16 + 2 * e + 1]);
@@ -584,10 +597,13 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                                 e0 = pow2(e0), e1 = pow2(e1);
                                 add2(sum0, sum1, e0, e1);
                                 v[e] = pack16<TP>(e0, e1);
-                                const float2 r = unpack16(v[e], TP());
-                                v[8 + e] = pack16<TP>(e0 - r.x, e1 - r.y);
+                                if constexpr (REST) {
+                                    const float2 r = unpack16(v[e], TP());
+                                    v[8 + e] = pack16<TP>(e0 - r.x, e1 - r.y);
+                                }
                             }
-                            tmem_st16(tp + 16 * g, v);
+                            if constexpr (REST) tmem_st16(tp + 16 * g, v);
+                            else tmem_st8(tp + 16 * g, v);
                         }
                         const float now = fmaxf(top[0], top[1]) * scale2;
                         const bool grown = now > m + PG_SLACK;

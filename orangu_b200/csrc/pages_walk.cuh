@@ -111,7 +111,7 @@ struct PaWalk {
             total *= a.pg.n_kv;
             share(total, pieces);
             uint32_t each = 1;
-            if (pieces <= gridDim.x)
+            if (pieces <= gridDim.x && per < a.apart)
                 for (uint32_t more = 0; more < 2 && !apart; ++more) {
                     each = (uint32_t)per + more * ((uint32_t)per / PA_MORE + 1);  // (about a piece's pages at most: 32 bits)
                     uint64_t parts = 0;
@@ -179,8 +179,8 @@ struct PaWalk {
 
 // The end of a piece: the warps' parts of its rows in shared memory (so: [warp][row][PITCH] outputs, sml: [warp][row][2] maximum and sum; all of them
 // written, no barrier since) become outputs, or a part that others go on with.  The maxima and sums are those of weights made 2^raise times as large.
-// The whole CTA.
-template <typename T, int HD, bool TREE>
+// The whole CTA.  DEEP: entries of parts under way.
+template <typename T, int HD, bool TREE, uint32_t DEEP = 16>
 __device__ __forceinline__ void pa_finish(const PagedAttnArgs &a, const PaWalk<TREE> &wk, const float *so, const float *sml, uint32_t row0, uint32_t n_rows, uint32_t head, uint32_t to, float raise,
                                           uint32_t &s_last) {
     using H = Half2<T>;
@@ -231,10 +231,10 @@ __device__ __forceinline__ void pa_finish(const PagedAttnArgs &a, const PaWalk<T
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    // 16 entries of parts are under way at once: a sequence of 32,000 positions, whose eight pieces have 55 parts each, takes 51 us for 16 rows of
+    // 16 entries of parts under way at once: a sequence of 32,000 positions, whose eight pieces have 55 parts each, takes 51 us for 16 rows of
     // 128 and 49 us for 4; with one row after the other 16 rows took 67 us
     auto add_up = [&](auto rows) {
-        constexpr uint32_t MINE = decltype(rows)::value, APART = PA_THREADS / VEC, AHEAD = 16 / MINE;  // rows of a thread, from one to the next, parts
+        constexpr uint32_t MINE = decltype(rows)::value, APART = PA_THREADS / VEC, AHEAD = DEEP / MINE;  // rows of a thread, from one to the next, parts
         const uint32_t r0 = threadIdx.x / VEC, c = threadIdx.x % VEC;
         float top[MINE], l[MINE];
         float4 x[MINE];

@@ -30,9 +30,10 @@ def seen_by(first, n_ctx, visible, s, n_positions):
     return out
 
 
-def attend_tokens(q, k, v, there, first, n_ctx, visible, scale, out, mass, rel_of):
+def attend_tokens(q, k, v, there, first, n_ctx, visible, scale, out, mass, rel_of, rounded=0.0):
     """q [tokens, heads, dim]; k, v: per sequence [positions, kv, dim]; there: per sequence which positions exist.  Writes out and mass [sequences, kv, positions];
-    returns the bounds of their errors.  rel_of(qk, n): a weight's relative error where sum |q k| is at most qk and n positions are seen."""
+    returns the bounds of their errors.  rel_of(qk, n): a weight's relative error where sum |q k| is at most qk and n positions are seen;
+    rounded: that of the weights on their way into the products with values, which goes into sum w v as it is."""
     tol, mass_tol = np.zeros(out.shape[:2]), None if mass is None else np.zeros(mass.shape)
     kv = k[0].shape[1] if len(k) else 1
     group = q.shape[1] // kv
@@ -56,7 +57,7 @@ def attend_tokens(q, k, v, there, first, n_ctx, visible, scale, out, mass, rel_o
                     w /= w.sum()
                     out[first[s] + t, h * group + g] = w @ vh
                     rel = rel_of(size, n)
-                    tol[first[s] + t, h * group + g] = 2 * rel * (w @ np.abs(vh)).max() + np.abs(vh[sees[t]]).max() * (n * 2.0 ** -32 + 2.0 ** -22)
+                    tol[first[s] + t, h * group + g] = (2 * rel + rounded) * (w @ np.abs(vh)).max() + np.abs(vh[sees[t]]).max() * (n * 2.0 ** -32 + 2.0 ** -22)
                     got += w
                     got_tol += 2 * rel * w + 2.0 ** -40
             if mass is not None:
