@@ -6,7 +6,7 @@
 // since the r-th residual max(r' - q, 0) / sum is max(p - c q, 0) / T.  Where no child is accepted the next token is the first v at which the sum of
 // max(p - c q, 0) exceeds u_0 times all of it.  Without draft rows a drafted token had probability one: accepted if u T < p(x), otherwise p(x) = 0, T -= p(x).
 //
-// A cluster of CTAs per sequence: eight, or as many fewer as let all sequences run at once.  The numbers that the tests need, two a node, are read for all nodes at
+// A cluster of CTAs per sequence: eight, or fewer where there are many sequences.  The numbers that the tests need, two a node, are read for all nodes at
 // once; a path is then walked in shared memory, by every CTA for itself.  Rows of the vocabulary are read only where a child was rejected and for the last
 // node, a part by each warp, and the parts' sums meet through distributed shared memory.  Sums are in 64 bits, so that the token does not depend on their order.
 #include <cooperative_groups.h>
@@ -22,7 +22,7 @@ namespace ob {
 
 namespace {
 
-constexpr uint32_t DV_CTAS = 8 /* at most */, DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_PARTS = DV_CTAS * DV_WARPS, DV_DEEP = 8, DV_TILE = 1024;
+constexpr uint32_t DV_CTAS = 8 /* at most */, DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_PARTS = DV_CTAS * DV_WARPS, DV_DEEP = 4, DV_TILE = 1024;
 
 __device__ __forceinline__ float number(float v) { return v; }
 __device__ __forceinline__ float number(__half v) { return __half2float(v); }
@@ -30,12 +30,28 @@ __device__ __forceinline__ float number(bf16 v) { return __bfloat162float(v); }
 // What is not a positive finite number counts as zero.
 template <typename T> __device__ __forceinline__ double clean(T v) {
     const float f = number(v);
-    return f > 0.0f && f <= 3.4028234664e38f ? (double)f : 0.0;
+    return __float_as_uint(f) - 1u < 0x7f7fffffu ? (double)f : 0.0;
 }
+__device__ __forceinline__ double above(double w) { return __double2hiint(w) < 0 ? 0.0 : w; }  // max(w, 0)
+
+// 16 bytes of a row as numbers.
+template <typename T> struct Vec {
+    static constexpr uint32_t N = 16 / sizeof(T);
+    uint4 u;
+    __device__ __forceinline__ T operator[](uint32_t i) const {
+        const uint32_t w = i * sizeof(T) / 4 == 0 ? u.x : i * sizeof(T) / 4 == 1 ? u.y : i * sizeof(T) / 4 == 2 ? u.z : u.w;  // (i is known to the compiler)
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w);
+        } else {
+            const uint16_t h = (uint16_t)(i % 2 ? w >> 16 : w);
+            return *reinterpret_cast<const T *>(&h);
+        }
+    }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __grid_constant__ DraftsVerifyArgs a) {
-    __shared__ double s_sum[DV_WARPS];     // of this CTA's parts, for the others
+    __shared__ double s_sum[2][DV_WARPS];  // of this CTA's parts, for the others; one after the other
     __shared__ double s_parts[DV_PARTS];   // of all
     __shared__ double s_tile[DV_TILE + DV_TILE / 32];  // weights of neighbouring tokens, 32 a lane
     __shared__ double s_p[DRAFTS_MOST], s_q[DRAFTS_MOST];  // of node i's token in its parent's rows
@@ -67,9 +83,10 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
     uint32_t node = 0, n_path = 1, n_gone = 0;
     double c = 0.0, total = 1.0;
     bool summed = false;
+    uint32_t turn = 0;
     auto weight = [&](const T *p, const T *q, uint32_t v) {
         const double x = clean(p[v]);
-        if (q) return fmax(x - c * clean(q[v]), 0.0);
+        if (q) return above(x - c * clean(q[v]));
         for (uint32_t i = 0; i < n_gone; ++i)
             if ((uint32_t)s_gone[i] == v) return 0.0;
         return x;
@@ -85,19 +102,32 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
         const T *p = target + (uint64_t)node * a.target_stride, *q = draft && c > 0.0 ? draft + (uint64_t)node * a.draft_stride : nullptr;
         const uint32_t v0 = min(mine * span, a.n_vocab), v1 = min(v0 + span, a.n_vocab);
         double s = 0.0;
+        auto one = [&](uint32_t v) { s += q ? above(clean(p[v]) - c * clean(q[v])) : clean(p[v]); };
+        // 16 bytes a lane where both rows allow it (a whole span of them is 64 KB under way per CTA and row), single numbers elsewhere
+        constexpr uint32_t N = Vec<T>::N;
+        const uintptr_t pa = reinterpret_cast<uintptr_t>(p + v0), qa = q ? reinterpret_cast<uintptr_t>(q + v0) : pa;
+        uint32_t from = v1, to = v1;  // what is read in vectors
+        if (((pa ^ qa) & 15) == 0) {
+            from = min(v1, v0 + (uint32_t)((16 - (pa & 15)) % 16 / sizeof(T)));
+            to = from + (v1 - from) / N * N;
+        }
+        for (uint32_t v = v0 + lane; v < from; v += 32) one(v);
+        for (uint32_t v = to + lane; v < v1; v += 32) one(v);
 #pragma unroll 1
-        for (uint32_t v = v0 + lane; v < v1; v += 32 * DV_DEEP) {
-            T x[DV_DEEP], y[DV_DEEP];
+        for (uint32_t v = from + N * lane; v < to; v += 32 * N * DV_DEEP) {
+            Vec<T> x[DV_DEEP], y[DV_DEEP];
 #pragma unroll
             for (uint32_t u = 0; u < DV_DEEP; ++u) {
-                x[u] = y[u] = T(0.0f);
-                if (v + 32 * u < v1) {
-                    x[u] = p[v + 32 * u];
-                    if (q) y[u] = q[v + 32 * u];
+                x[u].u = y[u].u = make_uint4(0, 0, 0, 0);
+                if (v + 32 * N * u < to) {
+                    x[u].u = __ldg(reinterpret_cast<const uint4 *>(p + v + 32 * N * u));
+                    if (q) y[u].u = __ldg(reinterpret_cast<const uint4 *>(q + v + 32 * N * u));
                 }
             }
 #pragma unroll
-            for (uint32_t u = 0; u < DV_DEEP; ++u) s += q ? fmax(clean(x[u]) - c * clean(y[u]), 0.0) : clean(x[u]);
+            for (uint32_t u = 0; u < DV_DEEP; ++u)
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) s += q ? above(clean(x[u][i]) - c * clean(y[u][i])) : clean(x[u][i]);
         }
         for (uint32_t i = 0; i < n_gone; ++i) {  // (few, and each of them in one part only)
             const uint32_t v = (uint32_t)s_gone[i];
@@ -105,10 +135,11 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) s_sum[warp] = fmax(s, 0.0);
-        cluster.sync();
-        if (threadIdx.x < n_parts) s_parts[threadIdx.x] = cluster.map_shared_rank(s_sum, threadIdx.x / DV_WARPS)[threadIdx.x % DV_WARPS];
-        cluster.sync();  // (all have read before anybody's sums are written again, or its memory goes away)
+        if (lane == 0) s_sum[turn][warp] = fmax(s, 0.0);
+        cluster.sync();  // (between two writes of one place lies the other's sync, before which all have read this one's)
+        if (threadIdx.x < n_parts) s_parts[threadIdx.x] = cluster.map_shared_rank(s_sum[turn], threadIdx.x / DV_WARPS)[threadIdx.x % DV_WARPS];
+        turn ^= 1;
+        __syncthreads();
         summed = true;
         return all_of();
     };
@@ -180,19 +211,20 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
             const int src = hits ? __ffs(hits) - 1 : 31 - __clz(some);
             part = __shfl_sync(0xffffffffu, part, src), start = __shfl_sync(0xffffffffu, start, src);
             if (!hits) start = -INFINITY;  // (nothing passes r there: its last one)
-            if (part == mine) {
+            if (part / DV_WARPS == rank) {  // (alike for the whole CTA, which reads; its first warp looks for the token)
                 const T *p = target + (uint64_t)node * a.target_stride, *q = draft && c > 0.0 ? draft + (uint64_t)node * a.draft_stride : nullptr;
                 const uint32_t v0 = min(part * span, a.n_vocab), v1 = min(v0 + span, a.n_vocab);
                 int32_t last = -1;
 #pragma unroll 1
-                for (uint32_t t0 = v0; t0 < v1 && next < 0; t0 += DV_TILE) {
-                    __syncwarp();
-#pragma unroll 8
-                    for (uint32_t k = 0; k < DV_TILE / 32; ++k) {
-                        const uint32_t v = t0 + k * 32 + lane;
-                        s_tile[k * 33 + lane] = v < v1 ? weight(p, q, v) : 0.0;
+                for (uint32_t t0 = v0; t0 < v1; t0 += DV_TILE) {
+                    __syncthreads();
+#pragma unroll
+                    for (uint32_t k = 0; k < DV_TILE / DV_THREADS; ++k) {
+                        const uint32_t i = k * DV_THREADS + threadIdx.x, v = t0 + i;
+                        s_tile[i / 32 * 33 + i % 32] = v < v1 ? weight(p, q, v) : 0.0;
                     }
-                    __syncwarp();
+                    __syncthreads();
+                    if (warp || next >= 0) continue;
                     const double *own = s_tile + lane * 33;  // tokens t0 + 32 lane ..
                     double sum = 0.0;
 #pragma unroll 8
@@ -222,8 +254,7 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
                     }
                     start += __shfl_sync(0xffffffffu, upto, 31);
                 }
-                if (next < 0) next = last;
-                if (lane == 0) a.next[seq] = next;
+                if (threadIdx.x == 0) a.next[seq] = next < 0 ? last : next;
             }
         } else if (rank == 0 && threadIdx.x == 0) {
             a.next[seq] = -1;
@@ -231,8 +262,8 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
     } else if (rank == 0 && threadIdx.x == 0) {
         a.next[seq] = -1;
     }
+    cluster.sync();  // (nobody's memory goes away while others may read it)
     if (rank == 0) {
-        __syncthreads();
         for (uint32_t j = threadIdx.x; j < a.kept_stride; j += DV_THREADS) a.kept[(uint64_t)seq * a.kept_stride + j] = n && j < n_path ? s_path[j] : -1;
         if (threadIdx.x == 0) a.n_kept[seq] = n ? min(n_path, a.kept_stride) : 0u;
     }
@@ -242,8 +273,10 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
 
 cudaError_t launch_drafts_verify(const DraftsVerifyArgs &a, uint32_t n_seq, uint32_t type, int sm_count, cudaStream_t st) {
     auto kernel = type == 0 ? drafts_verify_kernel<float> : type == 1 ? drafts_verify_kernel<__half> : drafts_verify_kernel<bf16>;
-    uint32_t ctas = DV_CTAS;  // two a multiprocessor at once
-    while (ctas > 1 && (uint64_t)n_seq * ctas > 2ull * sm_count) ctas /= 2;
+    // Two CTAs run on a multiprocessor at once; with up to twice as many, sequences that reject often still have all of them in the second round (64 trees of up to
+    // 16 nodes: 46 us with eight CTAs each and 56 with four; chains of up to 8, which reject once, 22 and 17).
+    uint32_t ctas = DV_CTAS;
+    while (ctas > 1 && (uint64_t)n_seq * ctas > 4ull * sm_count) ctas /= 2;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
