@@ -16,7 +16,7 @@ namespace ob {
 namespace {
 
 constexpr uint32_t EV_HELD = 32768;  // words of masses in shared memory at most
-constexpr uint32_t EV_THREADS = 256, EV_DEEP = 4;  // pieces of a thread in flight
+constexpr uint32_t EV_DEEP = 4;  // pieces of a thread in flight
 
 // Larger masses have larger words; what is no number has the smallest.
 __device__ __forceinline__ uint32_t mass_word(float s) {
@@ -89,9 +89,11 @@ struct Row4 {  // eight entries each, then units
     }
 };
 
-// grid (layers x sequences x heads, 3): keys, values, masses.
-template <typename R>
-__global__ void __launch_bounds__(EV_THREADS) pages_evict_move_kernel(const __grid_constant__ PagedEvictArgs a) {
+// grid (layers x sequences x heads, 3): keys, values, masses.  While a batch is copied the pages of the next one and the list of the one after are read: the three loads
+// that depend on each other are under way at once.  8 sequences of up to 4100, 32 layers of 8 heads of 128, to 2048: 397 us without, 331 with (5 TB/s in pieces of 256 bytes);
+// more CTAs on a multiprocessor made it slower (three quarters of the registers each: 553).
+template <typename R, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS) pages_evict_move_kernel(const __grid_constant__ PagedEvictArgs a) {
     pdl_release();
     pdl_wait();
     const uint32_t head = blockIdx.x % a.pg.n_kv, seq = blockIdx.x / a.pg.n_kv % a.n_seq, layer = blockIdx.x / a.pg.n_kv / a.n_seq;
@@ -100,18 +102,25 @@ __global__ void __launch_bounds__(EV_THREADS) pages_evict_move_kernel(const __gr
     const int32_t *kept = a.kept + (uint64_t)blockIdx.x * a.n_keep;
     if (blockIdx.y == 2) {
         float *mass = a.mass + (uint64_t)blockIdx.x * a.mass_stride;
+        uint32_t src[EV_DEEP];
+        auto list = [&](uint32_t j0) {
+#pragma unroll
+            for (uint32_t u = 0; u < EV_DEEP; ++u) {
+                const uint32_t j = j0 + u * THREADS + threadIdx.x;
+                src[u] = j < a.n_keep ? (uint32_t)kept[j] : 0u;
+            }
+        };
+        list(a.keep_first);
 #pragma unroll 1
-        for (uint32_t j0 = a.keep_first; j0 < a.n_keep; j0 += EV_DEEP * EV_THREADS) {
+        for (uint32_t j0 = a.keep_first; j0 < a.n_keep; j0 += EV_DEEP * THREADS) {
             float x[EV_DEEP];
 #pragma unroll
-            for (uint32_t u = 0; u < EV_DEEP; ++u) {
-                const uint32_t j = j0 + u * EV_THREADS + threadIdx.x;
-                if (j < a.n_keep) x[u] = mass[kept[j]];
-            }
-            __syncthreads();
+            for (uint32_t u = 0; u < EV_DEEP; ++u) x[u] = mass[src[u]];
+            list(j0 + EV_DEEP * THREADS);
+            __syncthreads();  // a batch has been read before it is written; what the next one reads lies behind it
 #pragma unroll
             for (uint32_t u = 0; u < EV_DEEP; ++u) {
-                const uint32_t j = j0 + u * EV_THREADS + threadIdx.x;
+                const uint32_t j = j0 + u * THREADS + threadIdx.x;
                 if (j < a.n_keep) mass[j] = x[u];
             }
         }
@@ -120,31 +129,48 @@ __global__ void __launch_bounds__(EV_THREADS) pages_evict_move_kernel(const __gr
     const bool value = blockIdx.y;
     uint8_t *pool = static_cast<uint8_t *>(const_cast<void *>(value ? a.pg.v : a.pg.k)) + layer * a.layer_bytes + (uint64_t)head * R::BLOCK;
     const int32_t *table = a.pg.tables + (uint64_t)seq * a.pg.stride;
-    constexpr uint32_t ROWS = EV_DEEP * EV_THREADS / R::PIECES;  // positions of a batch
+    constexpr uint32_t ROWS = EV_DEEP * THREADS / R::PIECES;  // positions of a batch
     const uint64_t page_bytes = (uint64_t)a.pg.n_kv * R::BLOCK;
+    uint32_t src[EV_DEEP], now[EV_DEEP];  // of the next batch's rows, of this one's; a row that stays has itself
+    int32_t ps[EV_DEEP], pd[EV_DEEP];
+    auto row = [&](uint32_t u) { return (u * THREADS + threadIdx.x) / R::PIECES; };
+    auto list = [&](uint32_t j0) {
+#pragma unroll
+        for (uint32_t u = 0; u < EV_DEEP; ++u) {
+            const uint32_t r = row(u), j = j0 + r;
+            src[u] = r < ROWS && j < a.n_keep ? (uint32_t)kept[j] : j;
+        }
+    };
+    auto pages = [&](uint32_t j0) {
+#pragma unroll
+        for (uint32_t u = 0; u < EV_DEEP; ++u) {
+            const uint32_t j = j0 + row(u);
+            now[u] = src[u], ps[u] = pd[u] = -1;
+            if (src[u] != j) ps[u] = table[src[u] / KV_PAGE], pd[u] = table[j / KV_PAGE];
+        }
+    };
+    list(a.keep_first);
+    pages(a.keep_first);
+    list(a.keep_first + ROWS);
 #pragma unroll 1
     for (uint32_t j0 = a.keep_first; j0 < a.n_keep; j0 += ROWS) {
         typename R::Word x[EV_DEEP];
         uint8_t *to[EV_DEEP];
-        const uint32_t rows = min(ROWS, a.n_keep - j0);
+        uint32_t at[EV_DEEP];
 #pragma unroll
         for (uint32_t u = 0; u < EV_DEEP; ++u) {
-            const uint32_t i = u * EV_THREADS + threadIdx.x, r = i / R::PIECES, piece = i - r * R::PIECES, j = j0 + r;
-            to[u] = nullptr;
-            if (r >= rows) continue;
-            const uint32_t src = (uint32_t)kept[j];
-            if (src == j) continue;
-            const int32_t ps = table[src / KV_PAGE], pd = table[j / KV_PAGE];
-            if ((uint32_t)ps >= a.pg.n_pages || (uint32_t)pd >= a.pg.n_pages) continue;
-            x[u] = R::load(pool + (uint32_t)ps * page_bytes, value, src % KV_PAGE, piece);
-            to[u] = pool + (uint32_t)pd * page_bytes;
+            const uint32_t r = row(u), piece = u * THREADS + threadIdx.x - r * R::PIECES;
+            to[u] = nullptr, at[u] = piece;
+            if ((uint32_t)ps[u] >= a.pg.n_pages || (uint32_t)pd[u] >= a.pg.n_pages) continue;
+            x[u] = R::load(pool + (uint32_t)ps[u] * page_bytes, value, now[u] % KV_PAGE, piece);
+            to[u] = pool + (uint32_t)pd[u] * page_bytes;
         }
+        pages(j0 + ROWS);
+        list(j0 + 2 * ROWS);
         __syncthreads();  // a batch has been read before it is written; what the next one reads lies behind it
 #pragma unroll
-        for (uint32_t u = 0; u < EV_DEEP; ++u) {
-            const uint32_t i = u * EV_THREADS + threadIdx.x, r = i / R::PIECES;
-            if (to[u]) R::store(to[u], value, (j0 + r) % KV_PAGE, i - r * R::PIECES, x[u]);
-        }
+        for (uint32_t u = 0; u < EV_DEEP; ++u)
+            if (to[u]) R::store(to[u], value, (j0 + row(u)) % KV_PAGE, at[u], x[u]);
     }
 }
 
@@ -219,8 +245,12 @@ cudaError_t launch_pages_evict(const PagedEvictArgs &a, uint32_t n_layer, uint32
     if (cudaError_t e = max_pos <= 4096 ? launch_pdl(pages_evict_choose_kernel<256>, dim3(pairs), dim3(256), (size_t)held * 4, st, a, held)
                                         : launch_pdl(pages_evict_choose_kernel<1024>, dim3(pairs), dim3(1024), (size_t)held * 4, st, a, held))
         return e;
-    auto kernel = q4 ? (a.pg.dim == 64 ? pages_evict_move_kernel<Row4<64>> : pages_evict_move_kernel<Row4<128>>) : (a.pg.dim == 64 ? pages_evict_move_kernel<Row16<64>> : pages_evict_move_kernel<Row16<128>>);
-    return launch_pdl(kernel, dim3(pairs, 3), dim3(EV_THREADS), 0, st, a);
+    // Large CTAs where they are few: fewer batches, one after the other, of a head.
+    auto move = [&](auto small, auto large) {
+        return pairs < 512 ? launch_pdl(large, dim3(pairs, 3), dim3(512), 0, st, a) : launch_pdl(small, dim3(pairs, 3), dim3(256), 0, st, a);
+    };
+    if (q4) return a.pg.dim == 64 ? move(pages_evict_move_kernel<Row4<64>, 256>, pages_evict_move_kernel<Row4<64>, 512>) : move(pages_evict_move_kernel<Row4<128>, 256>, pages_evict_move_kernel<Row4<128>, 512>);
+    return a.pg.dim == 64 ? move(pages_evict_move_kernel<Row16<64>, 256>, pages_evict_move_kernel<Row16<64>, 512>) : move(pages_evict_move_kernel<Row16<128>, 256>, pages_evict_move_kernel<Row16<128>, 512>);
 }
 cudaError_t launch_pages_keep_q4(const PagedKeepArgs &a, uint32_t n_seq, uint32_t n_layer, cudaStream_t st) {
     return launch_pdl(a.pg.dim == 64 ? pages_keep_q4_kernel<64> : pages_keep_q4_kernel<128>, dim3(n_seq, 2 * n_layer * a.pg.n_kv), dim3(256), 0, st, a);
