@@ -30,20 +30,6 @@ struct P4Shape {
     static_assert(PaResult<HD>::BYTES <= RINGS && SLOT % 16 == 0, "the warps' results meet in the rings");
 };
 
-__device__ __forceinline__ uint32_t lds32(uint32_t at) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t at) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
-    return v;
-}
-template <int N> __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t at) {
-    if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
-    else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // of 8 x 8 halves, two of a row a lane
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));

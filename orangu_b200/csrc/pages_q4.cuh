@@ -57,4 +57,19 @@ __device__ __forceinline__ uint32_t q4_offset(uint32_t d) {  // -72 d, exact
     return n;
 }
 
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    return v;
+}
+template <int N> __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t at) {
+    if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
+    else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
+}
+
 }  // namespace ob
