@@ -537,7 +537,7 @@ int ob_pages_attention_tree(ob_pages *p, uint32_t layer, uint32_t n_seq, const v
     a.pg = view(p, layer);
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.group = n_head / p->d.n_head_kv, a.n_units = n_seq, a.scale = scale;
-    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx, a.block = max_drafts, a.blocks = 1;
+    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_drafts, a.max_ctx = max_ctx, a.block = max_drafts, a.blocks = 1, a.apart = ~0u;  // (as it was: sums of other parts are other bits)
     use_workspace(p, a);
     if (max_drafts * a.group > PG_FEW_ROWS) {
         // (the walk over all pieces counts their tiles, and PG_START more for each, in 31 bits)
@@ -704,13 +704,15 @@ int ob_pages_attention_tokens(ob_pages *p, uint32_t layer, uint32_t n_seq, const
     a.pg = view(p, layer);
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.group = n_head / p->d.n_head_kv, a.scale = scale;
-    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_tokens, a.max_ctx = max_ctx;
+    a.first = first_token, a.n_ctx = n_ctx, a.visible = visible, a.n_tokens = n_tokens, a.max_drafts = max_tokens, a.max_ctx = max_ctx, a.apart = PG_APART;
     use_workspace(p, a);
     if (mass) a.stats = reinterpret_cast<float2 *>(p->ws.mem + PG_WORKSPACE - PG_STATS);
-    a.block = std::min(PG_MAX_DRAFTS, max_tokens);
+    // Over 4-bit pages few rows are units of up to 16: their tiles are made anew for each, but rows of 128 would be mostly padding.
+    const bool few = std::min(PG_MAX_DRAFTS, max_tokens) * a.group <= (q4 ? P4_FEW_ROWS : PG_FEW_ROWS);
+    a.block = std::min(q4 && few ? std::max(1u, PG_FEW_ROWS / a.group) : PG_MAX_DRAFTS, max_tokens);
     a.blocks = (max_tokens + a.block - 1) / a.block;
     const uint64_t units = (uint64_t)n_seq * a.blocks;
-    const bool wide = a.block * a.group > PG_FEW_ROWS;
+    const bool wide = !few;
     // (a walk over all pieces counts their pages or tiles, and PG_START more for each, in 31 bits)
     if (units >= (1ull << 24) || (wide && units * p->d.n_head_kv * (((uint64_t)p->d.table_stride + PG_PAGES - 1) / PG_PAGES + PG_START) * ((a.block * a.group + 127) / 128) >= (1ull << 31)))
         return fail(p->ctx, OB_ERR_CAPACITY, "pages_attention_tokens: too many tokens, or the tables of all sequences together have room for too many positions");

@@ -16,6 +16,10 @@ constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
 // dimension 128: 16.4 and 18.4 us for one sequence of 512, 45.1 and 51.2 for 32 of 1024, 195 and 223 for 32 of 8192; 64: 14.3 and 16.4, 30.7 and
 // 43.0, 119 and 166.  More rows would read all pages once per 16.
 constexpr uint32_t PG_FEW_ROWS = 16;
+constexpr uint32_t P4_FEW_ROWS = 32;     // the same over 4-bit pages, there in units of tokens that have up to 16
+// Shares of a CTA from which on all are even (PA_MORE): 32 sequences of 2 to 8 k in 4 bits 59.5 us, and 68.0 with pieces that all begin a CTA; 8 of
+// 2000 12.6 us, and 15.5 with even shares.
+constexpr uint32_t PG_APART = 64;
 constexpr float PG_SLACK = 8.0f;         // growth of a row's maximum (powers of two) that is put up with before its output is rescaled
 // Weights are made 2^PG_RAISE times as large, in numerator and denominator alike.  An f16 weight has steps of 2^-24 at best: of the running maximum's
 // weight as 1, those below 2^-25 would vanish and those below 2^-14 lose bits, raised they are off by 2^-32.  (131,000 positions of 2^-21 behind one of 1:
@@ -56,7 +60,7 @@ struct PagedAttnArgs {
     const uint32_t *n_ctx;    // [n_units]
     const uint64_t *visible;  // [n_tokens]
     uint32_t n_tokens, max_drafts, max_ctx;  // visible may be null: a token sees those before it and itself
-    uint32_t block, blocks;   // tokens of a unit, units of a sequence (n_units: all of them); several with visible == null only
+    uint32_t block, blocks;   // tokens of a unit, units of a sequence (n_units: all of them); several with visible == null, or (mma.sync) over 4-bit pages
     float2 *stats;            // [n_tokens][n_kv * group] or null: a row's maximum and the inverse of its sum, so that a weight is 2^(score - maximum) times that
     // list
     const int32_t *list;      // [n_units][n_kv][n_list]
@@ -68,9 +72,9 @@ struct PagedAttnArgs {
     PagePiece *pieces;
     float *partial;
     uint32_t *status;  // pinned host memory: 1 when a bounded wait ran out and the outputs are not valid
+    uint32_t apart;    // mma.sync forms: shares of this many pages and more are even, whatever pieces begin in their middle
     // filled in by the launcher
     uint32_t row_tiles;
-    uint32_t apart;    // shares of this many pages and more are even, whatever pieces begin in their middle
 };
 // With `tree`, max_drafts * group is at most PG_FEW_ROWS.
 cudaError_t launch_pages_attention(const PagedAttnArgs &a, bool tree, int sm_count, cudaStream_t st);

@@ -273,7 +273,6 @@ cudaError_t launch(PagedAttnArgs a, int sm_count, cudaStream_t st) {
     const uint64_t pages = TREE ? (std::min(a.max_ctx, a.pg.stride * KV_PAGE) + a.max_drafts + KV_PAGE - 1) / KV_PAGE : a.n_list;  // (tree: about, of a sequence)
     const uint64_t most = std::min<uint64_t>({(uint64_t)sm_count * PA_CTAS, PG_COUNTERS, PG_PARTS / (2 * S::PART * 4)});
     const uint64_t grid = std::min(most, std::max<uint64_t>(1, a.n_units * ((pages + PA_LEAST - 1) / PA_LEAST) * a.pg.n_kv));
-    a.apart = ~0u;
     return launch_pdl(kernel, dim3((uint32_t)grid), dim3(PA_THREADS), S::RINGS, st, a);
 }
 

@@ -20,8 +20,6 @@ namespace ob {
 
 namespace {
 
-constexpr uint32_t P4_APART = 64;
-
 template <int HD>
 struct P4Shape {
     static constexpr uint32_t BLOCK = Q4Block<HD>::BYTES, SLOT = 2 * BLOCK;
@@ -282,7 +280,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 3) pages_q4_attentio
 }
 
 template <typename T, int HD, int NT>
-cudaError_t launch(PagedAttnArgs a, int sm_count, cudaStream_t st) {
+cudaError_t launch(const PagedAttnArgs &a, int sm_count, cudaStream_t st) {
     using S = P4Shape<HD>;
     auto kernel = pages_q4_attention_kernel<T, HD, NT>;
     static PerDeviceOnce once;
@@ -290,7 +288,6 @@ cudaError_t launch(PagedAttnArgs a, int sm_count, cudaStream_t st) {
     const uint64_t pages = (std::min<uint64_t>(a.max_ctx, (uint64_t)a.pg.stride * KV_PAGE) + a.max_drafts + KV_PAGE - 1) / KV_PAGE;  // about, of a sequence
     const uint64_t most = std::min<uint64_t>({(uint64_t)sm_count * (NT == 1 ? 4 : 3), PG_COUNTERS, PG_PARTS / (2 * PaResult<HD>::PART * 4)});
     const uint64_t grid = std::min(most, std::max<uint64_t>(1, a.n_units * ((pages + PA_LEAST - 1) / PA_LEAST) * a.pg.n_kv));
-    a.apart = P4_APART;
     return launch_pdl(kernel, dim3((uint32_t)grid), dim3(PA_THREADS), S::RINGS, st, a);
 }
 template <typename T>

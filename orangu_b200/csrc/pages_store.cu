@@ -3,11 +3,10 @@
 //   m = the entry of largest magnitude of 32 (of equal ones the negative one), d = -m / 8 made larger to 7 significant bits (and a multiple of 2^-24), c = rint(x / d) from -8 to 7
 //
 // so that m itself is -8 d or a little less.  No number counts as 0, and magnitudes above 7168 as 7168, which keeps d an f16 number and every entry c d one, too.
-// The quotient comes from a product with about 1 / d; where that lies near the middle between two codes the division is done.
+// The quotient is a product with about 1 / d and one step of Newton's, so that ties are ties.
 //
-// Half a warp has a key's or value's 128 entries, eight a lane (a quarter 64), and the same head of several tokens, so that where a row lies is worked
-// out once for keys and values of all heads and the loads of two rows are under way at once.  The arithmetic is the larger part: about 100 instructions for eight
-// entries.  Maxima are taken two at a time in the rows' type; codes are whole numbers in the low bits of a sum with 1.5 2^23, put together as
+// Half a warp has a key's or value's 128 entries, eight a lane (a quarter 64), the same place of several pages.  The arithmetic is the larger part: about 100
+// instructions for eight entries.  Maxima are taken two at a time in the rows' type; codes are whole numbers in the low bits of a sum with 1.5 2^23, put together as
 // one number of base 16 by fused multiply-adds.
 #include <algorithm>
 #include <numeric>
@@ -49,56 +48,60 @@ template <> struct Pair<bf16> {
 };
 constexpr uint32_t SIGNS = 0x80008000u;
 
-// The rows of a group of lanes: one head's keys or values of tokens j, j + step, ...
+// What a group of lanes has: one head's keys or values, positions `pos`, `pos` + `step`, ... of the sequence.  P neighbouring groups have P neighbouring positions, from a
+// multiple of P on.
 struct PgRows {
-    uint32_t head, j, step, count, room;
+    uint32_t head, pos, step, ctx, end;  // new positions: from ctx to end
     bool value;
     int32_t first;
-    uint32_t ctx;
     const int32_t *table;
 };
-template <uint32_t ROWS>
+template <uint32_t GROUPS, uint32_t P>
 __device__ __forceinline__ PgRows rows_of(const PagedMoveArgs &a, uint32_t group) {
     PgRows r;
-    const uint32_t per = 2 * a.pg.n_kv, i = blockIdx.x * ROWS + group, part = i % per, seq = blockIdx.y;
-    r.j = i / per, r.step = gridDim.x * ROWS / per;  // (the grid is made so that there is no remainder)
-    r.value = part >= a.pg.n_kv, r.head = r.value ? part - a.pg.n_kv : part;
+    constexpr uint32_t SETS = GROUPS / P;  // of a CTA
+    const uint32_t per = 2 * a.pg.n_kv, i = blockIdx.x * SETS + group / P, part = i % per, seq = blockIdx.y;
     const int32_t f0 = a.first[seq], f1 = a.first[seq + 1];
-    r.ctx = a.n_ctx[seq], r.first = f0, r.room = a.pg.stride * KV_PAGE;
-    r.count = f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens || r.ctx >= r.room ? 0u : min(min((uint32_t)(f1 - f0), a.max_tokens), r.room - r.ctx);
+    const uint32_t room = a.pg.stride * KV_PAGE;
+    r.ctx = a.n_ctx[seq], r.first = f0;
+    r.end = f0 < 0 || f1 <= f0 || (uint32_t)f1 > a.n_tokens || r.ctx >= room ? 0u : r.ctx + min(min((uint32_t)(f1 - f0), a.max_tokens), room - r.ctx);
+    r.pos = r.ctx / P * P + i / per * P + group % P, r.step = gridDim.x * SETS / per * P;  // (the grid is made so that there is no remainder)
+    r.value = part >= a.pg.n_kv, r.head = r.value ? part - a.pg.n_kv : part;
     r.table = a.pg.tables + (uint64_t)seq * a.pg.stride;
     return r;
 }
-__device__ __forceinline__ int32_t page_of(const PagedMoveArgs &a, const PgRows &r, uint32_t j) {
-    const int32_t id = j < r.count ? r.table[(r.ctx + j) / KV_PAGE] : -1;
+__device__ __forceinline__ int32_t page_of(const PagedMoveArgs &a, const PgRows &r, uint32_t pos) {
+    const int32_t id = pos >= r.ctx && pos < r.end ? r.table[pos / KV_PAGE] : -1;
     return (uint32_t)id < a.pg.n_pages ? id : -1;
 }
 
 constexpr uint32_t ST_DEEP = 2;  // rows of a lane under way
 
-// grid (groups of lanes: (token, head, keys or values), sequences)
-template <typename T, int HD>
+// grid (sets of P positions x heads x keys and values, sequences).  With P = 16 a page's positions of one head are a CTA's (two pages with head dimension 64), so that
+// its sectors are read and written together: 32000 rows of 8 heads of 128 take 82 us to store and to load again (floor 51), with P = 1 101.  That is for few
+// positions: a step of 64 sequences takes 3.5 and 5 us then, and 7 each with P = 16.
+template <typename T, int HD, uint32_t P>
 __global__ void __launch_bounds__(256) pages_store_kernel(const __grid_constant__ PagedMoveArgs a) {
     using B = Q4Block<HD>;
     constexpr uint32_t LANES = HD / 8, ROWS = 256 / LANES;
     pdl_release();
     pdl_wait();
     const uint32_t w = threadIdx.x % LANES;
-    const PgRows r = rows_of<ROWS>(a, threadIdx.x / LANES);
+    const PgRows r = rows_of<ROWS, P>(a, threadIdx.x / LANES);
     const T *src = static_cast<const T *>(r.value ? a.v : a.k) + (uint64_t)(uint32_t)r.first * (r.value ? a.v_stride : a.k_stride) + (uint64_t)r.head * HD + w * 8;
     const uint64_t stride = r.value ? a.v_stride : a.k_stride;
     uint8_t *pool = static_cast<uint8_t *>(const_cast<void *>(r.value ? a.pg.v : a.pg.k)) + (uint64_t)r.head * B::BYTES;
     const uint64_t page_bytes = (uint64_t)a.pg.n_kv * B::BYTES;
     constexpr uint32_t lanes = 0xffffffffu;  // (a warp's groups go on as long as one of them has rows)
-    for (uint32_t j0 = r.j; __any_sync(lanes, j0 < r.count); j0 += ST_DEEP * r.step) {
+    for (uint32_t pos = r.pos; __any_sync(lanes, pos < r.end); pos += ST_DEEP * r.step) {
         uint4 u[ST_DEEP];
         int32_t id[ST_DEEP];
 #pragma unroll
         for (uint32_t k = 0; k < ST_DEEP; ++k) {
-            const uint32_t j = j0 + k * r.step;
+            const uint32_t x = pos + k * r.step;
             u[k] = make_uint4(0, 0, 0, 0);
-            if (j < r.count) u[k] = ldg128_stream(src + j * stride);
-            id[k] = page_of(a, r, j);
+            if (x >= r.ctx && x < r.end) u[k] = ldg128_stream(src + (x - r.ctx) * stride);
+            id[k] = page_of(a, r, x);
         }
 #pragma unroll
         for (uint32_t k = 0; k < ST_DEEP; ++k) {
@@ -134,26 +137,24 @@ __global__ void __launch_bounds__(256) pages_store_kernel(const __grid_constant_
             const float eighth = fmaxf(most, least) * 0.125f;
             // up to 7 significant bits; below 2^-18 to a multiple of 2^-24, the steps of f16
             float d = __uint_as_float((__float_as_uint(eighth) + 0x1ffffu) & ~0x1ffffu);
-            if (eighth < 0x1p-18f) d = ceilf(eighth * 0x1p24f) * 0x1p-24f;
+            if (__builtin_expect(eighth < 0x1p-18f, 0)) d = ceilf(eighth * 0x1p24f) * 0x1p-24f;
             if (most > least) d = -d;
-            const float by = d != 0.0f ? d : 1.0f, inverse = __frcp_rn(by);
+            const float by = d != 0.0f ? d : 1.0f;
+            float inverse, c[8];
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(by));
             constexpr float MAGIC = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers, ties to even
-            float c[8], off = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float t = fmaf(x[e], inverse, MAGIC) - MAGIC;
-                off = fmaxf(off, fabsf(fmaf(x[e], inverse, -t)));  // (off by 8 times 2^-24 and a rounding)
-                c[e] = fminf(t, 7.0f);
-            }
-            if (off > 0.5f - 0x1p-19f) {  // next to the middle between two codes
-#pragma unroll
-                for (int e = 0; e < 8; ++e) c[e] = fmaxf(-8.0f, fminf(rintf(__fdiv_rn(x[e], by)), 7.0f));
+                // a product with about 1 / d, and what is left over (exact: 11 bits less 4 times 7) once more: a quotient of 5 bits, as one in the middle between two codes is,
+                // comes out as it is, and any other is further from the middle (2^-12 of it) than it is off (2^-23)
+                const float q = x[e] * inverse;
+                c[e] = fminf((fmaf(fmaf(-q, by, x[e]), inverse, q) + MAGIC) - MAGIC, 7.0f);
             }
             // c + 8 in base 16: even entries in the low half, odd ones in the high half
             constexpr float EIGHTS = 8.0f * 0x1111;
             const float low = fmaf(fmaf(fmaf(c[6], 16.0f, c[4]), 16.0f, c[2]), 16.0f, c[0]) + (EIGHTS + MAGIC), high = fmaf(fmaf(fmaf(c[7], 16.0f, c[5]), 16.0f, c[3]), 16.0f, c[1]) + (EIGHTS + MAGIC);
             if (id[k] < 0) continue;
-            const uint32_t p = (r.ctx + j0 + k * r.step) % KV_PAGE;
+            const uint32_t p = (pos + k * r.step) % KV_PAGE;
             uint8_t *block = pool + (uint32_t)id[k] * page_bytes;
             if (r.value) {
                 uint16_t *at = reinterpret_cast<uint16_t *>(block + B::value(p, w));
@@ -167,26 +168,26 @@ __global__ void __launch_bounds__(256) pages_store_kernel(const __grid_constant_
 }
 
 constexpr uint32_t LD_DEEP = 4;
-template <typename T, int HD>
+template <typename T, int HD, uint32_t P>
 __global__ void __launch_bounds__(256) pages_load_kernel(const __grid_constant__ PagedMoveArgs a) {
     using B = Q4Block<HD>;
     constexpr uint32_t LANES = HD / 8, ROWS = 256 / LANES;
     pdl_release();
     pdl_wait();
     const uint32_t w = threadIdx.x % LANES;
-    const PgRows r = rows_of<ROWS>(a, threadIdx.x / LANES);
+    const PgRows r = rows_of<ROWS, P>(a, threadIdx.x / LANES);
     T *dst = static_cast<T *>(const_cast<void *>(r.value ? a.v : a.k)) + (uint64_t)(uint32_t)r.first * (r.value ? a.v_stride : a.k_stride) + (uint64_t)r.head * HD + w * 8;
     const uint64_t stride = r.value ? a.v_stride : a.k_stride;
     const uint8_t *pool = static_cast<const uint8_t *>(r.value ? a.pg.v : a.pg.k) + (uint64_t)r.head * B::BYTES;
     const uint64_t page_bytes = (uint64_t)a.pg.n_kv * B::BYTES;
-    for (uint32_t j0 = r.j; j0 < r.count; j0 += LD_DEEP * r.step) {
+    for (uint32_t pos = r.pos; pos < r.end; pos += LD_DEEP * r.step) {
         uint32_t code[LD_DEEP], unit[LD_DEEP];
         int32_t id[LD_DEEP];
 #pragma unroll
-        for (uint32_t k = 0; k < LD_DEEP; ++k) id[k] = page_of(a, r, j0 + k * r.step);
+        for (uint32_t k = 0; k < LD_DEEP; ++k) id[k] = page_of(a, r, pos + k * r.step);
 #pragma unroll
         for (uint32_t k = 0; k < LD_DEEP; ++k) {
-            const uint32_t p = (r.ctx + j0 + k * r.step) % KV_PAGE;
+            const uint32_t p = (pos + k * r.step) % KV_PAGE;
             const uint8_t *block = pool + (uint32_t)max(id[k], 0) * page_bytes;
             code[k] = unit[k] = 0;
             if (id[k] < 0) continue;
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(256) pages_load_kernel(const __grid_constant__
                     u[e] = pack2(f.x, f.y, T());
                 }
             }
-            __stcs(reinterpret_cast<uint4 *>(dst + (j0 + k * r.step) * stride), make_uint4(u[0], u[1], u[2], u[3]));
+            __stcs(reinterpret_cast<uint4 *>(dst + (pos + k * r.step - r.ctx) * stride), make_uint4(u[0], u[1], u[2], u[3]));
         }
     }
 }
@@ -219,13 +220,20 @@ __global__ void __launch_bounds__(256) pages_load_kernel(const __grid_constant__
 }  // namespace
 
 cudaError_t launch_pages_store(const PagedMoveArgs &a, bool is_bf16, bool load, int sm_count, cudaStream_t st) {
-    // Whole rounds of (head, keys or values), and CTAs for all places (eight an SM); fewer where there are few tokens.
-    const uint32_t rows = 256 / (a.pg.dim / 8), per = 2 * a.pg.n_kv, round = per / std::gcd(per, rows);
-    const uint64_t all = ((uint64_t)a.max_tokens * per + rows - 1) / rows, most = std::max<uint64_t>(1, 8ull * sm_count / a.n_seq);
+    // Whole rounds of (head, keys or values), and CTAs for all places (eight an SM); fewer where there are few positions.
+    const bool whole = a.max_tokens >= KV_PAGE;  // pages
+    const uint32_t positions = whole ? KV_PAGE : 1, sets = 256 / (a.pg.dim / 8) / positions, per = 2 * a.pg.n_kv, round = per / std::gcd(per, sets);
+    const uint64_t all = (((uint64_t)(a.max_tokens - 1) / positions + whole + 1) * per + sets - 1) / sets, most = std::max<uint64_t>(1, 8ull * sm_count / a.n_seq);  // (positions that do not begin a page touch one more)
     const dim3 grid((uint32_t)((std::min(all, most) + round - 1) / round * round), a.n_seq);
-    auto pick = [&](auto k64, auto k128) { return launch_pdl(a.pg.dim == 64 ? k64 : k128, grid, dim3(256), 0, st, a); };
-    if (load) return is_bf16 ? pick(pages_load_kernel<bf16, 64>, pages_load_kernel<bf16, 128>) : pick(pages_load_kernel<__half, 64>, pages_load_kernel<__half, 128>);
-    return is_bf16 ? pick(pages_store_kernel<bf16, 64>, pages_store_kernel<bf16, 128>) : pick(pages_store_kernel<__half, 64>, pages_store_kernel<__half, 128>);
+    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, dim3(256), 0, st, a); };
+    auto dim = [&](auto type, auto p) {
+        using T = decltype(type);
+        constexpr uint32_t P = decltype(p)::value;
+        if (load) return a.pg.dim == 64 ? go(pages_load_kernel<T, 64, P>) : go(pages_load_kernel<T, 128, P>);
+        return a.pg.dim == 64 ? go(pages_store_kernel<T, 64, P>) : go(pages_store_kernel<T, 128, P>);
+    };
+    auto pick = [&](auto type) { return whole ? dim(type, std::integral_constant<uint32_t, KV_PAGE>()) : dim(type, std::integral_constant<uint32_t, 1>()); };
+    return is_bf16 ? pick(bf16()) : pick(__half());
 }
 
 }  // namespace ob
