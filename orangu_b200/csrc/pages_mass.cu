@@ -83,16 +83,19 @@ __global__ void __launch_bounds__(PA_THREADS, 3) pages_mass_kernel(const __grid_
 #pragma unroll 1
             for (uint32_t i = 0; i + 1 < DEPTH; ++i) request(i);
             __syncthreads();  // (of the columns before)
+            // ---- rows: a row that sees nothing has a maximum of minus infinity and an inverse of zero; it counts as a row of zeros, as one that is none does
+            for (uint32_t c = threadIdx.x; c < sets * 8; c += PA_THREADS) {
+                const uint32_t r = c0 + c, tok = r / a.group;
+                const float2 st = r < n_cols ? a.stats[((uint64_t)row0 + tok) * a.group * a.pg.n_kv + head * a.group + r - tok * a.group] : make_float2(0.0f, 0.0f);
+                s_row[c] = make_float4(scale2, st.y != 0.0f ? -st.x : 0.0f, st.y, __uint_as_float(tok));
+            }
+            __syncthreads();
             // ---- queries: a warp a set of eight at a time, as B fragments; the order of a product's terms is that of the keys
+#pragma unroll 2
             for (uint32_t k = warp; k < sets; k += PA_WARPS) {
-                const uint32_t r = c0 + k * 8 + g, tok = r / a.group;
-                const bool live = r < n_cols;
-                const uint64_t token = (uint64_t)row0 + tok;
-                const uint32_t h = head * a.group + r - tok * a.group;
-                // A row that sees nothing has a maximum of minus infinity and an inverse of zero: it counts as a row of zeros, as one that is none does.
-                const float2 st = live ? a.stats[token * a.group * a.pg.n_kv + h] : make_float2(0.0f, 0.0f);
-                const bool counts = st.y != 0.0f;
-                const T *row = static_cast<const T *>(a.q) + (live ? token * a.q_stride + (uint64_t)h * HD : 0u);
+                const uint32_t r = c0 + k * 8 + g, tok = r / a.group, h = head * a.group + r - tok * a.group;
+                const bool counts = r < n_cols && s_row[k * 8 + g].z != 0.0f;
+                const T *row = static_cast<const T *>(a.q) + (r < n_cols ? ((uint64_t)row0 + tok) * a.q_stride + (uint64_t)h * HD : 0u);
                 uint32_t q[HD / 8];
                 if constexpr (Q4) {
 #pragma unroll
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) pages_mass_kernel(const __grid_
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < KW; ++i) s_q[(k * KW + i) * 32 + lane] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
-                if (t == 0) s_row[k * 8 + g] = make_float4(factor * scale2, counts ? -st.x : 0.0f, st.y, __uint_as_float(tok));
+                if (Q4 && !std::is_same<T, __half>::value && t == 0) s_row[k * 8 + g].x = factor * scale2;
             }
             __syncthreads();
 #pragma unroll 1
