@@ -23,7 +23,7 @@ __device__ __forceinline__ uint32_t warps_before(uint32_t mine, uint32_t *parts)
 // largest word that is not SEL_FORCED, as far as this thread has seen, and more than `want` words are not.  The whole CTA, once.
 // keys: anything that keys[i] gives the word of place i of.
 template <uint32_t THREADS, typename K>
-__device__ __forceinline__ void pick(uint32_t want, const K &keys, uint32_t n, uint32_t lo, uint32_t hi, int32_t *out) {
+__device__ __forceinline__ void pick(uint32_t want, K keys, uint32_t n, uint32_t lo, uint32_t hi, int32_t *out) {
     constexpr uint32_t NW = THREADS / 32, BINS = SEL_BINS / THREADS;  // bins of a thread
     __shared__ uint32_t s_hist[SEL_BINS], s_parts[5][32], s_pick[3];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

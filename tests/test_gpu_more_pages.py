@@ -328,6 +328,24 @@ def test_many_sequences_and_a_layer_of_several(backend, pages, kind):
     run_tokens(made, 4, ctx, counts, None, weighed=True, layer=1)
 
 
+@pytest.mark.parametrize("pages,kind,group", [("q4", "f16", 4), ("q4", "bf16", 16), ("bf16", "bf16", 8)])
+def test_prompts_that_reach_past_their_table_and_rows_before_the_first(backend, pages, kind, group):
+    """Positions behind a table's last page are nobody's: the tokens there see what there is.  Rows of no sequence are left as they were, in front, too."""
+    import torch
+
+    made = Held(backend, pages, kind, 1, 64, [96, 40], seed=4)  # tables of six pages
+    ctx, first = [20, 39], [3, 103, 104]
+    q, qb = plain.bits16((110, group, 64), made.r, kind, 1.5)
+    out = torch.full((110, group, 64), 7.0, dtype=torch.float16 if kind == "f16" else torch.bfloat16, device="cuda")
+    mass = torch.zeros((2, 1, 96), device="cuda")
+    made.cache.attention_tokens(device16(qb, kind), ints(first), ints(ctx), 0.125, out, max_tokens=100, max_context=39, mass=mass, stream=current())
+    made.cache.synchronize(current())
+    want, mass64 = np.full((110, group, 64), 7.0), np.zeros((2, 1, 96))
+    tol, mass_tol = more.attend_tokens(q, made.k[0], made.v[0], made.there, first, ctx, None, 0.125, want, mass64, weight_error(64), U["f16"] if pages == "q4" and kind == "bf16" else 0.0)
+    off = np.abs(float64(out) - want) - (tol[..., None] + U[kind] * (np.abs(want) + tol[..., None]) + 2.0 ** -25)
+    assert off.max() <= 0 and (np.abs(mass.cpu().numpy() - mass64) <= mass_tol).all()
+
+
 # ------------------------------------------------------------------------------------------- cutting caches down
 def run_evict(made, n_pos, n_keep, first, last, mass, max_pos=None, width=None):
     import torch
@@ -490,6 +508,18 @@ def test_verify(backend, kind, drafted, vocab, sizes, chain):
             row = draft[first[s] + parent[i]]
             tokens[i] = r.choice(vocab, p=row / row.sum()) if row.sum() else 0
     run_verify(backend, kind, target, draft if drafted else None, tokens, parent, first, r.random(n), pad=3)
+
+
+@pytest.mark.parametrize("vocab,sequences", [(700, 100), (700, 200), (20_000, 300)])
+def test_verify_of_many_sequences(backend, vocab, sequences):
+    """Fewer CTAs a sequence, and parts of more than 1024 tokens."""
+    r = np.random.default_rng(sequences)
+    sizes = r.integers(1, 4, sequences)
+    first, n = np.concatenate([[0], np.cumsum(sizes)]), int(sizes.sum())
+    target, draft = distributions(r, n, vocab, "f32")
+    parent = np.concatenate([[-1, 0, 0][:m] for m in sizes])
+    tokens = np.array([r.choice(vocab, p=row / row.sum()) for row in draft])
+    run_verify(backend, "f32", target, draft, tokens, parent, first, r.random(n))
 
 
 def test_verify_at_the_edges(backend):
