@@ -723,7 +723,8 @@ int ob_pages_attention_tokens(ob_pages *p, uint32_t layer, uint32_t n_seq, const
                              : (wide ? launch_pages_tree_tc5(a, p->maps[layer], p->ctx->sm_count, st) : launch_pages_attention(a, true, p->ctx->sm_count, st));
     if (int rc = launched(p, who, e, wide ? 2 : 1)) return rc;
     if (!mass) return OB_OK;
-    return launched(p, who, launch_pages_mass(a, q_bf16, q4, n_seq, mass, mass_stride, p->ctx->sm_count, st));
+    const bool many = (uint64_t)max_tokens * a.group > (q4 && q_bf16 ? P4_MASS_ROWS_BF16 : PG_MASS_ROWS);
+    return launched(p, who, (many ? launch_pages_mass_tc5 : launch_pages_mass)(a, q_bf16, q4, n_seq, mass, mass_stride, p->ctx->sm_count, st));
 }
 
 namespace {

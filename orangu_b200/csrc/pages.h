@@ -93,6 +93,11 @@ cudaError_t launch_pages_q4_tc5(const PagedAttnArgs &a, bool q_bf16, int sm_coun
 // After an attention with `stats`, whose units are of n_seq sequences: [n_seq][n_kv][mass_stride].
 cudaError_t launch_pages_mass(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, int sm_count, cudaStream_t st);
 
+// Rows a key/value head up to which the first of the two is taken: 64 and 128 rows over f16 pages, 16 sequences of 2000, attention among it: 72.9 and 94.6 us with it, 75.9
+// and 81.0 on tcgen05.  Where bfloat16 queries have to become f16 ones for every tile it is more: 128 rows over 4-bit pages 95.0 and 101.0, 512 (one of 12,000) 175 and 170.
+constexpr uint32_t PG_MASS_ROWS = 96, P4_MASS_ROWS_BF16 = 256;
+cudaError_t launch_pages_mass_tc5(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, int sm_count, cudaStream_t st);
+
 struct PagedMoveArgs {  // rows into 4-bit pages, or out of them
     PageView pg;
     const void *k, *v;  // [n_tokens][n_kv][dim], strides in elements
