@@ -190,7 +190,7 @@ int ob_attention_decode_static(ob_ctx *ctx, const float *q_dev, const void *k_pa
 /* ------------------------------------------------- pages of a cache that the caller holds
  * Operators of speculative decoding and of long contexts over caller-owned device memory, beside ob_attention_decode_static.  No
  * counterpart in the reference, whose caches are contiguous.  A cache is K and V apart, [layer][page][n_head_kv][16][head_dim], f16 or
- * bfloat16 (queries and outputs are of the same type), and a table of page numbers per sequence: position x of sequence s lies in slot
+ * bfloat16 (queries and outputs are of the same type), or in 4 bits (OB_TYPE_Q4_PAGES), and a table of page numbers per sequence: position x of sequence s lies in slot
  * x % 16 of page tables[s][x / 16].  An entry outside [0, n_pages) holds no positions: nobody sees them, nothing is read or written there.
  *
  * All pointers but `desc` are device memory of the context's GPU (refused otherwise).  Calls are asynchronous on `stream` (a cudaStream_t
@@ -200,7 +200,8 @@ int ob_attention_decode_static(ob_ctx *ctx, const float *q_dev, const void *k_pa
  * them a range, what lies outside is left out, never followed.  Products accumulate in fp32, softmax statistics are fp32. */
 #define OB_TYPE_F16 1u /* with OB_TYPE_BF16 below: types of pages; neither is a type of weights here */
 #define OB_TYPE_Q4_PAGES 256u /* pages in 4 bits, [layer][page][n_head_kv][9 * head_dim] bytes, for keys and for values: written by ob_pages_store, read by
-                               * ob_pages_load and ob_pages_attention_tokens; copied, forked and kept like the others */
+                               * ob_pages_load and ob_pages_attention_tokens; copied, forked, kept and cut like the others; refused
+                               * (OB_ERR_UNSUPPORTED) by ob_pages_attention_tree, _bounds, _select and _attention */
 typedef struct ob_pages ob_pages;
 typedef struct ob_pages_desc {
     void *k, *v;            /* aligned to 16 bytes */
@@ -217,7 +218,7 @@ typedef struct ob_pages_desc {
  * below 2^31 - 128, n_layer at most 16383, n_head_kv 4096, n_seq 2^24, table_stride 2^26 (OB_ERR_UNSUPPORTED). */
 int ob_pages_create(ob_ctx *ctx, const ob_pages_desc *desc, ob_pages **out);
 void ob_pages_destroy(ob_pages *pages);
-/* Waits for `stream`, on which the handle was used.  Every wait inside the kernels is bounded: OB_ERR_CUDA when ob_pages_attention_tree, called or replayed
+/* Waits for `stream`, on which the handle was used.  Every wait inside the kernels is bounded: OB_ERR_CUDA when ob_pages_attention_tree or ob_pages_attention_tokens, called or replayed
  * from a capture, gave one up since this was last asked, and its output is not valid.  (Never seen; a call returns before its kernels run and cannot
  * say so itself.)  ob_synchronize reports it, too, for all of a context's handles, but waits for the context's stream only. */
 int ob_pages_synchronize(ob_pages *pages, void *stream);
@@ -305,7 +306,7 @@ int ob_pages_attention_tokens(ob_pages *pages, uint32_t layer, uint32_t n_seq, c
  * sequence's new keys are rotated by the token's own number, not by where they lie. */
 int ob_pages_evict(ob_pages *pages, uint32_t n_seq, const uint32_t *n_pos, float *mass, uint64_t mass_stride, uint32_t max_pos, uint32_t n_keep,
                    uint32_t keep_first, uint32_t keep_last, int32_t *kept, uint32_t *n_left, void *stream);
-/* ob_pages_keep for the masses of all layers: call both. */
+/* ob_pages_keep for the masses of all layers: call both.  The same limit. */
 int ob_pages_keep_mass(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, const int32_t *kept, uint32_t kept_stride, const uint32_t *n_kept,
                        float *mass, uint64_t mass_stride, void *stream);
 

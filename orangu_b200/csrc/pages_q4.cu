@@ -9,8 +9,10 @@
 // remainder; where it is bfloat16 their value alone, which is off by 2^-12 at most, an eighth of what the output's own rounding is (64 sequences of 4 to 16 k, 4 rows of
 // 128: 165 us, and 183 with remainders).
 //
-// 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, so that its arithmetic comes close to its bytes: of an SM's 472 issue slots
-// in the time that 2304 bytes take at 6.5 TB/s, about 180 make the entries, 24 are products, 30 reads of shared memory.
+// 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, and its arithmetic is what bounds it: about 345 instructions a page of 128 (4-bit words to
+// entries 176, products 16, copies, scores and weights the rest) against 472 issue slots of an SM in the time that the bytes take.  64 sequences of 4 to
+// 16 k, 8 heads of 128, 4 rows: 165 us (4.2 TB/s; 115 with the copies alone, 124 without the values' half), 64 of 64 entries 112 us.  More CTAs an SM, deeper rings, products apart or
+// two sums of scores at once changed nothing; instructions did (373 a page, with remainders: 183).
 #include <algorithm>
 
 #include "pages_q4.cuh"
