@@ -25,8 +25,8 @@
 // two on the fused multiply-adds, 1/8 to 1/2 of them, took from 2 % less to 6 % more.
 //
 // Over 4-bit pages (Q4) warps make the f16 operand tiles out of codes, where TMA brings them otherwise; rows of bfloat16 have weights without remainders.  Four warps
-// do it, two for keys and two for values: of a step of 64 positions they are a fifth (10 sequences of 2000 in the caches, 128 rows of 128: 38 us, f16 pages 33).  8 x 16
-// tokens of 4 heads at 8k: 43 us; 1000 tokens of 8 heads at 8000: 338 us, 820 TFLOP/s of scores and values.
+// do it, two for keys and two for values.  8 x 16 tokens of 4 heads at 8192: 67 us (f16 pages 61); with three quarters of any one part left out, making of tiles, softmax, products or
+// copies, 56 to 66: no one of them bounds it, and 17 are the same at 512 positions.  1000 tokens of 8 heads at 8000: 334 us, 830 TFLOP/s of scores and values.
 //
 // Context positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
 // per thread.  There, values of positions that nobody has, or that are no numbers, are set to zero in shared memory (0 times them
@@ -218,7 +218,7 @@ struct PgWalk {
 template <int HD, bool VALUE>
 struct P4Tile {
     using B = Q4Block<HD>;
-    static constexpr uint32_t QUADS = HD / 32, EACH = PG_KEYS * QUADS / 32, WORDS = B::BYTES / 16, BYTES = PG_PAGES * B::BYTES;  // 16 bytes of codes: 32 entries with one unit; a row's, a lane's
+    static constexpr uint32_t QUADS = HD / 32, WORDS = B::BYTES / 16, BYTES = PG_PAGES * B::BYTES;  // 16 bytes of codes: 32 entries with one unit; a row's, a lane's
 
     // id: lane p < PG_PAGES has the number of the tile's page p, or -1 (zeros: its entries are zero).
     static __device__ __forceinline__ void request(uint32_t dst, const uint8_t *pool, uint32_t n_kv, uint32_t head, int32_t id) {
@@ -231,38 +231,52 @@ struct P4Tile {
             for (uint32_t c = lane; c < WORDS; c += 32) cp16(dst + p * B::BYTES + c * 16, block + c * 16, page >= 0);
         }
     }
-    static __device__ __forceinline__ void put(uint8_t *operand, uint32_t row, uint32_t c, uint32_t x, uint32_t d, uint32_t n) {  // eight entries
-        *reinterpret_cast<uint4 *>(operand + c / 8 * PG_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-            make_uint4(q4_field(x, 0, d, n), q4_field(x, 1, d, n), q4_field(x, 2, d, n), q4_field(x, 3, d, n));
+    static __device__ __forceinline__ void put(uint32_t at, uint32_t x, uint32_t d, uint32_t n) {  // eight entries
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q4_field(x, 0, d, n)), "r"(q4_field(x, 1, d, n)), "r"(q4_field(x, 2, d, n)), "r"(q4_field(x, 3, d, n)) : "memory");
     }
-    static __device__ __forceinline__ void make(const uint8_t *src, uint8_t *operand) {
-        uint32_t lane = threadIdx.x & 31;
-        asm volatile("" : "+r"(lane));  // (places are worked out where they are used)
-#pragma unroll 1
-        for (uint32_t i = 0; i < EACH; ++i) {
-            const uint32_t at = i * 32 + lane, page = at / (QUADS * KV_PAGE), in_page = at % (QUADS * KV_PAGE);
-            const uint8_t *block = src + page * B::BYTES;
-            const uint4 code = reinterpret_cast<const uint4 *>(block)[in_page];
-            // eight lanes write two rows, or one: those of the second block of columns (head dimension 64: of the second row) have another order, so that no two
-            // are in one bank
-            if constexpr (VALUE) {
-                const uint32_t r = in_page / (2 * QUADS), w = B::eight(r, 2 * (in_page % (2 * QUADS))), row = page * KV_PAGE + 2 * r;
-                const bool other = HD == 128 ? (w & 8) != 0 : (r & 1) != 0;
-                const uint32_t u = *reinterpret_cast<const uint32_t *>(block + B::unit(true, 2 * r, w / 4));
-                const uint32_t d0 = __byte_perm(u, u, 0x1010), d1 = __byte_perm(u, u, 0x3232), n0 = q4_offset(d0), n1 = q4_offset(d1);
-                const uint32_t x0 = other ? code.z : code.x, y0 = other ? code.w : code.y, x1 = other ? code.x : code.z, y1 = other ? code.y : code.w, w0 = other ? w + 1 : w, w1 = other ? w : w + 1;
-                put(operand, row, w0, __byte_perm(x0, y0, 0x5410), d0, n0);
-                put(operand, row + 1, w0, __byte_perm(x0, y0, 0x7632), d1, n1);
-                put(operand, row, w1, __byte_perm(x1, y1, 0x5410), d0, n0);
-                put(operand, row + 1, w1, __byte_perm(x1, y1, 0x7632), d1, n1);
-            } else {
-                const uint32_t pos = in_page / QUADS, q = in_page % QUADS, row = page * KV_PAGE + pos;
-                const bool other = HD == 128 && (q & 2);
-                const uint32_t d = *reinterpret_cast<const uint16_t *>(block + B::unit(false, pos, q)) * 0x10001u, n = q4_offset(d);
-                const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+    // A lane's words of a page are ROWS positions apart, a multiple of 8: where it reads and writes within them and how its rows are swizzled stays the same.
+    // (With addresses made for every word, 8 x 16 tokens of 4 heads at 8192 took 77 us, and 67 so.)
+    static constexpr uint32_t PER = QUADS * KV_PAGE / 32, ROWS = KV_PAGE / PER;
+    static __device__ __forceinline__ void make(uint32_t src, uint32_t operand) {
+        const uint32_t lane = threadIdx.x & 31;
+        // eight lanes write two rows, or one: those of the second block of columns (head dimension 64: of the second row) have another order, so that no two
+        // are in one bank
+        const uint32_t r = lane / (2 * QUADS), w = B::eight(r, 2 * (lane % (2 * QUADS))), pos = VALUE ? 2 * r : lane / QUADS, q = VALUE ? w / 4 : lane % QUADS;
+        const bool other = VALUE ? (HD == 128 ? (w & 8) != 0 : (r & 1) != 0) : HD == 128 && (q & 2);
+        uint32_t to[4];  // by the order of its stores; values: two eights of two positions
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) put(operand, row, 4 * q + (other ? e ^ 2 : e), other ? w[e ^ 2] : w[e], d, n);
+        for (uint32_t e = 0; e < 4; ++e) {
+            const uint32_t row = VALUE ? pos + (e & 1) : pos, c = VALUE ? (e / 2 ^ (other ? 1 : 0)) + w : 4 * q + (other ? e ^ 2 : e);
+            to[e] = operand + c / 8 * PG_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        }
+        const uint32_t unit = B::unit(VALUE, pos, q);
+#pragma unroll 1
+        for (uint32_t page = 0; page < PG_PAGES; ++page, src += B::BYTES) {
+            uint32_t code[PER][4], u[PER];
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i) {
+                lds_words(code[i], src + i * 512 + lane * 16);
+                u[i] = VALUE ? lds32(src + unit + B::unit(true, i * ROWS, 0) - B::CODES) : lds16(src + unit + B::unit(false, i * ROWS, 0) - B::CODES);
             }
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i) {
+                const uint32_t a0 = other ? code[i][2] : code[i][0], b0 = other ? code[i][3] : code[i][1], a1 = other ? code[i][0] : code[i][2], b1 = other ? code[i][1] : code[i][3], at = i * ROWS * 128;
+                if constexpr (VALUE) {
+                    const uint32_t d0 = __byte_perm(u[i], u[i], 0x1010), d1 = __byte_perm(u[i], u[i], 0x3232), n0 = q4_offset(d0), n1 = q4_offset(d1);
+                    put(to[0] + at, __byte_perm(a0, b0, 0x5410), d0, n0);
+                    put(to[1] + at, __byte_perm(a0, b0, 0x7632), d1, n1);
+                    put(to[2] + at, __byte_perm(a1, b1, 0x5410), d0, n0);
+                    put(to[3] + at, __byte_perm(a1, b1, 0x7632), d1, n1);
+                } else {
+                    const uint32_t d = __byte_perm(u[i], u[i], 0x1010), n = q4_offset(d);
+                    put(to[0] + at, a0, d, n);
+                    put(to[1] + at, b0, d, n);
+                    put(to[2] + at, a1, d, n);
+                    put(to[3] + at, b1, d, n);
+                }
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) to[e] += KV_PAGE * 128;
         }
     }
 };
@@ -351,7 +365,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     const uint32_t st = n % PLACES, from = slot + 1 == P4_AHEAD ? 0 : slot + 1;
                     ok = mbar_wait_warp(empty + 8 * st, ((n / PLACES) & 1u) ^ 1u, abort);  // (a place that was not used yet is empty)
                     if (!ok) break;
-                    Tile::make(own + from * Tile::BYTES, smem + (VALUE ? P::V : P::K) + st * PLACE);
+                    Tile::make(smem_addr(own) + from * Tile::BYTES, sbase + (VALUE ? P::V : P::K) + st * PLACE);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();  // (all of the warp's rows are written, and its codes read)
                     if (lane == 0) mbar_arrive(full + 8 * st);
