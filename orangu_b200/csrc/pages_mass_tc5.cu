@@ -8,8 +8,8 @@
 // One operand stays and the other streams: with up to 128 columns the queries of a (sequence, head) stay and its keys go by; with more the keys of 128
 // positions stay and the queries go by.  The pages of all pieces are shared out evenly (pages_walk.cuh), a tile is eight of them.  A position has one
 // writer, columns are added up in order: no atomics.  Its floor is the special function unit's, 16 powers of two a clock: 500 tokens of 4 heads a head at 12,000, 8 heads of 128, 46 us.
-// It takes 241 us (the mma.sync form 627): a column's four numbers are read from shared memory for every position, and the tiles of queries come anew for every
-// 128 positions (bfloat16 ones over 4-bit pages are made f16 each time: 431 us).  All waits are bounded; after one that was given up
+// It takes 236 us (the mma.sync form 627): a warp's step of 128 positions and 64 columns is some 1100 instructions, of which weights are a third, and issues half of the
+// time; tiles of queries come anew for every 128 positions (bfloat16 ones over 4-bit pages are made f16 each time: 431 us).  All waits are bounded; after one that was given up
 // every warp still goes through its loop, so that none is missed at a barrier.
 #include <algorithm>
 
@@ -76,8 +76,18 @@ template <typename T, int HD, bool Q4> struct MtKeys : MtTurns<HD> {
         }
     }
 };
-// Columns c0 .. of the piece's n_cols as rows of a tile, and of each its factor, minus its maximum, the inverse of its sum and its token; columns that are none have
-// an inverse of zero.
+// Columns c0 .. of the piece's n_cols as rows of a tile, and what is known of each, two neighbours together where both are read at once: minus its maximum, the
+// inverse of its sum, its token (-1: none, or it sees nothing: no weights, whatever its scores), and its factor where they are not all the same.
+struct MtRows {
+    float pair[MT_ROWS / 2][4];  // maximum, maximum, inverse, inverse
+    int32_t token[MT_ROWS];
+    float factor[MT_ROWS];
+};
+__device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
 template <typename T, int HD, bool Q4> struct MtQueries : MtTurns<HD> {
     using M = MtTurns<HD>;
     static constexpr bool FACTORS = Q4 && !std::is_same<T, __half>::value;  // bfloat16 queries become f16 ones (pages_q4.cu)
@@ -97,7 +107,7 @@ template <typename T, int HD, bool Q4> struct MtQueries : MtTurns<HD> {
         stat = make_float2(0.0f, 0.0f);
         if (threadIdx.x < MT_ROWS && c < n_cols) stat = a.stats[((uint64_t)row0 + tok) * a.group * a.pg.n_kv + head * a.group + c - tok * a.group];
     }
-    __device__ __forceinline__ void finish(uint32_t c0, uint32_t magic, float scale2, uint8_t *tile, float4 *rows) {
+    __device__ __forceinline__ void finish(uint32_t c0, uint32_t magic, float scale2, uint8_t *tile, MtRows &rows) {
         if constexpr (FACTORS) {
 #pragma unroll
             for (uint32_t i = 0; i < M::TURNS; ++i) {
@@ -114,13 +124,13 @@ template <typename T, int HD, bool Q4> struct MtQueries : MtTurns<HD> {
                     u[x] = Half2<__half>::pack(f.x * up, f.y * up);
                 }
                 *reinterpret_cast<uint4 *>(tile + M::place(i)) = make_uint4(u[0], u[1], u[2], u[3]);
-                if (M::word() == 0) rows[M::row(i)].x = __uint_as_float((uint32_t)(127 - e) << 23) * scale2;
+                if (M::word() == 0) rows.factor[M::row(i)] = __uint_as_float((uint32_t)(127 - e) << 23) * scale2;
             }
         }
         if (threadIdx.x < MT_ROWS) {
-            float4 &r = rows[threadIdx.x];
-            if (!FACTORS) r.x = scale2;
-            r.y = stat.y != 0.0f ? -stat.x : 0.0f, r.z = stat.y, r.w = __uint_as_float(token_of(c0 + threadIdx.x, magic));
+            float *pair = rows.pair[threadIdx.x / 2] + threadIdx.x % 2;
+            pair[0] = stat.y != 0.0f ? -stat.x : 0.0f, pair[2] = stat.y;
+            rows.token[threadIdx.x] = stat.y != 0.0f ? (int32_t)token_of(c0 + threadIdx.x, magic) : -1;
         }
     }
 };
@@ -130,6 +140,8 @@ __global__ void __launch_bounds__(MT_THREADS, MT_CTAS) pages_mass_tc5_kernel(con
     using P = MtPlan<HD>;
     using TP = typename std::conditional<Q4, __half, T>::type;  // of the operands
     constexpr uint32_t TILE = P::TILE;
+    constexpr bool FACTORS = MtQueries<T, HD, Q4>::FACTORS;
+    static_assert(sizeof(MtRows) == 16 * MT_ROWS, "as many bytes as are set apart");
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem), bar = sbase + P::BAR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(smem + P::BAR + MB_ABORT);
@@ -178,7 +190,7 @@ __global__ void __launch_bounds__(MT_THREADS, MT_CTAS) pages_mass_tc5_kernel(con
         const uint32_t from = tmem + ((warp % 4 * 32) << 16) + half * 64;
         const float scale2 = a.scale * 1.4426950408889634f;
         const uint32_t magic = a.group > 1 ? 0xffffffffu / a.group + 1 : 0u;
-        float4 *rows = reinterpret_cast<float4 *>(smem + P::BAR + MB_ROWS);  // [4][column]: of product n at n % 4 (with keys that stream: of the piece at 0)
+        MtRows *rows = reinterpret_cast<MtRows *>(smem + P::BAR + MB_ROWS);  // of product n at n % 4 (with keys that stream: of the piece at 0)
         volatile float *xchg = reinterpret_cast<volatile float *>(smem + P::BAR + MB_XCHG);
         float *pending = nullptr;  // where the sum of the tile before goes: the other half's part is known only after the next barrier
         float pending_old = 0.0f, pending_sum = 0.0f;
@@ -212,13 +224,13 @@ __global__ void __launch_bounds__(MT_THREADS, MT_CTAS) pages_mass_tc5_kernel(con
                 };
                 auto finish = [&](uint32_t i) {
                     if (keys_stream) keys.finish(smem + place(i));
-                    else queries.finish(i * MT_ROWS, magic, scale2, smem + place(i), rows + (n0 + i & 3) * MT_ROWS);
+                    else queries.finish(i * MT_ROWS, magic, scale2, smem + place(i), rows[n0 + i & 3]);
                 };
                 mt_sync();  // (all have read the rows of the piece before, and its products are done)
                 settle();
                 if (keys_stream) {
                     queries.issue(a, row0, head, n_cols, 0, magic, sbase);
-                    queries.finish(0, magic, scale2, smem, rows);
+                    queries.finish(0, magic, scale2, smem, rows[0]);
                 } else {
                     keys.issue(a, table, head, wk.page + group * MT_PAGES, last, sbase);
                     keys.finish(smem);
@@ -244,34 +256,47 @@ __global__ void __launch_bounds__(MT_THREADS, MT_CTAS) pages_mass_tc5_kernel(con
                     if (i + 2 < length) issue(i + 2);
                     cp_commit();
                     if (first) sum = 0.0f;
-                    const float4 *col = rows + (keys_stream ? 0u : n & 3) * MT_ROWS + half * 64;
+                    const MtRows &col = rows[keys_stream ? 0u : n & 3];
                     float part = 0.0f;
-                    // Without bits a position is seen by the tokens from `least` on.  (A row that sees nothing has no weights, whatever its score.)
-                    const uint32_t least = x < ctx ? 0u : x < limit ? x - ctx : ~0u;
-                    const bool bits = a.visible && x - r + MT_ROWS > ctx;  // (alike for all threads)
+                    // Without bits a position is seen by the tokens from `least` on.
+                    const int32_t least = x < ctx ? 0 : x < limit ? (int32_t)(x - ctx) : 0x7fffffff;
+                    const bool inside = x - r + MT_ROWS <= ctx, bits = a.visible && !inside;  // (alike for all threads)
+                    const bool plain = inside && __all_sync(0xffffffffu, min(col.token[half * 64 + lane], col.token[half * 64 + 32 + lane]) >= 0);  // every column sees every position
 #pragma unroll 1
                     for (uint32_t c = 0; c < 64; c += 16) {
+                        const uint32_t c0 = half * 64 + c;
                         uint32_t u[16];
                         tmem_ld16(from + b * MT_ROWS + c, u);
                         tmem_ld_wait();
                         float p[2] = {0.0f, 0.0f};
                         if (!bits) {
 #pragma unroll
-                            for (uint32_t e = 0; e < 16; ++e) {
-                                const float4 w = col[c + e];
-                                const float f = pow2(fmaf(__uint_as_float(u[e]), w.x, w.y));
-                                if (w.z != 0.0f && __float_as_uint(w.w) >= least) p[e & 1] = fmaf(f, w.z, p[e & 1]);
+                            for (uint32_t e = 0; e < 16; e += 2) {
+                                const float4 w = *reinterpret_cast<const float4 *>(col.pair[(c0 + e) / 2]);
+                                float2 k = make_float2(scale2, scale2);
+                                if constexpr (FACTORS) k = *reinterpret_cast<const float2 *>(col.factor + c0 + e);
+                                float f0, f1;
+                                fma2(f0, f1, __uint_as_float(u[e]), __uint_as_float(u[e + 1]), k.x, k.y, w.x, w.y);
+                                f0 = pow2(f0), f1 = pow2(f1);
+                                if (plain) {
+                                    fma2(p[0], p[1], f0, f1, w.z, w.w, p[0], p[1]);
+                                } else {
+                                    const int2 tok = *reinterpret_cast<const int2 *>(col.token + c0 + e);
+                                    if (tok.x >= least) p[0] = fmaf(f0, w.z, p[0]);
+                                    if (tok.y >= least) p[1] = fmaf(f1, w.w, p[1]);
+                                }
                             }
                         } else {
 #pragma unroll 1
                             for (uint32_t e = 0; e < 16; ++e) {
-                                const float4 w = col[c + e];
-                                bool see = x < ctx && w.z != 0.0f;
-                                if (x >= ctx && x < limit && w.z != 0.0f) see = a.visible[row0 + __float_as_uint(w.w)] >> ((x - ctx) & 63) & 1;
+                                const float *w = col.pair[(c0 + e) / 2] + e % 2;
+                                const int32_t tok = col.token[c0 + e];
+                                bool see = x < ctx && tok >= 0;
+                                if (x >= ctx && x < limit && tok >= 0) see = a.visible[row0 + tok] >> ((x - ctx) & 63) & 1;
                                 float s = __uint_as_float(u[0]);
 #pragma unroll
                                 for (uint32_t k = 1; k < 16; ++k) s = e == k ? __uint_as_float(u[k]) : s;
-                                if (see) p[0] = fmaf(pow2(fmaf(s, w.x, w.y)), w.z, p[0]);
+                                if (see) p[0] = fmaf(pow2(fmaf(s, FACTORS ? col.factor[c0 + e] : scale2, w[0])), w[2], p[0]);
                             }
                         }
                         part += p[0] + p[1];
