@@ -8,8 +8,8 @@
 // One operand stays and the other streams: with up to 128 columns the queries of a (sequence, head) stay and its keys go by; with more the keys of 128
 // positions stay and the queries go by.  The pages of all pieces are shared out evenly (pages_walk.cuh), a tile is eight of them.  A position has one
 // writer, columns are added up in order: no atomics.  Its floor is the special function unit's, 16 powers of two a clock: 500 tokens of 4 heads a head at 12,000, 8 heads of 128, 46 us.
-// It takes 236 us (the mma.sync form 627): a warp's step of 128 positions and 64 columns is some 1100 instructions, of which weights are a third, and issues half of the
-// time; tiles of queries come anew for every 128 positions (bfloat16 ones over 4-bit pages are made f16 each time: 431 us).  All waits are bounded; after one that was given up
+// It takes 200 us (the mma.sync form 627; 236 with a least share of the square root of a piece's pages, as attention has it, for which there were too few CTAs): a warp's step of 128 positions and 64 columns is some 1100 instructions, of which weights are a third, and issues half of the
+// time; tiles of queries come anew for every 128 positions (bfloat16 ones over 4-bit pages are made f16 each time: 366 us).  All waits are bounded; after one that was given up
 // every warp still goes through its loop, so that none is missed at a barrier.
 #include <algorithm>
 
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(MT_THREADS, MT_CTAS) pages_mass_tc5_kernel(con
     pdl_release();  // (only now: a CTA of the next kernel must not take the tensor memory first, it would keep it until this grid is done)
     pdl_wait();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + P::BAR + MB_SLOT);
-    PaWalk<true> wk;
+    PaWalk<true, MT_PAGES> wk;
     wk.start(a);
     uint32_t n = 0;  // products so far: number n has place n % 2 of what streams, and of the scores
     if (warp == MT_MMA_WARP) {
@@ -351,7 +351,7 @@ cudaError_t launch(PagedAttnArgs a, uint32_t n_seq, float *mass, uint64_t stride
     const uint64_t pages = (std::min<uint64_t>(a.max_ctx, (uint64_t)a.pg.stride * KV_PAGE) + a.max_drafts + KV_PAGE - 1) / KV_PAGE;  // about, of a sequence
     a.block = a.max_drafts, a.blocks = 1, a.n_units = n_seq;  // whole sequences
     a.apart = 0;
-    const uint64_t grid = std::min<uint64_t>((uint64_t)sm_count * MT_CTAS, std::max<uint64_t>(1, n_seq * ((pages + PA_LEAST - 1) / PA_LEAST) * a.pg.n_kv));
+    const uint64_t grid = std::min<uint64_t>((uint64_t)sm_count * MT_CTAS, std::max<uint64_t>(1, n_seq * ((pages + MT_PAGES - 1) / MT_PAGES) * a.pg.n_kv));
     return launch_pdl(kernel, dim3((uint32_t)grid), dim3(MT_THREADS), P::BYTES, st, a, mass, stride);
 }
 template <typename T>

@@ -87,8 +87,9 @@ __device__ __forceinline__ PaUnit pa_tree_unit(const PagedAttnArgs &a, uint32_t 
     return u;
 }
 // Pieces in the order (unit, head); every warp holds the same walk.  Where the grid has a CTA for every `per` pages of every piece, a piece begins a new
-// CTA (`apart`): none has the end of one and the start of the next.
-template <bool TREE>
+// CTA (`apart`): none has the end of one and the start of the next.  UNIT: where a cut piece
+// costs nothing, the least share is so many pages, and no more.
+template <bool TREE, uint32_t UNIT = 0>
 struct PaWalk {
     uint64_t at, end, per;  // pages of this CTA, pages a CTA; with `apart`, every piece counts as a multiple of `per`
     uint32_t unit, head, page;
@@ -166,7 +167,8 @@ struct PaWalk {
     __device__ __forceinline__ void share(uint64_t total, uint64_t pieces) {
         const float piece = (float)total / (float)pieces;  // pages of a piece, about
         const uint64_t even = total >> 32 ? (total + gridDim.x - 1) / gridDim.x : total ? ((uint32_t)total - 1) / gridDim.x + 1 : 0;
-        per = max(even, (uint64_t)max(PA_LEAST, (uint32_t)sqrtf(TREE ? piece : 0.5f * piece)));
+        if constexpr (UNIT != 0) per = max(even, (uint64_t)UNIT);
+        else per = max(even, (uint64_t)max(PA_LEAST, (uint32_t)sqrtf(TREE ? piece : 0.5f * piece)));
     }
     __device__ __forceinline__ bool more() const { return at < end; }
     __device__ __forceinline__ uint32_t last() const { return (uint32_t)min((uint64_t)u.n_pages, page + (end - at)); }  // the present piece is pages [page, last())
