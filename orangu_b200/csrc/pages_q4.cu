@@ -5,14 +5,14 @@
 // output^T += values^T x weights^T (16 dimensions x 8 rows), whose weights come out of the scores' registers by one exchange of 8 x 8 halves.  Up to 8
 // rows are half the products that 16 rows on the other side would be.  The order of a product's terms is free: a lane takes 16 neighbouring bytes of a key and
 // of two values.  Queries are f16; bfloat16 ones become that after a power of two per row has been taken out (their 8 bits fit, and what
-// falls below 2^-24 of 2^14 is less than 2^-38 of the row's largest).  Weights are f16 numbers raised by 2^7, as over f16 pages: where the output is f16, as value and
-// remainder; where it is bfloat16 their value alone, which is off by 2^-12 at most, an eighth of what the output's own rounding is (64 sequences of 4 to 16 k, 4 rows of
-// 128: 165 us, and 183 with remainders).
+// falls below 2^-24 of 2^14 is less than 2^-38 of the row's largest).  Weights enter as value and remainder, raised by 2^7, as over f16 pages: the value alone is off by up to
+// 2^-11, which is more than a bfloat16 output's own rounding where values cancel.
 //
-// 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, and its arithmetic is what bounds it: about 345 instructions a page of 128 (4-bit words to
-// entries 176, products 16, copies, scores and weights the rest) against 472 issue slots of an SM in the time that the bytes take.  64 sequences of 4 to
-// 16 k, 8 heads of 128, 4 rows: 165 us (4.2 TB/s; 115 with the copies alone, 124 without the values' half), 64 of 64 entries 112 us.  More CTAs an SM, deeper rings, products apart or
-// two sums of scores at once changed nothing; instructions did (373 a page, with remainders: 183).
+// 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, and about 373 instructions with 128 entries (4-bit words to entries 176, products 24, copies, scores and
+// weights the rest), of the 472 issue slots that an SM has in the time of the bytes.  64 sequences of 4 to 16 k, 8 heads of 128, 4 rows: 183 us (3.8 TB/s; 115 with the
+// copies alone), 64 of 64 entries 121 us.  Issued without gaps the instructions would take 85 us: more than half of the slots are empty, and no pipe is busy half of the time.  What it
+// waits for are latencies, one instruction's after the other's, with 16 warps an SM; more CTAs an SM, deeper rings, products apart or two sums of scores at once changed
+// nothing, shorter chains did.
 #include <algorithm>
 
 #include "pages_q4.cuh"
@@ -42,7 +42,6 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 3) pages_q4_attentio
     using F = Half2<__half>;
     using S = P4Shape<HD>;
     using B = Q4Block<HD>;
-    constexpr bool REST = std::is_same<T, __half>::value;  // weights with their remainders
     constexpr int DEPTH = S::DEPTH, KW = HD / 32, MT = HD / 16;  // words of a lane: of a key, of two values; tiles of dimensions
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t s_last;
@@ -220,7 +219,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 3) pages_q4_attentio
                         for (int i = 0; i < MT; ++i) o[i][n][c] *= keep, o[i][n][2 + c] *= keep;
                     }
             }
-            uint32_t w[NT][2], rest[NT][2];  // (REST)
+            uint32_t w[NT][2], rest[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -228,11 +227,8 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 3) pages_q4_attentio
                     const float e0 = pow2(fmaf(s[n][2 * h], fac[n][0], off[n][0])), e1 = pow2(fmaf(s[n][2 * h + 1], fac[n][1], off[n][1]));
                     sum[n][0] += e0, sum[n][1] += e1;
                     const uint32_t u = F::pack(e0, e1);
-                    w[n][h] = transposed(u);
-                    if constexpr (REST) {
-                        const float2 r = F::unpack(u);
-                        rest[n][h] = transposed(F::pack(e0 - r.x, e1 - r.y));
-                    }
+                    const float2 r = F::unpack(u);
+                    w[n][h] = transposed(u), rest[n][h] = transposed(F::pack(e0 - r.x, e1 - r.y));
                 }
             }
             // ---- outputs of the lane's dimensions: positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9
@@ -254,7 +250,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 4 : 3) pages_q4_attentio
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         F::mma(o[2 * i + j][n], f, w[n][0], w[n][1]);
-                        if constexpr (REST) F::mma(o[2 * i + j][n], f, rest[n][0], rest[n][1]);
+                        F::mma(o[2 * i + j][n], f, rest[n][0], rest[n][1]);
                     }
                 }
         }

@@ -24,7 +24,7 @@
 // for 32 sequences of 8192 with 512 rows in a call of its own, 855 in a loop, where the clocks fall under the power limit (floor 335).  A part of the powers of
 // two on the fused multiply-adds, 1/8 to 1/2 of them, took from 2 % less to 6 % more.
 //
-// Over 4-bit pages (Q4) warps make the f16 operand tiles out of codes, where TMA brings them otherwise; rows of bfloat16 have weights without remainders.  Four warps
+// Over 4-bit pages (Q4) warps make the f16 operand tiles out of codes, where TMA brings them otherwise.  Four warps
 // do it, two for keys and two for values.  8 x 16 tokens of 4 heads at 8192: 67 us (f16 pages 61); with three quarters of any one part left out, making of tiles, softmax, products or
 // copies, 56 to 66: no one of them bounds it, and 17 are the same at 512 positions.  1000 tokens of 8 heads at 8000: 334 us, 830 TFLOP/s of scores and values.
 //
@@ -286,7 +286,6 @@ __global__ void __launch_bounds__(Q4 ? P4_THREADS : PG_THREADS, 1)
 pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnArgs a) {
     using P = PgPlan<HD, WIDE, Q4>;
     using TP = typename std::conditional<Q4, __half, T>::type;  // of the operands
-    constexpr bool REST = !Q4 || std::is_same<T, __half>::value;  // weights with their remainders; f16 ones for bfloat16 outputs without (pages_q4.cu)
     constexpr uint32_t KST = P::KST, VST = P::VST, G = P::G, PLACE = P::PLACE, OPERAND = P::OPERAND, ROWS = P::ROWS, NB = P::NB, MR = P::MR;
     extern __shared__ __align__(1024) uint8_t smem[];  // (no other shared memory: the operand tiles' swizzle counts on the alignment)
     const uint32_t sbase = smem_u32(smem);
@@ -437,7 +436,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 #pragma unroll
                     for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add; 16 positions: eight columns of values, eight of remainders
                         umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
-                        if constexpr (REST) umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
+                        umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
                     }
                     umma_commit_warp(bar + PB_PV_DONE + 8 * s);
                     if (i % G == G - 1 || step + 1 == (int)steps) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
@@ -605,7 +604,7 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                         sum0 = sum1 = 0.0f;
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {  // 16 positions
-                            uint32_t v[REST ? 16 : 8];
+                            uint32_t v[16];
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 const float x0 = __uint_as_float(u[g / 2][g % 2 * 16 + 2 * e]), x1 = __uint_as_float(u[g / 2][g % 2 * 16 + 2 * e + 1]);
@@ -615,13 +614,10 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                                 e0 = pow2(e0), e1 = pow2(e1);
                                 add2(sum0, sum1, e0, e1);
                                 v[e] = pack16<TP>(e0, e1);
-                                if constexpr (REST) {
-                                    const float2 r = unpack16(v[e], TP());
-                                    v[8 + e] = pack16<TP>(e0 - r.x, e1 - r.y);
-                                }
+                                const float2 r = unpack16(v[e], TP());
+                                v[8 + e] = pack16<TP>(e0 - r.x, e1 - r.y);
                             }
-                            if constexpr (REST) tmem_st16(tp + 16 * g, v);
-                            else tmem_st8(tp + 16 * g, v);
+                            tmem_st16(tp + 16 * g, v);
                         }
                         const float now = fmaxf(top[0], top[1]) * scale2;
                         const bool grown = now > m + PG_SLACK;

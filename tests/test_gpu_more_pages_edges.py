@@ -1,0 +1,46 @@
+"""4-bit pages, weights per position, cut caches and verified drafts where they went wrong once: values that cancel, keys that are no finite numbers, paths longer than
+their list, numbers that are none."""
+import numpy as np
+import pytest
+
+import more_pages_plain as more
+import pages_plain as plain
+from gpu_common import backend  # noqa: F401
+from test_gpu_more_pages import U, Held, current, distributions, run_verify, weight_error
+from test_gpu_pages import PAGE, device16, float64, ints, words
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(made, q, kind, ctx, counts, bits, scale, mass=None):
+    """Output of attention_tokens over `made`, as float64; `mass` (a device array) is added to."""
+    import torch
+
+    qd = device16(plain.to16(q, kind)[1], kind)
+    out = torch.full_like(qd, 7.0)
+    made.cache.attention_tokens(qd, ints(np.concatenate([[0], np.cumsum(counts)])), ints(ctx), scale, out, max_tokens=max(counts), max_context=max(ctx), visible=words(bits) if bits is not None else None, mass=mass,
+                                stream=current())
+    made.cache.synchronize(current())
+    return float64(out)
+
+
+# ------------------------------------------------------------------------------------------- weights and their remainders
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,group,count", [(128, 4, 1), (64, 8, 1), (128, 2, 8), (64, 4, 8), (128, 4, 16), (64, 16, 7), (128, 8, 64), (64, 4, 64)])
+def test_values_that_cancel(backend, kind, dim, group, count):
+    """Two positions with nearly the same weight and opposite values: what is left of them is off by the weights' errors, which the output's rounding does not hide.  A
+    weight that were one number of 11 bits would be off by up to 2^-11, a few times the bound (sum |q k| is about a half here)."""
+    made = Held(backend, "q4", kind, 2, dim, [2 + count], seed=dim + group + count)
+    x = made.r.standard_normal((2 + count, 2, dim))
+    y = made.r.standard_normal((2 + count, 2, dim))
+    y[1] = -y[0]
+    rows = [plain.to16(z, kind) for z in (x, y)]
+    made.cache.store(*(device16(b, kind) for _, b in rows), ints([0, 2 + count]), ints([0]), max_tokens=2 + count, stream=current())
+    k, v = (more.in_four_bits(z) for z, _ in rows)
+    q = plain.to16(made.r.standard_normal((count, 2 * group, dim)) * 0.1, kind)[0]
+    scale, first, bits = 0.25 * 64 / dim / 4, [0, count], [0] * count  # drafts see the context alone
+    want = np.zeros(q.shape)
+    tol, _ = more.attend_tokens(q, [k], [v], made.there, first, [2], bits, scale, want, None, weight_error(dim))
+    got = attend(made, q, kind, [2], [count], bits, scale)
+    off = np.abs(got - want) - (tol[..., None] + U[kind] * (np.abs(want) + tol[..., None]) + 2.0 ** -25)
+    assert off.max() <= 0, f"{off.max()} over the bound ({tol.max()}) at {np.unravel_index(off.argmax(), off.shape)}"
