@@ -325,142 +325,145 @@ pages_tree_tc5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     auto steps_of = [&](uint32_t s, uint32_t tiles, uint32_t rows) { return WIDE ? (s == 0 || rows > PG_ROWS ? tiles : 0u) : (tiles + 1 - s) / 2; };
     auto tile_of = [&](uint32_t s, uint32_t step) { return WIDE ? step : s + 2 * step; };
 
-    if (Q4 && warp >= PG_TMA_WARP) {
-        if constexpr (Q4) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-            auto make = [&](auto value, uint32_t mine) {
-                constexpr bool VALUE = decltype(value)::value;
-                using Tile = P4Tile<HD, VALUE>;
-                constexpr uint32_t PLACES = VALUE ? VST : KST;
-                static_assert(PLACES % P4_TURNS == 0 && G == 1, "a place is always the same warp's");
-                const uint32_t full = bar + (VALUE ? PB_V_FULL : PB_K_FULL), empty = bar + (VALUE ? PB_V_EMPTY : PB_K_EMPTY);
-                const uint8_t *pool = static_cast<const uint8_t *>(VALUE ? a.pg.v : a.pg.k);
-                uint8_t *own = smem + P::CODES + (warp - PG_TMA_WARP) * P4_AHEAD * Tile::BYTES;
-                // The warp's next tile: number `at` of all tiles, those of its places.
-                uint32_t at = mine, before = 0;  // tiles of the pieces before
-                auto request = [&](uint32_t slot) {
-                    for (; w.more() && at - before >= w.last() - w.tile; w.next(a)) before += w.last() - w.tile;
-                    if (w.more()) {
-                        const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
-                        const uint32_t p = (w.tile + at - before) * PG_PAGES + lane % PG_PAGES;
-                        int32_t id = p < w.q.n_pages ? table[p] : -1;
-                        if ((uint32_t)id >= a.pg.n_pages) id = -1;
-                        Tile::request(smem_addr(own) + slot * Tile::BYTES, pool, a.pg.n_kv, w.head, id);
-                    }
-                    cp_commit();
-                    const bool any = w.more();
-                    at += P4_TURNS;
-                    return any;
-                };
-                bool ok = true;
-                uint32_t end = ~0u;  // the first of the warp's tiles that there is not
-#pragma unroll 1
-                for (uint32_t n = mine, slot = 0; ok; slot = slot + 1 == P4_AHEAD ? 0 : slot + 1) {
-                    if (!request(slot)) end = min(end, at - P4_TURNS);
-                    if (at < mine + P4_AHEAD * P4_TURNS) continue;  // (the first ones are only asked for)
-                    if (n >= end) break;
-                    cp_wait<P4_AHEAD - 1>();
-                    __syncwarp();
-                    const uint32_t st = n % PLACES, from = slot + 1 == P4_AHEAD ? 0 : slot + 1;
-                    ok = mbar_wait_warp(empty + 8 * st, ((n / PLACES) & 1u) ^ 1u, abort);  // (a place that was not used yet is empty)
-                    if (!ok) break;
-                    Tile::make(smem_addr(own) + from * Tile::BYTES, sbase + (VALUE ? P::V : P::K) + st * PLACE);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();  // (all of the warp's rows are written, and its codes read)
-                    if (lane == 0) mbar_arrive(full + 8 * st);
-                    n += P4_TURNS;
-                }
-                cp_wait<0>();
-            };
-            const uint32_t role = warp - PG_TMA_WARP;  // (two warps only fill their warpgroup)
-            if (role < P4_CODE_WARPS && (role & 1)) make(std::true_type{}, role / 2);
-            else if (role < P4_CODE_WARPS) make(std::false_type{}, role / 2);
-        }
-    } else if (warp >= PG_TMA_WARP) {
-        const bool values = warp > PG_TMA_WARP;
-        const CUtensorMap *map = values ? &tm_v : &tm_k;
-        const uint32_t ring = sbase + (values ? P::V : P::K), full = bar + (values ? PB_V_FULL : PB_K_FULL), empty = bar + (values ? PB_V_EMPTY : PB_K_EMPTY), places = values ? VST : KST;
-        uint32_t st = 0, par = 1;  // the tile's place, and the parity of its last use: a place that was not used yet is empty
-        bool ok = true;
-        const uint32_t nowhere = a.pg.n_pages * a.pg.n_kv * KV_PAGE;  // the row behind the pool: reads as zero
-        const uint32_t page = lane % (G * PG_PAGES), box = lane / (G * PG_PAGES), at = page / PG_PAGES * OPERAND + box * PG_BLOCK + page % PG_PAGES * (KV_PAGE * 128);  // a lane a copy
-        for (; w.more() && ok; w.next(a)) {
-            const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
-            const uint32_t end = w.last();
-            auto row_of = [&](uint32_t tile) {  // the first row of the lane's page of the tiles from this one on
-                const uint32_t p = tile * PG_PAGES + page;
-                const int32_t id = p < min(end * PG_PAGES, w.q.n_pages) ? table[p] : -1;
-                return (uint32_t)id < a.pg.n_pages ? ((uint32_t)id * a.pg.n_kv + w.head) * KV_PAGE : nowhere;
-            };
-            uint32_t y = row_of(w.tile);
-            for (uint32_t i = w.tile; i < end; i += G) {
-                const uint32_t next = row_of(i + G);
-                if (!(ok = mbar_wait_warp(empty + 8 * st, par, abort))) break;
-                if (lane == 0) mbar_expect_tx(full + 8 * st, PLACE);
-                __syncwarp();
-                if (box < NB) tma_load_2d(ring + st * PLACE + at, map, (int32_t)(box * 64), (int32_t)y, full + 8 * st);
-                __syncwarp();
-                y = next;
-                if (++st == places) st = 0, par ^= 1;
-            }
-        }
-    } else if (warp >= PG_MMA_WARP) {
+    if (warp >= PG_MMA_WARP) {
+        // One instruction for all warps of a warpgroup, before their roles part.  256 threads x 104 and 256 x 152 are the 512 x 128 of the launch.
+        static_assert(PG_MMA_WARP % 4 == 0 && P4_THREADS == 2 * PG_SOFT, "whole warpgroups");
         if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        constexpr uint32_t F16 = EXPONENT16<TP> == EXPONENT16<bf16> ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
-        const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
-        const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
-        uint32_t n = 0, turn = 0, done = 0;  // places, pieces and tiles of the stream so far
-        bool ok = true;
-        const uint64_t q_desc = umma_desc_sw128(sbase + (WIDE ? s * ROWS : 0u)), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
-        for (; w.more() && ok; w.next(a), ++turn) {
-            const uint32_t tiles = w.last() - w.tile, steps = steps_of(s, tiles, w.q.drafts * a.group - w.rt * MR);
-            ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);  // (of every piece: a phase that is not waited for could be taken for the next one)
-            if (WIDE && steps == 0)  // no rows: only says of every tile that it does not need it
-                for (uint32_t i = 0; i < (tiles + G - 1) / G && ok; ++i) {
-                    const uint32_t kt = (n + i) % KST, vt = (n + i) % VST;
-                    ok = mbar_wait_warp(bar + PB_K_FULL + 8 * kt, ((n + i) / KST) & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * vt, ((n + i) / VST) & 1u, abort);
-                    if (ok && lane == 0) mbar_arrive(bar + PB_K_EMPTY + 8 * kt), mbar_arrive(bar + PB_V_EMPTY + 8 * vt);
-                    __syncwarp();
-                }
+        if (Q4 && warp >= PG_TMA_WARP) {
+            if constexpr (Q4) {
+                auto make = [&](auto value, uint32_t mine) {
+                    constexpr bool VALUE = decltype(value)::value;
+                    using Tile = P4Tile<HD, VALUE>;
+                    constexpr uint32_t PLACES = VALUE ? VST : KST;
+                    static_assert(PLACES % P4_TURNS == 0 && G == 1, "a place is always the same warp's");
+                    const uint32_t full = bar + (VALUE ? PB_V_FULL : PB_K_FULL), empty = bar + (VALUE ? PB_V_EMPTY : PB_K_EMPTY);
+                    const uint8_t *pool = static_cast<const uint8_t *>(VALUE ? a.pg.v : a.pg.k);
+                    uint8_t *own = smem + P::CODES + (warp - PG_TMA_WARP) * P4_AHEAD * Tile::BYTES;
+                    // The warp's next tile: number `at` of all tiles, those of its places.
+                    uint32_t at = mine, before = 0;  // tiles of the pieces before
+                    auto request = [&](uint32_t slot) {
+                        for (; w.more() && at - before >= w.last() - w.tile; w.next(a)) before += w.last() - w.tile;
+                        if (w.more()) {
+                            const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
+                            const uint32_t p = (w.tile + at - before) * PG_PAGES + lane % PG_PAGES;
+                            int32_t id = p < w.q.n_pages ? table[p] : -1;
+                            if ((uint32_t)id >= a.pg.n_pages) id = -1;
+                            Tile::request(smem_addr(own) + slot * Tile::BYTES, pool, a.pg.n_kv, w.head, id);
+                        }
+                        cp_commit();
+                        const bool any = w.more();
+                        at += P4_TURNS;
+                        return any;
+                    };
+                    bool ok = true;
+                    uint32_t end = ~0u;  // the first of the warp's tiles that there is not
 #pragma unroll 1
-            for (int step = -2; step < (int)steps && ok; ++step) {  // -2, -1: only the first scores
-                const uint32_t place = (done + step) & 1u;
-                if (step >= 0) {
-                    const uint32_t i = tile_of(s, step), at = n + i / G, st = at % VST;
-                    if (i % G == 0) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / VST) & 1u, abort);
-                    ok = ok && mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * place, (done + step) >> 1 & 1u, abort);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t p = ts + place * PG_KEYS;
-                    const uint64_t vd = v_desc + ((st * PLACE + i % G * OPERAND) >> 4);
-#pragma unroll
-                    for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add; 16 positions: eight columns of values, eight of remainders
-                        umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
-                        umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
+                    for (uint32_t n = mine, slot = 0; ok; slot = slot + 1 == P4_AHEAD ? 0 : slot + 1) {
+                        if (!request(slot)) end = min(end, at - P4_TURNS);
+                        if (at < mine + P4_AHEAD * P4_TURNS) continue;  // (the first ones are only asked for)
+                        if (n >= end) break;
+                        cp_wait<P4_AHEAD - 1>();
+                        __syncwarp();
+                        const uint32_t st = n % PLACES, from = slot + 1 == P4_AHEAD ? 0 : slot + 1;
+                        ok = mbar_wait_warp(empty + 8 * st, ((n / PLACES) & 1u) ^ 1u, abort);  // (a place that was not used yet is empty)
+                        if (!ok) break;
+                        Tile::make(smem_addr(own) + from * Tile::BYTES, sbase + (VALUE ? P::V : P::K) + st * PLACE);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();  // (all of the warp's rows are written, and its codes read)
+                        if (lane == 0) mbar_arrive(full + 8 * st);
+                        n += P4_TURNS;
                     }
-                    umma_commit_warp(bar + PB_PV_DONE + 8 * s);
-                    if (i % G == G - 1 || step + 1 == (int)steps) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
-                }
-                const uint32_t next = step + 2;
-                if (next < steps) {
-                    const uint32_t i = tile_of(s, next), at = n + i / G, st = at % KST;
-                    if (i % G == 0) ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / KST) & 1u, abort);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t kd = k_desc + ((st * PLACE + i % G * OPERAND) >> 4);
-#pragma unroll
-                    for (uint32_t b = 0; b < HD / 16; ++b)
-                        umma_bf16_warp(ts + place * PG_KEYS, q_desc + (b / 4) * (PG_QBLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
-                    umma_commit_warp(bar + PB_S_FULL + 16 * s + 8 * place);
-                    if (i % G == G - 1 || next + 1 == steps) umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
-                } else if (next == steps + 1 && steps > 0) {
-                    umma_commit_warp(bar + PB_O_FULL + 8 * s);
+                    cp_wait<0>();
+                };
+                const uint32_t role = warp - PG_TMA_WARP;  // (two warps only fill their warpgroup)
+                if (role < P4_CODE_WARPS && (role & 1)) make(std::true_type{}, role / 2);
+                else if (role < P4_CODE_WARPS) make(std::false_type{}, role / 2);
+            }
+        } else if (warp >= PG_TMA_WARP) {
+            const bool values = warp > PG_TMA_WARP;
+            const CUtensorMap *map = values ? &tm_v : &tm_k;
+            const uint32_t ring = sbase + (values ? P::V : P::K), full = bar + (values ? PB_V_FULL : PB_K_FULL), empty = bar + (values ? PB_V_EMPTY : PB_K_EMPTY), places = values ? VST : KST;
+            uint32_t st = 0, par = 1;  // the tile's place, and the parity of its last use: a place that was not used yet is empty
+            bool ok = true;
+            const uint32_t nowhere = a.pg.n_pages * a.pg.n_kv * KV_PAGE;  // the row behind the pool: reads as zero
+            const uint32_t page = lane % (G * PG_PAGES), box = lane / (G * PG_PAGES), at = page / PG_PAGES * OPERAND + box * PG_BLOCK + page % PG_PAGES * (KV_PAGE * 128);  // a lane a copy
+            for (; w.more() && ok; w.next(a)) {
+                const int32_t *table = a.pg.tables + (uint64_t)(a.blocks > 1 ? w.seq / a.blocks : w.seq) * a.pg.stride;
+                const uint32_t end = w.last();
+                auto row_of = [&](uint32_t tile) {  // the first row of the lane's page of the tiles from this one on
+                    const uint32_t p = tile * PG_PAGES + page;
+                    const int32_t id = p < min(end * PG_PAGES, w.q.n_pages) ? table[p] : -1;
+                    return (uint32_t)id < a.pg.n_pages ? ((uint32_t)id * a.pg.n_kv + w.head) * KV_PAGE : nowhere;
+                };
+                uint32_t y = row_of(w.tile);
+                for (uint32_t i = w.tile; i < end; i += G) {
+                    const uint32_t next = row_of(i + G);
+                    if (!(ok = mbar_wait_warp(empty + 8 * st, par, abort))) break;
+                    if (lane == 0) mbar_expect_tx(full + 8 * st, PLACE);
+                    __syncwarp();
+                    if (box < NB) tma_load_2d(ring + st * PLACE + at, map, (int32_t)(box * 64), (int32_t)y, full + 8 * st);
+                    __syncwarp();
+                    y = next;
+                    if (++st == places) st = 0, par ^= 1;
                 }
             }
-            n += (tiles + G - 1) / G, done += steps;
+        } else {
+            constexpr uint32_t F16 = EXPONENT16<TP> == EXPONENT16<bf16> ? 0u : (1u << 7) | (1u << 10);  // the operands' format bits: zero for f16
+            const uint32_t id_s = umma_idesc_bf16(PG_KEYS) & ~F16, id_o = (umma_idesc_bf16(HD) & ~F16) | UMMA_B_MN_MAJOR;
+            const uint32_t s = warp - PG_MMA_WARP, ts = tmem + PG_TMEM_S + s * 2 * PG_KEYS, to = tmem + PG_TMEM_O + s * 128;
+            uint32_t n = 0, turn = 0, done = 0;  // places, pieces and tiles of the stream so far
+            bool ok = true;
+            const uint64_t q_desc = umma_desc_sw128(sbase + (WIDE ? s * ROWS : 0u)), k_desc = umma_desc_sw128(sbase + P::K), v_desc = umma_desc_sw128_mn(sbase + P::V, PG_BLOCK);
+            for (; w.more() && ok; w.next(a), ++turn) {
+                const uint32_t tiles = w.last() - w.tile, steps = steps_of(s, tiles, w.q.drafts * a.group - w.rt * MR);
+                ok = mbar_wait_warp(bar + PB_Q_FULL, turn & 1u, abort);  // (of every piece: a phase that is not waited for could be taken for the next one)
+                if (WIDE && steps == 0)  // no rows: only says of every tile that it does not need it
+                    for (uint32_t i = 0; i < (tiles + G - 1) / G && ok; ++i) {
+                        const uint32_t kt = (n + i) % KST, vt = (n + i) % VST;
+                        ok = mbar_wait_warp(bar + PB_K_FULL + 8 * kt, ((n + i) / KST) & 1u, abort) && mbar_wait_warp(bar + PB_V_FULL + 8 * vt, ((n + i) / VST) & 1u, abort);
+                        if (ok && lane == 0) mbar_arrive(bar + PB_K_EMPTY + 8 * kt), mbar_arrive(bar + PB_V_EMPTY + 8 * vt);
+                        __syncwarp();
+                    }
+#pragma unroll 1
+                for (int step = -2; step < (int)steps && ok; ++step) {  // -2, -1: only the first scores
+                    const uint32_t place = (done + step) & 1u;
+                    if (step >= 0) {
+                        const uint32_t i = tile_of(s, step), at = n + i / G, st = at % VST;
+                        if (i % G == 0) ok = mbar_wait_warp(bar + PB_V_FULL + 8 * st, (at / VST) & 1u, abort);
+                        ok = ok && mbar_wait_warp(bar + PB_P_FULL + 16 * s + 8 * place, (done + step) >> 1 & 1u, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t p = ts + place * PG_KEYS;
+                        const uint64_t vd = v_desc + ((st * PLACE + i % G * OPERAND) >> 4);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < PG_KEYS / 16; ++kk) {  // the stream's first product writes, the others add; 16 positions: eight columns of values, eight of remainders
+                            umma_bf16_ta_warp(to, p + kk * 16, vd + kk * 128, id_o, step || kk ? 1u : 0u);
+                            umma_bf16_ta_warp(to, p + kk * 16 + 8, vd + kk * 128, id_o, 1u);
+                        }
+                        umma_commit_warp(bar + PB_PV_DONE + 8 * s);
+                        if (i % G == G - 1 || step + 1 == (int)steps) umma_commit_warp(bar + PB_V_EMPTY + 8 * st);
+                    }
+                    const uint32_t next = step + 2;
+                    if (next < steps) {
+                        const uint32_t i = tile_of(s, next), at = n + i / G, st = at % KST;
+                        if (i % G == 0) ok = mbar_wait_warp(bar + PB_K_FULL + 8 * st, (at / KST) & 1u, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t kd = k_desc + ((st * PLACE + i % G * OPERAND) >> 4);
+#pragma unroll
+                        for (uint32_t b = 0; b < HD / 16; ++b)
+                            umma_bf16_warp(ts + place * PG_KEYS, q_desc + (b / 4) * (PG_QBLOCK >> 4) + 2 * (b % 4), kd + (b / 4) * (PG_BLOCK >> 4) + 2 * (b % 4), id_s, b ? 1u : 0u);
+                        umma_commit_warp(bar + PB_S_FULL + 16 * s + 8 * place);
+                        if (i % G == G - 1 || next + 1 == steps) umma_commit_warp(bar + PB_K_EMPTY + 8 * st);
+                    } else if (next == steps + 1 && steps > 0) {
+                        umma_commit_warp(bar + PB_O_FULL + 8 * s);
+                    }
+                }
+                n += (tiles + G - 1) / G, done += steps;
+            }
         }
-    } else if (warp < PG_MMA_WARP) {
-        if constexpr (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");  // 256 threads x 152 and 256 x 104 are the 512 x 128 of the launch
+    } else {
+        if constexpr (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const uint32_t s = warp / 4, quad = warp % 4, r = quad * 32 + lane;
         const uint32_t magic = (65536 + a.group - 1) / a.group;  // x / group = x magic / 65536 for x below 4096, group up to 16
         float scale2 = a.scale * 1.4426950408889634f;  // weights are powers of two of the scaled score
