@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) pages_mass_kernel(const __grid_
                                         const uint32_t x = pos0 + i * KV_PAGE + g + 8 * h;
                                         if (row.z != 0.0f && (x < ctx || (x < limit && (a.visible ? (bits >> ((x - ctx) & 63) & 1) != 0 : x - ctx <= tok)))) part[i][h] = fmaf(e, row.z, part[i][h]);
                                     } else {
-                                        part[i][h] = fmaf(e, row.z, part[i][h]);
+                                        if (row.z != 0.0f) part[i][h] = fmaf(e, row.z, part[i][h]);  // (a column of zeros: an infinite entry of a key would make it none)
                                     }
                                 }
                         }

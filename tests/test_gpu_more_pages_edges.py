@@ -44,3 +44,30 @@ def test_values_that_cancel(backend, kind, dim, group, count):
     got = attend(made, q, kind, [2], [count], bits, scale)
     off = np.abs(got - want) - (tol[..., None] + U[kind] * (np.abs(want) + tol[..., None]) + 2.0 ** -25)
     assert off.max() <= 0, f"{off.max()} over the bound ({tol.max()}) at {np.unravel_index(off.argmax(), off.shape)}"
+
+
+# ------------------------------------------------------------------------------------------- weights where keys are no finite numbers
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,group,count", [(64, 1, 1), (128, 3, 1), (64, 4, 5), (128, 3, 40), (64, 7, 20)])
+def test_a_key_that_every_row_puts_at_minus_infinity(backend, kind, dim, group, count):
+    """Its weight is zero in every row, and in the columns that fill up a set there is none: what the position had gathered stays, whatever kernel the number of rows takes."""
+    import torch
+
+    ctx, at, entry = 50, 21, 5
+    made = Held(backend, kind, kind, 2, dim, [ctx + count], seed=dim + group + count)
+    page = int(made.tables[0, at // PAGE])
+    made.kd[0, page, :, at % PAGE, entry] = float("inf")
+    q = plain.to16(made.r.standard_normal((count, 2 * group, dim)), kind)[0]
+    q[..., entry] = -np.abs(q[..., entry]) - 0.25
+    q = plain.to16(q, kind)[0]  # as the device has them
+    mass = made.r.exponential(1.0, (1, 2, made.tables.shape[1] * PAGE)).astype(np.float32)
+    md, want, mass64 = torch.from_numpy(mass).cuda(), np.zeros(q.shape), mass.astype(np.float64)
+    there = [made.there[0].copy()]
+    there[0][at] = False  # a weight of zero
+    tol, mass_tol = more.attend_tokens(q, made.k[0], made.v[0], there, [0, count], [ctx], None, dim ** -0.5, want, mass64, weight_error(dim))
+    got = attend(made, q, kind, [ctx], [count], None, dim ** -0.5, md)
+    off = np.abs(got - want) - (tol[..., None] + U[kind] * (np.abs(want) + tol[..., None]) + 2.0 ** -25)
+    assert off.max() <= 0
+    masses = md.cpu().numpy()
+    assert np.isfinite(masses).all() and np.array_equal(masses[0, :, at], mass[0, :, at])
+    assert (np.abs(masses - mass64) <= mass_tol).all()
