@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
     };
     if (threadIdx.x == 0 && n) s_path[0] = 0;
 #pragma unroll 1
-    for (uint32_t i = 1; i < n; ++i) {
+    for (uint32_t i = 1; i < n && n_path < a.kept_stride; ++i) {  // (a full list ends the path: what is drawn next follows its last node)
         if (s_parent[i] != (int32_t)node) continue;
         const double u = fmax((double)s_u[i], 0.0);
         double p = s_p[i];
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(DV_THREADS, 2) drafts_verify_kernel(const __gr
     cluster.sync();  // (nobody's memory goes away while others may read it)
     if (rank == 0) {
         for (uint32_t j = threadIdx.x; j < a.kept_stride; j += DV_THREADS) a.kept[(uint64_t)seq * a.kept_stride + j] = n && j < n_path ? s_path[j] : -1;
-        if (threadIdx.x == 0) a.n_kept[seq] = n ? min(n_path, a.kept_stride) : 0u;
+        if (threadIdx.x == 0) a.n_kept[seq] = n ? n_path : 0u;
     }
 }
 

@@ -247,8 +247,8 @@ class PagedCache:
 def verify_drafts(backend: CudaBackend, target, draft, tokens, parent, first_token, uniform, kept, n_kept, next_token, stream=None):
     """Which drafted tokens are accepted.  Node i of sequence s (nodes first_token[s] .. first_token[s + 1] - 1, node 0 the last certain token) is token tokens[i] and
     continues node parent[i] < i of its sequence; ``target`` [nodes, vocabulary] are the probabilities of what follows each node, ``draft`` those that its children were drawn
-    from (None: each was certain), ``uniform`` [nodes] random numbers from [0, 1).  kept [sequences, up to 64] int32: node 0 and the accepted ones, -1
-    behind them, as ``PagedCache.keep`` takes them; n_kept; next_token: what is drawn after the last of them."""
+    from (None: each was certain), ``uniform`` [nodes] random numbers from [0, 1).  kept [sequences, up to 64] int32: node 0 and the accepted ones, no
+    more than it has places, -1 behind them, as ``PagedCache.keep`` takes them; n_kept; next_token: what is drawn after the last of them."""
     t = _type_of[target.dtype]
     if t is None:
         raise ValueError(f"target is {target.dtype}, expected float32, float16 or bfloat16")

@@ -71,3 +71,54 @@ def test_a_key_that_every_row_puts_at_minus_infinity(backend, kind, dim, group, 
     masses = md.cpu().numpy()
     assert np.isfinite(masses).all() and np.array_equal(masses[0, :, at], mass[0, :, at])
     assert (np.abs(masses - mass64) <= mass_tol).all()
+
+
+# ------------------------------------------------------------------------------------------- verification
+def in_list(parent, first, width):
+    """The tree without the nodes whose paths are longer than the list: nobody's children."""
+    out = np.array(parent).copy()
+    for a, b in zip(first[:-1], first[1:]):
+        depth = np.zeros(b - a, int)
+        for i in range(1, b - a):
+            depth[i] = depth[parent[a + i]] + 1
+            if depth[i] >= width:
+                out[a + i] = -1
+    return out
+
+
+def chain_with_siblings(m):
+    """Every third node is the child of a node that has one already; the others go on from each other."""
+    parent, last = [-1], 0
+    for i in range(1, m):
+        parent.append(last if i % 3 else max(0, parent[last]))
+        last = i if i % 3 else last
+    return parent
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("width", [1, 2, 3, 5])
+def test_a_path_ends_with_its_list(backend, kind, drafted, width):
+    """No more nodes are accepted than the list holds, and the next token follows the last one in it."""
+    import torch
+
+    from orangu_b200 import verify_drafts
+
+    r = np.random.default_rng(width)
+    vocab, sizes = 300, [7, 1, 12, 64, 4] * 3
+    first, n = np.concatenate([[0], np.cumsum(sizes)]), sum(sizes)
+    target, draft = distributions(r, n, vocab, kind)
+    draft = plain.to16(0.7 * target + 0.3 * draft, kind)[0] if kind != "f32" else (0.7 * target + 0.3 * draft).astype(np.float32).astype(np.float64)  # mostly accepted
+    parent = np.concatenate([chain_with_siblings(m) for m in sizes])
+    above = np.repeat(first[:-1], sizes) + np.maximum(parent, 0)
+    tokens = np.array([r.choice(vocab, p=draft[a] / draft[a].sum()) if drafted else int(target[a].argmax()) for a in above])
+    uniform = r.random(n).astype(np.float32) * (1.0 if drafted else 0.02)
+    uniform[first[:-1]] = r.random(len(sizes))
+    want = more.verify(target, draft if drafted else None, tokens, in_list(parent, first, width), first, uniform, width)
+    assert (want[1] == width).sum() >= 5  # lists that are full
+    device = lambda x: torch.from_numpy(x.astype(np.float32)).cuda() if kind == "f32" else device16(plain.to16(x, kind)[1], kind)  # noqa: E731
+    kept, count, token = torch.full((len(sizes), width), 7, dtype=torch.int32, device="cuda"), ints([7] * len(sizes)), ints([7] * len(sizes))
+    verify_drafts(backend, device(target), device(draft) if drafted else None, ints(tokens), ints(parent), ints(first), torch.from_numpy(uniform).cuda(), kept, count, token, stream=current())
+    torch.cuda.synchronize()
+    for got, w in zip((kept, count, token), want):
+        assert np.array_equal(got.cpu().numpy(), w), (got, w)
