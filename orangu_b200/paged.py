@@ -79,6 +79,7 @@ class PagedCache:
         if len(tables.shape) != 2:
             raise ValueError(f"tables is {list(tables.shape)}, expected [sequences, pages each]")
         self.backend, self._lib, self._arrays = backend, backend._lib, (k, v, tables)
+        self._device = getattr(k, "device", None)
         self.n_layer, self.n_pages, self.n_head_kv = shape[:3]
         self.head_dim = shape[3] // 9 if self._q4 else shape[4]
         self.n_seq, self.table_stride = tuple(tables.shape)
@@ -189,8 +190,13 @@ class PagedCache:
             self._check(self._lib.ob_pages_keep_mass(self._h, n_seq, *p, *m, _stream(stream)))
 
     def _mass(self, mass, n_seq, *layers):
-        """Address and row stride of weights [(layers,) sequences, kv heads, positions]."""
-        return _array("mass", mass, layers + (n_seq, self.n_head_kv, mass.shape[-1]), _FLOAT), mass.shape[-1]
+        """Address and row stride of weights [(layers,) sequences, kv heads, positions], a table's positions or more."""
+        width = mass.shape[-1]
+        if width < self.table_stride * _PAGE:
+            raise ValueError(f"mass is {list(mass.shape)}, expected at least {self.table_stride * _PAGE} positions")
+        if getattr(mass, "device", None) != self._device:
+            raise ValueError(f"mass is on {mass.device}, the cache on {self._device}")
+        return _array("mass", mass, layers + (n_seq, self.n_head_kv, width), _FLOAT), width
 
     def _moved(self, call, k, v, first_token, n_ctx, max_tokens, layer, stream):
         t = _type_of[k.dtype]
