@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(THREADS) pages_evict_choose_kernel(const __gri
     int32_t *out = a.kept + (uint64_t)blockIdx.x * a.n_keep;
     if (blockIdx.x % a.pg.n_kv == 0 && blockIdx.x / a.pg.n_kv < a.n_seq && threadIdx.x == 0) a.n_left[seq] = min(n, a.n_keep);
     if (n <= a.n_keep) {
-        for (uint32_t i = threadIdx.x; i < a.n_keep; i += THREADS) out[i] = i < n ? (int32_t)i : -1;
+        for (uint64_t i = threadIdx.x; i < a.n_keep; i += THREADS) out[i] = i < n ? (int32_t)i : -1;  // (in 32 bits the last turn of a list of almost 2^32 would begin anew)
         return;
     }
     const MassWords words{a.mass + (uint64_t)blockIdx.x * a.mass_stride, a.keep_first, n - a.keep_last};

@@ -73,6 +73,23 @@ def test_a_key_that_every_row_puts_at_minus_infinity(backend, kind, dim, group, 
     assert (np.abs(masses - mass64) <= mass_tol).all()
 
 
+# ------------------------------------------------------------------------------------------- cutting caches down
+def test_a_list_of_almost_all_numbers(backend):
+    """n_keep may be anything that 32 bits hold: what lies behind the last position is filled up to the end."""
+    import torch
+
+    n_keep = (1 << 32) - 1
+    if torch.cuda.mem_get_info()[0] < 6 * n_keep:
+        pytest.skip("not enough memory")
+    made = Held(backend, "q4", "f16", 1, 64, [40], seed=1)
+    kept, left, mass = torch.zeros((1, 1, 1, n_keep), dtype=torch.int32, device="cuda"), ints([0]), torch.ones((1, 1, 1, made.tables.shape[1] * PAGE), device="cuda")
+    made.cache.evict(ints([40]), mass, kept, left, max_pos=40, stream=current())
+    torch.cuda.synchronize()
+    flat = kept.view(-1)
+    assert left.item() == 40 and torch.equal(flat[:40].cpu(), torch.arange(40, dtype=torch.int32))
+    assert all(bool((part == -1).all()) for part in flat[40:].split(1 << 28))
+
+
 # ------------------------------------------------------------------------------------------- verification
 def in_list(parent, first, width):
     """The tree without the nodes whose paths are longer than the list: nobody's children."""
