@@ -314,11 +314,12 @@ int ob_pages_keep_mass(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, c
  * past it are left out), as ob_pages_attention_tokens had them: node 0 is its last certain token, node i the drafted token tokens[i] that continues node
  * parent[i] < i (numbers within the sequence; the root's entries of both are not read).  Row i of target, [n_tokens][n_vocab] f32, f16 or bfloat16, target_stride elements apart:
  * the target's probabilities of what follows node i; draft: those that node i's children were drawn from independently, or NULL (each was certain).
- * uniform: [n_tokens] numbers from [0, 1).  From node 0 on the children of the present node are tried in ascending order; c = 0 and T = 1 at first:
+ * uniform: [n_tokens] numbers from [0, 1); what is no number, or below, counts as 0.
+ * From node 0 on the children of the present node are tried in ascending order; c = 0 and T = 1 at first:
  *   with draft     child x is accepted where uniform[x] T q(x) < p(x) - c q(x); if not, c becomes c + T and T the sum of max(p - c q, 0)
  *   without        where uniform[x] T < p(x); if not, T becomes T - p(x) and p(x) zero
- * until no child of the present node is accepted, or kept_stride nodes are kept: the children of the last one are not tried then.  next_token[s] is then the first v at which the sum of max(p - c q, 0) (without draft: p) exceeds uniform[0] times all of
- * it; if all of it is zero, the same of the target's row, and -1 if that is zero, too.  kept [n_seq][kept_stride <= 64]: 0 and the accepted nodes, -1 behind
+ * until no child of the present node is accepted, or kept_stride nodes are kept (the children of the last one are not tried then).  next_token[s] is then the first v
+ * at which the sum of max(p - c q, 0) (without draft: p) exceeds uniform[0] times all of it; if all of it is zero, the same of the target's row, and -1 if that is zero, too.  kept [n_seq][kept_stride <= 64]: 0 and the accepted nodes, -1 behind
  * them, as ob_pages_keep takes them, n_kept how many.  A probability that is not a positive finite number counts as zero; a node whose
  * parent or token is out of range is never accepted.  A sequence without nodes: n_kept 0, next_token -1.  Sums are in 64 bits. */
 int ob_drafts_verify(ob_ctx *ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t n_vocab, uint32_t type, const void *target, uint64_t target_stride, const void *draft,

@@ -139,3 +139,13 @@ def test_a_path_ends_with_its_list(backend, kind, drafted, width):
     torch.cuda.synchronize()
     for got, w in zip((kept, count, token), want):
         assert np.array_equal(got.cpu().numpy(), w), (got, w)
+
+
+@pytest.mark.parametrize("drafted", [True, False])
+def test_random_numbers_that_are_none(backend, drafted):
+    """They count as 0, as numbers below it do."""
+    r = np.random.default_rng(8)
+    target, draft = distributions(r, 6, 50, "f32")
+    tokens, parent, first = np.array([0, 3, 4, 5, 6, 7]), np.array([-1, 0, 0, 1, 1, 2]), np.array([0, 6])
+    for u in (np.full(6, np.nan), np.array([np.nan, 0.9, 0.9, 0.9, 0.9, 0.9]), np.array([0.7, 1.0, np.nan, 1.0, 1.0, np.nan]), np.array([-np.inf, np.inf, -1.0, 0.99, np.nan, 0.5])):
+        run_verify(backend, "f32", target, draft if drafted else None, tokens, parent, first, u)
