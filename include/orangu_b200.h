@@ -314,7 +314,7 @@ int ob_pages_keep_mass(ob_pages *pages, uint32_t n_seq, const uint32_t *n_ctx, c
  * past it are left out), as ob_pages_attention_tokens had them: node 0 is its last certain token, node i the drafted token tokens[i] that continues node
  * parent[i] < i (numbers within the sequence; the root's entries of both are not read).  Row i of target, [n_tokens][n_vocab] f32, f16 or bfloat16, target_stride elements apart:
  * the target's probabilities of what follows node i; draft: those that node i's children were drawn from independently, or NULL (each was certain).
- * uniform: [n_tokens] numbers from [0, 1); what is no number, or below, counts as 0.
+ * uniform: [n_tokens] numbers from [0, 1); what is no number, or below, counts as 0.  With n_tokens 0 these five may be NULL.
  * From node 0 on the children of the present node are tried in ascending order; c = 0 and T = 1 at first:
  *   with draft     child x is accepted where uniform[x] T q(x) < p(x) - c q(x); if not, c becomes c + T and T the sum of max(p - c q, 0)
  *   without        where uniform[x] T < p(x); if not, T becomes T - p(x) and p(x) zero

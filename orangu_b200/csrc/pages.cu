@@ -810,9 +810,10 @@ int ob_drafts_verify(ob_ctx *ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t n_
     if (n_seq > (1u << 24)) return invalid("too many sequences");
     if (n_seq == 0) return OB_OK;
     const size_t size = type == OB_TYPE_F32 ? 4 : 2;
-    const Named list[] = {{target, "target", size}, {draft, "draft", size}, {tokens, "tokens", 4}, {parent, "parent", 4}, {first_token, "first_token", 4}, {uniform, "uniform", 4}, {kept, "kept", 4}, {n_kept, "n_kept", 4}, {next_token, "next_token", 4}};
+    const Named list[] = {{draft, "draft", size}, {target, "target", size}, {tokens, "tokens", 4}, {parent, "parent", 4}, {uniform, "uniform", 4}, {first_token, "first_token", 4}, {kept, "kept", 4}, {n_kept, "n_kept", 4}, {next_token, "next_token", 4}};
+    constexpr int OF_NODES = 5;  // the first of them: nobody reads them where there are no nodes
     for (const Named &n : list) {
-        if (!n.p && n.p == draft && &n == list + 1) continue;
+        if (!n.p && (&n == list || (n_tokens == 0 && &n < list + OF_NODES))) continue;
         if (!n.p) return invalid(std::string(n.name) + " is null");
         if (!aligned(n.p, n.align)) return invalid(std::string(n.name) + " is not aligned to " + std::to_string(n.align) + " bytes");
         if (!on_device(ctx, n.p)) return invalid(std::string(n.name) + " is not memory of the context's device");

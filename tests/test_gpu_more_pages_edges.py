@@ -142,6 +142,20 @@ def test_a_path_ends_with_its_list(backend, kind, drafted, width):
 
 
 @pytest.mark.parametrize("drafted", [True, False])
+def test_no_nodes_at_all(backend, drafted):
+    """A batch without drafts or certain tokens: empty arrays have no memory, and every sequence its answer."""
+    import torch
+
+    from orangu_b200 import verify_drafts
+
+    rows, none = torch.zeros((0, 50), device="cuda"), ints([])
+    kept, count, token = torch.full((3, 5), 7, dtype=torch.int32, device="cuda"), ints([7] * 3), ints([7] * 3)
+    verify_drafts(backend, rows, rows if drafted else None, none, none, ints([0, 0, 0, 0]), torch.zeros(0, device="cuda"), kept, count, token, stream=current())
+    torch.cuda.synchronize()
+    assert bool((kept == -1).all()) and count.tolist() == [0, 0, 0] and token.tolist() == [-1, -1, -1]
+
+
+@pytest.mark.parametrize("drafted", [True, False])
 def test_random_numbers_that_are_none(backend, drafted):
     """They count as 0, as numbers below it do."""
     r = np.random.default_rng(8)
