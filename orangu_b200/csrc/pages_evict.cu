@@ -242,10 +242,13 @@ cudaError_t launch_pages_evict(const PagedEvictArgs &a, uint32_t n_layer, uint32
         }))
         return e;
     const uint32_t pairs = n_layer * a.n_seq * a.pg.n_kv, held = std::min({std::max(max_pos, 1u), a.pg.stride * KV_PAGE, EV_HELD});
-    if (cudaError_t e = max_pos <= 4096 ? launch_pdl(pages_evict_choose_kernel<256>, dim3(pairs), dim3(256), (size_t)held * 4, st, a, held)
+    // Threads of the choice: 256 for short caches, many of which run at once, 1024 above.  2048 rows (32 layers of eight sequences, 8 heads of 128), the cut as a whole: of 200 positions 51 us
+    // with 256 and 76 with 1024, of 600 114 and 99, of 2050 375 and 354, of 4100 828 and 673; 64 entries: of 600 74 and 82, of 1500 172 and 149.
+    if (cudaError_t e = max_pos <= 1024 ? launch_pdl(pages_evict_choose_kernel<256>, dim3(pairs), dim3(256), (size_t)held * 4, st, a, held)
                                         : launch_pdl(pages_evict_choose_kernel<1024>, dim3(pairs), dim3(1024), (size_t)held * 4, st, a, held))
         return e;
-    // Large CTAs where they are few: fewer batches, one after the other, of a head.
+    // Large CTAs for the moves where they are few: fewer batches, one after the other, of a head.  8 heads of 128, 128 rows of 4100 positions: 41 us with them and 69 with small ones, in 4 bits 53
+    // and 111.  512 rows of 200: 21 and 17, 2048 rows of 1000: 162 and 188 (4 bits: 183 and 176), of 4100 619 and 673 (4 bits: 657 and 597).
     auto move = [&](auto small, auto large) {
         return pairs < 512 ? launch_pdl(large, dim3(pairs, 3), dim3(512), 0, st, a) : launch_pdl(small, dim3(pairs, 3), dim3(256), 0, st, a);
     };
