@@ -16,7 +16,10 @@ constexpr uint32_t PG_MAX_GROUP = 16;    // query heads of a key/value head
 // dimension 128: 16.4 and 18.4 us for one sequence of 512, 45.1 and 51.2 for 32 of 1024, 195 and 223 for 32 of 8192; 64: 14.3 and 16.4, 30.7 and
 // 43.0, 119 and 166.  More rows would read all pages once per 16.
 constexpr uint32_t PG_FEW_ROWS = 16;
-constexpr uint32_t P4_FEW_ROWS = 32;     // the same over 4-bit pages, there in units of tokens that have up to 16
+// The same over 4-bit pages, there in units of tokens that have up to 16 rows, each of which reads the pages for itself.  Both at 32 and 48 rows, f16 queries, 8 heads of 128: one sequence of
+// 2048 16.5 and 18.6, 18.6 and 18.6 us; eight of 2048 28.9 and 30.8, 37.0 and 30.9; 32 of 2048 73.9 and 79.6, 101 and 82; eight of 8192 68.5 and 64.3, 94.3 and 65.4; with 64
+// entries 45.2 and 57.5, 61.6 and 57.2.
+constexpr uint32_t P4_FEW_ROWS = 32;
 // Shares of a CTA from which on all are even (PA_MORE): 32 sequences of 2 to 8 k in 4 bits 59.5 us, and 68.0 with pieces that all begin a CTA; 8 of
 // 2000 12.6 us, and 15.5 with even shares.
 constexpr uint32_t PG_APART = 64;
@@ -93,8 +96,9 @@ cudaError_t launch_pages_q4_tc5(const PagedAttnArgs &a, bool q_bf16, int sm_coun
 // After an attention with `stats`, whose units are of n_seq sequences: [n_seq][n_kv][mass_stride].
 cudaError_t launch_pages_mass(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, int sm_count, cudaStream_t st);
 
-// Rows a key/value head up to which the first of the two is taken: 64 and 128 rows over f16 pages, 16 sequences of 2000, attention among it: 72.9 and 94.6 us with it, 75.9
-// and 81.0 on tcgen05.  Where bfloat16 queries have to become f16 ones for every tile it is more: 128 rows over 4-bit pages 95.0 and 101.0, 512 (one of 12,000) 175 and 170.
+// Rows a key/value head up to which the first of the two is taken.  Both at 64 and 128 rows over f16 pages, 16 sequences of 2000, attention among it: 71.4 and 72.4 us, 93.3 and 77.6.
+// Where bfloat16 queries have to become f16 ones for every tile it is more, and depends on the sequences, too: 256 and 512 rows over 4-bit pages, one sequence of 12,000: 108 and 101,
+// 181 and 160; four of 12,000: 202 and 256, 388 and 457; 2000 rows, one sequence: 627 and 366.
 constexpr uint32_t PG_MASS_ROWS = 96, P4_MASS_ROWS_BF16 = 256;
 cudaError_t launch_pages_mass_tc5(const PagedAttnArgs &a, bool q_bf16, bool q4, uint32_t n_seq, float *mass, uint64_t mass_stride, int sm_count, cudaStream_t st);
 

@@ -8,11 +8,10 @@
 // falls below 2^-24 of 2^14 is less than 2^-38 of the row's largest).  Weights enter as value and remainder, raised by 2^7, as over f16 pages: the value alone is off by up to
 // 2^-11, which is more than a bfloat16 output's own rounding where values cancel.
 //
-// 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, and about 373 instructions with 128 entries (4-bit words to entries 176, products 24, copies, scores and
-// weights the rest), of the 472 issue slots that an SM has in the time of the bytes.  64 sequences of 4 to 16 k, 8 heads of 128, 4 rows: 183 us (3.8 TB/s; 115 with the
-// copies alone), 64 of 64 entries 121 us.  Issued without gaps the instructions would take 85 us: more than half of the slots are empty, and no pipe is busy half of the time.  What it
-// waits for are latencies, one instruction's after the other's, with 16 warps an SM; more CTAs an SM, deeper rings, products apart or two sums of scores at once changed
-// nothing, shorter chains did.
+// 9 bits for two entries: a page of a head is 18 HD bytes, keys and values, and with 128 entries about 373 instructions of the loop (4-bit words to entries 176, products 24, copies, scores
+// and weights the rest), 401 with starts and ends.  In the time of the bytes an SM can issue 396 (at 1.9 GHz): the two floors are the same, and there is little room for a gap.  64
+// sequences of 4 to 16 k, 8 heads of 128, 4 rows: 183 us, 3.8 TB/s (115 with the copies alone), 64 of 64 entries 121 us.  59 % of the issue slots are used and no pipe more than 42 %;
+// what the warps, 16 an SM, wait for most are the latencies of their own instructions.  More CTAs an SM, deeper rings, products apart or two sums of scores at once changed nothing.
 #include <algorithm>
 
 #include "pages_q4.cuh"

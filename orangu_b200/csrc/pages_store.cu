@@ -5,8 +5,8 @@
 // so that m itself is -8 d or a little less.  No number counts as 0, and magnitudes above 7168 as 7168, which keeps d an f16 number and every entry c d one, too.
 // The quotient is a product with about 1 / d and one step of Newton's, so that ties are ties.
 //
-// Half a warp has a key's or value's 128 entries, eight a lane (a quarter 64), the same place of several pages.  The arithmetic is the larger part: about 100
-// instructions for eight entries.  Maxima are taken two at a time in the rows' type; codes are whole numbers in the low bits of a sum with 1.5 2^23, put together as
+// Half a warp has a key's or value's 128 entries, eight a lane (a quarter 64), the same place of several pages.  The arithmetic is the larger part of storing: 167
+// instructions for eight entries, issued in 77 % of the slots (loading: 82, which wait for their loads).  Maxima are taken two at a time in the rows' type; codes are whole numbers in the low bits of a sum with 1.5 2^23, put together as
 // one number of base 16 by fused multiply-adds.
 #include <algorithm>
 #include <numeric>

@@ -26,7 +26,8 @@
 //
 // Over 4-bit pages (Q4) warps make the f16 operand tiles out of codes, where TMA brings them otherwise.  Four warps
 // do it, two for keys and two for values.  8 x 16 tokens of 4 heads at 8192: 67 us (f16 pages 61); with three quarters of any one part left out, making of tiles, softmax, products or
-// copies, 56 to 66: no one of them bounds it, and 17 are the same at 512 positions.  1000 tokens of 8 heads at 8000: 334 us, 830 TFLOP/s of scores and values.
+// copies, 56 to 66: no one of them bounds it, and 17 are the same at 512 positions.  1000 tokens of 8 heads at 8000: 405 us, 685 TFLOP/s of scores and values
+// (1030 with the products of the remainders).
 //
 // Context positions are seen by every row: only tiles that reach past the context, or have a page that is not there, are masked, a 64-bit word
 // per thread.  There, values of positions that nobody has, or that are no numbers, are set to zero in shared memory (0 times them

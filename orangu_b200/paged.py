@@ -105,8 +105,8 @@ class PagedCache:
             capi.check(self.backend._h, rc)
 
     def synchronize(self, stream=None):
-        """Waits for ``stream``.  Raises OranguError if a wait inside a kernel of attention_tree ran out since this was last asked: its output is not
-        valid then."""
+        """Waits for ``stream``.  Raises OranguError if a wait inside a kernel of attention_tree or attention_tokens ran out since this was last asked: its
+        output is not valid then."""
         self._check(self._lib.ob_pages_synchronize(self._h, _stream(stream)))
 
     def _rows(self, name, a, dtype=None):

@@ -88,6 +88,8 @@ def test_a_list_of_almost_all_numbers(backend):
     flat = kept.view(-1)
     assert left.item() == 40 and torch.equal(flat[:40].cpu(), torch.arange(40, dtype=torch.int32))
     assert all(bool((part == -1).all()) for part in flat[40:].split(1 << 28))
+    del kept, flat
+    torch.cuda.empty_cache()  # (17 GB)
 
 
 # ------------------------------------------------------------------------------------------- verification
