@@ -20,8 +20,8 @@ constexpr uint32_t PG_FEW_ROWS = 16;
 // 2048 16.5 and 18.6, 18.6 and 18.6 us; eight of 2048 28.9 and 30.8, 37.0 and 30.9; 32 of 2048 73.9 and 79.6, 101 and 82; eight of 8192 68.5 and 64.3, 94.3 and 65.4; with 64
 // entries 45.2 and 57.5, 61.6 and 57.2.
 constexpr uint32_t P4_FEW_ROWS = 32;
-// Shares of a CTA from which on all are even (PA_MORE): 32 sequences of 2 to 8 k in 4 bits 59.5 us, and 68.0 with pieces that all begin a CTA; 8 of
-// 2000 12.6 us, and 15.5 with even shares.
+// Shares of a CTA from which on all are even (PA_MORE).  4-bit pages, bfloat16 rows, 8 heads of 128: 32 sequences of 2 to 8 k 59.6 us, and 67.7 with pieces that all begin a CTA; one of
+// 4000 12.4 us, and 15.7 with even shares, two of 1000 with four tokens 14.5 and 20.7 (eight of 2000 16.5 and 14.8).
 constexpr uint32_t PG_APART = 64;
 constexpr float PG_SLACK = 8.0f;         // growth of a row's maximum (powers of two) that is put up with before its output is rescaled
 // Weights are made 2^PG_RAISE times as large, in numerator and denominator alike.  An f16 weight has steps of 2^-24 at best: of the running maximum's
